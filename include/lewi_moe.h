@@ -348,6 +348,43 @@ int lewi_gdn_chunk_bwd(void* stream, const void* q, const void* k, const void* v
                        float* dg, void* dbeta, float* dh0, int B, int S, int H, int K, int V);
 
 /* ------------------------------------------------------------------------------------------------
+ * Single-token steps of both, for decoding.  A row of the batch has its state at slots[b] of a pool of N (slots null: at b, N >= B);
+ * the state is read, moved one token on and written back.  slots[b] < 0: an idle row, zeros out, no state touched.  A slot past the
+ * pool, or one that an earlier row of the batch has: the same, and LEWI_STATUS_BAD_INDEX.  `*_stride` is the distance of two rows of
+ * the batch in elements; within a row inputs are contiguous.
+ *   convolution: y[b,c] = sum_{j<K} w[j,c] z[j,c], z = (state, x); state <- z[1..].  x, y bf16 [B,C], w bf16 [K,C], state bf16 [N,K-1,C]
+ *     (the K-1 inputs before this one, oldest first; zeros where there were none).  K <= 8, C a multiple of 8, all 16-byte aligned.
+ *   gated delta rule: S <- S exp(g), S <- S + k (x) beta (v - k^T S), o = (q / sqrt(K))^T S.  q, k bf16 [B,Hk,K], v, o bf16 [B,H,V],
+ *     g, beta [B,H] of g_dtype, beta_dtype; state f32 [N,H,K,V].  Value head h has the keys of head h / (H / Hk).  K <= 128; K and V
+ *     multiples of 8; state 16-byte, o 8-byte aligned.  Products and sums float32.
+ * ---------------------------------------------------------------------------------------------- */
+int lewi_causal_conv1d_step(void* stream, const void* x, int64_t x_stride, const void* w, void* state, const int32_t* slots, void* y,
+                            int B, int N, int C, int K);
+int lewi_gdn_step(void* stream, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                  const void* g, int g_dtype, const void* beta, int beta_dtype, float* state, const int32_t* slots, void* o, int B,
+                  int N, int Hk, int H, int K, int V);
+
+/* ------------------------------------------------------------------------------------------------
+ * A paged key-value cache: k_cache, v_cache bf16 [pages][page][Hkv][D], pages page_stride elements apart; sequence b has the pages
+ * tables[b][0..max_pages) (i32) and lengths[b] (i32) tokens in them, the new ones among them.  D <= 256, a multiple of 8; caches
+ * 16-byte aligned, page_stride a multiple of 8.  Table entries past a sequence's length are not read.  A length past the table counts
+ * as the table's, a page that does not exist is left out, both with LEWI_STATUS_BAD_INDEX; a length of zero or less is an idle row.
+ *   write: tokens cu_seqlens[b] .. cu_seqlens[b+1] of k, v bf16 [T][Hkv][D] (i32, ascending; null: one token per sequence, T = B) become
+ *     the last ones of sequence b.  Tokens of no sequence are left out.  Two tokens on one cell leave either.
+ *   attention of one new token per sequence: o[b,h] = softmax_j(scale q[b,h].k[j]) v[j] over the sequence's cells j, with the key head
+ *     h / (Hq / Hkv).  q, o bf16 [B][Hq][D]; zeros for an idle row.  Scores, softmax and sums float32, p rounded to bf16 for its
+ *     product with v.  The order of the sums depends on the lengths of the whole batch, not on chance: equal calls have equal bits.
+ * Cells that no sequence names are neither read nor written, so what they hold does not matter.
+ * ---------------------------------------------------------------------------------------------- */
+int lewi_paged_cache_write(void* stream, const void* k, int64_t k_stride, const void* v, int64_t v_stride, void* k_cache, void* v_cache,
+                           int64_t page_stride, const int32_t* tables, const int32_t* lengths, const int32_t* cu_seqlens, int T, int B,
+                           int Hkv, int D, int64_t pages, int page, int max_pages);
+int64_t lewi_paged_attention_workspace_bytes(int D);
+int lewi_paged_attention(void* stream, const void* q, int64_t q_stride, const void* k_cache, const void* v_cache, int64_t page_stride,
+                         const int32_t* tables, const int32_t* lengths, void* o, void* workspace, int64_t workspace_bytes, int B,
+                         int Hq, int Hkv, int D, int64_t pages, int page, int max_pages, float scale);
+
+/* ------------------------------------------------------------------------------------------------
  * The whole layer in two calls.  lewi_moe_fwd / lewi_moe_bwd queue the complete launch sequence of the MoE layer of
  * the MaxText `qwen3_5` block as the reference patches it: router (softmax -> top-k -> renormalise,
  * configs/stage1.yml:33-41) -> `_route_activations` (modal/moe_permute.py:399-404) -> the three `ragged_dot`s of the

@@ -74,6 +74,12 @@ SIGNATURES = {
     "lewi_causal_conv1d_bwd": (c_int, [P, P, P, P, P, P, c_int, P, c_int64, c_int, c_int, c_int, c_int]),
     "lewi_gdn_chunk_workspace_bytes": (c_int64, [c_int, c_int, c_int, c_int, c_int]),
     "lewi_gdn_chunk_fwd": (c_int, [P, P, P, P, P, P, P, P, P, P, c_int64, c_int, c_int, c_int, c_int, c_int]),
+    "lewi_causal_conv1d_step": (c_int, [P, P, c_int64, P, P, P, P, c_int, c_int, c_int, c_int]),
+    "lewi_gdn_step": (c_int, [P, P, c_int64, P, c_int64, P, c_int64, P, c_int, P, c_int, P, P, P] + [c_int] * 6),
+    "lewi_paged_cache_write": (c_int, [P, P, c_int64, P, c_int64, P, P, c_int64, P, P, P, c_int, c_int, c_int, c_int, c_int64, c_int, c_int]),
+    "lewi_paged_attention_workspace_bytes": (c_int64, [c_int]),
+    "lewi_paged_attention": (c_int, [P, P, c_int64, P, P, c_int64, P, P, P, P, c_int64, c_int, c_int, c_int, c_int, c_int64, c_int, c_int,
+                                     c_float]),
     "lewi_moe_residual_layout": (c_int64, [c_int64, c_int, c_int, c_int, c_int, c_int, c_int, P]),
     "lewi_moe_workspace_bytes": (c_int64, [c_int64, c_int, c_int, c_int, c_int, c_int, c_int]),
     "lewi_moe_router_prepared_bytes": (c_int64, [c_int, c_int]),
@@ -150,3 +156,42 @@ def last_status():
   if rc < 0:
     check(rc, "lewi_last_status")
   return rc
+
+
+def one_device(*tensors):
+  """A context in which the device of all these CUDA tensors (None is left out) is the current one."""
+  import contextlib
+  import torch
+  devices = {t.device for t in tensors if t is not None}
+  if len(devices) != 1 or next(iter(devices)).type != "cuda":
+    raise LewiError(f"expected CUDA tensors of one device, got {sorted(map(str, devices))}: the kernels have no CPU path")
+  index = next(iter(devices)).index
+  return contextlib.nullcontext() if index == torch.cuda.current_device() else torch.cuda.device(index)
+
+
+def index_table(t, what):
+  """A table of int32 as the kernels read it; int64 values that int32 cannot hold stay out of range."""
+  import torch
+  if t is None:
+    return None
+  if t.dtype == torch.int64:
+    t = t.clamp(-1, 2 ** 31 - 1).to(torch.int32)
+  if t.dtype != torch.int32:
+    raise LewiError(f"{what} holds int32 or int64 indices")
+  return t.contiguous()
+
+
+def rows_of(t, align):
+  """`t` with its trailing dimensions packed (only rows may be apart) and rows and address multiples of `align` bytes; a copy where they
+  are not."""
+  packed, n = True, 1
+  for size, step in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+    packed &= size == 1 or step == n
+    n *= size
+  rows = t.stride(0) if t.shape[0] > 1 else n
+  if not packed or rows < n or t.data_ptr() % align or rows * t.element_size() % align:
+    t = t.contiguous()
+    rows = n
+    if t.data_ptr() % align:
+      t = t.clone()
+  return t, rows

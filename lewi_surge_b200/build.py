@@ -5,14 +5,12 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-SRC = os.path.join(HERE, "csrc", "lewi_moe.cu")
+UNITS = ("lewi_moe.cu", "mixers.cu")   # compiled side by side, then linked
 OUT = os.path.join(HERE, "liblewi_moe.so")
-NVCC_FLAGS = [
-    "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
-    "-shared", "-Xcompiler", "-fPIC",
-]
+NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC"]
 
 
 def _sources():
@@ -35,15 +33,22 @@ def build(force=False, verbose=False):
   if not force and not is_stale():
     return OUT
   nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
-  cmd = [nvcc, *NVCC_FLAGS, "-o", OUT, SRC]
+  extra = ["-Xptxas", "-v"] if verbose else []
+  with tempfile.TemporaryDirectory() as tmp:
+    objects = [os.path.join(tmp, u + ".o") for u in UNITS]
+    runs = [subprocess.Popen([nvcc, *extra, *NVCC_FLAGS, "-c", "-o", o, os.path.join(HERE, "csrc", u)], stdout=subprocess.PIPE,
+                             stderr=subprocess.STDOUT, text=True) for u, o in zip(UNITS, objects)]
+    said = [r.communicate()[0] for r in runs]
+    if any(r.returncode != 0 for r in runs):
+      raise RuntimeError("nvcc failed:\n" + "\n".join(said))
+    linked = os.path.join(tmp, "lib.so")   # (moved into place whole: a process that loads it meanwhile has the old one)
+    res = subprocess.run([nvcc, *NVCC_FLAGS, "-shared", "-o", linked, *objects], capture_output=True, text=True)
+    if res.returncode != 0:
+      raise RuntimeError("linking failed:\n" + res.stdout + res.stderr)
+    shutil.copy(linked, OUT + ".new")
+    os.replace(OUT + ".new", OUT)
   if verbose:
-    cmd.insert(1, "-Xptxas")
-    cmd.insert(2, "-v")
-  res = subprocess.run(cmd, capture_output=True, text=True)
-  if res.returncode != 0:
-    raise RuntimeError("nvcc failed:\n" + res.stdout + res.stderr)
-  if verbose:
-    print(res.stderr)
+    print("\n".join(said))
   return OUT
 
 

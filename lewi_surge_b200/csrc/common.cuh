@@ -17,10 +17,18 @@ namespace lewi {
 constexpr int kWarp = 32;
 constexpr int kNumSMsDefault = 148;
 
-// Per-device status word.  Kernels OR bits into it; lewi_last_status() reads and clears it.
-__device__ int g_status = 0;
+// Per-device status word of this translation unit's kernels, which OR bits into it; lewi_last_status() reads and clears all of them.
+static __device__ int g_status = 0;
 
 __device__ __forceinline__ void raise_status(int bit) { atomicOr(&g_status, bit); }
+
+// The status word, and 0 in its place; negative: an error code.
+static inline int take_status_word() {
+  int v = 0, zero = 0;
+  if (cudaMemcpyFromSymbol(&v, g_status, sizeof(int)) != cudaSuccess) return LEWI_ERR_CUDA;
+  if (v != 0 && cudaMemcpyToSymbol(g_status, &zero, sizeof(int)) != cudaSuccess) return LEWI_ERR_CUDA;
+  return v;
+}
 
 struct alignas(16) U4 {
   uint32_t x, y, z, w;

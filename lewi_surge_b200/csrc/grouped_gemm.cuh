@@ -18,6 +18,7 @@
 
 #include "common.cuh"
 #include "tcgen05.cuh"
+#include "tensor_map.cuh"
 
 namespace lewi {
 namespace gg {
@@ -1010,41 +1011,6 @@ __global__ void __launch_bounds__(256) tn_reduce_ragged_kernel(const float* __re
 }
 
 // ------------------------------------------------------------------------------------------------ host side
-
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-inline EncodeTiledFn encode_fn() {
-  static const EncodeTiledFn fn = [] {   // (host threads that come here at the same time wait for the first)
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-                    q == cudaDriverEntryPointSuccess;
-    return ok ? reinterpret_cast<EncodeTiledFn>(p) : nullptr;
-  }();
-  return fn;
-}
-
-// Tiles of 128-byte swizzled rows.  The encoder is a driver function and wants the device's context in the calling host thread, which a
-// thread has only after its first runtime call that needs one (an autograd thread whose first work is a product has none yet).
-inline bool encode_tiled(CUtensorMap* m, CUtensorMapDataType type, cuuint32_t rank, const void* ptr, const cuuint64_t* dims,
-                         const cuuint64_t* strides, const cuuint32_t* box) {
-  const EncodeTiledFn fn = encode_fn();
-  if (fn == nullptr) return false;
-  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
-  auto encode = [&] {
-    return fn(m, type, rank, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  };
-  CUresult r = encode();
-  if (r == CUDA_ERROR_INVALID_CONTEXT) {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return false;
-    r = encode();
-  }
-  return r == CUDA_SUCCESS;
-}
 
 // bf16 (or f32) tensor [d2][d1][d0] (d0 contiguous); box [b2][b1][b0]; rank 2 when d2 == 0.
 inline bool make_map(CUtensorMap* m, const void* ptr, uint64_t d0, uint64_t d1, uint64_t d2, uint32_t b0,

@@ -17,6 +17,10 @@
 
 using namespace lewi;
 
+namespace lewi {
+int take_mixer_status();   // the status word of mixers.cu
+}
+
 // Scratch for lewi_router_topk_static(): lives in the library image, so every GPU that loads the
 // library holds these bytes until the process exits.  Host code must not pass this name to a kernel:
 // on the host it is only a handle; the device address comes from cudaGetSymbolAddress().
@@ -54,10 +58,8 @@ int64_t lewi_launch_count(void) { return launch_counter(); }
 
 int lewi_last_status(void* stream) {
   if (cudaStreamSynchronize(as_stream(stream)) != cudaSuccess) return LEWI_ERR_CUDA;
-  int v = 0, zero = 0;
-  if (cudaMemcpyFromSymbol(&v, g_status, sizeof(int)) != cudaSuccess) return LEWI_ERR_CUDA;
-  if (v != 0 && cudaMemcpyToSymbol(g_status, &zero, sizeof(int)) != cudaSuccess) return LEWI_ERR_CUDA;
-  return v;
+  const int here = take_status_word(), mixers = take_mixer_status();
+  return here < 0 ? here : mixers < 0 ? mixers : here | mixers;
 }
 
 int64_t lewi_padded_rows_bound(int64_t m, int num_experts, int block) {

@@ -1,0 +1,148 @@
+// C ABI of what mixes along the sequence, apart from the whole-sequence kernels of lewi_moe.cu: single-token steps of the convolution
+// and the gated delta rule, the paged cache, attention (declarations and contracts: include/lewi_moe.h).
+#include "common.cuh"
+#include "paged.cuh"
+#include "step.cuh"
+
+using namespace lewi;
+
+namespace lewi {
+int take_mixer_status() { return take_status_word(); }
+}
+
+namespace {
+
+inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
+inline bool aligned(const void* p, int to) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(to - 1)) == 0; }
+inline bool is_dtype(int d) { return d == LEWI_BF16 || d == LEWI_F32; }
+typedef __nv_bfloat16 bf16;
+
+// Checks of a paged cache; 0 or an error code.
+int check_cache(const void* k, const void* v, const int32_t* tables, const int32_t* lengths, int B, int Hkv, int D, int64_t pages, int page,
+                int max_pages, int64_t page_stride) {
+  if (!k || !v || !tables || !lengths || B <= 0 || Hkv <= 0 || D <= 0 || pages <= 0 || page <= 0 || max_pages <= 0) return LEWI_ERR_ARG;
+  if (D > 256 || pages > 0x7fffffff || (int64_t)max_pages * page > 0x7fffffff - 64) return LEWI_ERR_LIMIT;
+  if (D % 8 != 0 || !aligned(k, 16) || !aligned(v, 16) || page_stride % 8 != 0 || page_stride < (int64_t)page * Hkv * D) return LEWI_ERR_SHAPE;
+  return LEWI_OK;
+}
+
+template <int D>
+int launch_paged(cudaStream_t st, const paged::Args& a) {
+  static bool done[64] = {false};
+  using S = paged::Shape<D>;
+  if (!allow_smem(paged::attend_kernel<D>, S::kSmem, done)) return LEWI_ERR_CUDA;
+  if (launch_kernel(paged::attend_kernel<D>, a.ctas, paged::kThreads, S::kSmem, st, false, a) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return LEWI_ERR_CUDA;
+  }
+  ++launch_counter();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((a.Hq + paged::kWarps - 1) / paged::kWarps), (unsigned)a.c.B);
+  cfg.blockDim = dim3(paged::kThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, paged::join_kernel, a) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return LEWI_ERR_CUDA;
+  }
+  ++launch_counter();
+  return LEWI_OK;
+}
+
+inline int paged_ctas(int D) { return num_sms() * (D > 128 ? 1 : 2); }
+
+}  // namespace
+
+extern "C" {
+
+// ------------------------------------------------------------------------------------------------ single-token steps
+
+int lewi_causal_conv1d_step(void* stream, const void* x, int64_t x_stride, const void* w, void* state, const int32_t* slots, void* y, int B,
+                            int N, int C, int K) {
+  if (!x || !w || !y || B <= 0 || N <= 0 || C <= 0 || K <= 0 || (K > 1 && !state) || (!slots && N < B)) return LEWI_ERR_ARG;
+  if (K > 8 || B > 65535) return LEWI_ERR_LIMIT;
+  if (C % 8 != 0 || x_stride % 8 != 0 || x_stride < C || !aligned(x, 16) || !aligned(w, 16) || !aligned(state, 16) || !aligned(y, 16))
+    return LEWI_ERR_SHAPE;
+  const step::ConvArgs a{reinterpret_cast<const bf16*>(x), x_stride, reinterpret_cast<const bf16*>(w), reinterpret_cast<bf16*>(state), slots,
+                         reinterpret_cast<bf16*>(y), N, C};
+  const dim3 grid((unsigned)((C / 8 + step::kThreads - 1) / step::kThreads), (unsigned)B);
+  cudaStream_t st = as_stream(stream);
+  switch (K) {
+    case 1: step::conv_step_kernel<1><<<grid, step::kThreads, 0, st>>>(a); break;
+    case 2: step::conv_step_kernel<2><<<grid, step::kThreads, 0, st>>>(a); break;
+    case 3: step::conv_step_kernel<3><<<grid, step::kThreads, 0, st>>>(a); break;
+    case 4: step::conv_step_kernel<4><<<grid, step::kThreads, 0, st>>>(a); break;
+    case 5: step::conv_step_kernel<5><<<grid, step::kThreads, 0, st>>>(a); break;
+    case 6: step::conv_step_kernel<6><<<grid, step::kThreads, 0, st>>>(a); break;
+    case 7: step::conv_step_kernel<7><<<grid, step::kThreads, 0, st>>>(a); break;
+    default: step::conv_step_kernel<8><<<grid, step::kThreads, 0, st>>>(a); break;
+  }
+  LEWI_CHECK_LAUNCH();
+  return LEWI_OK;
+}
+
+int lewi_gdn_step(void* stream, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                  const void* g, int g_dtype, const void* beta, int beta_dtype, float* state, const int32_t* slots, void* o, int B, int N,
+                  int Hk, int H, int K, int V) {
+  if (!q || !k || !v || !g || !beta || !state || !o || B <= 0 || N <= 0 || Hk <= 0 || H <= 0 || K <= 0 || V <= 0) return LEWI_ERR_ARG;
+  if (!is_dtype(g_dtype) || !is_dtype(beta_dtype) || (!slots && N < B)) return LEWI_ERR_ARG;
+  if (K > step::kMaxK || H > 65535 || B > 65535) return LEWI_ERR_LIMIT;
+  if (K % 8 != 0 || V % 8 != 0 || H % Hk != 0 || !aligned(state, 16) || !aligned(o, 8)) return LEWI_ERR_SHAPE;
+  if (q_stride < (int64_t)Hk * K || k_stride < (int64_t)Hk * K || v_stride < (int64_t)H * V) return LEWI_ERR_SHAPE;
+  const step::GdnArgs a{reinterpret_cast<const bf16*>(q), reinterpret_cast<const bf16*>(k), reinterpret_cast<const bf16*>(v), q_stride, k_stride,
+                        v_stride, g, beta, g_dtype == LEWI_F32, beta_dtype == LEWI_F32, state, slots, reinterpret_cast<bf16*>(o), N, Hk, H, K, V,
+                        1.f / sqrtf((float)K)};
+  const dim3 grid((unsigned)((V + step::kCols - 1) / step::kCols), (unsigned)H, (unsigned)B);
+  step::gdn_step_kernel<<<grid, step::kThreads, 0, as_stream(stream)>>>(a);
+  LEWI_CHECK_LAUNCH();
+  return LEWI_OK;
+}
+
+// ------------------------------------------------------------------------------------------------ paged cache
+
+int lewi_paged_cache_write(void* stream, const void* k, int64_t k_stride, const void* v, int64_t v_stride, void* k_cache, void* v_cache,
+                           int64_t page_stride, const int32_t* tables, const int32_t* lengths, const int32_t* cu_seqlens, int T, int B,
+                           int Hkv, int D, int64_t pages, int page, int max_pages) {
+  if (!k || !v || T <= 0) return LEWI_ERR_ARG;
+  if (const int rc = check_cache(k_cache, v_cache, tables, lengths, B, Hkv, D, pages, page, max_pages, page_stride)) return rc;
+  if (!cu_seqlens && T != B) return LEWI_ERR_ARG;
+  const int64_t row = (int64_t)Hkv * D;
+  if (!aligned(k, 16) || !aligned(v, 16) || k_stride % 8 != 0 || v_stride % 8 != 0 || k_stride < row || v_stride < row) return LEWI_ERR_SHAPE;
+  const paged::WriteArgs a{{tables, lengths, reinterpret_cast<bf16*>(k_cache), reinterpret_cast<bf16*>(v_cache), page_stride, B, Hkv, D,
+                            (int)pages, page, max_pages},
+                           reinterpret_cast<const bf16*>(k), reinterpret_cast<const bf16*>(v), k_stride, v_stride, cu_seqlens, T};
+  constexpr int per = paged::kWriteThreads / 32;
+  paged::write_kernel<<<(unsigned)((T + per - 1) / per), paged::kWriteThreads, 0, as_stream(stream)>>>(a);
+  LEWI_CHECK_LAUNCH();
+  return LEWI_OK;
+}
+
+int64_t lewi_paged_attention_workspace_bytes(int D) {
+  if (D <= 0) return LEWI_ERR_ARG;
+  return (int64_t)2 * paged_ctas(D) * paged::kRows * (D + 2) * 4;
+}
+
+int lewi_paged_attention(void* stream, const void* q, int64_t q_stride, const void* k_cache, const void* v_cache, int64_t page_stride,
+                         const int32_t* tables, const int32_t* lengths, void* o, void* workspace, int64_t workspace_bytes, int B, int Hq,
+                         int Hkv, int D, int64_t pages, int page, int max_pages, float scale) {
+  if (!q || !o || Hq <= 0) return LEWI_ERR_ARG;
+  if (const int rc = check_cache(k_cache, v_cache, tables, lengths, B, Hkv, D, pages, page, max_pages, page_stride)) return rc;
+  if (B > 65535) return LEWI_ERR_LIMIT;
+  if (Hq % Hkv != 0 || !aligned(q, 4) || q_stride % 2 != 0 || q_stride < (int64_t)Hq * D || !aligned(o, 8)) return LEWI_ERR_SHAPE;
+  if (!workspace || !aligned(workspace, 16) || workspace_bytes < lewi_paged_attention_workspace_bytes(D)) return LEWI_ERR_WORKSPACE;
+  const int G = Hq / Hkv, MT = (G + paged::kRows - 1) / paged::kRows;
+  const paged::Args a{{tables, lengths, const_cast<bf16*>(reinterpret_cast<const bf16*>(k_cache)),
+                       const_cast<bf16*>(reinterpret_cast<const bf16*>(v_cache)), page_stride, B, Hkv, D, (int)pages, page, max_pages},
+                      reinterpret_cast<const bf16*>(q), q_stride, reinterpret_cast<bf16*>(o), reinterpret_cast<float*>(workspace), Hq, G, MT,
+                      paged_ctas(D), scale * 1.4426950408889634f};
+  cudaStream_t st = as_stream(stream);
+  if (D <= 64) return launch_paged<64>(st, a);
+  if (D <= 128) return launch_paged<128>(st, a);
+  return launch_paged<256>(st, a);
+}
+
+}  // extern "C"

@@ -1,0 +1,444 @@
+// A paged key-value cache: new tokens written to their cells, attention of one new token per sequence over what is there.
+//
+// k_cache, v_cache [pages][page][Hkv][D] bf16 (pages `page_stride` elements apart); a sequence's tokens lie in the pages of its row of
+// `tables` [B][max_pages], `lengths[b]` of them.  A length past the table is cut to it and a page that does not exist is left out
+// (LEWI_STATUS_BAD_INDEX either way); entries past a sequence's length are not read.
+#pragma once
+
+#include "common.cuh"
+#include "gdn_mma.cuh"
+#include "tcgen05.cuh"
+
+namespace lewi {
+namespace paged {
+
+struct Cache {
+  const int32_t *tables, *lengths;
+  __nv_bfloat16 *k, *v;
+  long long page_stride;
+  int B, Hkv, D, pages, page, max_pages;
+};
+
+// tokens of sequence b that the cache can hold
+__device__ __forceinline__ int length_of(const Cache& c, int b) {
+  return max(0, (int)min((long long)c.lengths[b], (long long)c.max_pages * c.page));
+}
+// Element at which cell `pos` of sequence b starts (head 0), -1 where its page does not exist.
+__device__ __forceinline__ long long cell_of(const Cache& c, int b, int pos) {
+  const unsigned p = (unsigned)pos / (unsigned)c.page;
+  const int id = c.tables[(long long)b * c.max_pages + p];
+  if (id < 0 || id >= c.pages) return -1;
+  return id * c.page_stride + (long long)(pos - (int)p * c.page) * c.Hkv * c.D;
+}
+
+// ---------------------------------------------------------------- write
+// Token i of sequence b (tokens cu[b] .. cu[b+1]; without cu one token per sequence) goes to cell lengths[b] - n_b + i.  A warp per
+// token: 16-byte pieces, every one requested before the first is stored.  Tokens of no sequence are left out; a token before
+// the cache's start or past its table raises LEWI_STATUS_BAD_INDEX and is left out.
+constexpr int kWriteThreads = 128;
+struct WriteArgs {
+  Cache c;
+  const __nv_bfloat16 *k, *v;   // [T][Hkv][D], tokens ks, vs elements apart
+  long long ks, vs;
+  const int32_t* cu;
+  int T;
+};
+
+__device__ __forceinline__ void write_row(const __nv_bfloat16* __restrict__ src, __nv_bfloat16* __restrict__ dst,
+                                          const __nv_bfloat16* __restrict__ src2, __nv_bfloat16* __restrict__ dst2, int vecs, int lane) {
+  constexpr int kAhead = 4;
+  for (int i0 = lane; i0 < vecs; i0 += 32 * kAhead) {
+    uint4 a[kAhead], b[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (i0 + 32 * j < vecs) {
+        a[j] = ld_nc_v4(src + (i0 + 32 * j) * 8);
+        b[j] = ld_nc_v4(src2 + (i0 + 32 * j) * 8);
+      }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (i0 + 32 * j < vecs) {
+        st_v4(dst + (i0 + 32 * j) * 8, a[j]);
+        st_v4(dst2 + (i0 + 32 * j) * 8, b[j]);
+      }
+  }
+}
+
+__global__ void __launch_bounds__(kWriteThreads) write_kernel(const WriteArgs a) {
+  const int t = (blockIdx.x * kWriteThreads + threadIdx.x) >> 5, lane = threadIdx.x & 31;
+  if (t >= a.T) return;
+  int b = t, back = 1;   // the token's sequence, and how far from its end it is
+  if (a.cu != nullptr) {
+    // the last b with cu[b] <= t, 32 bounds at a time; [lo, hi) holds it
+    int lo = 0, hi = a.c.B + 1;
+    while (hi - lo > 1) {
+      const int stride = (hi - lo + 31) / 32, at = lo + lane * stride;
+      const unsigned le = __ballot_sync(0xffffffffu, at < hi && a.cu[at] <= t);
+      if (le == 0u) break;   // before the first sequence (or bounds that fall)
+      const int last = 31 - __clz(le);
+      lo += last * stride;
+      hi = min(hi, lo + stride);
+    }
+    if (lo >= a.c.B) return;
+    const int first = a.cu[lo], end = a.cu[lo + 1];
+    if (first > t || end <= t) return;
+    b = lo;
+    back = end - t;
+  }
+  const int len = length_of(a.c, b);
+  const long long pos = (long long)a.c.lengths[b] - back;
+  const long long cell = pos >= 0 && pos < len ? cell_of(a.c, b, (int)pos) : -1;
+  if (cell < 0) {
+    if (lane == 0 && (a.cu != nullptr || a.c.lengths[b] > 0)) raise_status(LEWI_STATUS_BAD_INDEX);   // (length 0: an idle row)
+    return;
+  }
+  write_row(a.k + t * a.ks, a.c.k + cell, a.v + t * a.vs, a.c.v + cell, a.c.Hkv * a.c.D / 8, lane);
+}
+
+// ---------------------------------------------------------------- attention of one token
+// o[b,h] = sum_j p_j v_j, p = softmax(scale q.k_j) over the sequence's cells; one pass with a running maximum and sum (float32).
+//
+// Bound by the cache's way from HBM: 4 Hkv D bytes per cell.  The cells of all sequences and key heads are one long list of tiles of
+// 64 cells, of which every CTA takes an equal run, whatever the lengths (they are read on the device, so a captured launch follows
+// them).  The query heads that share a key head are the 16 rows of an `mma.sync` (m16n8k16), a warp's 16 cells its columns; a
+// warp has its own ring of tiles in shared memory (cp.async) and its own softmax, and nothing is synchronised before a head's
+// tiles end.  There the four warps' results are joined; a head that one CTA has whole is written out, of the others every CTA leaves
+// its part (at most two per CTA) and `join_kernel` adds them up in the order of the cells.
+// p is rounded to bf16 for its product with v (relative 2^-9, like the output's own rounding); its sum is taken before.
+constexpr int kWarps = 4, kThreads = kWarps * 32, kChunk = 16, kTile = kWarps * kChunk, kRows = 16, kJoinCols = 32;
+
+template <int D>
+struct Shape {
+  static constexpr int kStage = 2 * kChunk * D * 2;                    // a warp's K and V of 16 cells
+  static constexpr int kStages = D == 64 ? 6 : 3;
+  static constexpr int kCtas = D == 256 ? 1 : 2;                       // per SM
+  static constexpr int kRing = kWarps * kStages * kStage;
+  static constexpr int kSmem = kRing + kWarps * kRows * kJoinCols * 4 + 2 * kWarps * kRows * 4 + kWarps * kStages * 4 + 128;
+};
+
+struct Args {
+  Cache c;
+  const __nv_bfloat16* q;   // [B][Hq][D], rows of the batch qs elements apart
+  long long qs;
+  __nv_bfloat16* o;         // [B][Hq][D]
+  float* part;              // [2 per CTA][16][D] sums, then [2 per CTA][16] maxima, then as many sums of p
+  int Hq, G, MT, ctas;      // query heads per key head, groups of 16 of them, CTAs of the list
+  float scale_log2;
+};
+
+// Where the list stands: tile t of `nt` of row group r of sequence b.
+struct Cursor {
+  int b, r, t, nt;
+};
+
+__device__ __forceinline__ int tiles_of(const Cache& c, int b) { return (length_of(c, b) + kTile - 1) / kTile; }
+
+__device__ __forceinline__ void next_tile(Cursor& u, const Cache& c, int R) {
+  if (++u.t < u.nt) return;
+  u.t = 0;
+  if (++u.r < R) return;
+  u.r = 0;
+  do {
+    if (++u.b >= c.B) return;
+    u.nt = tiles_of(c, u.b);
+  } while (u.nt == 0);
+}
+
+// Tiles of all sequences and of those before `upto` (both times R: places in the list); all threads of the CTA call it.
+__device__ __forceinline__ longlong2 count_tiles(const Cache& c, int upto, long long (&s)[2][kWarps]) {
+  long long all = 0, before = 0;
+  for (int b = threadIdx.x; b < c.B; b += kThreads) {
+    const int n = tiles_of(c, b);
+    all += n;
+    if (b < upto) before += n;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    all += __shfl_xor_sync(0xffffffffu, all, o);
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+  }
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) {
+    s[0][threadIdx.x >> 5] = all;
+    s[1][threadIdx.x >> 5] = before;
+  }
+  __syncthreads();
+  return make_longlong2(s[0][0] + s[0][1] + s[0][2] + s[0][3], s[1][0] + s[1][1] + s[1][2] + s[1][3]);
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, Shape<D>::kCtas) attend_kernel(const Args a) {
+  using S = Shape<D>;
+  constexpr int ST = S::kStages, KS = D / 16, VR = D / 8;   // 16-wide steps over D, 16-byte vectors of a row
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ long long s_count[2][kWarps];
+  __shared__ Cursor s_start;
+  grid_launch();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, R = a.c.Hkv * a.MT;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~(uintptr_t)127);
+  float* s_o = reinterpret_cast<float*>(smem + S::kRing);                       // [warp][16][32]
+  float* s_m = s_o + kWarps * kRows * kJoinCols;                                // [warp][16]
+  float* s_l = s_m + kWarps * kRows;
+  uint32_t* s_mask = reinterpret_cast<uint32_t*>(s_l + kWarps * kRows) + warp * ST;   // cells of a stage that count
+  const uint32_t ring = ptx::smem_u32(smem) + warp * ST * S::kStage;
+  const gdn::LaneOff L = gdn::lane_off(lane);
+
+  // this CTA's run of the list, and where it starts
+  const long long total = count_tiles(a.c, 0, s_count).x * R;
+  const long long n_ctas = min(total, (long long)a.ctas);   // (so that no run is empty)
+  if (blockIdx.x >= n_ctas) return;
+  const long long w0 = blockIdx.x * total / n_ctas, w1 = (blockIdx.x + 1) * total / n_ctas;
+  if (warp == 0) {   // 32 sequences at a time
+    long long at = 0;
+    for (int b0 = 0; b0 < a.c.B; b0 += 32) {
+      const int n = b0 + lane < a.c.B ? tiles_of(a.c, b0 + lane) : 0;
+      long long upto = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, (at + upto) * R > w0);
+      if (past != 0u) {
+        if (lane == __ffs(past) - 1) {
+          const long long in = w0 - (at + upto - n) * R;   // place in the sequence's own tiles
+          s_start = Cursor{b0 + lane, (int)(in / n), (int)(in % n), n};
+        }
+        break;
+      }
+      at += __shfl_sync(0xffffffffu, upto, 31);
+    }
+  }
+  __syncthreads();
+  Cursor use = s_start, get = use;
+
+  // The cells of the tile that is requested next: a lane (of the first 16) has one cell, whose page is looked up one request ahead.
+  long long cell = -1;
+  bool bad = false;
+  auto look = [&] {
+    cell = -1;
+    const int pos = get.t * kTile + warp * kChunk + lane;
+    if (lane < kChunk && pos < length_of(a.c, get.b)) {
+      cell = cell_of(a.c, get.b, pos);
+      bad |= cell < 0;
+    }
+  };
+  const int vecs = a.c.D / 8;
+  long long got = w0;
+  look();
+  auto request = [&](int stage) {
+    if (got < w1) {
+      const uint32_t mask = __ballot_sync(0xffffffffu, cell >= 0);
+      if (lane == 0) s_mask[stage] = mask;
+      const uint32_t at = ring + stage * S::kStage;
+      const int head = get.r / a.MT * a.c.D;
+#pragma unroll
+      for (int i = 0; i < VR / 2; ++i) {
+        const int row = (i * 32 + lane) / VR, vec = (i * 32 + lane) % VR;
+        const long long from = __shfl_sync(0xffffffffu, cell, row);
+        const bool in = from >= 0 && vec < vecs;
+        const long long e = in ? from + head + vec * 8 : 0;
+        const uint32_t dst = gdn::swz(at + (vec >> 3) * (kChunk * 128), row, vec & 7);
+        ptx::cp_async16(dst, a.c.k + e, in ? 16u : 0u);
+        ptx::cp_async16(dst + kChunk * D * 2, a.c.v + e, in ? 16u : 0u);
+      }
+      ++got;
+      if (got < w1) {
+        next_tile(get, a.c, R);
+        look();
+      }
+    }
+    ptx::cp_async_commit();   // (always a group, so that the groups count the tiles)
+  };
+#pragma unroll
+  for (int s = 0; s < ST - 1; ++s) request(s);
+
+  uint32_t qf[KS][4];
+  float o[D / 8][4], m[2], l[2];
+  int stage = 0, part = 2 * blockIdx.x;   // where a part is left: the first head's, then the last one's
+  for (long long w = w0; w < w1; ++w) {
+    if (w == w0 || use.t == 0) {   // a head starts: its queries, nothing seen yet
+      const __nv_bfloat16* q = a.q + use.b * a.qs + ((long long)(use.r / a.MT) * a.G + use.r % a.MT * kRows) * a.c.D;
+      const int rows = min(kRows, a.G - use.r % a.MT * kRows), r = lane >> 2, c = (lane & 3) * 2;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int row = r + (e & 1) * 8, col = ks * 16 + c + (e >> 1) * 8;
+          qf[ks][e] = row < rows && col < a.c.D ? *reinterpret_cast<const uint32_t*>(q + (long long)row * a.c.D + col) : 0u;
+        }
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) gdn::zero4(o[i]);
+      m[0] = m[1] = -INFINITY;
+      l[0] = l[1] = 0.f;
+    }
+    request(stage == 0 ? ST - 1 : stage - 1);   // into the stage that was worked through last
+    ptx::cp_async_wait<ST - 1>();
+    __syncwarp();
+    const uint32_t kt = ring + stage * S::kStage, vt = kt + kChunk * D * 2, mask = s_mask[stage];
+    float s[2][4] = {};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) gdn::mma2(s[0], s[1], qf[ks], gdn::ld_b(kt, 0, ks, L, kChunk * 128));
+    float top[2] = {m[0], m[1]};
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool seen = mask >> (j * 8 + (lane & 3) * 2 + (e & 1)) & 1u;
+        s[j][e] = seen ? s[j][e] * a.scale_log2 : -INFINITY;
+        top[e >> 1] = fmaxf(top[e >> 1], s[j][e]);
+      }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+      top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+    }
+    if (__any_sync(0xffffffffu, top[0] != m[0] || top[1] != m[1])) {   // the sums so far, to the new maximum
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float f = m[r] == top[r] ? 1.f : exp2f(m[r] - top[r]);   // (a first maximum: 0; both -inf: 1, of nothing)
+        l[r] *= f;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          o[i][2 * r] *= f;
+          o[i][2 * r + 1] *= f;
+        }
+        m[r] = top[r];
+      }
+    }
+    uint32_t p[4];
+    {
+      const float z0 = m[0] == -INFINITY ? 0.f : m[0], z1 = m[1] == -INFINITY ? 0.f : m[1];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float p0 = exp2f(s[j][0] - z0), p1 = exp2f(s[j][1] - z0), p2 = exp2f(s[j][2] - z1), p3 = exp2f(s[j][3] - z1);
+        l[0] += p0 + p1;
+        l[1] += p2 + p3;
+        p[2 * j] = pack_bf16(p0, p1);
+        p[2 * j + 1] = pack_bf16(p2, p3);
+      }
+    }
+#pragma unroll
+    for (int np = 0; np < D / 16; ++np) gdn::mma2(o[2 * np], o[2 * np + 1], p, gdn::ld_b_t(vt, 0, np, L, kChunk * 128));
+    __syncwarp();   // (the stage may be written again)
+    stage = stage + 1 == ST ? 0 : stage + 1;
+
+    if (use.t + 1 == use.nt || w + 1 == w1) {   // the head ends here, or this CTA's share of it
+      const int rows = min(kRows, a.G - use.r % a.MT * kRows), r0 = lane >> 2;
+      const bool from_start = w - w0 >= use.t, whole = from_start && use.t + 1 == use.nt;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+        if ((lane & 3) == 0) {
+          s_m[warp * kRows + r0 + r * 8] = m[r];
+          s_l[warp * kRows + r0 + r * 8] = l[r];
+        }
+      }
+      __syncthreads();
+      float f[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float mm = -INFINITY;
+#pragma unroll
+        for (int x = 0; x < kWarps; ++x) mm = fmaxf(mm, s_m[x * kRows + r0 + r * 8]);
+        f[r] = m[r] == -INFINITY ? 0.f : m[r] == mm ? 1.f : exp2f(m[r] - mm);
+      }
+      const int row = threadIdx.x >> 3, c4 = (threadIdx.x & 7) * 4;   // what this thread joins: 4 columns of a row
+      float mm = -INFINITY, ll = 0.f;
+#pragma unroll
+      for (int x = 0; x < kWarps; ++x) mm = fmaxf(mm, s_m[x * kRows + row]);
+#pragma unroll
+      for (int x = 0; x < kWarps; ++x) {
+        const float mx = s_m[x * kRows + row];
+        ll += mx == -INFINITY ? s_l[x * kRows + row] * 0.f : s_l[x * kRows + row] * (mx == mm ? 1.f : exp2f(mx - mm));
+      }
+      const float inv = ll == 0.f ? 0.f : 1.f / ll;
+#pragma unroll
+      for (int c0 = 0; c0 < D; c0 += kJoinCols) {
+#pragma unroll
+        for (int i = 0; i < kJoinCols / 8; ++i)
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+            *reinterpret_cast<float2*>(s_o + (warp * kRows + r0 + r * 8) * kJoinCols + i * 8 + (lane & 3) * 2) =
+                make_float2(o[c0 / 8 + i][2 * r] * f[r], o[c0 / 8 + i][2 * r + 1] * f[r]);
+        __syncthreads();
+        if (row < rows && c0 + c4 < a.c.D) {
+          float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int x = 0; x < kWarps; ++x) {
+            const float4 v = *reinterpret_cast<const float4*>(s_o + (x * kRows + row) * kJoinCols + c4);
+            sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+          }
+          if (whole) {
+            const long long at = ((long long)use.b * a.Hq + (use.r / a.MT) * a.G + use.r % a.MT * kRows + row) * a.c.D + c0 + c4;
+            *reinterpret_cast<uint2*>(a.o + at) = make_uint2(pack_bf16(sum.x * inv, sum.y * inv), pack_bf16(sum.z * inv, sum.w * inv));
+          } else {
+            *reinterpret_cast<float4*>(a.part + ((long long)part * kRows + row) * a.c.D + c0 + c4) = sum;
+          }
+        }
+        __syncthreads();
+      }
+      if (!whole && (threadIdx.x & 7) == 0) {
+        float* stats = a.part + (long long)2 * a.ctas * kRows * a.c.D + part * kRows + row;
+        stats[0] = mm;
+        stats[2 * a.ctas * kRows] = ll;
+      }
+      __syncthreads();   // (s_m and s_l may be written again)
+      part = 2 * blockIdx.x + 1;
+    }
+    if (w + 1 < w1) next_tile(use, a.c, R);
+  }
+  ptx::cp_async_wait_all();
+  if (bad) raise_status(LEWI_STATUS_BAD_INDEX);
+}
+
+// Adds up the parts of the heads that several CTAs worked on, in the order of the cells, and writes zeros for sequences without
+// cells.  A warp per query head.
+__global__ void __launch_bounds__(kThreads) join_kernel(const Args a) {
+  __shared__ long long s_count[2][kWarps];
+  const int b = blockIdx.y, lane = threadIdx.x & 31, R = a.c.Hkv * a.MT;
+  const int head = blockIdx.x * kWarps + (threadIdx.x >> 5);
+  const longlong2 count = count_tiles(a.c, b, s_count);
+  const int nt = tiles_of(a.c, b);
+  grid_wait();   // (every CTA, so that what follows this kernel follows the one before it, too)
+  if (threadIdx.x == 0 && blockIdx.x == 0 && a.c.lengths[b] > (long long)a.c.max_pages * a.c.page) raise_status(LEWI_STATUS_BAD_INDEX);
+  if (head >= a.Hq) return;
+  __nv_bfloat16* o = a.o + ((long long)b * a.Hq + head) * a.c.D;
+  if (nt == 0) {
+    for (int c = lane * 4; c < a.c.D; c += 128) *reinterpret_cast<uint2*>(o + c) = make_uint2(0u, 0u);
+    return;
+  }
+  const int g = head % a.G, row = g % kRows;
+  const long long total = count.x * R, w0 = count.y * R + (long long)((head / a.G) * a.MT + g / kRows) * nt, w1 = w0 + nt;
+  const long long n_ctas = min(total, (long long)a.ctas);
+  auto cta_of = [&](long long w) { return (int)(((w + 1) * n_ctas - 1) / total); };
+  const int c0 = cta_of(w0), c1 = cta_of(w1 - 1);
+  if (c0 == c1) return;   // written already
+  const int slot0 = 2 * c0 + (w0 == c0 * total / n_ctas ? 0 : 1);   // (every other CTA's run starts inside the head)
+  const float* stats = a.part + (long long)2 * a.ctas * kRows * a.c.D + row;
+  auto slot_of = [&](int c) { return c == c0 ? slot0 : 2 * c; };
+  float mm = -INFINITY, ll = 0.f;
+  for (int c = c0 + lane; c <= c1; c += 32) mm = fmaxf(mm, stats[slot_of(c) * kRows]);
+  mm = warp_max(mm);
+  for (int c = c0 + lane; c <= c1; c += 32) {
+    const float mx = stats[slot_of(c) * kRows], lx = stats[(2 * a.ctas + slot_of(c)) * kRows];
+    ll += mx == -INFINITY ? lx * 0.f : lx * (mx == mm ? 1.f : exp2f(mx - mm));
+  }
+  ll = warp_sum(ll);
+  const float inv = ll == 0.f ? 0.f : 1.f / ll;
+  for (int col = lane * 4; col < a.c.D; col += 128) {
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int c = c0; c <= c1; ++c) {
+      const float mx = stats[slot_of(c) * kRows];
+      const float f = mx == -INFINITY ? 0.f : mx == mm ? 1.f : exp2f(mx - mm);
+      const float4 v = *reinterpret_cast<const float4*>(a.part + ((long long)slot_of(c) * kRows + row) * a.c.D + col);
+      sum.x = fmaf(f, v.x, sum.x); sum.y = fmaf(f, v.y, sum.y); sum.z = fmaf(f, v.z, sum.z); sum.w = fmaf(f, v.w, sum.w);
+    }
+    *reinterpret_cast<uint2*>(o + col) = make_uint2(pack_bf16(sum.x * inv, sum.y * inv), pack_bf16(sum.z * inv, sum.w * inv));
+  }
+}
+
+}  // namespace paged
+}  // namespace lewi

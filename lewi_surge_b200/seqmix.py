@@ -110,3 +110,66 @@ def chunk_gated_delta_rule(query, key, value, g, beta, chunk_size=64, initial_st
     raise LewiError("chunk_gated_delta_rule takes bfloat16 q, k, v")
   o, hf = _ChunkGatedDeltaRule.apply(query, key, value, g, beta, initial_state)
   return o, (hf.to(torch.bfloat16) if initial_state is not None else None)
+
+
+def _check_slots(what, b, state, slots):
+  if slots is None and state.shape[0] < b:
+    raise LewiError(f"{what}: {b} rows and no slots, but {state.shape[0]} states")
+  if slots is not None and slots.shape != (b,):
+    raise LewiError(f"{what}: slots [B] are required")
+
+
+def causal_conv1d_step(x, w, state, slots=None):
+  """One more input of the sequences of `causal_conv1d`: x [B,C] bf16, w [K,1,C], state [N,K-1,C] bf16 holds the K-1 inputs before this
+  one, oldest first (zeros at the start of a sequence) and is moved on in place.  Row b has the state slots[b] (int32 or int64; none:
+  state b).  A negative slot is an idle row: zeros out, no state touched; a slot past the pool, or an earlier row's, as well, with
+  `LEWI_STATUS_BAD_INDEX` in `_lib.last_status()`.  Not differentiable; the values are `causal_conv1d`'s bit for bit."""
+  lib = _lib.load()
+  if x.dim() != 2 or w.dim() != 3 or w.shape[1] != 1 or w.shape[2] != x.shape[1]:
+    raise LewiError("causal_conv1d_step: x [B,C] and a depthwise kernel w [K,1,C] are required")
+  if x.dtype != torch.bfloat16 or state.dtype != torch.bfloat16:
+    raise LewiError("causal_conv1d_step takes bfloat16 activations and state")
+  (b, c), k = x.shape, w.shape[0]
+  if state.dim() != 3 or state.shape[1:] != (k - 1, c):
+    raise LewiError("causal_conv1d_step: state [N,K-1,C] is required")
+  _check_slots("causal_conv1d_step", b, state, slots)
+  with torch.no_grad(), _lib.one_device(x, w, state, slots):
+    x, x_rows = _lib.rows_of(x, 16)
+    w = w.to(torch.bfloat16).contiguous()
+    slots = _lib.index_table(slots, "slots")
+    y = torch.empty((b, c), dtype=torch.bfloat16, device=x.device)
+    if b > 0:
+      check(lib.lewi_causal_conv1d_step(stream(), x.data_ptr(), x_rows, ptr(w), ptr(state), ptr(slots), ptr(y), b, state.shape[0], c, k),
+            "lewi_causal_conv1d_step")
+  return y
+
+
+def gated_delta_step(query, key, value, g, beta, state, slots=None):
+  """One more token of the sequences of `chunk_gated_delta_rule`, with the same arguments without their S: query, key [B,Hk,K],
+  value [B,H,V] bf16, g (log decay), beta [B,H] (float32 or bf16) and the state [N,H,K,V] float32, which is moved on in place; returns
+  o [B,H,V] bf16.  H is a multiple of Hk: value head h has the query and key of head h // (H // Hk).  Row b has the state slots[b]
+  (int32 or int64; none: state b); idle and refused rows are those of `causal_conv1d_step`.  K up to 128, K and V multiples of 8.
+  Rows of the batch may lie apart (views of one projection need no copy).  Not differentiable.  Everything is float32 inside, where
+  `chunk_gated_delta_rule` rounds some products to bf16 as the reference does, so the two agree to bf16's precision."""
+  lib = _lib.load()
+  if any(t.dtype != torch.bfloat16 for t in (query, key, value)) or state.dtype != torch.float32:
+    raise LewiError("gated_delta_step takes bfloat16 q, k, v and a float32 state")
+  if query.dim() != 3 or key.shape != query.shape or value.dim() != 3 or value.shape[0] != query.shape[0]:
+    raise LewiError("gated_delta_step: query, key [B,Hk,K] and value [B,H,V] are required")
+  (b, hk, kd), (_, h, vd) = query.shape, value.shape
+  if state.dim() != 4 or state.shape[1:] != (h, kd, vd):
+    raise LewiError("gated_delta_step: state [N,H,K,V] is required")
+  if g.shape != (b, h) or beta.shape != (b, h):
+    raise LewiError("gated_delta_step: g and beta [B,H] are required")
+  _check_slots("gated_delta_step", b, state, slots)
+  dt = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
+  if g.dtype not in dt or beta.dtype not in dt:
+    raise LewiError("gated_delta_step takes float32 or bfloat16 g and beta")
+  with torch.no_grad(), _lib.one_device(query, key, value, g, beta, state, slots):
+    (q, qs), (k, ks), (v, vs) = (_lib.rows_of(t, 2) for t in (query, key, value))
+    g, beta, slots = g.contiguous(), beta.contiguous(), _lib.index_table(slots, "slots")
+    o = torch.empty((b, h, vd), dtype=torch.bfloat16, device=q.device)
+    if b > 0:
+      check(lib.lewi_gdn_step(stream(), q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, ptr(g), dt[g.dtype], ptr(beta), dt[beta.dtype],
+                              ptr(state), ptr(slots), ptr(o), b, state.shape[0], hk, h, kd, vd), "lewi_gdn_step")
+  return o
