@@ -385,6 +385,26 @@ int lewi_paged_attention(void* stream, const void* q, int64_t q_stride, const vo
                          int Hq, int Hkv, int D, int64_t pages, int page, int max_pages, float scale);
 
 /* ------------------------------------------------------------------------------------------------
+ * Causal attention over packed sequences, forward and backward: o[t,h] = softmax_j(scale q[t,h].k[j]) v[j] over the rows j <= t of t's own
+ * sequence, with the key head h / (Hq / Hkv).  q, o bf16 [T][Hq][D], k, v bf16 [T][Hkv][D]; sequence s has the rows
+ * cu_seqlens[s] .. cu_seqlens[s+1] (i32 [n_seqs + 1], ascending; null: n_seqs sequences of T / n_seqs rows).  Rows of no sequence get zeros, in o
+ * and in the gradients, whatever they hold.  Bounds that fall or leave the rows raise LEWI_STATUS_BAD_INDEX; what they cut is
+ * undefined.  lse f32 [Hq][T] is for the backward pass (log2 of the softmax's denominator; rows of no sequence are left as they are).
+ * D <= 128, a multiple of 8; scale > 0; all tensors 16-byte aligned, `*_stride` (elements from row to row; heads are contiguous) multiples
+ * of 8.  Scores, softmax and sums float32; p and the gradient of the scores are rounded to bf16 for their products.
+ * The backward call makes dq and/or dk and dv (bf16, contiguous; dk and dv together) out of d_o (bf16 [T][Hq][D], contiguous).  No
+ * atomics: equal calls have equal bits.
+ * ---------------------------------------------------------------------------------------------- */
+int lewi_causal_attention_fwd(void* stream, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                              int64_t v_stride, const int32_t* cu_seqlens, int n_seqs, void* o, float* lse, int T, int Hq, int Hkv, int D,
+                              float scale);
+int64_t lewi_causal_attention_bwd_workspace_bytes(int T, int Hq);
+int lewi_causal_attention_bwd(void* stream, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                              int64_t v_stride, const void* o, const float* lse, const void* d_o, const int32_t* cu_seqlens, int n_seqs,
+                              void* dq, void* dk, void* dv, void* workspace, int64_t workspace_bytes, int T, int Hq, int Hkv, int D,
+                              float scale);
+
+/* ------------------------------------------------------------------------------------------------
  * The whole layer in two calls.  lewi_moe_fwd / lewi_moe_bwd queue the complete launch sequence of the MoE layer of
  * the MaxText `qwen3_5` block as the reference patches it: router (softmax -> top-k -> renormalise,
  * configs/stage1.yml:33-41) -> `_route_activations` (modal/moe_permute.py:399-404) -> the three `ragged_dot`s of the

@@ -1,5 +1,5 @@
-"""Softmax attention of the decoder block's full-attention layers, beside the mixers of `seqmix`: the paged key-value cache
-(`paged_cache_write`, `paged_attention`) for decoding.
+"""Softmax attention of the decoder block's full-attention layers, beside the mixers of `seqmix`: `causal_attention` over whole
+sequences for training and prompts, the paged key-value cache (`paged_cache_write`, `paged_attention`) for decoding.
 
 Everything is bfloat16 with float32 scores, softmax and sums; no fallback path."""
 from __future__ import annotations
@@ -74,3 +74,70 @@ def paged_attention(query, key_cache, value_cache, block_tables, lengths, scale=
                                    ptr(o), ptr(ws), ws_bytes, b, hq, heads, d, key_cache.shape[0], page, tables.shape[1],
                                    d ** -0.5 if scale is None else float(scale)), "lewi_paged_attention")
   return o
+
+
+class _CausalAttention(torch.autograd.Function):
+
+  @staticmethod
+  def forward(ctx, q, k, v, cu, n_seqs, scale):
+    lib = _lib.load()
+    with _lib.one_device(q, k, v, cu):
+      (q, qs), (k, ks), (v, vs) = (_lib.rows_of(t, 16) for t in (q, k, v))
+      cu = _lib.index_table(cu, "cu_seqlens")
+      t, hq, d = q.shape
+      o = torch.empty((t, hq, d), dtype=torch.bfloat16, device=q.device)
+      lse = torch.empty((hq, t), dtype=torch.float32, device=q.device)
+      check(lib.lewi_causal_attention_fwd(stream(), q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, ptr(cu), n_seqs, ptr(o), ptr(lse),
+                                          t, hq, k.shape[1], d, scale), "lewi_causal_attention_fwd")
+    ctx.save_for_backward(q, k, v, o, lse, cu)
+    ctx.call = n_seqs, scale
+    return o
+
+  @staticmethod
+  def backward(ctx, g):
+    lib = _lib.load()
+    q, k, v, o, lse, cu = ctx.saved_tensors
+    n_seqs, scale = ctx.call
+    t, hq, d = q.shape
+    with _lib.one_device(q, g):
+      (q, qs), (k, ks), (v, vs) = (_lib.rows_of(x, 16) for x in (q, k, v))
+      g, _ = _lib.rows_of(g.contiguous(), 16)
+      dq = torch.empty((t, hq, d), dtype=torch.bfloat16, device=q.device) if ctx.needs_input_grad[0] else None
+      dk, dv = (torch.empty(k.shape, dtype=torch.bfloat16, device=q.device) if any(ctx.needs_input_grad[1:3]) else None for _ in range(2))
+      ws_bytes = int(lib.lewi_causal_attention_bwd_workspace_bytes(t, hq))
+      ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+      check(lib.lewi_causal_attention_bwd(stream(), q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, ptr(o), ptr(lse), ptr(g), ptr(cu), n_seqs,
+                                          ptr(dq), ptr(dk), ptr(dv), ptr(ws), ws_bytes, t, hq, k.shape[1], d, scale),
+            "lewi_causal_attention_bwd")
+    return dq, dk, dv, None, None, None
+
+
+def causal_attention(query, key, value, cu_seqlens=None, scale=None):
+  """softmax(scale q k^T) v over the rows of a sequence up to the query's own.  Packed: query [T, Hq, D], key, value [T, Hkv, D] bf16, sequence s
+  the rows cu_seqlens[s] .. cu_seqlens[s+1] (int32 or int64 [N + 1], ascending, empty ones among them; none: one sequence), or sequences of one
+  length: query [B, S, Hq, D], key, value [B, S, Hkv, D].  Head h has the keys of head h // (Hq // Hkv); D up to 128, a multiple of 8;
+  `scale` > 0 defaults to D ** -0.5.  Returns bf16 of the query's shape; differentiable through `torch.autograd` in query, key and value.
+  Rows of no sequence give zeros and get zero gradients, whatever they hold.  Bounds that fall or leave the rows:
+  `LEWI_STATUS_BAD_INDEX` in `_lib.last_status()`.  Rows may lie apart (views of one projection need no copy).
+
+  A value of v that is not finite reaches back to the start of its 128 rows of the sequence (as those of q, k and the upstream gradient do in the
+  gradients), never into another sequence."""
+  if any(x.dtype != torch.bfloat16 for x in (query, key, value)):
+    raise LewiError("causal_attention takes bfloat16 q, k, v")
+  if query.dim() not in (3, 4) or key.dim() != query.dim() or value.shape != key.shape or query.shape[:-2] != key.shape[:-2] or \
+      query.shape[-1] != key.shape[-1] or key.shape[-2] == 0 or query.shape[-2] % key.shape[-2]:
+    raise LewiError("causal_attention: query [T, Hq, D] and key, value [T, Hkv, D], or all three [B, S, ..], Hq a multiple of Hkv, are required")
+  if cu_seqlens is not None and (query.dim() == 4 or cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 2):
+    raise LewiError("causal_attention: cu_seqlens [N + 1] belongs to packed rows [T, H, D]")
+  scale = query.shape[-1] ** -0.5 if scale is None else float(scale)
+  if not scale > 0:
+    raise LewiError("causal_attention: scale must be positive")
+  shape = query.shape
+  n_seqs = 1 if query.dim() == 3 else shape[0]
+  if query.dim() == 4:
+    query, key, value = (x.reshape(-1, *x.shape[2:]) for x in (query, key, value))
+  if cu_seqlens is not None:
+    n_seqs = cu_seqlens.shape[0] - 1
+  if query.numel() == 0:
+    return query.clone()
+  return _CausalAttention.apply(query, key, value, cu_seqlens, n_seqs, scale).view(shape)

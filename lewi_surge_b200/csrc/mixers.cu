@@ -1,5 +1,6 @@
 // C ABI of what mixes along the sequence, apart from the whole-sequence kernels of lewi_moe.cu: single-token steps of the convolution
 // and the gated delta rule, the paged cache, attention (declarations and contracts: include/lewi_moe.h).
+#include "attention.cuh"
 #include "common.cuh"
 #include "paged.cuh"
 #include "step.cuh"
@@ -50,6 +51,52 @@ int launch_paged(cudaStream_t st, const paged::Args& a) {
     return LEWI_ERR_CUDA;
   }
   ++launch_counter();
+  return LEWI_OK;
+}
+
+// Checks of what forward and backward of causal attention share.
+int check_attention(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride, const int32_t* cu, int n_seqs,
+                    const void* o, const float* lse, int T, int Hq, int Hkv, int D, float scale) {
+  if (!q || !k || !v || !o || !lse || T <= 0 || n_seqs <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || !(scale > 0.f)) return LEWI_ERR_ARG;
+  if (!cu && T % n_seqs != 0) return LEWI_ERR_ARG;
+  if (D > attn::kMaxD || T > 0x7fffffff - attn::kTile) return LEWI_ERR_LIMIT;
+  if ((attn::most_tiles(T, n_seqs) + n_seqs) * Hq > 0x7fffffff) return LEWI_ERR_LIMIT;
+  if (D % 8 != 0 || Hq % Hkv != 0 || !aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(o, 16)) return LEWI_ERR_SHAPE;
+  if (q_stride % 8 != 0 || k_stride % 8 != 0 || v_stride % 8 != 0) return LEWI_ERR_SHAPE;
+  if (q_stride < (int64_t)Hq * D || k_stride < (int64_t)Hkv * D || v_stride < (int64_t)Hkv * D) return LEWI_ERR_SHAPE;
+  return LEWI_OK;
+}
+
+template <int DP>
+int attention_fwd(cudaStream_t st, const attn::Args& a, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv) {
+  static bool done[64] = {false};
+  if (!allow_smem(attn::fwd_kernel<DP>, attn::FwdShape<DP>::kSmem, done)) return LEWI_ERR_CUDA;
+  // pairs of units of all sequences: half their tiles times heads, and one to round up for each
+  const long long pairs = (attn::most_tiles(a.seqs.T, a.seqs.n) * a.G + a.seqs.n + 1) / 2;
+  attn::fwd_kernel<DP><<<(unsigned)(pairs * a.Hkv), attn::kFwdThreads, attn::FwdShape<DP>::kSmem, st>>>(tq, tk, tv, a);
+  LEWI_CHECK_LAUNCH();
+  return LEWI_OK;
+}
+
+template <int DP>
+int attention_bwd(cudaStream_t st, const attn::Args& a, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& td,
+                  const bf16* d_o) {
+  const long long rows = (long long)a.seqs.T * a.Hq, per = attn::kDeltaThreads / (DP / 8);
+  attn::delta_kernel<DP><<<(unsigned)((rows + per - 1) / per), attn::kDeltaThreads, 0, st>>>(a.o, d_o, a.delta, a.seqs.T, a.Hq, a.D);
+  LEWI_CHECK_LAUNCH();
+  const long long tiles = attn::most_tiles(a.seqs.T, a.seqs.n);
+  if (a.dk != nullptr) {
+    static bool done[64] = {false};
+    if (!allow_smem(attn::dkv_kernel<DP>, attn::DkvShape<DP>::kSmem, done)) return LEWI_ERR_CUDA;
+    attn::dkv_kernel<DP><<<(unsigned)(tiles * a.Hkv), attn::kBwdThreads, attn::DkvShape<DP>::kSmem, st>>>(tq, tk, tv, td, a);
+    LEWI_CHECK_LAUNCH();
+  }
+  if (a.dq != nullptr) {
+    static bool done[64] = {false};
+    if (!allow_smem(attn::dq_kernel<DP>, attn::DqShape<DP>::kSmem, done)) return LEWI_ERR_CUDA;
+    attn::dq_kernel<DP><<<(unsigned)(tiles * a.Hq), attn::kDqThreads, attn::DqShape<DP>::kSmem, st>>>(tq, tk, tv, td, a);
+    LEWI_CHECK_LAUNCH();
+  }
   return LEWI_OK;
 }
 
@@ -143,6 +190,43 @@ int lewi_paged_attention(void* stream, const void* q, int64_t q_stride, const vo
   if (D <= 64) return launch_paged<64>(st, a);
   if (D <= 128) return launch_paged<128>(st, a);
   return launch_paged<256>(st, a);
+}
+
+// ------------------------------------------------------------------------------------------------ causal attention
+
+int lewi_causal_attention_fwd(void* stream, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                              const int32_t* cu_seqlens, int n_seqs, void* o, float* lse, int T, int Hq, int Hkv, int D, float scale) {
+  if (const int rc = check_attention(q, q_stride, k, k_stride, v, v_stride, cu_seqlens, n_seqs, o, lse, T, Hq, Hkv, D, scale)) return rc;
+  CUtensorMap tq, tk, tv;
+  if (!attn::make_rows_map(&tq, q, T, Hq, D, q_stride) || !attn::make_rows_map(&tk, k, T, Hkv, D, k_stride) ||
+      !attn::make_rows_map(&tv, v, T, Hkv, D, v_stride))
+    return LEWI_ERR_CUDA;
+  const attn::Args a{{cu_seqlens, n_seqs, T}, Hq, Hkv, Hq / Hkv, D, scale, scale * 1.4426950408889634f, reinterpret_cast<bf16*>(o), lse,
+                     nullptr, nullptr, nullptr, nullptr};
+  return D <= 64 ? attention_fwd<64>(as_stream(stream), a, tq, tk, tv) : attention_fwd<128>(as_stream(stream), a, tq, tk, tv);
+}
+
+int64_t lewi_causal_attention_bwd_workspace_bytes(int T, int Hq) {
+  if (T <= 0 || Hq <= 0) return LEWI_ERR_ARG;
+  return (int64_t)T * Hq * 4;
+}
+
+int lewi_causal_attention_bwd(void* stream, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                              const void* o, const float* lse, const void* d_o, const int32_t* cu_seqlens, int n_seqs, void* dq, void* dk,
+                              void* dv, void* workspace, int64_t workspace_bytes, int T, int Hq, int Hkv, int D, float scale) {
+  if (const int rc = check_attention(q, q_stride, k, k_stride, v, v_stride, cu_seqlens, n_seqs, o, lse, T, Hq, Hkv, D, scale)) return rc;
+  if (!d_o || (!dq && !dk) || !dk != !dv) return LEWI_ERR_ARG;
+  if (!aligned(d_o, 16) || !aligned(dq, 16) || !aligned(dk, 16) || !aligned(dv, 16)) return LEWI_ERR_SHAPE;
+  if (!workspace || !aligned(workspace, 4) || workspace_bytes < lewi_causal_attention_bwd_workspace_bytes(T, Hq)) return LEWI_ERR_WORKSPACE;
+  CUtensorMap tq, tk, tv, td;
+  if (!attn::make_rows_map(&tq, q, T, Hq, D, q_stride) || !attn::make_rows_map(&tk, k, T, Hkv, D, k_stride) ||
+      !attn::make_rows_map(&tv, v, T, Hkv, D, v_stride) || !attn::make_rows_map(&td, d_o, T, Hq, D, (int64_t)Hq * D))
+    return LEWI_ERR_CUDA;
+  const attn::Args a{{cu_seqlens, n_seqs, T}, Hq, Hkv, Hq / Hkv, D, scale, scale * 1.4426950408889634f,
+                     const_cast<bf16*>(reinterpret_cast<const bf16*>(o)), const_cast<float*>(lse), reinterpret_cast<float*>(workspace),
+                     reinterpret_cast<bf16*>(dq), reinterpret_cast<bf16*>(dk), reinterpret_cast<bf16*>(dv)};
+  const bf16* g = reinterpret_cast<const bf16*>(d_o);
+  return D <= 64 ? attention_bwd<64>(as_stream(stream), a, tq, tk, tv, td, g) : attention_bwd<128>(as_stream(stream), a, tq, tk, tv, td, g);
 }
 
 }  // extern "C"

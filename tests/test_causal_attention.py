@@ -1,0 +1,256 @@
+"""Causal attention over packed sequences, forward and backward, against its formulas in 64 bits.
+
+Tolerances: a rounding to bf16 is off by u = 2^-8 of the value at most.  p is rounded for its product with v, so o is off by u sum p |v| and its
+own rounding.  delta is a sum over the rounded o.  dS is rounded for its products, so dQ is off by scale (u |dS| + p |delta's error|) |K|
+and its own rounding, and so on.  1e-4 of the magnitudes is room for float32: scores of magnitude up to 40 with sums of 128 products."""
+import pytest
+import torch
+
+from lewi_surge_b200 import LewiError, _lib, attention
+
+U, F32 = 2.0 ** -8, 1e-4
+F64 = torch.float64
+
+
+def formulas(q, k, v, cu, scale, d_o=None, f32=F32):
+  """Outputs and gradients in 64 bits with their bounds, {name: (value, bound)}; rows of no sequence are zero."""
+  t, hq, d = q.shape
+  g = hq // k.shape[1]
+  q, k, v = (x.to(F64) for x in (q, k, v))
+  zeros = lambda x: torch.zeros_like(x)
+  o, ob, dq, dqb, dk, dkb, dv, dvb = zeros(q), zeros(q), zeros(q), zeros(q), zeros(k), zeros(k), zeros(v), zeros(v)
+  for a, b in zip(cu, cu[1:]):
+    if a >= b:
+      continue
+    seen = torch.ones(b - a, b - a, dtype=torch.bool).tril()
+    for h in range(hq):
+      qh, kh, vh = q[a:b, h], k[a:b, h // g], v[a:b, h // g]
+      p = torch.softmax((qh @ kh.t() * scale).masked_fill(~seen, float("-inf")), -1)
+      oh = p @ vh
+      o[a:b, h], ob[a:b, h] = oh, U * oh.abs() + (U + f32) * (p @ vh.abs())
+      if d_o is None:
+        continue
+      do = d_o[a:b, h].to(F64)
+      dv[a:b, h // g] += p.t() @ do
+      dvb[a:b, h // g] += (U + f32) * (p.t() @ do.abs())
+      delta, delta_b = (do * oh).sum(-1, keepdim=True), (do.abs() * ob[a:b, h]).sum(-1, keepdim=True)
+      ds = p * (do @ vh.t() - delta)
+      ds_b = U * ds.abs() + p * (delta_b + f32 * (do.abs() @ vh.abs().t() + (do * oh).abs().sum(-1, keepdim=True)))
+      dq[a:b, h], dqb[a:b, h] = scale * (ds @ kh), scale * (ds_b @ kh.abs())
+      dk[a:b, h // g] += scale * (ds.t() @ qh)
+      dkb[a:b, h // g] += scale * (ds_b.t() @ qh.abs())
+  out = {"o": (o, ob)}
+  if d_o is not None:
+    out.update(dq=(dq, dqb + U * dq.abs()), dk=(dk, dkb + U * dk.abs()), dv=(dv, dvb + U * dv.abs()))
+  return out
+
+
+def within(got, want, what):
+  value, bound = want
+  off = (got.detach().to(F64).cpu() - value).abs()
+  assert not torch.isnan(off).any(), what
+  bound = bound + 1e-31   # (float32: a p below 2^-126 is zero, times sums of at most 10^6)
+  assert (off <= bound).all(), f"{what} is off by {(off / bound).max().item():.2f} of its bound"
+
+
+def rnd(gen, *shape):
+  return torch.randn(*shape, generator=gen).bfloat16()
+
+
+def test_refusals():
+  bf = torch.bfloat16
+  q, k = torch.zeros(6, 4, 16, dtype=bf), torch.zeros(6, 2, 16, dtype=bf)
+  cu = torch.tensor([0, 6])
+  for bad in (lambda: attention.causal_attention(q, k, k), lambda: attention.causal_attention(q.float(), k, k),
+              lambda: attention.causal_attention(q, k, k[:5]), lambda: attention.causal_attention(q[:, :3], k, k),
+              lambda: attention.causal_attention(q, k[..., :8], k[..., :8]), lambda: attention.causal_attention(q, k, k, cu[:1]),
+              lambda: attention.causal_attention(q[None], k[None], k[None], cu), lambda: attention.causal_attention(q, k, k, scale=0.0),
+              lambda: attention.causal_attention(q, k, k, scale=-1.0), lambda: attention.causal_attention(q[0], k[0], k[0])):
+    with pytest.raises(LewiError):
+      bad()
+  lib, at = _lib.load(), 1 << 20   # (addresses that are never used)
+  call = lambda q=at, qs=256, n=1, t=64, hq=4, hkv=2, d=64, scale=1.0: lib.lewi_causal_attention_fwd(None, q, qs, at, 128, at, 128, None, n, at, at, t, hq, hkv, d, scale)
+  assert call(q=None) == -1 and call(t=0) == -1 and call(n=3) == -1 and call(scale=float("nan")) == -1
+  assert call(q=at + 2) == -2 and call(qs=255) == -2 and call(qs=264 - 16) == -2 and call(hq=3) == -2 and call(d=60) == -2 and call(d=136) == -5
+  bwd = lambda dq=at, dk=at, dv=at, ws=1 << 20: lib.lewi_causal_attention_bwd(None, at, 256, at, 128, at, 128, at, at, at, None, 1, dq, dk, dv, at, ws, 64, 4, 2, 64, 1.0)
+  assert bwd(dq=None, dk=None, dv=None) == -1 and bwd(dv=None) == -1 and bwd(dq=at + 8) == -2 and bwd(ws=16) == -3
+
+
+def test_the_formulas_are_the_gradients():
+  """The 64-bit formulas above against differences of their own forward pass."""
+  gen = torch.Generator().manual_seed(0)
+  q, k, v, d_o = (torch.randn(11, h, 8, generator=gen, dtype=F64) for h in (4, 2, 2, 4))
+  cu, scale, step = [0, 4, 4, 11], 0.4, 1e-5
+  grads = formulas(q, k, v, cu, scale, d_o)
+  for name, i in (("dq", 0), ("dk", 1), ("dv", 2)):
+    along = torch.randn((q, k, v)[i].shape, generator=gen, dtype=F64)
+    loss = lambda s: (formulas(*(x + s * along if j == i else x for j, x in enumerate((q, k, v))), cu, scale)["o"][0] * d_o).sum()
+    assert abs((loss(step) - loss(-step)) / (2 * step) - (grads[name][0] * along).sum()) <= 1e-7 * (grads[name][0] * along).abs().sum()
+
+
+CASES = [([1], 1, 1, 8), ([128], 2, 1, 64), ([129], 1, 1, 128), ([127, 1, 0, 128, 2, 300], 4, 2, 64), ([1000], 6, 2, 128), ([256, 257, 255, 5], 3, 1, 96),
+         ([13] * 37, 2, 2, 80), ([0, 0, 640, 0], 5, 1, 64), ([3, 130] * 200, 2, 1, 32), ([700], 7, 7, 120), ([200] + [1] * 400 + [129], 3, 3, 16)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,hq,hkv,d", CASES)
+def test_packed_sequences_forward_and_backward(cuda, lens, hq, hkv, d):
+  gen = torch.Generator().manual_seed(sum(lens) + hq)
+  before, behind = (0, 0) if len(lens) == 1 else (3, 140)   # rows of no sequence, of NaN
+  t = before + sum(lens) + behind
+  cu = (torch.tensor([0] + lens).cumsum(0) + before).tolist()
+  fused = rnd(gen, t, (hq + 2 * hkv) * d)
+  fused[:before] = float("nan")
+  fused[t - behind:] = float("nan")
+  d_o = rnd(gen, t, hq, d)
+  d_o[:before] = float("nan")
+  d_o[t - behind:] = float("nan")
+  split = lambda x: [p.view(t, h, d) for p, h in zip(x.split([hq * d, hkv * d, hkv * d], 1), (hq, hkv, hkv))]
+  scale = 0.2 if d == 80 else None
+  want = formulas(*split(fused), cu, scale or d ** -0.5, d_o)
+  F = fused.to(cuda).requires_grad_(True)
+  seqs = torch.tensor(cu, device=cuda) if before or len(lens) > 1 else None
+  q, k, v = split(F)   # views of one projection
+  o = attention.causal_attention(q, k, v, seqs, scale=scale)
+  dF, = torch.autograd.grad(o, F, d_o.to(cuda), retain_graph=True)
+  assert _lib.last_status() == 0
+  within(o, want["o"], "o")
+  for name, x in zip(("dq", "dk", "dv"), split(dF)):
+    within(x, want[name], name)
+  again, = torch.autograd.grad(attention.causal_attention(*split(F), seqs, scale=scale), F, d_o.to(cuda))
+  assert torch.equal(again, dF)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("b,s,hq,hkv,d", [(3, 1, 2, 1, 64), (2, 128, 4, 4, 64), (3, 150, 2, 2, 128), (1, 400, 3, 1, 64), (70, 20, 2, 1, 72)])
+def test_sequences_of_one_length(cuda, b, s, hq, hkv, d):
+  """[B, S, H, D]: the bits of the packed call, and each gradient alone those of all three."""
+  gen = torch.Generator().manual_seed(s)
+  q, k, v, d_o = (rnd(gen, b, s, h, d).to(cuda) for h in (hq, hkv, hkv, hq))
+  leaves = [x.clone().requires_grad_(True) for x in (q, k, v)]
+  o = attention.causal_attention(*leaves)
+  grads = torch.autograd.grad(o, leaves, d_o)
+  flat = [x.flatten(0, 1).requires_grad_(True) for x in (q, k, v)]
+  o2 = attention.causal_attention(*flat, torch.arange(0, b * s + 1, s, device=cuda))
+  assert torch.equal(o.flatten(0, 1), o2)
+  for g, g2 in zip(grads, torch.autograd.grad(o2, flat, d_o.flatten(0, 1))):
+    assert torch.equal(g.flatten(0, 1), g2)
+  for i in range(3):
+    only = [x.clone().requires_grad_(j == i) for j, x in enumerate((q, k, v))]
+    g, = torch.autograd.grad(attention.causal_attention(*only), only[i], d_o)
+    assert torch.equal(g, grads[i])
+  within(o.flatten(0, 1), formulas(*(x.flatten(0, 1).detach().cpu() for x in (q, k, v)), list(range(0, b * s + 1, s)), d ** -0.5)["o"], "o")
+
+
+@pytest.mark.gpu
+def test_scores_that_grow_along_the_keys(cuda):
+  """The running maximum grows in every block, by more and by less than what makes the sums so far be scaled anew."""
+  gen = torch.Generator().manual_seed(8)
+  t, d = 900, 64
+  q, k, v, d_o = (rnd(gen, t, 2, d) for _ in range(4))
+  for slope in (0.002, 0.02, -0.02):
+    ks = (k.float() * 0.1 + slope * torch.arange(t)[:, None, None] * q.float().mean(0, keepdim=True).sign()).bfloat16()
+    qs = (q.float().abs() * q.float().mean(0, keepdim=True).sign()).bfloat16()
+    want = formulas(qs, ks, v, [0, t], d ** -0.5, d_o, f32=5e-4)   # (scores of up to 120, sums of 64 products: 2^-24 64 120)
+    leaves = [x.to(cuda).requires_grad_(True) for x in (qs, ks, v)]
+    o = attention.causal_attention(*leaves)
+    within(o, want["o"], "o")
+    for name, g in zip(("dq", "dk", "dv"), torch.autograd.grad(o, leaves, d_o.to(cuda))):
+      within(g, want[name], name)
+
+
+@pytest.mark.gpu
+def test_bad_bounds_are_recorded_and_write_nothing_outside(cuda):
+  gen = torch.Generator().manual_seed(2)
+  q, k, v = (rnd(gen, 300, h, 64).to(cuda) for h in (2, 1, 1))
+  for cu in ([0, 400], [-5, 300], [0, 200, 100, 300], [0, 2 ** 40]):
+    o = attention.causal_attention(q, k, v, torch.tensor(cu, device=cuda))
+    assert _lib.last_status() == _lib.STATUS_BAD_INDEX and o.shape == q.shape
+  good = attention.causal_attention(q, k, v)
+  assert torch.equal(attention.causal_attention(q, k, v, torch.tensor([0, 400], device=cuda)), good)   # cut to the rows there are
+  assert _lib.last_status() == _lib.STATUS_BAD_INDEX
+
+
+@pytest.mark.gpu
+def test_a_value_that_is_not_finite_stays_in_its_sequence(cuda):
+  gen = torch.Generator().manual_seed(3)
+  q, k, v = (rnd(gen, 500, h, 64).to(cuda) for h in (2, 1, 1))
+  cu = torch.tensor([0, 130, 131, 400, 500], device=cuda)
+  want = attention.causal_attention(q, k, v, cu)
+  for x in (q, k, v):
+    x[131 + 140:400] = float("nan")
+  got = attention.causal_attention(q, k, v, cu)
+  whole = torch.ones(500, dtype=torch.bool, device=cuda)
+  whole[131 + 128:400] = False   # its tile and what comes behind it
+  assert torch.equal(got[whole], want[whole]) and got[131 + 140:400].isnan().all()
+
+
+@pytest.mark.gpu
+def test_a_captured_training_step_follows_its_inputs_and_bounds(cuda):
+  from lewi_surge_b200 import layer
+  gen = torch.Generator().manual_seed(4)
+  data = [[rnd(gen, 600, h, 64).to(cuda) for h in (4, 2, 2, 4)] for _ in range(4)]
+  bounds = [[0, 600, 600, 600], [0, 1, 2, 600], [0, 300, 301, 550], [100, 228, 400, 400]]
+  q, k, v, d_o = (x.clone() for x in data[0])
+  cu = torch.zeros(4, dtype=torch.int32, device=cuda)
+  def step():
+    leaves = [x.detach().requires_grad_(True) for x in (q, k, v)]
+    o = attention.causal_attention(*leaves, cu)
+    return o.detach(), *torch.autograd.grad(o, leaves, d_o)
+  step()
+  run = layer.CapturedStep(step)
+  for new, b in zip(data * 2, bounds * 2):
+    for x, y in zip((q, k, v, d_o), new):
+      x.copy_(y)
+    cu.copy_(torch.tensor(b))
+    got = [x.clone() for x in run()]
+    for x, y in zip(got, step()):
+      assert torch.equal(x, y)
+  assert _lib.last_status() == 0
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once(cuda):
+  gen = torch.Generator().manual_seed(5)
+  sets = [[rnd(gen, 1500, h, 128).to(cuda).requires_grad_(True) for h in (4, 2, 2)] for _ in range(2)]
+  d_o = rnd(gen, 1500, 4, 128).to(cuda)
+  def call(leaves):
+    o = attention.causal_attention(*leaves)
+    return o.detach(), *torch.autograd.grad(o, leaves, d_o)
+  want = [call(x) for x in sets]
+  streams = [torch.cuda.Stream() for _ in range(2)]
+  torch.cuda.synchronize()
+  got = [[], []]
+  for _ in range(6):
+    for i, st in enumerate(streams):
+      with torch.cuda.stream(st):
+        got[i].append(call(sets[i]))
+  torch.cuda.synchronize()
+  for i in range(2):
+    for r in got[i]:
+      assert all(torch.equal(x, y) for x, y in zip(r, want[i]))
+
+
+@pytest.mark.gpu
+def test_a_prompt_and_the_tokens_after_it_are_one_sequence(cuda):
+  """Prompts by causal_attention and their keys into pages, then tokens one by one over the pages: as causal attention over everything."""
+  gen = torch.Generator().manual_seed(6)
+  lens, more, hq, hkv, d, page = [130, 5, 257], 4, 8, 2, 64, 16
+  rows = [[rnd(gen, n + more, h, d) for h in (hq, hkv, hkv)] for n in lens]
+  pack = lambda i, part: torch.cat([r[i][part(n)] for r, n in zip(rows, lens)]).to(cuda)
+  q, k, v = (pack(i, lambda n: slice(0, n)) for i in range(3))
+  cu = torch.tensor([0] + lens, device=cuda).cumsum(0)
+  tables = torch.randperm(3 * 20, generator=gen).view(3, 20).to(cuda)
+  kc, vc = (torch.full((60, page, hkv, d), float("nan"), dtype=torch.bfloat16, device=cuda) for _ in range(2))
+  ln = torch.tensor(lens, device=cuda)
+  attention.paged_cache_write(k, v, kc, vc, tables, ln, cu)
+  got = [attention.causal_attention(q, k, v, cu).split(lens)]
+  for i in range(more):
+    q1, k1, v1 = (torch.stack([r[j][n + i] for r, n in zip(rows, lens)]).to(cuda) for j in range(3))
+    ln += 1
+    attention.paged_cache_write(k1, v1, kc, vc, tables, ln)
+    got.append([x[None] for x in attention.paged_attention(q1, kc, vc, tables, ln).unbind()])
+  assert _lib.last_status() == 0
+  for b, n in enumerate(lens):
+    want = formulas(*rows[b], [0, n + more], d ** -0.5)["o"]
+    within(torch.cat([g[b] for g in got]), want, f"sequence {b}")
