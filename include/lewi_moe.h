@@ -398,7 +398,7 @@ int lewi_paged_attention(void* stream, const void* q, int64_t q_stride, const vo
 int lewi_causal_attention_fwd(void* stream, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
                               int64_t v_stride, const int32_t* cu_seqlens, int n_seqs, void* o, float* lse, int T, int Hq, int Hkv, int D,
                               float scale);
-int64_t lewi_causal_attention_bwd_workspace_bytes(int T, int Hq);
+int64_t lewi_causal_attention_bwd_workspace_bytes(int T, int n_seqs, int Hq, int Hkv, int D);
 int lewi_causal_attention_bwd(void* stream, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
                               int64_t v_stride, const void* o, const float* lse, const void* d_o, const int32_t* cu_seqlens, int n_seqs,
                               void* dq, void* dk, void* dv, void* workspace, int64_t workspace_bytes, int T, int Hq, int Hkv, int D,

@@ -81,7 +81,7 @@ SIGNATURES = {
     "lewi_paged_attention": (c_int, [P, P, c_int64, P, P, c_int64, P, P, P, P, c_int64, c_int, c_int, c_int, c_int, c_int64, c_int, c_int,
                                      c_float]),
     "lewi_causal_attention_fwd": (c_int, [P, P, c_int64, P, c_int64, P, c_int64, P, c_int, P, P] + [c_int] * 4 + [c_float]),
-    "lewi_causal_attention_bwd_workspace_bytes": (c_int64, [c_int, c_int]),
+    "lewi_causal_attention_bwd_workspace_bytes": (c_int64, [c_int] * 5),
     "lewi_causal_attention_bwd": (c_int, [P, P, c_int64, P, c_int64, P, c_int64, P, P, P, P, c_int, P, P, P, P, c_int64] + [c_int] * 4 +
                                   [c_float]),
     "lewi_moe_residual_layout": (c_int64, [c_int64, c_int, c_int, c_int, c_int, c_int, c_int, P]),
@@ -162,40 +162,45 @@ def last_status():
   return rc
 
 
-def one_device(*tensors):
-  """A context in which the device of all these CUDA tensors (None is left out) is the current one."""
-  import contextlib
+def elsewhere(*tensors):
+  """Whether these CUDA tensors (None is left out) lie on a device that is not the current one; they have to lie on one."""
   import torch
-  devices = {t.device for t in tensors if t is not None}
-  if len(devices) != 1 or next(iter(devices)).type != "cuda":
-    raise LewiError(f"expected CUDA tensors of one device, got {sorted(map(str, devices))}: the kernels have no CPU path")
-  index = next(iter(devices)).index
-  return contextlib.nullcontext() if index == torch.cuda.current_device() else torch.cuda.device(index)
+  index = tensors[0].get_device()
+  for t in tensors:
+    if t is not None and (t.get_device() != index or index < 0):
+      raise LewiError(f"expected CUDA tensors of one device, got {t.device} and {tensors[0].device}: the kernels have no CPU path")
+  return index != torch._C._cuda_getDevice()
 
 
 def index_table(t, what):
   """A table of int32 as the kernels read it; int64 values that int32 cannot hold stay out of range."""
   import torch
-  if t is None:
-    return None
-  if t.dtype == torch.int64:
+  if t is None or (t.dtype is torch.int32 and t.is_contiguous()):
+    return t
+  if t.dtype is torch.int64:
     t = t.clamp(-1, 2 ** 31 - 1).to(torch.int32)
-  if t.dtype != torch.int32:
+  if t.dtype is not torch.int32:
     raise LewiError(f"{what} holds int32 or int64 indices")
   return t.contiguous()
 
 
 def rows_of(t, align):
-  """`t` with its trailing dimensions packed (only rows may be apart) and rows and address multiples of `align` bytes; a copy where they
-  are not."""
-  packed, n = True, 1
-  for size, step in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
-    packed &= size == 1 or step == n
-    n *= size
-  rows = t.stride(0) if t.shape[0] > 1 else n
-  if not packed or rows < n or t.data_ptr() % align or rows * t.element_size() % align:
-    t = t.contiguous()
+  """`t` with its trailing dimensions packed (only rows may be apart) and rows and address multiples of `align` bytes, a copy where they
+  are not; and the distance of its rows in elements."""
+  size = t.element_size()
+  n = 1
+  for m in t.shape[1:]:
+    n *= m
+  if t.is_contiguous():
     rows = n
-    if t.data_ptr() % align:
-      t = t.clone()
+  else:
+    packed, step = True, 1
+    for m, st in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+      packed &= m == 1 or st == step
+      step *= m
+    rows = t.stride(0) if t.shape[0] > 1 else n
+    if not packed or rows < n or rows * size % align:
+      t, rows = t.contiguous(), n
+  if t.data_ptr() % align:
+    t, rows = t.new_empty(t.shape).copy_(t), n
   return t, rows

@@ -16,9 +16,10 @@ def _check_cache(what, key_cache, value_cache, block_tables, lengths):
   if key_cache.dim() != 4 or value_cache.shape != key_cache.shape:
     raise LewiError(f"{what}: caches [pages, page, Hkv, D] of one shape are required")
   _, page, heads, d = key_cache.shape
-  for t in (key_cache, value_cache):
-    if t.stride()[1:] != (heads * d, d, 1) or (t.shape[0] > 1 and t.stride(0) != key_cache.stride(0)):
-      raise LewiError(f"{what}: pages that are contiguous and as far apart in both caches are required")
+  if not (key_cache.is_contiguous() and value_cache.is_contiguous()):
+    for t in (key_cache, value_cache):
+      if t.stride()[1:] != (heads * d, d, 1) or (t.shape[0] > 1 and t.stride(0) != key_cache.stride(0)):
+        raise LewiError(f"{what}: pages that are contiguous and as far apart in both caches are required")
   if block_tables.dim() != 2 or lengths.shape != (block_tables.shape[0],):
     raise LewiError(f"{what}: block_tables [B, max_pages] and lengths [B] are required")
   page_stride = key_cache.stride(0) if key_cache.shape[0] > 1 else page * heads * d
@@ -43,12 +44,15 @@ def paged_cache_write(key, value, key_cache, value_cache, block_tables, lengths,
     raise LewiError("paged_cache_write: without cu_seqlens there is one token per sequence")
   if t == 0 or b == 0:
     return
-  with torch.no_grad(), _lib.one_device(key, value, key_cache, value_cache, block_tables, lengths, cu_seqlens):
-    (k, ks), (v, vs) = _lib.rows_of(key, 16), _lib.rows_of(value, 16)
-    tables, lens, cu = (_lib.index_table(x, n) for x, n in ((block_tables, "block_tables"), (lengths, "lengths"), (cu_seqlens, "cu_seqlens")))
-    check(lib.lewi_paged_cache_write(stream(), k.data_ptr(), ks, v.data_ptr(), vs, key_cache.data_ptr(), value_cache.data_ptr(), page_stride,
-                                     ptr(tables), ptr(lens), ptr(cu), t, b, heads, d, key_cache.shape[0], page, tables.shape[1]),
-          "lewi_paged_cache_write")
+  if _lib.elsewhere(key_cache, key, value, value_cache, block_tables, lengths, cu_seqlens):
+    with torch.cuda.device(key_cache.device):
+      return paged_cache_write(key, value, key_cache, value_cache, block_tables, lengths, cu_seqlens)
+  (k, ks), (v, vs) = _lib.rows_of(key, 16), _lib.rows_of(value, 16)
+  tables, lens = _lib.index_table(block_tables, "block_tables"), _lib.index_table(lengths, "lengths")
+  cu = _lib.index_table(cu_seqlens, "cu_seqlens")
+  check(lib.lewi_paged_cache_write(stream(), k.data_ptr(), ks, v.data_ptr(), vs, key_cache.data_ptr(), value_cache.data_ptr(), page_stride,
+                                   tables.data_ptr(), lens.data_ptr(), ptr(cu), t, b, heads, d, key_cache.shape[0], page, tables.shape[1]),
+        "lewi_paged_cache_write")
 
 
 def paged_attention(query, key_cache, value_cache, block_tables, lengths, scale=None):
@@ -62,33 +66,39 @@ def paged_attention(query, key_cache, value_cache, block_tables, lengths, scale=
   if query.dtype != torch.bfloat16 or query.dim() != 3 or query.shape[2] != d or query.shape[1] % heads or query.shape[0] != block_tables.shape[0]:
     raise LewiError("paged_attention: query [B, Hq, D] bfloat16 with Hq a multiple of the caches' heads is required")
   b, hq = query.shape[:2]
-  with torch.no_grad(), _lib.one_device(query, key_cache, value_cache, block_tables, lengths):
-    q, qs = _lib.rows_of(query, 4)
-    o = torch.empty((b, hq, d), dtype=torch.bfloat16, device=q.device)
-    if b == 0 or hq == 0:
-      return o
-    tables, lens = _lib.index_table(block_tables, "block_tables"), _lib.index_table(lengths, "lengths")
-    ws_bytes = int(lib.lewi_paged_attention_workspace_bytes(d))
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
-    check(lib.lewi_paged_attention(stream(), q.data_ptr(), qs, key_cache.data_ptr(), value_cache.data_ptr(), page_stride, ptr(tables), ptr(lens),
-                                   ptr(o), ptr(ws), ws_bytes, b, hq, heads, d, key_cache.shape[0], page, tables.shape[1],
-                                   d ** -0.5 if scale is None else float(scale)), "lewi_paged_attention")
+  if _lib.elsewhere(query, key_cache, value_cache, block_tables, lengths):
+    with torch.cuda.device(query.device):
+      return paged_attention(query, key_cache, value_cache, block_tables, lengths, scale)
+  q, qs = _lib.rows_of(query, 4)
+  o = torch.empty((b, hq, d), dtype=torch.bfloat16, device=q.device)
+  if b == 0 or hq == 0:
+    return o
+  tables, lens = _lib.index_table(block_tables, "block_tables"), _lib.index_table(lengths, "lengths")
+  ws_bytes = lib.lewi_paged_attention_workspace_bytes(d)
+  ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+  check(lib.lewi_paged_attention(stream(), q.data_ptr(), qs, key_cache.data_ptr(), value_cache.data_ptr(), page_stride, tables.data_ptr(),
+                                 lens.data_ptr(), o.data_ptr(), ws.data_ptr(), ws_bytes, b, hq, heads, d, key_cache.shape[0], page, tables.shape[1],
+                                 d ** -0.5 if scale is None else float(scale)), "lewi_paged_attention")
   return o
+
+
+def _attention_fwd(q, k, v, cu, n_seqs, scale):
+  """Output, log-sum-exp and the operands as the kernels read them."""
+  (q, qs), (k, ks), (v, vs) = _lib.rows_of(q, 16), _lib.rows_of(k, 16), _lib.rows_of(v, 16)
+  cu = _lib.index_table(cu, "cu_seqlens")
+  t, hq, d = q.shape
+  o = torch.empty((t, hq, d), dtype=torch.bfloat16, device=q.device)
+  lse = torch.empty((hq, t), dtype=torch.float32, device=q.device)
+  check(_lib.load().lewi_causal_attention_fwd(stream(), q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, ptr(cu), n_seqs, o.data_ptr(),
+                                              lse.data_ptr(), t, hq, k.shape[1], d, scale), "lewi_causal_attention_fwd")
+  return o, lse, q, k, v, cu
 
 
 class _CausalAttention(torch.autograd.Function):
 
   @staticmethod
   def forward(ctx, q, k, v, cu, n_seqs, scale):
-    lib = _lib.load()
-    with _lib.one_device(q, k, v, cu):
-      (q, qs), (k, ks), (v, vs) = (_lib.rows_of(t, 16) for t in (q, k, v))
-      cu = _lib.index_table(cu, "cu_seqlens")
-      t, hq, d = q.shape
-      o = torch.empty((t, hq, d), dtype=torch.bfloat16, device=q.device)
-      lse = torch.empty((hq, t), dtype=torch.float32, device=q.device)
-      check(lib.lewi_causal_attention_fwd(stream(), q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, ptr(cu), n_seqs, ptr(o), ptr(lse),
-                                          t, hq, k.shape[1], d, scale), "lewi_causal_attention_fwd")
+    o, lse, q, k, v, cu = _attention_fwd(q, k, v, cu, n_seqs, scale)
     ctx.save_for_backward(q, k, v, o, lse, cu)
     ctx.call = n_seqs, scale
     return o
@@ -99,16 +109,15 @@ class _CausalAttention(torch.autograd.Function):
     q, k, v, o, lse, cu = ctx.saved_tensors
     n_seqs, scale = ctx.call
     t, hq, d = q.shape
-    with _lib.one_device(q, g):
-      (q, qs), (k, ks), (v, vs) = (_lib.rows_of(x, 16) for x in (q, k, v))
-      g, _ = _lib.rows_of(g.contiguous(), 16)
-      dq = torch.empty((t, hq, d), dtype=torch.bfloat16, device=q.device) if ctx.needs_input_grad[0] else None
-      dk, dv = (torch.empty(k.shape, dtype=torch.bfloat16, device=q.device) if any(ctx.needs_input_grad[1:3]) else None for _ in range(2))
-      ws_bytes = int(lib.lewi_causal_attention_bwd_workspace_bytes(t, hq))
-      ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
-      check(lib.lewi_causal_attention_bwd(stream(), q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, ptr(o), ptr(lse), ptr(g), ptr(cu), n_seqs,
-                                          ptr(dq), ptr(dk), ptr(dv), ptr(ws), ws_bytes, t, hq, k.shape[1], d, scale),
-            "lewi_causal_attention_bwd")
+    (q, qs), (k, ks), (v, vs) = _lib.rows_of(q, 16), _lib.rows_of(k, 16), _lib.rows_of(v, 16)
+    g, _ = _lib.rows_of(g.contiguous(), 16)
+    dq = torch.empty((t, hq, d), dtype=torch.bfloat16, device=q.device) if ctx.needs_input_grad[0] else None
+    dk, dv = (torch.empty(k.shape, dtype=torch.bfloat16, device=q.device) if any(ctx.needs_input_grad[1:3]) else None for _ in range(2))
+    ws_bytes = lib.lewi_causal_attention_bwd_workspace_bytes(t, n_seqs, hq, k.shape[1], d)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+    check(lib.lewi_causal_attention_bwd(stream(), q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, o.data_ptr(), lse.data_ptr(), g.data_ptr(),
+                                        ptr(cu), n_seqs, ptr(dq), ptr(dk), ptr(dv), ws.data_ptr(), ws_bytes, t, hq, k.shape[1], d, scale),
+          "lewi_causal_attention_bwd")
     return dq, dk, dv, None, None, None
 
 
@@ -122,7 +131,7 @@ def causal_attention(query, key, value, cu_seqlens=None, scale=None):
 
   A value of v that is not finite reaches back to the start of its 128 rows of the sequence (as those of q, k and the upstream gradient do in the
   gradients), never into another sequence."""
-  if any(x.dtype != torch.bfloat16 for x in (query, key, value)):
+  if not query.dtype == key.dtype == value.dtype == torch.bfloat16:
     raise LewiError("causal_attention takes bfloat16 q, k, v")
   if query.dim() not in (3, 4) or key.dim() != query.dim() or value.shape != key.shape or query.shape[:-2] != key.shape[:-2] or \
       query.shape[-1] != key.shape[-1] or key.shape[-2] == 0 or query.shape[-2] % key.shape[-2]:
@@ -140,4 +149,9 @@ def causal_attention(query, key, value, cu_seqlens=None, scale=None):
     n_seqs = cu_seqlens.shape[0] - 1
   if query.numel() == 0:
     return query.clone()
-  return _CausalAttention.apply(query, key, value, cu_seqlens, n_seqs, scale).view(shape)
+  if _lib.elsewhere(query, key, value, cu_seqlens):
+    with torch.cuda.device(query.device):
+      return causal_attention(query.view(shape), key.view(*shape[:-2], *key.shape[-2:]), value.view(*shape[:-2], *key.shape[-2:]), cu_seqlens, scale)
+  if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad):
+    return _CausalAttention.apply(query, key, value, cu_seqlens, n_seqs, scale).view(shape)
+  return _attention_fwd(query, key, value, cu_seqlens, n_seqs, scale)[0].view(shape)

@@ -13,6 +13,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "f32x2.cuh"
 #include "tcgen05.cuh"
 #include "tensor_map.cuh"
 
@@ -134,12 +135,25 @@ __device__ __forceinline__ void zero_gaps(const Seqs& q, __nv_bfloat16* out, int
 }
 
 // ---------------------------------------------------------------- pieces
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
+// 2^(x scale + shift) of two scores.  The special function unit gives 16 a cycle and SM, so 128 x 128 of them take as long as two products
+// of 128 x 128 x 128; every OF-th pair is made by multiply-adds instead (0: none).
+template <int OF>
+__device__ __forceinline__ F2 ex2_pair(uint32_t x0, uint32_t x1, F2 scale, F2 shift, int pair) {
+  const F2 x = fma2(f2(__uint_as_float(x0), __uint_as_float(x1)), scale, shift);
+  if (OF > 0 && pair % (OF > 0 ? OF : 1) == OF - 1) return ex2_poly(x);
+  float lo, hi;
+  f2_split(x, lo, hi);
+  return f2(ex2(lo), ex2(hi));
 }
+// The backward pass does so where D <= 64, whose products are half as long (T = 8192, 32 heads over 8: dQ 488 -> 465, dK and dV 695 ->
+// 670 us); at D = 128 it costs (dQ 648 -> 661, dK and dV 845 -> 875 us).
+template <int DP> constexpr int kBwdPoly = DP == 64 ? 4 : 0;
 
+__device__ __forceinline__ F2 hide(F2 v, bool lo_hidden, bool hi_hidden) {
+  float lo, hi;
+  f2_split(v, lo, hi);
+  return f2(lo_hidden ? 0.f : lo, hi_hidden ? 0.f : hi);
+}
 // Operand tiles in shared memory: boxes of [128 rows][64 columns], 128-byte swizzled, 16 KB apart.
 constexpr int kBox = kTile * 128;
 template <int DP> constexpr int kTileBytes = kTile * DP * 2;
@@ -212,6 +226,8 @@ struct Args {
   __nv_bfloat16* o;        // [T][Hq][D]
   float *lse, *delta;      // [Hq][T], lse in units of log 2
   __nv_bfloat16 *dq, *dk, *dv;
+  int parts;               // of a group's heads, one CTA each for dK and dV
+  float* sums;             // [part][dV, dK][T][Hkv][D] where there are several
 };
 
 __device__ __forceinline__ void store_row32(__nv_bfloat16* dst, const uint32_t (&v)[32], float f, int cols) {
@@ -224,13 +240,21 @@ __device__ __forceinline__ void store_row32(__nv_bfloat16* dst, const uint32_t (
                                     pack_bf16(__uint_as_float(v[8 * i + 6]) * f, __uint_as_float(v[8 * i + 7]) * f)));
 }
 
+__device__ __forceinline__ void store_part32(float* dst, const uint32_t (&v)[32], float f, int cols) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i * 4 < cols)
+      *reinterpret_cast<float4*>(dst + i * 4) = make_float4(__uint_as_float(v[4 * i]) * f, __uint_as_float(v[4 * i + 1]) * f,
+                                                            __uint_as_float(v[4 * i + 2]) * f, __uint_as_float(v[4 * i + 3]) * f);
+}
+
 // ---------------------------------------------------------------- forward
 // A CTA works on two tiles of queries that share their keys (two heads, or two tiles of one head): while one tile's softmax is made by its
 // four warps, the tensor cores multiply for the other, and every key and value tile that is brought serves both.  Warps 0-3 and 4-7: a
 // row of S per thread; warp 8: TMA; warp 9: MMA.  Products are issued in the order S0(j+1) after P0 V(j), S1(j+1) after P1 V(j): a
 // softmax that finds its scores knows that the product before them is done, so it may scale O then.  It does so only where the
 // maximum has grown by more than 8 (in powers of 2; p stays below 2^8, which bf16 and float32 hold as well as 1).
-constexpr int kFwdThreads = 320;
+constexpr int kFwdThreads = 384;   // (warps 10 and 11 have nothing to do: registers move between warpgroups of four warps)
 template <int DP>
 struct FwdShape {
   static constexpr int kStages = DP == 64 ? 6 : 5;
@@ -306,6 +330,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
   auto s_at = [&](int t) { return tmem + t * 128; };
   auto o_at = [&](int t) { return tmem + 256 + t * 128; };
 
+  // registers: 8 x 216 + 4 x 72 = 12 x 168 a thread, what the launch has
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
   if (warp == 8) {
     // ---------------------------------------------------------------- queries, then K0, V0, K1, V1, ..
     bool ok = true;
@@ -369,8 +396,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
       if (!ok) settle();
     }
     __syncwarp();
+  }
   } else {
     // ---------------------------------------------------------------- softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const int t = warp >> 2, row = (warp & 3) * 32 + lane, n_blocks = blocks[t];
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;   // this warp's lanes of tensor memory
     const uint32_t sp = s_at(t) + lanes, op = o_at(t) + lanes;
@@ -416,28 +445,26 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
         }
         ptx::tmem_st_wait();
       }
-      const float ms = m * a.scale_log2;
-      float sum[4] = {};
+      const F2 scale = f2(a.scale_log2, a.scale_log2), shift = f2(-m * a.scale_log2, -m * a.scale_log2);
+      F2 sum[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         uint32_t p[32];
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const float p0 = ex2(fmaf(__uint_as_float(s[2 * half + c][i]), a.scale_log2, -ms));
-            const float p1 = ex2(fmaf(__uint_as_float(s[2 * half + c][i + 1]), a.scale_log2, -ms));
-            sum[(i >> 1) & 1] += p0;
-            sum[2 + ((i >> 1) & 1)] += p1;
-            p[c * 16 + i / 2] = pack_bf16(p0, p1);
-          }
+        for (int i = 0; i < 32; ++i) {
+          const F2 x = ex2_pair<4>(s[2 * half + i / 16][i % 16 * 2], s[2 * half + i / 16][i % 16 * 2 + 1], scale, shift, i);
+          sum[i & 1] = add2(sum[i & 1], x);
+          p[i] = f2_bf16(x);
+        }
         ptx::tmem_st_32x32(sp + half * 32, p);
         ptx::tmem_st_wait();
         ptx::tc_fence_before();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(p_full(t, half));
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      float lo, hi;
+      f2_split(add2(sum[0], sum[1]), lo, hi);
+      l += lo + hi;
     }
     if (ok && n_blocks > 0) ok = warp_wait(o_full(t), 0, abort_flag);
     if (ok && n_blocks > 0) {
@@ -486,8 +513,8 @@ __global__ void __launch_bounds__(kDeltaThreads) delta_kernel(const __nv_bfloat1
 }
 
 // ---------------------------------------------------------------- backward: dK and dV
-// A CTA has one tile of keys and works through the queries that see it, head by head of the group, so that dK and dV stay in tensor memory
-// and no sum needs an atomic.  Scores transposed (a row is a key): P^T and dS^T are the A operands of dV = P^T dO and dK = dS^T Q.
+// A CTA has one tile of keys and works through the queries that see it, head by head of the group (or of a part of it: dkv_parts), so that
+// dK and dV stay in tensor memory and no sum needs an atomic.  Scores transposed (a row is a key): P^T and dS^T are the A operands of dV = P^T dO and dK = dS^T Q.
 // Warps 0-7: elementwise, a thread has 64 of the 128 queries of a row; warp 8: TMA; warp 9: MMA; warp 10: lse and delta.
 // Order of products: S(0) dP(0) | dV(i) S(i+1) after P(i), dK(i) dP(i+1) after dS(i): exponentials are made while dK and dP run,
 // dS while dV and S do.
@@ -512,13 +539,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dkv_kernel(const __grid_consta
     return;
   }
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int hk = blockIdx.x % a.Hkv;
+  const int hk = blockIdx.x % a.Hkv, part = blockIdx.x / a.Hkv % a.parts;
   zero_gaps(a.seqs, a.dk, a.Hkv * a.D / 8, kBwdThreads);
   zero_gaps(a.seqs, a.dv, a.Hkv * a.D / 8, kBwdThreads);
-  const Work w = find_work<kBwdThreads>(a.seqs, blockIdx.x / a.Hkv, [](int tiles) { return tiles; });
+  const Work w = find_work<kBwdThreads>(a.seqs, blockIdx.x / (a.Hkv * a.parts), [](int tiles) { return tiles; });
   if (!w.any) return;
-  const int tiles = (w.len + kTile - 1) / kTile, key_tile = tiles - 1 - w.level, per_head = w.level + 1, n_it = per_head * a.G;
-  auto head_of = [&](int it) { return hk * a.G + it / per_head; };
+  const int head0 = part * a.G / a.parts, heads = (part + 1) * a.G / a.parts - head0;   // of the group
+  const int tiles = (w.len + kTile - 1) / kTile, key_tile = tiles - 1 - w.level, per_head = w.level + 1, n_it = per_head * heads;
+  auto head_of = [&](int it) { return hk * a.G + head0 + it / per_head; };
   auto tile_of = [&](int it) { return key_tile + it % per_head; };
 
   const uint32_t k_at = base, v_at = base + TB, ring = base + 2 * TB;   // [stage][Q, dO]
@@ -628,8 +656,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dkv_kernel(const __grid_consta
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int r = tile_of(it) * kTile + lane + 32 * i;
-        x[i] = r < w.len ? a.lse[at + r] : INFINITY;   // (behind the end: p = 0)
-        y[i] = r < w.len ? a.delta[at + r] : 0.f;
+        x[i] = r < w.len ? -a.lse[at + r] : -INFINITY;   // (behind the end: p = 0)
+        y[i] = r < w.len ? -a.delta[at + r] : 0.f;
       }
       ok = warp_wait(st_empty(s), (it / ST & 1) ^ 1u, abort_flag);
       if (!ok) break;
@@ -644,66 +672,57 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dkv_kernel(const __grid_consta
   } else {
     const int half = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+    const F2 scale = f2(a.scale_log2, a.scale_log2);
     bool ok = true;
     for (int it = 0; it < n_it; ++it) {
       const int s = it % ST;
       const bool diagonal = tile_of(it) == key_tile;
-      const float4* lse = reinterpret_cast<const float4*>(stats + s * 2 * kTile + half * 64);
-      const float4* delta = reinterpret_cast<const float4*>(stats + (s * 2 + 1) * kTile + half * 64);
+      const ulonglong2* lse = reinterpret_cast<const ulonglong2*>(stats + s * 2 * kTile + half * 64);   // (both negative, in pairs)
+      const ulonglong2* delta = reinterpret_cast<const ulonglong2*>(stats + (s * 2 + 1) * kTile + half * 64);
       ok = warp_wait(st_full(s), it / ST & 1, abort_flag) && warp_wait(s_full, it & 1, abort_flag);
       if (!ok) break;
       ptx::tc_fence_after();
-      float p[64];
-      {
-        uint32_t x[2][32], pk[32];
-        ptx::tmem_ld_32x32(t_s + lanes + half * 64, x[0]);
-        ptx::tmem_ld_32x32(t_s + lanes + half * 64 + 32, x[1]);
-        ptx::tmem_ld_wait();
+      F2 p[32];
+      uint32_t x[2][32], out[32];
+      ptx::tmem_ld_32x32(t_s + lanes + half * 64, x[0]);
+      ptx::tmem_ld_32x32(t_s + lanes + half * 64 + 32, x[1]);
+      ptx::tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 64; i += 4) {
-          const float4 e = lse[i / 4];
-          p[i] = ex2(fmaf(__uint_as_float(x[i / 32][i % 32]), a.scale_log2, -e.x));
-          p[i + 1] = ex2(fmaf(__uint_as_float(x[i / 32][i % 32 + 1]), a.scale_log2, -e.y));
-          p[i + 2] = ex2(fmaf(__uint_as_float(x[i / 32][i % 32 + 2]), a.scale_log2, -e.z));
-          p[i + 3] = ex2(fmaf(__uint_as_float(x[i / 32][i % 32 + 3]), a.scale_log2, -e.w));
-        }
-        if (diagonal) {
-#pragma unroll
-          for (int i = 0; i < 64; ++i)
-            if (half * 64 + i < row) p[i] = 0.f;
-        }
-#pragma unroll
-        for (int i = 0; i < 32; ++i) pk[i] = pack_bf16(p[2 * i], p[2 * i + 1]);
-        ptx::tmem_st_32x32(t_s + lanes + half * 64, pk);
-        ptx::tmem_st_wait();
-        ptx::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(p_ready);
+      for (int i = 0; i < 32; i += 2) {
+        const ulonglong2 e = lse[i / 2];
+        p[i] = ex2_pair<kBwdPoly<DP>>(x[i / 16][i % 16 * 2], x[i / 16][i % 16 * 2 + 1], scale, F2{e.x}, i);
+        p[i + 1] = ex2_pair<kBwdPoly<DP>>(x[i / 16][i % 16 * 2 + 2], x[i / 16][i % 16 * 2 + 3], scale, F2{e.y}, i + 1);
       }
+      if (diagonal) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) p[i] = hide(p[i], half * 64 + 2 * i < row, half * 64 + 2 * i + 1 < row);
+      }
+#pragma unroll
+      for (int i = 0; i < 32; ++i) out[i] = f2_bf16(p[i]);
+      ptx::tmem_st_32x32(t_s + lanes + half * 64, out);
+      ptx::tmem_st_wait();
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(p_ready);
       ok = warp_wait(dp_full, it & 1, abort_flag);
       if (!ok) break;
       ptx::tc_fence_after();
-      uint32_t ds[32];
+      ptx::tmem_ld_32x32(t_dp + lanes + half * 64, x[0]);
+      ptx::tmem_ld_32x32(t_dp + lanes + half * 64 + 32, x[1]);
+      ptx::tmem_ld_wait();
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t x[32];
-        ptx::tmem_ld_32x32(t_dp + lanes + half * 64 + c * 32, x);
-        ptx::tmem_ld_wait();
-#pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          const float4 e = delta[c * 8 + i / 4];
-          float d[4] = {p[c * 32 + i] * (__uint_as_float(x[i]) - e.x), p[c * 32 + i + 1] * (__uint_as_float(x[i + 1]) - e.y),
-                        p[c * 32 + i + 2] * (__uint_as_float(x[i + 2]) - e.z), p[c * 32 + i + 3] * (__uint_as_float(x[i + 3]) - e.w)};
-          if (diagonal) {   // (a pair that is masked adds nothing, whatever dP holds there)
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-              if (half * 64 + c * 32 + i + u < row) d[u] = 0.f;
-          }
-          ds[c * 16 + i / 2] = pack_bf16(d[0], d[1]);
-          ds[c * 16 + i / 2 + 1] = pack_bf16(d[2], d[3]);
-        }
+      for (int i = 0; i < 32; i += 2) {
+        const ulonglong2 e = delta[i / 2];
+        p[i] = mul2(p[i], add2(f2(__uint_as_float(x[i / 16][i % 16 * 2]), __uint_as_float(x[i / 16][i % 16 * 2 + 1])), F2{e.x}));
+        p[i + 1] = mul2(p[i + 1], add2(f2(__uint_as_float(x[i / 16][i % 16 * 2 + 2]), __uint_as_float(x[i / 16][i % 16 * 2 + 3])), F2{e.y}));
       }
-      ptx::tmem_st_32x32(t_dp + lanes + half * 64, ds);
+      if (diagonal) {   // (a pair that is masked adds nothing, whatever dP holds there)
+#pragma unroll
+        for (int i = 0; i < 32; ++i) p[i] = hide(p[i], half * 64 + 2 * i < row, half * 64 + 2 * i + 1 < row);
+      }
+#pragma unroll
+      for (int i = 0; i < 32; ++i) out[i] = f2_bf16(p[i]);
+      ptx::tmem_st_32x32(t_dp + lanes + half * 64, out);
       ptx::tmem_st_wait();
       ptx::tc_fence_before();
       __syncwarp();
@@ -716,16 +735,22 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dkv_kernel(const __grid_consta
     if (ok) {
       ptx::tc_fence_after();
       const int in_seq = key_tile * kTile + row;
-      const long long at = ((long long)(w.start + in_seq) * a.Hkv + hk) * a.D;
+      const long long at = ((long long)(w.start + in_seq) * a.Hkv + hk) * a.D, plane = (long long)a.seqs.T * a.Hkv * a.D;
 #pragma unroll 1
       for (int c = half * (DP / 2); c < (half + 1) * (DP / 2); c += 32) {
         uint32_t x[32];
         ptx::tmem_ld_32x32(t_dv + lanes + c, x);
         ptx::tmem_ld_wait();
-        if (in_seq < w.len) store_row32(a.dv + at + c, x, 1.f, a.D - c);
+        if (in_seq < w.len) {
+          if (a.parts == 1) store_row32(a.dv + at + c, x, 1.f, a.D - c);
+          else store_part32(a.sums + 2 * part * plane + at + c, x, 1.f, a.D - c);
+        }
         ptx::tmem_ld_32x32(t_dk + lanes + c, x);
         ptx::tmem_ld_wait();
-        if (in_seq < w.len) store_row32(a.dk + at + c, x, a.scale, a.D - c);
+        if (in_seq < w.len) {
+          if (a.parts == 1) store_row32(a.dk + at + c, x, a.scale, a.D - c);
+          else store_part32(a.sums + (2 * part + 1) * plane + at + c, x, a.scale, a.D - c);
+        }
       }
     }
   }
@@ -735,6 +760,26 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dkv_kernel(const __grid_consta
     ptx::tc_fence_after();
     ptx::tmem_dealloc(tmem, 512);
   }
+}
+
+// Adds up the parts, in their order; rows of no sequence have been zeroed and have no parts.
+constexpr int kSumThreads = 256;
+__global__ void __launch_bounds__(kSumThreads) dkv_sum_kernel(const Args a) {
+  const long long plane = (long long)a.seqs.T * a.Hkv * a.D, i = ((long long)blockIdx.x * kSumThreads + threadIdx.x) * 4;
+  if (i >= plane) return;
+  if (a.seqs.cu != nullptr) {
+    const int t = (int)(i / ((long long)a.Hkv * a.D));
+    if (t < a.seqs.cu[0] || t >= a.seqs.cu[a.seqs.n]) return;
+  }
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f), k = v;
+#pragma unroll 4
+  for (int p = 0; p < a.parts; ++p) {
+    const float4 x = *reinterpret_cast<const float4*>(a.sums + 2 * p * plane + i), y = *reinterpret_cast<const float4*>(a.sums + (2 * p + 1) * plane + i);
+    v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+    k.x += y.x; k.y += y.y; k.z += y.z; k.w += y.w;
+  }
+  *reinterpret_cast<uint2*>(a.dv + i) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+  *reinterpret_cast<uint2*>(a.dk + i) = make_uint2(pack_bf16(k.x, k.y), pack_bf16(k.z, k.w));
 }
 
 // ---------------------------------------------------------------- backward: dQ
@@ -855,40 +900,35 @@ __global__ void __launch_bounds__(kDqThreads, 1) dq_kernel(const __grid_constant
     const bool live = q_row + row < w.len;
     const long long at = (long long)head * a.seqs.T + w.start + q_row + row;
     const float lse = live ? a.lse[at] : INFINITY, delta = live ? a.delta[at] : 0.f;
+    const F2 scale = f2(a.scale_log2, a.scale_log2), shift = f2(-lse, -lse), minus_delta = f2(-delta, -delta);
     bool ok = true;
     for (int j = 0; j < nb; ++j) {
       const bool diagonal = j == nb - 1;
       ok = warp_wait(s_full(j & 1), j >> 1 & 1, abort_flag);
       if (!ok) break;
       ptx::tc_fence_after();
-      float p[64];
-      {
-        uint32_t x[2][32];
-        ptx::tmem_ld_32x32(t_s(j) + lanes + half * 64, x[0]);
-        ptx::tmem_ld_32x32(t_s(j) + lanes + half * 64 + 32, x[1]);
-        ptx::tmem_ld_wait();
+      F2 p[32];
+      uint32_t x[2][32], ds[32];
+      ptx::tmem_ld_32x32(t_s(j) + lanes + half * 64, x[0]);
+      ptx::tmem_ld_32x32(t_s(j) + lanes + half * 64 + 32, x[1]);
+      ptx::tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 64; ++i) p[i] = ex2(fmaf(__uint_as_float(x[i / 32][i % 32]), a.scale_log2, -lse));
-      }
+      for (int i = 0; i < 32; ++i) p[i] = ex2_pair<kBwdPoly<DP>>(x[i / 16][i % 16 * 2], x[i / 16][i % 16 * 2 + 1], scale, shift, i);
       ok = warp_wait(dp_full, j & 1, abort_flag);
       if (!ok) break;
       ptx::tc_fence_after();
-      uint32_t ds[32];
+      ptx::tmem_ld_32x32(t_dp + lanes + half * 64, x[0]);
+      ptx::tmem_ld_32x32(t_dp + lanes + half * 64 + 32, x[1]);
+      ptx::tmem_ld_wait();
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t x[32];
-        ptx::tmem_ld_32x32(t_dp + lanes + half * 64 + c * 32, x);
-        ptx::tmem_ld_wait();
+      for (int i = 0; i < 32; ++i)
+        p[i] = mul2(p[i], add2(f2(__uint_as_float(x[i / 16][i % 16 * 2]), __uint_as_float(x[i / 16][i % 16 * 2 + 1])), minus_delta));
+      if (diagonal) {
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          float d0 = p[c * 32 + i] * (__uint_as_float(x[i]) - delta), d1 = p[c * 32 + i + 1] * (__uint_as_float(x[i + 1]) - delta);
-          if (diagonal) {
-            if (half * 64 + c * 32 + i > row) d0 = 0.f;
-            if (half * 64 + c * 32 + i + 1 > row) d1 = 0.f;
-          }
-          ds[c * 16 + i / 2] = pack_bf16(d0, d1);
-        }
+        for (int i = 0; i < 32; ++i) p[i] = hide(p[i], half * 64 + 2 * i > row, half * 64 + 2 * i + 1 > row);
       }
+#pragma unroll
+      for (int i = 0; i < 32; ++i) ds[i] = f2_bf16(p[i]);
       ptx::tmem_st_32x32(t_s(j) + lanes + half * 64, ds);
       ptx::tmem_st_wait();
       ptx::tc_fence_before();
@@ -923,6 +963,13 @@ inline bool make_rows_map(CUtensorMap* m, const void* p, int T, int heads, int D
   const cuuint64_t strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)row * 2};
   const cuuint32_t box[3] = {64, 1, kTile};
   return encode_tiled(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, p, dims, strides, box);
+}
+
+// How many CTAs share the heads of a group for a tile of dK and dV.  A tile of the first keys of a long sequence has all its queries, times G
+// heads, so few key heads leave a few long runs: as many parts as make 2 CTAs per SM, at least one head each.
+inline int dkv_parts(long long tiles, int Hkv, int G) {
+  const long long want = 2ll * num_sms(), have = tiles * Hkv;
+  return (int)(have >= want ? 1 : (want + have - 1) / have < G ? (want + have - 1) / have : G);
 }
 
 // Units that `n` sequences of together T rows can have at most, `per` per tile and one to round up per sequence.

@@ -88,8 +88,13 @@ int attention_bwd(cudaStream_t st, const attn::Args& a, const CUtensorMap& tq, c
   if (a.dk != nullptr) {
     static bool done[64] = {false};
     if (!allow_smem(attn::dkv_kernel<DP>, attn::DkvShape<DP>::kSmem, done)) return LEWI_ERR_CUDA;
-    attn::dkv_kernel<DP><<<(unsigned)(tiles * a.Hkv), attn::kBwdThreads, attn::DkvShape<DP>::kSmem, st>>>(tq, tk, tv, td, a);
+    attn::dkv_kernel<DP><<<(unsigned)(tiles * a.Hkv * a.parts), attn::kBwdThreads, attn::DkvShape<DP>::kSmem, st>>>(tq, tk, tv, td, a);
     LEWI_CHECK_LAUNCH();
+    if (a.parts > 1) {
+      const long long vecs = (long long)a.seqs.T * a.Hkv * a.D / 4;
+      attn::dkv_sum_kernel<<<(unsigned)((vecs + attn::kSumThreads - 1) / attn::kSumThreads), attn::kSumThreads, 0, st>>>(a);
+      LEWI_CHECK_LAUNCH();
+    }
   }
   if (a.dq != nullptr) {
     static bool done[64] = {false};
@@ -99,6 +104,8 @@ int attention_bwd(cudaStream_t st, const attn::Args& a, const CUtensorMap& tq, c
   }
   return LEWI_OK;
 }
+
+inline int64_t delta_bytes(int T, int Hq) { return ((int64_t)T * Hq * 4 + 255) / 256 * 256; }
 
 inline int paged_ctas(int D) { return num_sms() * (D > 128 ? 1 : 2); }
 
@@ -202,13 +209,14 @@ int lewi_causal_attention_fwd(void* stream, const void* q, int64_t q_stride, con
       !attn::make_rows_map(&tv, v, T, Hkv, D, v_stride))
     return LEWI_ERR_CUDA;
   const attn::Args a{{cu_seqlens, n_seqs, T}, Hq, Hkv, Hq / Hkv, D, scale, scale * 1.4426950408889634f, reinterpret_cast<bf16*>(o), lse,
-                     nullptr, nullptr, nullptr, nullptr};
+                     nullptr, nullptr, nullptr, nullptr, 1, nullptr};
   return D <= 64 ? attention_fwd<64>(as_stream(stream), a, tq, tk, tv) : attention_fwd<128>(as_stream(stream), a, tq, tk, tv);
 }
 
-int64_t lewi_causal_attention_bwd_workspace_bytes(int T, int Hq) {
-  if (T <= 0 || Hq <= 0) return LEWI_ERR_ARG;
-  return (int64_t)T * Hq * 4;
+int64_t lewi_causal_attention_bwd_workspace_bytes(int T, int n_seqs, int Hq, int Hkv, int D) {
+  if (T <= 0 || n_seqs <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || Hq % Hkv != 0) return LEWI_ERR_ARG;
+  const int parts = attn::dkv_parts(attn::most_tiles(T, n_seqs), Hkv, Hq / Hkv);
+  return delta_bytes(T, Hq) + (parts > 1 ? (int64_t)parts * 2 * T * Hkv * D * 4 : 0);
 }
 
 int lewi_causal_attention_bwd(void* stream, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
@@ -217,14 +225,17 @@ int lewi_causal_attention_bwd(void* stream, const void* q, int64_t q_stride, con
   if (const int rc = check_attention(q, q_stride, k, k_stride, v, v_stride, cu_seqlens, n_seqs, o, lse, T, Hq, Hkv, D, scale)) return rc;
   if (!d_o || (!dq && !dk) || !dk != !dv) return LEWI_ERR_ARG;
   if (!aligned(d_o, 16) || !aligned(dq, 16) || !aligned(dk, 16) || !aligned(dv, 16)) return LEWI_ERR_SHAPE;
-  if (!workspace || !aligned(workspace, 4) || workspace_bytes < lewi_causal_attention_bwd_workspace_bytes(T, Hq)) return LEWI_ERR_WORKSPACE;
+  if (!workspace || !aligned(workspace, 16) || workspace_bytes < lewi_causal_attention_bwd_workspace_bytes(T, n_seqs, Hq, Hkv, D))
+    return LEWI_ERR_WORKSPACE;
   CUtensorMap tq, tk, tv, td;
   if (!attn::make_rows_map(&tq, q, T, Hq, D, q_stride) || !attn::make_rows_map(&tk, k, T, Hkv, D, k_stride) ||
       !attn::make_rows_map(&tv, v, T, Hkv, D, v_stride) || !attn::make_rows_map(&td, d_o, T, Hq, D, (int64_t)Hq * D))
     return LEWI_ERR_CUDA;
   const attn::Args a{{cu_seqlens, n_seqs, T}, Hq, Hkv, Hq / Hkv, D, scale, scale * 1.4426950408889634f,
                      const_cast<bf16*>(reinterpret_cast<const bf16*>(o)), const_cast<float*>(lse), reinterpret_cast<float*>(workspace),
-                     reinterpret_cast<bf16*>(dq), reinterpret_cast<bf16*>(dk), reinterpret_cast<bf16*>(dv)};
+                     reinterpret_cast<bf16*>(dq), reinterpret_cast<bf16*>(dk), reinterpret_cast<bf16*>(dv),
+                     attn::dkv_parts(attn::most_tiles(T, n_seqs), Hkv, Hq / Hkv),
+                     reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(workspace) + delta_bytes(T, Hq))};
   const bf16* g = reinterpret_cast<const bf16*>(d_o);
   return D <= 64 ? attention_bwd<64>(as_stream(stream), a, tq, tk, tv, td, g) : attention_bwd<128>(as_stream(stream), a, tq, tk, tv, td, g);
 }

@@ -12,6 +12,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "f32x2.cuh"
 #include "gather.cuh"
 #include "tcgen05.cuh"
 
@@ -88,33 +89,12 @@ __global__ void __launch_bounds__(kConvThreads) causal_conv1d_kernel(const __nv_
   }
 }
 
-// Two floats side by side (fma.rn.f32x2: each half rounded as a single fma).
-struct F2 {
-  unsigned long long v;
-};
-__device__ __forceinline__ F2 f2(float lo, float hi) {
-  F2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ void f2_split(F2 a, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(a.v)); }
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
 __device__ __forceinline__ void unpack2(uint4 v, F2 (&f)[4]) {
   f[0] = f2(bf16_lo(v.x), bf16_hi(v.x));
   f[1] = f2(bf16_lo(v.y), bf16_hi(v.y));
   f[2] = f2(bf16_lo(v.z), bf16_hi(v.z));
   f[3] = f2(bf16_lo(v.w), bf16_hi(v.w));
 }
-__device__ __forceinline__ uint32_t f2_bf16(F2 a) {
-  float lo, hi;
-  f2_split(a, lo, hi);
-  return pack_bf16(lo, hi);
-}
-
 // Both gradients in one pass over g: with the window g[t] .. g[t+K-1] in registers, dx[t] is its product with the taps and
 // x[t] times the window is what x[t] adds to dw (dw[j] = sum_t x[t] * g[t+(K-1)-j]).  A warp takes 32 channel vectors of one
 // run; the CTA adds up its warps' dw and leaves partial[(b * gridDim.y + blockIdx.y), j, c].

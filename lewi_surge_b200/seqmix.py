@@ -112,6 +112,9 @@ def chunk_gated_delta_rule(query, key, value, g, beta, chunk_size=64, initial_st
   return o, (hf.to(torch.bfloat16) if initial_state is not None else None)
 
 
+_GATES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
+
+
 def _check_slots(what, b, state, slots):
   if slots is None and state.shape[0] < b:
     raise LewiError(f"{what}: {b} rows and no slots, but {state.shape[0]} states")
@@ -133,14 +136,17 @@ def causal_conv1d_step(x, w, state, slots=None):
   if state.dim() != 3 or state.shape[1:] != (k - 1, c):
     raise LewiError("causal_conv1d_step: state [N,K-1,C] is required")
   _check_slots("causal_conv1d_step", b, state, slots)
-  with torch.no_grad(), _lib.one_device(x, w, state, slots):
-    x, x_rows = _lib.rows_of(x, 16)
-    w = w.to(torch.bfloat16).contiguous()
-    slots = _lib.index_table(slots, "slots")
-    y = torch.empty((b, c), dtype=torch.bfloat16, device=x.device)
-    if b > 0:
-      check(lib.lewi_causal_conv1d_step(stream(), x.data_ptr(), x_rows, ptr(w), ptr(state), ptr(slots), ptr(y), b, state.shape[0], c, k),
-            "lewi_causal_conv1d_step")
+  if _lib.elsewhere(x, w, state, slots):
+    with torch.cuda.device(x.device):
+      return causal_conv1d_step(x, w, state, slots)
+  x, x_rows = _lib.rows_of(x, 16)
+  if w.dtype is not torch.bfloat16 or not w.is_contiguous():
+    w = w.detach().to(torch.bfloat16).contiguous()
+  slots = _lib.index_table(slots, "slots")
+  y = torch.empty((b, c), dtype=torch.bfloat16, device=x.device)
+  if b > 0:
+    check(lib.lewi_causal_conv1d_step(stream(), x.data_ptr(), x_rows, ptr(w), ptr(state), ptr(slots), y.data_ptr(), b, state.shape[0], c, k),
+          "lewi_causal_conv1d_step")
   return y
 
 
@@ -152,7 +158,7 @@ def gated_delta_step(query, key, value, g, beta, state, slots=None):
   Rows of the batch may lie apart (views of one projection need no copy).  Not differentiable.  Everything is float32 inside, where
   `chunk_gated_delta_rule` rounds some products to bf16 as the reference does, so the two agree to bf16's precision."""
   lib = _lib.load()
-  if any(t.dtype != torch.bfloat16 for t in (query, key, value)) or state.dtype != torch.float32:
+  if not query.dtype == key.dtype == value.dtype == torch.bfloat16 or state.dtype != torch.float32:
     raise LewiError("gated_delta_step takes bfloat16 q, k, v and a float32 state")
   if query.dim() != 3 or key.shape != query.shape or value.dim() != 3 or value.shape[0] != query.shape[0]:
     raise LewiError("gated_delta_step: query, key [B,Hk,K] and value [B,H,V] are required")
@@ -162,14 +168,15 @@ def gated_delta_step(query, key, value, g, beta, state, slots=None):
   if g.shape != (b, h) or beta.shape != (b, h):
     raise LewiError("gated_delta_step: g and beta [B,H] are required")
   _check_slots("gated_delta_step", b, state, slots)
-  dt = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
-  if g.dtype not in dt or beta.dtype not in dt:
+  if g.dtype not in _GATES or beta.dtype not in _GATES:
     raise LewiError("gated_delta_step takes float32 or bfloat16 g and beta")
-  with torch.no_grad(), _lib.one_device(query, key, value, g, beta, state, slots):
-    (q, qs), (k, ks), (v, vs) = (_lib.rows_of(t, 2) for t in (query, key, value))
-    g, beta, slots = g.contiguous(), beta.contiguous(), _lib.index_table(slots, "slots")
-    o = torch.empty((b, h, vd), dtype=torch.bfloat16, device=q.device)
-    if b > 0:
-      check(lib.lewi_gdn_step(stream(), q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, ptr(g), dt[g.dtype], ptr(beta), dt[beta.dtype],
-                              ptr(state), ptr(slots), ptr(o), b, state.shape[0], hk, h, kd, vd), "lewi_gdn_step")
+  if _lib.elsewhere(query, key, value, g, beta, state, slots):
+    with torch.cuda.device(query.device):
+      return gated_delta_step(query, key, value, g, beta, state, slots)
+  (q, qs), (k, ks), (v, vs) = _lib.rows_of(query, 2), _lib.rows_of(key, 2), _lib.rows_of(value, 2)
+  g, beta, slots = g.contiguous(), beta.contiguous(), _lib.index_table(slots, "slots")
+  o = torch.empty((b, h, vd), dtype=torch.bfloat16, device=q.device)
+  if b > 0:
+    check(lib.lewi_gdn_step(stream(), q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, g.data_ptr(), _GATES[g.dtype], beta.data_ptr(),
+                            _GATES[beta.dtype], ptr(state), ptr(slots), o.data_ptr(), b, state.shape[0], hk, h, kd, vd), "lewi_gdn_step")
   return o
