@@ -38,99 +38,97 @@ __device__ __forceinline__ Rows rows_of(const Seqs& q, int s) {
   return {lo, hi - lo};
 }
 
-struct Work {
-  int start, len, level;   // the sequence's rows; level < its number of units
-  bool any;
+// What a CTA works on: unit `level` of the sequence at rows start .. start + len, `sub` of the unit's shares.  level < 0: nothing is left.
+struct Item {
+  int start, len, level, sub;
 };
 
-// The x-th unit of work in the order of falling levels, where sequence s has the levels 0 .. units(tiles of s) - 1 and a level's work
-// grows with it: long runs first, whatever the lengths, without a table.  F(i) = sum_s max(0, units - i) counts the units of level i and
-// above; the level is the largest i with F(i) > x, and the sequence the (x - F(i + 1))-th of those that have it.  All threads call it.
-template <int THREADS, class U>
-__device__ __forceinline__ Work find_work(const Seqs& q, int x, U units) {
-  constexpr int WARPS = THREADS / 32;
-  __shared__ int s_part[2][WARPS];
-  __shared__ int s_hit;
-  if (q.cu == nullptr) {
-    const int len = q.T / q.n, u = units((len + kTile - 1) / kTile), level = u - 1 - x / q.n;
-    return {len * (x % q.n), len, level, level >= 0};
-  }
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  auto units_of = [&](int s) { return units((rows_of(q, s).len + kTile - 1) / kTile); };
-  if (q.n == 1) {
-    const Rows r = rows_of(q, 0);
-    const int level = units((r.len + kTile - 1) / kTile) - 1 - x;
-    return {r.start, r.len, level, level >= 0};
-  }
-  if (q.n <= 32) {   // a sequence per lane, every warp for itself
-    const int u = lane < q.n ? units_of(lane) : 0;
-    auto count = [&](int i) { return __reduce_add_sync(0xffffffffu, max(0, u - i)); };
-    if (count(0) <= x) return {0, 0, 0, false};
-    int lo = 0, hi = __reduce_max_sync(0xffffffffu, u);   // F(lo) > x, F(hi) = 0
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (count(mid) > x) lo = mid;
-      else hi = mid;
+// The kernels run one CTA per SM, which takes items until none is left; a warp of its own looks the next one up while the others work.
+// Sequence s has the units 0 .. units(s) - 1 of `rows` rows, a unit's work grows with its number, and every unit has `subs` equal shares.
+// Items are numbered by falling unit, all shares of a unit together, and CTA c has the items c, 2 n - 1 - c, 2 n + c, 4 n - 1 - c, .. of n
+// CTAs: long runs first, and about as much work for everybody, whatever the lengths.  No table is needed: F(i) = sum_s max(0, units(s) - i)
+// counts the units from number i on, so the x-th unit's number is the largest i with F(i) > x, and its sequence is the
+// (x - F(i + 1))-th of those that have it.
+constexpr int kPlanned = 448;   // sequences whose units are kept in shared memory (further ones are looked up again)
+struct Plan {
+  int4 item[2];
+  int units[kPlanned];
+};
+
+// The whole warp calls it; `give` hands an item on and tells whether to go on.
+template <class Give>
+__device__ __forceinline__ void plan_items(const Seqs& q, int rows, int subs, Plan& plan, Give give) {
+  const int lane = threadIdx.x & 31, n = gridDim.x, c = blockIdx.x;
+  auto unit_count = [&](int s) { return (rows_of(q, s).len + rows - 1) / rows; };
+  const bool alike = q.cu == nullptr, kept = q.n <= kPlanned;
+  int most = 0;   // a sequence's units
+  if (alike) {
+    most = unit_count(0);
+  } else {
+    for (int s = lane; s < q.n; s += 32) {
+      const int u = unit_count(s);
+      if (kept) plan.units[s] = u;
+      most = max(most, u);
     }
-    unsigned have = __ballot_sync(0xffffffffu, u > lo);
-    for (int r = x - count(lo + 1); r > 0; --r) have &= have - 1;
-    const Rows r = rows_of(q, __ffs(have) - 1);
-    return {r.start, r.len, lo, true};
+    most = __reduce_max_sync(0xffffffffu, most);
+    __syncwarp();
   }
-  // runs of sequences per thread
-  const int per = (q.n + THREADS - 1) / THREADS, s0 = min(q.n, (int)threadIdx.x * per), s1 = min(q.n, s0 + per);
-  int flip = 0;
-  auto block_sum = [&](int v) {
-    const int w = __reduce_add_sync(0xffffffffu, v);
-    if (lane == 0) s_part[flip][warp] = w;
-    __syncthreads();
-    int sum = 0;
-    for (int i = 0; i < WARPS; ++i) sum += s_part[flip][i];
-    flip ^= 1;
-    return sum;
-  };
-  auto mine = [&](int i) {
+  auto units = [&](int s) { return kept ? plan.units[s] : unit_count(s); };
+  auto count = [&](int i) {
     int v = 0;
-    for (int s = s0; s < s1; ++s) v += max(0, units_of(s) - i);
-    return v;
+    for (int s = lane; s < q.n; s += 32) v += max(0, units(s) - i);
+    return __reduce_add_sync(0xffffffffu, v);
   };
-  if (block_sum(mine(0)) <= x) return {0, 0, 0, false};
-  int lo = 0, hi = units((q.T + kTile - 1) / kTile) + 1;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (block_sum(mine(mid)) > x) lo = mid;
-    else hi = mid;
+  const int all = alike ? most * q.n : count(0);
+  int top = most;   // F(top) <= the next x
+  for (int r = 0;; ++r) {
+    const long long id = (long long)r * n + ((r & 1) != 0 ? n - 1 - c : c);
+    const int x = (int)min(id / subs, 0x7fffffffll);
+    Item item{0, 0, -1, 0};
+    if (x < all) {
+      item.sub = (int)(id % subs);
+      int s, lo = 0;
+      if (alike) {
+        lo = most - 1 - x / q.n;
+        s = x % q.n;
+      } else {
+        int hi = top;   // F(lo) > x, F(hi) <= x
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (count(mid) > x) lo = mid;
+          else hi = mid;
+        }
+        int rank = x - count(lo + 1);
+        top = lo + 1;
+        s = 0;
+        for (int s0 = 0; s0 < q.n; s0 += 32) {
+          unsigned have = __ballot_sync(0xffffffffu, s0 + lane < q.n && units(min(s0 + lane, q.n - 1)) > lo);
+          if (rank >= __popc(have)) {
+            rank -= __popc(have);
+            continue;
+          }
+          for (; rank > 0; --rank) have &= have - 1;
+          s = s0 + __ffs(have) - 1;
+          break;
+        }
+      }
+      const Rows of = rows_of(q, s);
+      item.start = of.start;
+      item.len = of.len;
+      item.level = lo;
+    }
+    if (!give(r, item) || item.level < 0) return;
   }
-  int rank = x - block_sum(mine(lo + 1)), have = 0;
-  for (int s = s0; s < s1; ++s) have += units_of(s) > lo;
-  int upto = have;   // of this warp's threads up to this one
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += v;
-  }
-  if (lane == 31) s_part[flip][warp] = upto;
-  if (threadIdx.x == 0) s_hit = 0;
-  __syncthreads();
-  for (int i = 0; i < warp; ++i) upto += s_part[flip][i];
-  if (rank >= upto - have && rank < upto) {
-    rank -= upto - have;
-    for (int s = s0; s < s1; ++s)
-      if (units_of(s) > lo && rank-- == 0) s_hit = s;
-  }
-  __syncthreads();
-  const Rows r = rows_of(q, s_hit);
-  return {r.start, r.len, lo, true};
 }
 
-// Rows of no sequence become zero: a share of them for every CTA, `vecs` 16-byte pieces each.
-__device__ __forceinline__ void zero_gaps(const Seqs& q, __nv_bfloat16* out, int vecs, int threads) {
-  if (q.cu == nullptr || threadIdx.x >= threads) return;
-  const int first = min(max(q.cu[0], 0), q.T), end = min(max(q.cu[q.n], 0), q.T);
+// Rows of no sequence become zero: a share of them for every CTA, by one warp; `vecs` 16-byte pieces each.
+__device__ __forceinline__ void zero_gaps(const Seqs& q, __nv_bfloat16* out, int vecs) {
+  if (q.cu == nullptr) return;
+  const int lane = threadIdx.x & 31, first = min(max(q.cu[0], 0), q.T), end = min(max(q.cu[q.n], 0), q.T);
   for (int r = blockIdx.x; r < q.T; r += gridDim.x) {
     if (r >= first && r < end) r += (end - r + gridDim.x - 1) / gridDim.x * gridDim.x;
     if (r >= q.T) break;
-    for (int i = threadIdx.x; i < vecs; i += threads) st_v4(out + ((long long)r * vecs + i) * 8, make_uint4(0u, 0u, 0u, 0u));
+    for (int i = lane; i < vecs; i += 32) st_v4(out + ((long long)r * vecs + i) * 8, make_uint4(0u, 0u, 0u, 0u));
   }
 }
 
@@ -188,20 +186,21 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
   return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity, abort_flag));
 }
 
-// What a warp that brings tiles does for one of them.  `valid` rows belong to the sequence; the others are zeroed once the copy has
-// landed (on a barrier of the warp's own), and the tile is handed on after that.
+// A tile reaches into rows that are not its sequence's where `valid` < 128.  Such a tile lands on a barrier of its own (`raw`), and another warp
+// zeroes the foreign rows and hands the tile on (`mend_tile`), so that the warp that brings tiles waits for none of them (doing both
+// itself it took 1.4 us per such tile, and of short sequences every other tile is one).
 template <int DP>
-__device__ __forceinline__ bool bring_tile(uint32_t dst, const CUtensorMap* tm, uint32_t full, uint32_t raw, uint32_t& raw_phase, int head, int row,
-                                           int valid, volatile int* abort_flag) {
-  const bool whole = valid >= kTile;
+__device__ __forceinline__ void bring_tile(uint32_t dst, const CUtensorMap* tm, uint32_t full, uint32_t raw, int head, int row, int valid) {
   if (ptx::elect_one()) {
-    ptx::mbar_expect_tx(whole ? full : raw, kTileBytes<DP>);
-    load_tile<DP>(dst, tm, whole ? full : raw, head, row);
+    const uint32_t bar = valid >= kTile ? full : raw;
+    ptx::mbar_expect_tx(bar, kTileBytes<DP>);
+    load_tile<DP>(dst, tm, bar, head, row);
   }
   __syncwarp();
-  if (whole) return true;
-  if (!warp_wait(raw, raw_phase, abort_flag)) return false;
-  raw_phase ^= 1u;
+}
+template <int DP>
+__device__ __forceinline__ bool mend_tile(uint32_t dst, uint32_t full, uint32_t raw, uint32_t phase, int valid, volatile int* abort_flag) {
+  if (!warp_wait(raw, phase & 1u, abort_flag)) return false;
   for (int i = (threadIdx.x & 31); i < (kTile - valid) * (DP / 8); i += 32) {
     const uint32_t at = dst + (i & 7) * 16 + ((i >> 3) / (kTile - valid)) * kBox + (valid + (i >> 3) % (kTile - valid)) * 128;
     asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0u) : "memory");
@@ -230,35 +229,89 @@ struct Args {
   float* sums;             // [part][dV, dK][T][Hkv][D] where there are several
 };
 
-__device__ __forceinline__ void store_row32(__nv_bfloat16* dst, const uint32_t (&v)[32], float f, int cols) {
+// A warp's 32 rows x 64 bytes go through shared memory (2 KB of its own), so that a store writes 8 rows x 64 bytes and not a piece of each of
+// 32 rows (which took 3700 cycles for a tile of 128 x 128 bf16).  `v`: this lane's row; rows dst + r * stride for r < valid, `bytes` of the 64.
+constexpr int kStaging = 8 * 2048, kBarriers = 384;
+__device__ __forceinline__ void store_rows(uint8_t* stage, const uint32_t (&v)[16], uint8_t* dst, long long stride, int valid, int bytes) {
+  const int lane = threadIdx.x & 31;
+  uint4* mine = reinterpret_cast<uint4*>(stage) + lane * 4;
+  __syncwarp();   // (what was there has been read)
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (i * 8 < cols)
-      st_v4(dst + i * 8, make_uint4(pack_bf16(__uint_as_float(v[8 * i]) * f, __uint_as_float(v[8 * i + 1]) * f),
-                                    pack_bf16(__uint_as_float(v[8 * i + 2]) * f, __uint_as_float(v[8 * i + 3]) * f),
-                                    pack_bf16(__uint_as_float(v[8 * i + 4]) * f, __uint_as_float(v[8 * i + 5]) * f),
-                                    pack_bf16(__uint_as_float(v[8 * i + 6]) * f, __uint_as_float(v[8 * i + 7]) * f)));
+  for (int i = 0; i < 4; ++i) mine[i ^ (lane >> 1 & 3)] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = i * 8 + (lane >> 2), piece = lane & 3;
+    const uint4 x = reinterpret_cast<const uint4*>(stage)[row * 4 + (piece ^ (row >> 1 & 3))];
+    if (row < valid && piece * 16 < bytes) st_v4(dst + row * stride + piece * 16, x);
+  }
+}
+// 32 accumulator columns as bf16 / 16 of them as float32
+__device__ __forceinline__ void pack_row(uint32_t (&out)[16], const uint32_t (&v)[32], float f) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) out[i] = pack_bf16(__uint_as_float(v[2 * i]) * f, __uint_as_float(v[2 * i + 1]) * f);
+}
+__device__ __forceinline__ void half_row(uint32_t (&out)[16], const uint32_t (&v)[32], int half, float f) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) out[i] = __float_as_uint(__uint_as_float(v[16 * half + i]) * f);
 }
 
-__device__ __forceinline__ void store_part32(float* dst, const uint32_t (&v)[32], float f, int cols) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (i * 4 < cols)
-      *reinterpret_cast<float4*>(dst + i * 4) = make_float4(__uint_as_float(v[4 * i]) * f, __uint_as_float(v[4 * i + 1]) * f,
-                                                            __uint_as_float(v[4 * i + 2]) * f, __uint_as_float(v[4 * i + 3]) * f);
-}
+// What the roles of a kernel share: barriers of the items, the planning warp's loop, and how a warp or a thread takes an item.
+struct ItemQueue {
+  Plan* plan;
+  uint32_t bars;   // full[2], empty[2]
+  volatile int* abort_flag;
+  __device__ __forceinline__ void init(int readers) const {
+    for (int s = 0; s < 2; ++s) {
+      ptx::mbar_init(bars + 8u * s, 1);
+      ptx::mbar_init(bars + 16u + 8u * s, readers);
+    }
+  }
+  __device__ __forceinline__ void run(const Seqs& seqs, int rows, int subs) const {
+    plan_items(seqs, rows, subs, *plan, [&](int r, const Item& item) {
+      if (!warp_wait(bars + 16u + 8u * (r & 1), (r >> 1 & 1) ^ 1u, abort_flag)) return false;
+      if ((threadIdx.x & 31) == 0) {
+        plan->item[r & 1] = make_int4(item.start, item.len, item.level, item.sub);
+        ptx::mbar_arrive(bars + 8u * (r & 1));
+      }
+      __syncwarp();
+      return true;
+    });
+  }
+  __device__ __forceinline__ Item read(int r) const {
+    const volatile int4& v = plan->item[r & 1];
+    return {v.x, v.y, v.z, v.w};
+  }
+  // by a whole warp; level < 0 also where a wait ran out
+  __device__ __forceinline__ Item take(int r) const {
+    if (!warp_wait(bars + 8u * (r & 1), r >> 1 & 1, abort_flag)) return {0, 0, -1, 0};
+    const Item item = read(r);
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(bars + 16u + 8u * (r & 1));
+    return item;
+  }
+  // by one thread
+  __device__ __forceinline__ Item take_alone(int r) const {
+    if (!ptx::mbar_wait(bars + 8u * (r & 1), r >> 1 & 1, abort_flag)) return {0, 0, -1, 0};
+    const Item item = read(r);
+    ptx::mbar_arrive(bars + 16u + 8u * (r & 1));
+    return item;
+  }
+};
 
 // ---------------------------------------------------------------- forward
-// A CTA works on two tiles of queries that share their keys (two heads, or two tiles of one head): while one tile's softmax is made by its
-// four warps, the tensor cores multiply for the other, and every key and value tile that is brought serves both.  Warps 0-3 and 4-7: a
-// row of S per thread; warp 8: TMA; warp 9: MMA.  Products are issued in the order S0(j+1) after P0 V(j), S1(j+1) after P1 V(j): a
-// softmax that finds its scores knows that the product before them is done, so it may scale O then.  It does so only where the
-// maximum has grown by more than 8 (in powers of 2; p stays below 2^8, which bf16 and float32 hold as well as 1).
-constexpr int kFwdThreads = 384;   // (warps 10 and 11 have nothing to do: registers move between warpgroups of four warps)
+// A CTA works on two tiles of queries that share their keys: two heads of a group, or, where a group is odd, the tiles 2 u and 2 u + 1 of one
+// head.  While one tile's softmax is made by its four warps, the tensor cores multiply for the other, and every key and value tile
+// that is brought serves both.  Warps 0-3 and 4-7: a row of S per thread; warp 8: TMA; warp 9: MMA; warp 10: items; warp 11: rows of no
+// sequence, and those of other sequences in a tile.  Products are issued in the order S0(j+1) after P0 V(j), S1(j+1) after P1 V(j): a softmax that finds its scores knows that the
+// product before them is done, so it may scale O then.  It does so only where the maximum has grown by more than 8 (in powers of 2; p
+// stays below 2^8, which bf16 and float32 hold as well as 1).  The next item's queries, first keys and scores are on their way while O
+// of this one is written out.
+constexpr int kFwdThreads = 384;
 template <int DP>
 struct FwdShape {
-  static constexpr int kStages = DP == 64 ? 6 : 5;
-  static constexpr int kSmem = 2 * kTileBytes<DP> + kStages * kTileBytes<DP> + 256;
+  static constexpr int kStages = DP == 64 ? 6 : 4;
+  static constexpr int kSmem = (2 + kStages) * kTileBytes<DP> + kStaging + kBarriers;
 };
 
 template <int DP>
@@ -268,50 +321,34 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
   extern __shared__ __align__(1024) uint8_t attn_smem[];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
+  __shared__ Plan s_plan;
   const uint32_t base = ptx::smem_u32(attn_smem);
   if ((base & 1023u) != 0) {
     if (threadIdx.x == 0) raise_status(LEWI_STATUS_SMEM_LAYOUT);
     return;
   }
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int hk = blockIdx.x % a.Hkv;
-  zero_gaps(a.seqs, a.o, a.Hq * a.D / 8, kFwdThreads);
-  const Work w = find_work<kFwdThreads>(a.seqs, blockIdx.x / a.Hkv, [&](int tiles) { return (tiles * a.G + 1) / 2; });
-  if (!w.any) return;
-  // the two tiles: units 2 level and 2 level + 1 of the sequence's tiles x heads
-  const int tiles = (w.len + kTile - 1) / kTile;
-  int tile[2], head[2], blocks[2];
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const int u = 2 * w.level + t;
-    tile[t] = u / a.G;
-    head[t] = hk * a.G + u % a.G;
-    blocks[t] = tile[t] < tiles ? tile[t] + 1 : 0;
-  }
-  const int nb = max(blocks[0], blocks[1]);
-
-  const uint32_t kv = base + 2 * TB, bars = kv + ST * TB;
-  auto full = [&](int s) { return bars + 8u * s; };
-  auto empty = [&](int s) { return bars + 8u * (ST + s); };
+  const uint32_t kv = base + 2 * TB, bars = kv + ST * TB + kStaging;
+  auto full = [&](int n) { return bars + 8u * (n % ST); };
+  auto empty = [&](int n) { return bars + 8u * (ST + n % ST); };
   auto q_full = [&](int t) { return bars + 8u * (2 * ST + t); };
-  auto s_full = [&](int t) { return bars + 8u * (2 * ST + 2 + t); };
-  auto p_full = [&](int t, int half) { return bars + 8u * (2 * ST + 4 + 2 * t + half); };
-  auto o_full = [&](int t) { return bars + 8u * (2 * ST + 8 + t); };
-  const uint32_t raw = bars + 8u * (2 * ST + 10);
+  auto q_empty = [&](int t) { return bars + 8u * (2 * ST + 2 + t); };
+  auto s_full = [&](int t) { return bars + 8u * (2 * ST + 4 + t); };
+  auto p_full = [&](int t, int half) { return bars + 8u * (2 * ST + 6 + 2 * t + half); };
+  auto o_full = [&](int t) { return bars + 8u * (2 * ST + 10 + t); };
+  auto o_empty = [&](int t) { return bars + 8u * (2 * ST + 12 + t); };
+  auto raw = [&](int n) { return bars + 8u * (2 * ST + 14 + n % ST); };
   volatile int* abort_flag = &s_abort;
+  const ItemQueue items{&s_plan, bars + 8u * (3 * ST + 14), abort_flag};
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) {
-      ptx::mbar_init(full(s), 1);
-      ptx::mbar_init(empty(s), 1);
+      for (uint32_t b : {full(s), empty(s), raw(s)}) ptx::mbar_init(b, 1);
     }
     for (int t = 0; t < 2; ++t) {
-      ptx::mbar_init(q_full(t), 1);
-      ptx::mbar_init(s_full(t), 1);
-      ptx::mbar_init(p_full(t, 0), 4);
-      ptx::mbar_init(p_full(t, 1), 4);
-      ptx::mbar_init(o_full(t), 1);
+      for (uint32_t b : {q_full(t), q_empty(t), s_full(t), o_full(t)}) ptx::mbar_init(b, 1);
+      for (uint32_t b : {p_full(t, 0), p_full(t, 1), o_empty(t)}) ptx::mbar_init(b, 4);
     }
-    ptx::mbar_init(raw, 1);
+    items.init(11);
     s_abort = 0;
     ptx::mbar_fence_init();
     ptx::fence_proxy_async();
@@ -329,157 +366,211 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
   const uint32_t tmem = s_tmem;
   auto s_at = [&](int t) { return tmem + t * 128; };
   auto o_at = [&](int t) { return tmem + 256 + t * 128; };
+  const bool two_heads = a.G % 2 == 0;
+  auto tile_of = [&](const Item& w, int t) { return two_heads ? w.level : 2 * w.level + t; };
+  auto head_of = [&](const Item& w, int t) { return two_heads ? 2 * w.sub + t : w.sub; };
+  auto blocks_of = [&](const Item& w, int t) { return tile_of(w, t) * kTile < w.len ? tile_of(w, t) + 1 : 0; };
 
   // registers: 8 x 216 + 4 x 72 = 12 x 168 a thread, what the launch has
   if (warp >= 8) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-  if (warp == 8) {
-    // ---------------------------------------------------------------- queries, then K0, V0, K1, V1, ..
-    bool ok = true;
-    if (ptx::elect_one()) {
-      for (int t = 0; t < 2; ++t)
-        if (blocks[t] > 0) {
-          ptx::mbar_expect_tx(q_full(t), TB);
-          load_tile<DP>(base + t * TB, &tm_q, q_full(t), head[t], w.start + tile[t] * kTile);
-        }
-    }
-    __syncwarp();
-    uint32_t raw_phase = 0;
-    for (int n = 0; ok && n < 2 * nb; ++n) {
-      const int s = n % ST, j = n >> 1;
-      ok = warp_wait(empty(s), (n / ST & 1) ^ 1u, abort_flag);
-      if (!ok) break;
-      const int valid = (n & 1) != 0 ? w.len - j * kTile : kTile;   // (of K a foreign row only reaches scores that are masked)
-      ok = bring_tile<DP>(kv + s * TB, (n & 1) != 0 ? &tm_v : &tm_k, full(s), raw, raw_phase, hk, w.start + j * kTile, valid, abort_flag);
-    }
-    if (!ok) settle();
-  } else if (warp == 9) {
-    // ---------------------------------------------------------------- products
-    const uint32_t id_s = ptx::instr_desc_bf16(128, 128, 0, 0), id_o = ptx::instr_desc_bf16(128, DP, 0, 1);
-    if (ptx::elect_one()) {
-      bool ok = ptx::mbar_wait(full(0), 0, abort_flag);
-      auto scores = [&](int t, int s) {
-        ptx::tc_fence_after();
-        mma_kk<DP>(s_at(t), base + t * TB, kv + s * TB, id_s);
-        ptx::mma_commit(s_full(t));
-      };
-      for (int t = 0; ok && t < 2; ++t)
-        if (blocks[t] > 0) {
-          ok = ptx::mbar_wait(q_full(t), 0, abort_flag);
-          if (ok) scores(t, 0);
-        }
-      if (ok) ptx::mma_commit(empty(0));
-      for (int j = 0; ok && j < nb; ++j) {
-        const int nv = 2 * j + 1, nk = nv + 1, sv = nv % ST, sk = nk % ST;
-        ok = ptx::mbar_wait(full(sv), nv / ST & 1, abort_flag);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 8) {
+      // ---------------------------------------------------------------- queries, then K0, V0, K1, V1, ..
+      bool ok = true;
+      int n = 0, used[2] = {0, 0};
+      for (int r = 0; ok; ++r) {
+        const Item w = items.take(r);
+        if (w.level < 0) break;
+        const int hk = head_of(w, 0) / a.G, nb = max(blocks_of(w, 0), blocks_of(w, 1));
         for (int t = 0; ok && t < 2; ++t) {
-          if (j >= blocks[t]) continue;
-          ok = ptx::mbar_wait(p_full(t, 0), j & 1, abort_flag);
-          if (!ok) break;
-          ptx::tc_fence_after();
-          mma_tm<0, 4>(o_at(t), s_at(t), kv + sv * TB, id_o, j > 0, 32);
-          ok = ptx::mbar_wait(p_full(t, 1), j & 1, abort_flag);
-          if (!ok) break;
-          ptx::tc_fence_after();
-          mma_tm<4, 8>(o_at(t), s_at(t), kv + sv * TB, id_o, true, 32);
-          if (j + 1 < blocks[t]) {
-            ok = ptx::mbar_wait(full(sk), nk / ST & 1, abort_flag);
-            if (ok) scores(t, sk);
-          } else {
-            ptx::mma_commit(o_full(t));
+          if (blocks_of(w, t) == 0) continue;
+          ok = warp_wait(q_empty(t), (used[t] & 1) ^ 1u, abort_flag);
+          ++used[t];
+          if (ok && ptx::elect_one()) {
+            ptx::mbar_expect_tx(q_full(t), TB);
+            load_tile<DP>(base + t * TB, &tm_q, q_full(t), head_of(w, t), w.start + tile_of(w, t) * kTile);
           }
+          __syncwarp();
         }
-        if (!ok) break;
-        ptx::mma_commit(empty(sv));
-        if (j + 1 < nb) ptx::mma_commit(empty(sk));
+        for (int i = 0; ok && i < 2 * nb; ++i, ++n) {
+          const int j = i >> 1, valid = (i & 1) != 0 ? w.len - j * kTile : kTile;   // (of K a foreign row only reaches scores that are masked)
+          ok = warp_wait(empty(n), (n / ST & 1) ^ 1u, abort_flag);
+          if (!ok) break;
+          bring_tile<DP>(kv + n % ST * TB, (i & 1) != 0 ? &tm_v : &tm_k, full(n), raw(n), hk, w.start + j * kTile, valid);
+        }
       }
-      if (!ok) settle();
+      if (s_abort) settle();
+    } else if (warp == 9) {
+      // ---------------------------------------------------------------- products
+      const uint32_t id_s = ptx::instr_desc_bf16(128, 128, 0, 0), id_o = ptx::instr_desc_bf16(128, DP, 0, 1);
+      if (ptx::elect_one()) {
+        bool ok = true;
+        int n = 0, used[2] = {0, 0}, done[2] = {0, 0};   // ring position, items and blocks of each tile so far
+        for (int r = 0; ok; ++r) {
+          const Item w = items.take_alone(r);
+          if (w.level < 0) break;
+          const int blocks[2] = {blocks_of(w, 0), blocks_of(w, 1)}, nb = max(blocks[0], blocks[1]);
+          auto scores = [&](int t, int j) {
+            ptx::tc_fence_after();
+            mma_kk<DP>(s_at(t), base + t * TB, kv + (n + 2 * j) % ST * TB, id_s);
+            ptx::mma_commit(s_full(t));
+            if (j + 1 == blocks[t]) ptx::mma_commit(q_empty(t));
+          };
+          ok = ptx::mbar_wait(full(n), n / ST & 1, abort_flag);
+          for (int t = 0; ok && t < 2; ++t)
+            if (blocks[t] > 0) {
+              ok = ptx::mbar_wait(q_full(t), used[t] & 1, abort_flag);
+              if (ok) scores(t, 0);
+            }
+          if (!ok) break;
+          ptx::mma_commit(empty(n));
+          for (int j = 0; ok && j < nb; ++j) {
+            const int nv = n + 2 * j + 1, nk = nv + 1;
+            ok = ptx::mbar_wait(full(nv), nv / ST & 1, abort_flag);
+            for (int t = 0; ok && t < 2; ++t) {
+              if (j >= blocks[t]) continue;
+              ok = (j > 0 || ptx::mbar_wait(o_empty(t), (used[t] & 1) ^ 1u, abort_flag)) && ptx::mbar_wait(p_full(t, 0), done[t] & 1, abort_flag);
+              if (!ok) break;
+              ptx::tc_fence_after();
+              mma_tm<0, 4>(o_at(t), s_at(t), kv + nv % ST * TB, id_o, j > 0, 32);
+              ok = ptx::mbar_wait(p_full(t, 1), done[t] & 1, abort_flag);
+              if (!ok) break;
+              ptx::tc_fence_after();
+              mma_tm<4, 8>(o_at(t), s_at(t), kv + nv % ST * TB, id_o, true, 32);
+              ++done[t];
+              if (j + 1 < blocks[t]) {
+                ok = ptx::mbar_wait(full(nk), nk / ST & 1, abort_flag);
+                if (ok) scores(t, j + 1);
+              } else {
+                ptx::mma_commit(o_full(t));
+              }
+            }
+            if (!ok) break;
+            ptx::mma_commit(empty(nv));
+            if (j + 1 < nb) ptx::mma_commit(empty(nk));
+          }
+          n += 2 * nb;
+          for (int t = 0; t < 2; ++t) used[t] += blocks[t] > 0;
+        }
+        if (s_abort) settle();
+      }
+      __syncwarp();
+    } else if (warp == 10) {
+      items.run(a.seqs, two_heads ? kTile : 2 * kTile, two_heads ? a.Hq / 2 : a.Hq);
+    } else {
+      zero_gaps(a.seqs, a.o, a.Hq * a.D / 8);
+      bool ok = true;
+      int n = 0;
+      uint32_t phases = 0;   // of the raw barriers, a bit each
+      for (int r = 0; ok; ++r) {
+        const Item w = items.take(r);
+        if (w.level < 0) break;
+        const int nb = max(blocks_of(w, 0), blocks_of(w, 1)), valid = w.len - (nb - 1) * kTile;   // of the last values
+        n += 2 * nb;
+        if (valid >= kTile) continue;
+        const int s = (n - 1) % ST;
+        ok = mend_tile<DP>(kv + s * TB, full(s), raw(s), phases >> s, valid, abort_flag);
+        phases ^= 1u << s;
+      }
     }
-    __syncwarp();
-  }
   } else {
     // ---------------------------------------------------------------- softmax
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-    const int t = warp >> 2, row = (warp & 3) * 32 + lane, n_blocks = blocks[t];
+    const int t = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;   // this warp's lanes of tensor memory
     const uint32_t sp = s_at(t) + lanes, op = o_at(t) + lanes;
-    float m = 0.f, l = 0.f;
+    const F2 scale = f2(a.scale_log2, a.scale_log2);
+    int used = 0, done = 0;
     bool ok = true;
-    for (int j = 0; j < n_blocks; ++j) {
-      ok = warp_wait(s_full(t), j & 1, abort_flag);
-      if (!ok) break;
-      ptx::tc_fence_after();
-      uint32_t s[4][32];
+    for (int r = 0; ok; ++r) {
+      const Item w = items.take(r);
+      if (w.level < 0) break;
+      const int tile = tile_of(w, t), head = head_of(w, t), n_blocks = blocks_of(w, t);
+      if (n_blocks == 0) continue;
+      float m = 0.f, l = 0.f;
+      for (int j = 0; j < n_blocks; ++j, ++done) {
+        ok = warp_wait(s_full(t), done & 1, abort_flag);
+        if (!ok) break;
+        ptx::tc_fence_after();
+        uint32_t s[4][32];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) ptx::tmem_ld_32x32(sp + c * 32, s[c]);
-      ptx::tmem_ld_wait();
-      if (j == tile[t]) {   // the diagonal: keys behind the query
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (c * 32 + i > row) s[c][i] = 0xff800000u;
-      }
-      float mx[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        mx[c] = __uint_as_float(s[c][0]);
-#pragma unroll
-        for (int i = 1; i < 32; ++i) mx[c] = fmaxf(mx[c], __uint_as_float(s[c][i]));
-      }
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-      if (j == 0) {
-        m = top;
-      } else if (__any_sync(0xffffffffu, (top - m) * a.scale_log2 > 8.f)) {
-        const float grown = fmaxf(m, top), f = grown == m ? 1.f : ex2((m - grown) * a.scale_log2);
-        m = grown;
-        l *= f;
-#pragma unroll 1
-        for (int c = 0; c < DP; c += 32) {
-          uint32_t v[32];
-          ptx::tmem_ld_32x32(op + c, v);
-          ptx::tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
-          ptx::tmem_st_32x32(op + c, v);
-        }
-        ptx::tmem_st_wait();
-      }
-      const F2 scale = f2(a.scale_log2, a.scale_log2), shift = f2(-m * a.scale_log2, -m * a.scale_log2);
-      F2 sum[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t p[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const F2 x = ex2_pair<4>(s[2 * half + i / 16][i % 16 * 2], s[2 * half + i / 16][i % 16 * 2 + 1], scale, shift, i);
-          sum[i & 1] = add2(sum[i & 1], x);
-          p[i] = f2_bf16(x);
-        }
-        ptx::tmem_st_32x32(sp + half * 32, p);
-        ptx::tmem_st_wait();
-        ptx::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(p_full(t, half));
-      }
-      float lo, hi;
-      f2_split(add2(sum[0], sum[1]), lo, hi);
-      l += lo + hi;
-    }
-    if (ok && n_blocks > 0) ok = warp_wait(o_full(t), 0, abort_flag);
-    if (ok && n_blocks > 0) {
-      ptx::tc_fence_after();
-      const int in_seq = tile[t] * kTile + row;
-      const long long r = w.start + in_seq;
-      const float inv = 1.f / l;
-#pragma unroll 1
-      for (int c = 0; c < DP; c += 32) {
-        uint32_t v[32];
-        ptx::tmem_ld_32x32(op + c, v);
+        for (int c = 0; c < 4; ++c) ptx::tmem_ld_32x32(sp + c * 32, s[c]);
         ptx::tmem_ld_wait();
-        if (in_seq < w.len) store_row32(a.o + (r * a.Hq + head[t]) * a.D + c, v, inv, a.D - c);
+        if (j == tile) {   // the diagonal: keys behind the query
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (c * 32 + i > row) s[c][i] = 0xff800000u;
+        }
+        float mx[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          mx[c] = __uint_as_float(s[c][0]);
+#pragma unroll
+          for (int i = 1; i < 32; ++i) mx[c] = fmaxf(mx[c], __uint_as_float(s[c][i]));
+        }
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        if (j == 0) {
+          m = top;
+        } else if (__any_sync(0xffffffffu, (top - m) * a.scale_log2 > 8.f)) {
+          const float grown = fmaxf(m, top), f = grown == m ? 1.f : ex2((m - grown) * a.scale_log2);
+          m = grown;
+          l *= f;
+#pragma unroll 1
+          for (int c = 0; c < DP; c += 32) {
+            uint32_t v[32];
+            ptx::tmem_ld_32x32(op + c, v);
+            ptx::tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+            ptx::tmem_st_32x32(op + c, v);
+          }
+          ptx::tmem_st_wait();
+        }
+        const F2 shift = f2(-m * a.scale_log2, -m * a.scale_log2);
+        F2 sum[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t p[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const F2 x = ex2_pair<4>(s[2 * half + i / 16][i % 16 * 2], s[2 * half + i / 16][i % 16 * 2 + 1], scale, shift, i);
+            sum[i & 1] = add2(sum[i & 1], x);
+            p[i] = f2_bf16(x);
+          }
+          ptx::tmem_st_32x32(sp + half * 32, p);
+          ptx::tmem_st_wait();
+          ptx::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(p_full(t, half));
+        }
+        float lo, hi;
+        f2_split(add2(sum[0], sum[1]), lo, hi);
+        l += lo + hi;
       }
-      if (in_seq < w.len) a.lse[(long long)head[t] * a.seqs.T + r] = m * a.scale_log2 + log2f(l);
+      ok = ok && warp_wait(o_full(t), used & 1, abort_flag);
+      if (!ok) break;
+      ++used;
+      ptx::tc_fence_after();
+      const float inv = 1.f / l;
+      uint32_t out[DP / 32][16];
+#pragma unroll
+      for (int c = 0; c < DP / 32; ++c) {
+        uint32_t v[32];
+        ptx::tmem_ld_32x32(op + c * 32, v);
+        ptx::tmem_ld_wait();
+        pack_row(out[c], v, inv);
+      }
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(o_empty(t));
+      const int row0 = tile * kTile + (warp & 3) * 32, valid = w.len - row0;   // of this warp's rows
+      uint8_t* dst = reinterpret_cast<uint8_t*>(a.o + ((long long)(w.start + row0) * a.Hq + head) * a.D);
+#pragma unroll
+      for (int c = 0; c < DP / 32; ++c)
+        store_rows(attn_smem + (2 + ST) * TB + warp * 2048, out[c], dst + c * 64, (long long)a.Hq * a.D * 2, valid, (a.D - c * 32) * 2);
+      if (lane < valid) a.lse[(long long)head * a.seqs.T + w.start + row0 + lane] = m * a.scale_log2 + log2f(l);
     }
   }
   ptx::tc_fence_before();
@@ -497,6 +588,7 @@ template <int DP>
 __global__ void __launch_bounds__(kDeltaThreads) delta_kernel(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict__ d_o,
                                                               float* __restrict__ delta, int T, int Hq, int D) {
   constexpr int L = DP / 8;
+  grid_launch();
   const long long row = ((long long)blockIdx.x * kDeltaThreads + threadIdx.x) / L;
   const int c = threadIdx.x % L * 8;
   const bool live = row < (long long)T * Hq;
@@ -513,16 +605,16 @@ __global__ void __launch_bounds__(kDeltaThreads) delta_kernel(const __nv_bfloat1
 }
 
 // ---------------------------------------------------------------- backward: dK and dV
-// A CTA has one tile of keys and works through the queries that see it, head by head of the group (or of a part of it: dkv_parts), so that
-// dK and dV stay in tensor memory and no sum needs an atomic.  Scores transposed (a row is a key): P^T and dS^T are the A operands of dV = P^T dO and dK = dS^T Q.
-// Warps 0-7: elementwise, a thread has 64 of the 128 queries of a row; warp 8: TMA; warp 9: MMA; warp 10: lse and delta.
-// Order of products: S(0) dP(0) | dV(i) S(i+1) after P(i), dK(i) dP(i+1) after dS(i): exponentials are made while dK and dP run,
-// dS while dV and S do.
-constexpr int kBwdThreads = 352;
+// An item is a tile of keys: its CTA works through the queries that see it, head by head of the group (or of a part of it: dkv_parts), so that
+// dK and dV stay in tensor memory and no sum needs an atomic.  Scores transposed (a row is a key): P^T and dS^T are the A operands of
+// dV = P^T dO and dK = dS^T Q.  Warps 0-7: elementwise, a thread has 64 of the 128 queries of a row; warp 8: TMA; warp 9: MMA; warp 10: items;
+// warp 11: lse and delta, and the rows of other sequences in a tile.  Order of products: S(0) dP(0) | dV(i) S(i+1) after P(i), dK(i) dP(i+1) after dS(i): exponentials are made while
+// dK and dP run, dS while dV and S do.
+constexpr int kBwdThreads = 384;
 template <int DP>
 struct DkvShape {
   static constexpr int kStages = 2;
-  static constexpr int kSmem = (2 + 2 * kStages) * kTileBytes<DP> + kStages * 2 * kTile * 4 + 256;
+  static constexpr int kSmem = (2 + 2 * kStages) * kTileBytes<DP> + kStaging + kStages * 2 * kTile * 4 + kBarriers;
 };
 
 template <int DP>
@@ -533,46 +625,36 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dkv_kernel(const __grid_consta
   extern __shared__ __align__(1024) uint8_t attn_smem[];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
+  __shared__ Plan s_plan;
   const uint32_t base = ptx::smem_u32(attn_smem);
   if ((base & 1023u) != 0) {
     if (threadIdx.x == 0) raise_status(LEWI_STATUS_SMEM_LAYOUT);
     return;
   }
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int hk = blockIdx.x % a.Hkv, part = blockIdx.x / a.Hkv % a.parts;
-  zero_gaps(a.seqs, a.dk, a.Hkv * a.D / 8, kBwdThreads);
-  zero_gaps(a.seqs, a.dv, a.Hkv * a.D / 8, kBwdThreads);
-  const Work w = find_work<kBwdThreads>(a.seqs, blockIdx.x / (a.Hkv * a.parts), [](int tiles) { return tiles; });
-  if (!w.any) return;
-  const int head0 = part * a.G / a.parts, heads = (part + 1) * a.G / a.parts - head0;   // of the group
-  const int tiles = (w.len + kTile - 1) / kTile, key_tile = tiles - 1 - w.level, per_head = w.level + 1, n_it = per_head * heads;
-  auto head_of = [&](int it) { return hk * a.G + head0 + it / per_head; };
-  auto tile_of = [&](int it) { return key_tile + it % per_head; };
-
   const uint32_t k_at = base, v_at = base + TB, ring = base + 2 * TB;   // [stage][Q, dO]
-  float* stats = reinterpret_cast<float*>(attn_smem + (2 + 2 * ST) * TB);   // [stage][lse, delta][128]
-  const uint32_t bars = base + (2 + 2 * ST) * TB + ST * 2 * kTile * 4;
-  const uint32_t k_full = bars, v_full = bars + 8, s_full = bars + 16, dp_full = bars + 24, p_ready = bars + 32, ds_ready = bars + 40, done = bars + 48,
-                 raw = bars + 56;
-  auto q_full = [&](int s) { return bars + 64u + 8u * s; };
-  auto q_empty = [&](int s) { return bars + 64u + 8u * (ST + s); };
-  auto do_full = [&](int s) { return bars + 64u + 8u * (2 * ST + s); };
-  auto do_empty = [&](int s) { return bars + 64u + 8u * (3 * ST + s); };
-  auto st_full = [&](int s) { return bars + 64u + 8u * (4 * ST + s); };
-  auto st_empty = [&](int s) { return bars + 64u + 8u * (5 * ST + s); };
+  float* stats = reinterpret_cast<float*>(attn_smem + (2 + 2 * ST) * TB + kStaging);   // [stage][-lse, -delta][128]
+  const uint32_t bars = base + (2 + 2 * ST) * TB + kStaging + ST * 2 * kTile * 4;
+  const uint32_t k_full = bars, v_full = bars + 8, s_full = bars + 16, dp_full = bars + 24, p_ready = bars + 32, ds_ready = bars + 40, acc_full = bars + 48,
+                 k_empty = bars + 64, v_empty = bars + 72, acc_empty = bars + 80;
+  auto q_full = [&](int n) { return bars + 88u + 8u * (n % ST); };
+  auto q_empty = [&](int n) { return bars + 88u + 8u * (ST + n % ST); };
+  auto do_full = [&](int n) { return bars + 88u + 8u * (2 * ST + n % ST); };
+  auto do_empty = [&](int n) { return bars + 88u + 8u * (3 * ST + n % ST); };
+  auto st_full = [&](int n) { return bars + 88u + 8u * (4 * ST + n % ST); };
+  auto st_empty = [&](int n) { return bars + 88u + 8u * (5 * ST + n % ST); };
+  auto q_raw = [&](int n) { return bars + 88u + 8u * (6 * ST + n % ST); };
+  auto do_raw = [&](int n) { return bars + 88u + 8u * (7 * ST + n % ST); };
   volatile int* abort_flag = &s_abort;
+  const ItemQueue items{&s_plan, bars + 88u + 8u * (8 * ST), abort_flag};
   if (threadIdx.x == 0) {
-    for (uint32_t b : {k_full, v_full, s_full, dp_full, done, raw}) ptx::mbar_init(b, 1);
-    ptx::mbar_init(p_ready, 8);
-    ptx::mbar_init(ds_ready, 8);
+    for (uint32_t b : {k_full, v_full, k_empty, v_empty, s_full, dp_full, acc_full}) ptx::mbar_init(b, 1);
+    for (uint32_t b : {p_ready, ds_ready, acc_empty}) ptx::mbar_init(b, 8);
     for (int s = 0; s < ST; ++s) {
-      ptx::mbar_init(q_full(s), 1);
-      ptx::mbar_init(q_empty(s), 1);
-      ptx::mbar_init(do_full(s), 1);
-      ptx::mbar_init(do_empty(s), 1);
-      ptx::mbar_init(st_full(s), 1);
+      for (uint32_t b : {q_full(s), q_empty(s), do_full(s), do_empty(s), st_full(s), q_raw(s), do_raw(s)}) ptx::mbar_init(b, 1);
       ptx::mbar_init(st_empty(s), 8);
     }
+    items.init(11);
     s_abort = 0;
     ptx::mbar_fence_init();
     ptx::fence_proxy_async();
@@ -590,167 +672,256 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dkv_kernel(const __grid_consta
   ptx::tc_fence_after();
   const uint32_t tmem = s_tmem, t_s = tmem, t_dp = tmem + 128, t_dv = tmem + 256, t_dk = tmem + 384;
 
+  // An item's products: tile `key` of the keys with the tiles key .. key + per_head - 1 of the queries, head by head.
+  struct Span {
+    int hk, part, key, per_head, head0, n_it;
+  };
+  auto span_of = [&](const Item& w) {
+    Span s;
+    s.hk = w.sub % a.Hkv;
+    s.part = w.sub / a.Hkv;
+    s.key = (w.len + kTile - 1) / kTile - 1 - w.level;   // the first keys have the most queries
+    s.per_head = w.level + 1;
+    const int first = s.part * a.G / a.parts;
+    s.head0 = s.hk * a.G + first;
+    s.n_it = s.per_head * ((s.part + 1) * a.G / a.parts - first);
+    return s;
+  };
+
   if (warp == 8) {
     bool ok = true;
-    if (ptx::elect_one()) {
-      ptx::mbar_expect_tx(k_full, TB);
-      load_tile<DP>(k_at, &tm_k, k_full, hk, w.start + key_tile * kTile);
-      ptx::mbar_expect_tx(v_full, TB);
-      load_tile<DP>(v_at, &tm_v, v_full, hk, w.start + key_tile * kTile);
+    int n = 0;
+    for (int r = 0; ok; ++r) {
+      const Item w = items.take(r);
+      if (w.level < 0) break;
+      const Span sp = span_of(w);
+      ok = warp_wait(k_empty, (r & 1) ^ 1u, abort_flag);
+      if (!ok) break;
+      if (ptx::elect_one()) {
+        ptx::mbar_expect_tx(k_full, TB);
+        load_tile<DP>(k_at, &tm_k, k_full, sp.hk, w.start + sp.key * kTile);
+      }
+      __syncwarp();
+      for (int it = 0; it < sp.n_it; ++it, ++n) {
+        const int row = (sp.key + it % sp.per_head) * kTile, head = sp.head0 + it / sp.per_head;
+        const uint32_t ph = (n / ST & 1) ^ 1u, at = ring + n % ST * 2 * TB;
+        ok = warp_wait(q_empty(n), ph, abort_flag);
+        if (!ok) break;
+        bring_tile<DP>(at, &tm_q, q_full(n), q_raw(n), head, w.start + row, w.len - row);
+        if (it == 0) {   // (V is wanted after the first scores only)
+          ok = warp_wait(v_empty, (r & 1) ^ 1u, abort_flag);
+          if (!ok) break;
+          if (ptx::elect_one()) {
+            ptx::mbar_expect_tx(v_full, TB);
+            load_tile<DP>(v_at, &tm_v, v_full, sp.hk, w.start + sp.key * kTile);
+          }
+          __syncwarp();
+        }
+        ok = warp_wait(do_empty(n), ph, abort_flag);
+        if (!ok) break;
+        bring_tile<DP>(at + TB, &tm_do, do_full(n), do_raw(n), head, w.start + row, w.len - row);
+      }
     }
-    __syncwarp();
-    uint32_t raw_phase = 0;
-    for (int it = 0; ok && it < n_it; ++it) {
-      const int s = it % ST, row = tile_of(it) * kTile;
-      const uint32_t ph = (it / ST & 1) ^ 1u;
-      ok = warp_wait(q_empty(s), ph, abort_flag) &&
-           bring_tile<DP>(ring + 2 * s * TB, &tm_q, q_full(s), raw, raw_phase, head_of(it), w.start + row, w.len - row, abort_flag) &&
-           warp_wait(do_empty(s), ph, abort_flag) &&
-           bring_tile<DP>(ring + (2 * s + 1) * TB, &tm_do, do_full(s), raw, raw_phase, head_of(it), w.start + row, w.len - row, abort_flag);
-    }
-    if (!ok) settle();
+    if (s_abort) settle();
   } else if (warp == 9) {
     const uint32_t id_s = ptx::instr_desc_bf16(128, 128, 0, 0), id_d = ptx::instr_desc_bf16(128, DP, 0, 1);
     if (ptx::elect_one()) {
-      auto scores = [&](int it) {   // S^T = K Q^T
-        const int s = it % ST;
-        if (!ptx::mbar_wait(q_full(s), it / ST & 1, abort_flag)) return false;
-        ptx::tc_fence_after();
-        mma_kk<DP>(t_s, k_at, ring + 2 * s * TB, id_s);
-        ptx::mma_commit(s_full);
-        return true;
-      };
-      auto dps = [&](int it) {   // dP^T = V dO^T
-        const int s = it % ST;
-        if (!ptx::mbar_wait(do_full(s), it / ST & 1, abort_flag)) return false;
-        ptx::tc_fence_after();
-        mma_kk<DP>(t_dp, v_at, ring + (2 * s + 1) * TB, id_s);
-        ptx::mma_commit(dp_full);
-        return true;
-      };
-      bool ok = ptx::mbar_wait(k_full, 0, abort_flag) && scores(0) && ptx::mbar_wait(v_full, 0, abort_flag) && dps(0);
-      for (int it = 0; ok && it < n_it; ++it) {
-        const int s = it % ST;
-        ok = ptx::mbar_wait(p_ready, it & 1, abort_flag);
-        if (!ok) break;
-        ptx::tc_fence_after();
-        mma_tm<0, 8>(t_dv, t_s, ring + (2 * s + 1) * TB, id_d, it > 0, 64);
-        ptx::mma_commit(do_empty(s));
-        if (it + 1 < n_it) ok = scores(it + 1);
-        ok = ok && ptx::mbar_wait(ds_ready, it & 1, abort_flag);
-        if (!ok) break;
-        ptx::tc_fence_after();
-        mma_tm<0, 8>(t_dk, t_dp, ring + 2 * s * TB, id_d, it > 0, 64);
-        ptx::mma_commit(it + 1 < n_it ? q_empty(s) : done);
-        if (it + 1 < n_it) ok = dps(it + 1);
+      bool ok = true;
+      int n = 0;
+      for (int r = 0; ok; ++r) {
+        const Item w = items.take_alone(r);
+        if (w.level < 0) break;
+        const int n_it = span_of(w).n_it;
+        auto scores = [&](int it) {   // S^T = K Q^T
+          const int x = n + it;
+          if (!ptx::mbar_wait(q_full(x), x / ST & 1, abort_flag)) return false;
+          ptx::tc_fence_after();
+          mma_kk<DP>(t_s, k_at, ring + x % ST * 2 * TB, id_s);
+          ptx::mma_commit(s_full);
+          if (it + 1 == n_it) ptx::mma_commit(k_empty);
+          return true;
+        };
+        auto dps = [&](int it) {   // dP^T = V dO^T
+          const int x = n + it;
+          if (!ptx::mbar_wait(do_full(x), x / ST & 1, abort_flag)) return false;
+          ptx::tc_fence_after();
+          mma_kk<DP>(t_dp, v_at, ring + x % ST * 2 * TB + TB, id_s);
+          ptx::mma_commit(dp_full);
+          if (it + 1 == n_it) ptx::mma_commit(v_empty);
+          return true;
+        };
+        ok = ptx::mbar_wait(k_full, r & 1, abort_flag) && scores(0) && ptx::mbar_wait(v_full, r & 1, abort_flag) && dps(0);
+        for (int it = 0; ok && it < n_it; ++it) {
+          const int x = n + it, at = ring + x % ST * 2 * TB;
+          ok = ptx::mbar_wait(p_ready, x & 1, abort_flag) && (it > 0 || ptx::mbar_wait(acc_empty, (r & 1) ^ 1u, abort_flag));
+          if (!ok) break;
+          ptx::tc_fence_after();
+          mma_tm<0, 8>(t_dv, t_s, at + TB, id_d, it > 0, 64);
+          ptx::mma_commit(do_empty(x));
+          if (it + 1 < n_it) ok = scores(it + 1);
+          ok = ok && ptx::mbar_wait(ds_ready, x & 1, abort_flag);
+          if (!ok) break;
+          ptx::tc_fence_after();
+          mma_tm<0, 8>(t_dk, t_dp, at, id_d, it > 0, 64);
+          ptx::mma_commit(q_empty(x));
+          if (it + 1 < n_it) ok = dps(it + 1);
+          else ptx::mma_commit(acc_full);
+        }
+        n += n_it;
       }
-      if (!ok) settle();
+      if (s_abort) settle();
     }
     __syncwarp();
   } else if (warp == 10) {
+    items.run(a.seqs, kTile, a.Hkv * a.parts);
+  } else if (warp == 11) {
+    grid_wait();     // delta, which no other warp reads, is there ..
+    grid_launch();   // .. also for the kernel after this one
+    zero_gaps(a.seqs, a.dk, a.Hkv * a.D / 8);
+    zero_gaps(a.seqs, a.dv, a.Hkv * a.D / 8);
     bool ok = true;
-    for (int it = 0; ok && it < n_it; ++it) {
-      const int s = it % ST;
-      const long long at = (long long)head_of(it) * a.seqs.T + w.start;
-      float x[4], y[4];
+    int n = 0;
+    uint32_t phases = 0;   // of the raw barriers, a bit per stage
+    for (int r = 0; ok; ++r) {
+      const Item w = items.take(r);
+      if (w.level < 0) break;
+      const Span sp = span_of(w);
+      for (int it = 0; it < sp.n_it; ++it, ++n) {
+        const long long at = (long long)(sp.head0 + it / sp.per_head) * a.seqs.T + w.start;
+        float x[4], y[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = tile_of(it) * kTile + lane + 32 * i;
-        x[i] = r < w.len ? -a.lse[at + r] : -INFINITY;   // (behind the end: p = 0)
-        y[i] = r < w.len ? -a.delta[at + r] : 0.f;
-      }
-      ok = warp_wait(st_empty(s), (it / ST & 1) ^ 1u, abort_flag);
-      if (!ok) break;
+        for (int i = 0; i < 4; ++i) {
+          const int row = (sp.key + it % sp.per_head) * kTile + lane + 32 * i;
+          x[i] = row < w.len ? -a.lse[at + row] : -INFINITY;   // (behind the end: p = 0)
+          y[i] = row < w.len ? -a.delta[at + row] : 0.f;
+        }
+        ok = warp_wait(st_empty(n), (n / ST & 1) ^ 1u, abort_flag);
+        if (!ok) break;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        stats[s * 2 * kTile + lane + 32 * i] = x[i];
-        stats[(s * 2 + 1) * kTile + lane + 32 * i] = y[i];
+        for (int i = 0; i < 4; ++i) {
+          stats[n % ST * 2 * kTile + lane + 32 * i] = x[i];
+          stats[(n % ST * 2 + 1) * kTile + lane + 32 * i] = y[i];
+        }
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(st_full(n));
+        const int valid = w.len - (sp.key + it % sp.per_head) * kTile;
+        if (valid < kTile) {
+          const uint32_t at_q = ring + n % ST * 2 * TB, phase = phases >> n % ST;
+          ok = mend_tile<DP>(at_q, q_full(n), q_raw(n), phase, valid, abort_flag) && mend_tile<DP>(at_q + TB, do_full(n), do_raw(n), phase, valid, abort_flag);
+          phases ^= 1u << n % ST;
+          if (!ok) break;
+        }
       }
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(st_full(s));
     }
   } else {
     const int half = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
     const F2 scale = f2(a.scale_log2, a.scale_log2);
     bool ok = true;
-    for (int it = 0; it < n_it; ++it) {
-      const int s = it % ST;
-      const bool diagonal = tile_of(it) == key_tile;
-      const ulonglong2* lse = reinterpret_cast<const ulonglong2*>(stats + s * 2 * kTile + half * 64);   // (both negative, in pairs)
-      const ulonglong2* delta = reinterpret_cast<const ulonglong2*>(stats + (s * 2 + 1) * kTile + half * 64);
-      ok = warp_wait(st_full(s), it / ST & 1, abort_flag) && warp_wait(s_full, it & 1, abort_flag);
+    int n = 0;
+    for (int r = 0; ok; ++r) {
+      const Item w = items.take(r);
+      if (w.level < 0) break;
+      const Span sp = span_of(w);
+      for (int it = 0; it < sp.n_it; ++it, ++n) {
+        const bool diagonal = it % sp.per_head == 0;
+        const ulonglong2* lse = reinterpret_cast<const ulonglong2*>(stats + n % ST * 2 * kTile + half * 64);   // (both negative, in pairs)
+        const ulonglong2* delta = reinterpret_cast<const ulonglong2*>(stats + (n % ST * 2 + 1) * kTile + half * 64);
+        ok = warp_wait(st_full(n), n / ST & 1, abort_flag) && warp_wait(s_full, n & 1, abort_flag);
+        if (!ok) break;
+        ptx::tc_fence_after();
+        F2 p[32];
+        uint32_t x[2][32], out[32];
+        ptx::tmem_ld_32x32(t_s + lanes + half * 64, x[0]);
+        ptx::tmem_ld_32x32(t_s + lanes + half * 64 + 32, x[1]);
+        ptx::tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          const ulonglong2 e = lse[i / 2];
+          p[i] = ex2_pair<kBwdPoly<DP>>(x[i / 16][i % 16 * 2], x[i / 16][i % 16 * 2 + 1], scale, F2{e.x}, i);
+          p[i + 1] = ex2_pair<kBwdPoly<DP>>(x[i / 16][i % 16 * 2 + 2], x[i / 16][i % 16 * 2 + 3], scale, F2{e.y}, i + 1);
+        }
+        if (diagonal) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) p[i] = hide(p[i], half * 64 + 2 * i < row, half * 64 + 2 * i + 1 < row);
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) out[i] = f2_bf16(p[i]);
+        ptx::tmem_st_32x32(t_s + lanes + half * 64, out);
+        ptx::tmem_st_wait();
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(p_ready);
+        ok = warp_wait(dp_full, n & 1, abort_flag);
+        if (!ok) break;
+        ptx::tc_fence_after();
+        ptx::tmem_ld_32x32(t_dp + lanes + half * 64, x[0]);
+        ptx::tmem_ld_32x32(t_dp + lanes + half * 64 + 32, x[1]);
+        ptx::tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          const ulonglong2 e = delta[i / 2];
+          p[i] = mul2(p[i], add2(f2(__uint_as_float(x[i / 16][i % 16 * 2]), __uint_as_float(x[i / 16][i % 16 * 2 + 1])), F2{e.x}));
+          p[i + 1] = mul2(p[i + 1], add2(f2(__uint_as_float(x[i / 16][i % 16 * 2 + 2]), __uint_as_float(x[i / 16][i % 16 * 2 + 3])), F2{e.y}));
+        }
+        if (diagonal) {   // (a pair that is masked adds nothing, whatever dP holds there)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) p[i] = hide(p[i], half * 64 + 2 * i < row, half * 64 + 2 * i + 1 < row);
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) out[i] = f2_bf16(p[i]);
+        ptx::tmem_st_32x32(t_dp + lanes + half * 64, out);
+        ptx::tmem_st_wait();
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          ptx::mbar_arrive(ds_ready);
+          ptx::mbar_arrive(st_empty(n));
+        }
+      }
+      ok = ok && warp_wait(acc_full, r & 1, abort_flag);
       if (!ok) break;
       ptx::tc_fence_after();
-      F2 p[32];
-      uint32_t x[2][32], out[32];
-      ptx::tmem_ld_32x32(t_s + lanes + half * 64, x[0]);
-      ptx::tmem_ld_32x32(t_s + lanes + half * 64 + 32, x[1]);
-      ptx::tmem_ld_wait();
-#pragma unroll
-      for (int i = 0; i < 32; i += 2) {
-        const ulonglong2 e = lse[i / 2];
-        p[i] = ex2_pair<kBwdPoly<DP>>(x[i / 16][i % 16 * 2], x[i / 16][i % 16 * 2 + 1], scale, F2{e.x}, i);
-        p[i + 1] = ex2_pair<kBwdPoly<DP>>(x[i / 16][i % 16 * 2 + 2], x[i / 16][i % 16 * 2 + 3], scale, F2{e.y}, i + 1);
-      }
-      if (diagonal) {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) p[i] = hide(p[i], half * 64 + 2 * i < row, half * 64 + 2 * i + 1 < row);
-      }
-#pragma unroll
-      for (int i = 0; i < 32; ++i) out[i] = f2_bf16(p[i]);
-      ptx::tmem_st_32x32(t_s + lanes + half * 64, out);
-      ptx::tmem_st_wait();
-      ptx::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(p_ready);
-      ok = warp_wait(dp_full, it & 1, abort_flag);
-      if (!ok) break;
-      ptx::tc_fence_after();
-      ptx::tmem_ld_32x32(t_dp + lanes + half * 64, x[0]);
-      ptx::tmem_ld_32x32(t_dp + lanes + half * 64 + 32, x[1]);
-      ptx::tmem_ld_wait();
-#pragma unroll
-      for (int i = 0; i < 32; i += 2) {
-        const ulonglong2 e = delta[i / 2];
-        p[i] = mul2(p[i], add2(f2(__uint_as_float(x[i / 16][i % 16 * 2]), __uint_as_float(x[i / 16][i % 16 * 2 + 1])), F2{e.x}));
-        p[i + 1] = mul2(p[i + 1], add2(f2(__uint_as_float(x[i / 16][i % 16 * 2 + 2]), __uint_as_float(x[i / 16][i % 16 * 2 + 3])), F2{e.y}));
-      }
-      if (diagonal) {   // (a pair that is masked adds nothing, whatever dP holds there)
-#pragma unroll
-        for (int i = 0; i < 32; ++i) p[i] = hide(p[i], half * 64 + 2 * i < row, half * 64 + 2 * i + 1 < row);
-      }
-#pragma unroll
-      for (int i = 0; i < 32; ++i) out[i] = f2_bf16(p[i]);
-      ptx::tmem_st_32x32(t_dp + lanes + half * 64, out);
-      ptx::tmem_st_wait();
-      ptx::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        ptx::mbar_arrive(ds_ready);
-        ptx::mbar_arrive(st_empty(s));
-      }
-    }
-    if (ok) ok = warp_wait(done, 0, abort_flag);
-    if (ok) {
-      ptx::tc_fence_after();
-      const int in_seq = key_tile * kTile + row;
-      const long long at = ((long long)(w.start + in_seq) * a.Hkv + hk) * a.D, plane = (long long)a.seqs.T * a.Hkv * a.D;
-#pragma unroll 1
-      for (int c = half * (DP / 2); c < (half + 1) * (DP / 2); c += 32) {
-        uint32_t x[32];
-        ptx::tmem_ld_32x32(t_dv + lanes + c, x);
+      const int row0 = sp.key * kTile + (warp & 3) * 32, valid = w.len - row0;
+      const long long at = ((long long)(w.start + row0) * a.Hkv + sp.hk) * a.D, plane = (long long)a.seqs.T * a.Hkv * a.D;
+      uint8_t* stage = attn_smem + (2 + 2 * ST) * TB + warp * 2048;
+      // this warp's pieces of 32 columns: of dV, then of dK
+      auto column = [&](int i) { return half * (DP / 2) + i % (DP / 64) * 32; };
+      auto piece = [&](int i, uint32_t (&v)[32]) {
+        ptx::tmem_ld_32x32((i < DP / 64 ? t_dv : t_dk) + lanes + column(i), v);
         ptx::tmem_ld_wait();
-        if (in_seq < w.len) {
-          if (a.parts == 1) store_row32(a.dv + at + c, x, 1.f, a.D - c);
-          else store_part32(a.sums + 2 * part * plane + at + c, x, 1.f, a.D - c);
+      };
+      auto free_sums = [&] {
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(acc_empty);
+      };
+      if (a.parts == 1) {
+        uint32_t out[DP / 32][16];
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i) {
+          uint32_t v[32];
+          piece(i, v);
+          pack_row(out[i], v, i < DP / 64 ? 1.f : a.scale);
         }
-        ptx::tmem_ld_32x32(t_dk + lanes + c, x);
-        ptx::tmem_ld_wait();
-        if (in_seq < w.len) {
-          if (a.parts == 1) store_row32(a.dk + at + c, x, a.scale, a.D - c);
-          else store_part32(a.sums + (2 * part + 1) * plane + at + c, x, a.scale, a.D - c);
+        free_sums();   // (the next item's products may go on)
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i)
+          store_rows(stage, out[i], reinterpret_cast<uint8_t*>((i < DP / 64 ? a.dv : a.dk) + at + column(i)), (long long)a.Hkv * a.D * 2, valid,
+                     (a.D - column(i)) * 2);
+      } else {
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i) {
+          uint32_t v[32], out[16];
+          piece(i, v);
+          float* dst = a.sums + (2 * sp.part + (i < DP / 64 ? 0 : 1)) * plane + at + column(i);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            half_row(out, v, h, i < DP / 64 ? 1.f : a.scale);
+            store_rows(stage, out, reinterpret_cast<uint8_t*>(dst + h * 16), (long long)a.Hkv * a.D * 4, valid, (a.D - column(i) - h * 16) * 4);
+          }
         }
+        free_sums();
       }
     }
   }
@@ -783,49 +954,49 @@ __global__ void __launch_bounds__(kSumThreads) dkv_sum_kernel(const Args a) {
 }
 
 // ---------------------------------------------------------------- backward: dQ
-// A CTA has one tile of queries of one head and works through the keys that it sees, with S and dP as in the forward pass.  Scores have two
-// places in tensor memory, so that S(j+1) is there when dS(j) has been made; dS(j) takes the place of S(j).
-// Order of products: S(0) dP(0) S(1) | dP(j+1) dQ(j) S(j+2) after dS(j).
+// An item is a tile of queries of one head: its CTA works through the keys that it sees, with S and dP as in the forward pass.  Scores have two
+// places in tensor memory, so that S(j+1) is there when dS(j) has been made; dS(j) takes the place of S(j).  Warps as above; warp 11: rows of
+// no sequence and of other ones.  Its CTAs begin where those for dK and dV have finished.  Order of products: S(0) dP(0) S(1) | dP(j+1) dQ(j) S(j+2) after dS(j).
+// S(j+2) waits for K(j+2), whose place is that of K(j) where there are four: five places take what the staging would (8192 x 32 heads, D = 128:
+// 650 us with five, 780 with four), so at D = 128 dQ is stored row by row.
 template <int DP>
 struct DqShape {
   static constexpr int kStages = DP == 64 ? 6 : 5;
-  static constexpr int kSmem = (2 + kStages) * kTileBytes<DP> + 256;
+  static constexpr bool kStaged = DP == 64;
+  static constexpr int kSmem = (2 + kStages) * kTileBytes<DP> + (kStaged ? kStaging : 0) + kBarriers;
 };
-constexpr int kDqThreads = 320;
 
 template <int DP>
-__global__ void __launch_bounds__(kDqThreads, 1) dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                                                           const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
-                                                           const Args a) {
+__global__ void __launch_bounds__(kBwdThreads, 1) dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                                                            const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
+                                                            const Args a) {
   constexpr int ST = DqShape<DP>::kStages, TB = kTileBytes<DP>;
   extern __shared__ __align__(1024) uint8_t attn_smem[];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
+  __shared__ Plan s_plan;
   const uint32_t base = ptx::smem_u32(attn_smem);
   if ((base & 1023u) != 0) {
     if (threadIdx.x == 0) raise_status(LEWI_STATUS_SMEM_LAYOUT);
     return;
   }
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int head = blockIdx.x % a.Hq, hk = head / a.G;
-  zero_gaps(a.seqs, a.dq, a.Hq * a.D / 8, kDqThreads);
-  const Work w = find_work<kDqThreads>(a.seqs, blockIdx.x / a.Hq, [](int tiles) { return tiles; });
-  if (!w.any) return;
-  const int q_row = w.level * kTile, nb = w.level + 1;
-
-  const uint32_t q_at = base, do_at = base + TB, kv = base + 2 * TB, bars = kv + ST * TB;
-  const uint32_t q_full = bars, do_full = bars + 8, dp_full = bars + 16, ds_ready = bars + 24, done = bars + 32, raw = bars + 40;
-  auto s_full = [&](int b) { return bars + 48u + 8u * b; };
-  auto full = [&](int s) { return bars + 64u + 8u * s; };
-  auto empty = [&](int s) { return bars + 64u + 8u * (ST + s); };
+  const uint32_t q_at = base, do_at = base + TB, kv = base + 2 * TB, bars = kv + ST * TB + (DqShape<DP>::kStaged ? kStaging : 0);
+  const uint32_t q_full = bars, do_full = bars + 8, q_empty = bars + 16, do_empty = bars + 24, dp_full = bars + 32, ds_ready = bars + 40, acc_full = bars + 48,
+                 acc_empty = bars + 56;
+  auto s_full = [&](int b) { return bars + 72u + 8u * (b & 1); };
+  auto full = [&](int n) { return bars + 88u + 8u * (n % ST); };
+  auto empty = [&](int n) { return bars + 88u + 8u * (ST + n % ST); };
+  auto raw = [&](int n) { return bars + 88u + 8u * (2 * ST + n % ST); };
   volatile int* abort_flag = &s_abort;
+  const ItemQueue items{&s_plan, bars + 88u + 24u * ST, abort_flag};
   if (threadIdx.x == 0) {
-    for (uint32_t b : {q_full, do_full, dp_full, done, raw, s_full(0), s_full(1)}) ptx::mbar_init(b, 1);
-    ptx::mbar_init(ds_ready, 8);
+    for (uint32_t b : {q_full, do_full, q_empty, do_empty, dp_full, acc_full, s_full(0), s_full(1)}) ptx::mbar_init(b, 1);
+    for (uint32_t b : {ds_ready, acc_empty}) ptx::mbar_init(b, 8);
     for (int s = 0; s < ST; ++s) {
-      ptx::mbar_init(full(s), 1);
-      ptx::mbar_init(empty(s), 1);
+      for (uint32_t b : {full(s), empty(s), raw(s)}) ptx::mbar_init(b, 1);
     }
+    items.init(11);
     s_abort = 0;
     ptx::mbar_fence_init();
     ptx::fence_proxy_async();
@@ -842,109 +1013,167 @@ __global__ void __launch_bounds__(kDqThreads, 1) dq_kernel(const __grid_constant
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem = s_tmem, t_dp = tmem + 256, t_dq = tmem + 384;
-  auto t_s = [&](int j) { return tmem + (j & 1) * 128; };
+  auto t_s = [&](int b) { return tmem + (b & 1) * 128; };   // (b: blocks so far)
 
-  if (warp == 8) {   // Q, K0, dO, V0, K1, V1, ..
+  if (warp == 8) {   // Q, dO, K0, V0, K1, V1, ..
     bool ok = true;
-    uint32_t raw_phase = 0;
-    if (ptx::elect_one()) {
-      ptx::mbar_expect_tx(q_full, TB);
-      load_tile<DP>(q_at, &tm_q, q_full, head, w.start + q_row);
-      ptx::mbar_expect_tx(do_full, TB);
-      load_tile<DP>(do_at, &tm_do, do_full, head, w.start + q_row);
-    }
-    __syncwarp();
-    for (int n = 0; ok && n < 2 * nb; ++n) {
-      const int s = n % ST, j = n >> 1;
-      ok = warp_wait(empty(s), (n / ST & 1) ^ 1u, abort_flag);
+    int n = 0;
+    for (int r = 0; ok; ++r) {
+      const Item w = items.take(r);
+      if (w.level < 0) break;
+      const int q_row = w.start + w.level * kTile, nb = w.level + 1, hk = w.sub / a.G;
+      ok = warp_wait(q_empty, (r & 1) ^ 1u, abort_flag) && warp_wait(do_empty, (r & 1) ^ 1u, abort_flag);
       if (!ok) break;
-      const int valid = (n & 1) == 0 ? w.len - j * kTile : kTile;   // (of V a foreign row only reaches pairs that are masked)
-      ok = bring_tile<DP>(kv + s * TB, (n & 1) != 0 ? &tm_v : &tm_k, full(s), raw, raw_phase, hk, w.start + j * kTile, valid, abort_flag);
+      if (ptx::elect_one()) {
+        ptx::mbar_expect_tx(q_full, TB);
+        load_tile<DP>(q_at, &tm_q, q_full, w.sub, q_row);
+        ptx::mbar_expect_tx(do_full, TB);
+        load_tile<DP>(do_at, &tm_do, do_full, w.sub, q_row);
+      }
+      __syncwarp();
+      for (int i = 0; ok && i < 2 * nb; ++i, ++n) {
+        const int j = i >> 1, valid = (i & 1) == 0 ? w.len - j * kTile : kTile;   // (of V a foreign row only reaches pairs that are masked)
+        ok = warp_wait(empty(n), (n / ST & 1) ^ 1u, abort_flag);
+        if (!ok) break;
+        bring_tile<DP>(kv + n % ST * TB, (i & 1) != 0 ? &tm_v : &tm_k, full(n), raw(n), hk, w.start + j * kTile, valid);
+      }
     }
-    if (!ok) settle();
+    if (s_abort) settle();
   } else if (warp == 9) {
     const uint32_t id_s = ptx::instr_desc_bf16(128, 128, 0, 0), id_d = ptx::instr_desc_bf16(128, DP, 0, 1);
     if (ptx::elect_one()) {
-      auto scores = [&](int j) {
-        const int n = 2 * j, s = n % ST;
-        if (!ptx::mbar_wait(full(s), n / ST & 1, abort_flag)) return false;
-        ptx::tc_fence_after();
-        mma_kk<DP>(t_s(j), q_at, kv + s * TB, id_s);
-        ptx::mma_commit(s_full(j & 1));
-        return true;
-      };
-      auto dps = [&](int j) {
-        const int n = 2 * j + 1, s = n % ST;
-        if (!ptx::mbar_wait(full(s), n / ST & 1, abort_flag)) return false;
-        ptx::tc_fence_after();
-        mma_kk<DP>(t_dp, do_at, kv + s * TB, id_s);
-        ptx::mma_commit(dp_full);
-        ptx::mma_commit(empty(s));
-        return true;
-      };
-      bool ok = ptx::mbar_wait(q_full, 0, abort_flag) && scores(0) && ptx::mbar_wait(do_full, 0, abort_flag) && dps(0) && (nb < 2 || scores(1));
-      for (int j = 0; ok && j < nb; ++j) {
-        ok = ptx::mbar_wait(ds_ready, j & 1, abort_flag) && (j + 1 >= nb || dps(j + 1));
-        if (!ok) break;
-        ptx::tc_fence_after();
-        mma_tm<0, 8>(t_dq, t_s(j), kv + 2 * j % ST * TB, id_d, j > 0, 64);
-        ptx::mma_commit(j + 1 < nb ? empty(2 * j % ST) : done);
-        if (j + 2 < nb) ok = scores(j + 2);
+      bool ok = true;
+      int n = 0, b = 0;   // ring position, blocks so far
+      for (int r = 0; ok; ++r) {
+        const Item w = items.take_alone(r);
+        if (w.level < 0) break;
+        const int nb = w.level + 1;
+        auto scores = [&](int j) {
+          const int x = n + 2 * j;
+          if (!ptx::mbar_wait(full(x), x / ST & 1, abort_flag)) return false;
+          ptx::tc_fence_after();
+          mma_kk<DP>(t_s(b + j), q_at, kv + x % ST * TB, id_s);
+          ptx::mma_commit(s_full(b + j));
+          if (j + 1 == nb) ptx::mma_commit(q_empty);
+          return true;
+        };
+        auto dps = [&](int j) {
+          const int x = n + 2 * j + 1;
+          if (!ptx::mbar_wait(full(x), x / ST & 1, abort_flag)) return false;
+          ptx::tc_fence_after();
+          mma_kk<DP>(t_dp, do_at, kv + x % ST * TB, id_s);
+          ptx::mma_commit(dp_full);
+          ptx::mma_commit(empty(x));
+          if (j + 1 == nb) ptx::mma_commit(do_empty);
+          return true;
+        };
+        ok = ptx::mbar_wait(q_full, r & 1, abort_flag) && scores(0) && ptx::mbar_wait(do_full, r & 1, abort_flag) && dps(0) && (nb < 2 || scores(1));
+        for (int j = 0; ok && j < nb; ++j) {
+          const int x = n + 2 * j;
+          ok = ptx::mbar_wait(ds_ready, (b + j) & 1, abort_flag) && (j + 1 >= nb || dps(j + 1)) &&
+               (j > 0 || ptx::mbar_wait(acc_empty, (r & 1) ^ 1u, abort_flag));
+          if (!ok) break;
+          ptx::tc_fence_after();
+          mma_tm<0, 8>(t_dq, t_s(b + j), kv + x % ST * TB, id_d, j > 0, 64);
+          ptx::mma_commit(empty(x));
+          if (j + 1 == nb) ptx::mma_commit(acc_full);
+          if (j + 2 < nb) ok = scores(j + 2);
+        }
+        n += 2 * nb;
+        b += nb;
       }
-      if (!ok) settle();
+      if (s_abort) settle();
     }
     __syncwarp();
+  } else if (warp == 10) {
+    items.run(a.seqs, kTile, a.Hq);
+  } else if (warp == 11) {
+    zero_gaps(a.seqs, a.dq, a.Hq * a.D / 8);
+    bool ok = true;
+    int n = 0;
+    uint32_t phases = 0;   // of the raw barriers, a bit each
+    for (int r = 0; ok; ++r) {
+      const Item w = items.take(r);
+      if (w.level < 0) break;
+      const int valid = w.len - w.level * kTile, s = (n + 2 * w.level) % ST;   // of the last keys
+      n += 2 * (w.level + 1);
+      if (valid >= kTile) continue;
+      ok = mend_tile<DP>(kv + s * TB, full(s), raw(s), phases >> s, valid, abort_flag);
+      phases ^= 1u << s;
+    }
   } else {
     const int half = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
-    const bool live = q_row + row < w.len;
-    const long long at = (long long)head * a.seqs.T + w.start + q_row + row;
-    const float lse = live ? a.lse[at] : INFINITY, delta = live ? a.delta[at] : 0.f;
-    const F2 scale = f2(a.scale_log2, a.scale_log2), shift = f2(-lse, -lse), minus_delta = f2(-delta, -delta);
+    const F2 scale = f2(a.scale_log2, a.scale_log2);
     bool ok = true;
-    for (int j = 0; j < nb; ++j) {
-      const bool diagonal = j == nb - 1;
-      ok = warp_wait(s_full(j & 1), j >> 1 & 1, abort_flag);
-      if (!ok) break;
-      ptx::tc_fence_after();
-      F2 p[32];
-      uint32_t x[2][32], ds[32];
-      ptx::tmem_ld_32x32(t_s(j) + lanes + half * 64, x[0]);
-      ptx::tmem_ld_32x32(t_s(j) + lanes + half * 64 + 32, x[1]);
-      ptx::tmem_ld_wait();
+    int b = 0;
+    if (a.dk == nullptr) grid_wait();   // delta comes from the kernel before this one
+    for (int r = 0; ok; ++r) {
+      const Item w = items.take(r);
+      if (w.level < 0) break;
+      const int nb = w.level + 1, in_seq = w.level * kTile + row;
+      const long long at = (long long)w.sub * a.seqs.T + w.start + in_seq;
+      const float lse = in_seq < w.len ? a.lse[at] : INFINITY, delta = in_seq < w.len ? a.delta[at] : 0.f;
+      const F2 shift = f2(-lse, -lse), minus_delta = f2(-delta, -delta);
+      for (int j = 0; j < nb; ++j, ++b) {
+        ok = warp_wait(s_full(b), b >> 1 & 1, abort_flag);
+        if (!ok) break;
+        ptx::tc_fence_after();
+        F2 p[32];
+        uint32_t x[2][32], ds[32];
+        ptx::tmem_ld_32x32(t_s(b) + lanes + half * 64, x[0]);
+        ptx::tmem_ld_32x32(t_s(b) + lanes + half * 64 + 32, x[1]);
+        ptx::tmem_ld_wait();
 #pragma unroll
-      for (int i = 0; i < 32; ++i) p[i] = ex2_pair<kBwdPoly<DP>>(x[i / 16][i % 16 * 2], x[i / 16][i % 16 * 2 + 1], scale, shift, i);
-      ok = warp_wait(dp_full, j & 1, abort_flag);
-      if (!ok) break;
-      ptx::tc_fence_after();
-      ptx::tmem_ld_32x32(t_dp + lanes + half * 64, x[0]);
-      ptx::tmem_ld_32x32(t_dp + lanes + half * 64 + 32, x[1]);
-      ptx::tmem_ld_wait();
+        for (int i = 0; i < 32; ++i) p[i] = ex2_pair<kBwdPoly<DP>>(x[i / 16][i % 16 * 2], x[i / 16][i % 16 * 2 + 1], scale, shift, i);
+        ok = warp_wait(dp_full, b & 1, abort_flag);
+        if (!ok) break;
+        ptx::tc_fence_after();
+        ptx::tmem_ld_32x32(t_dp + lanes + half * 64, x[0]);
+        ptx::tmem_ld_32x32(t_dp + lanes + half * 64 + 32, x[1]);
+        ptx::tmem_ld_wait();
 #pragma unroll
-      for (int i = 0; i < 32; ++i)
-        p[i] = mul2(p[i], add2(f2(__uint_as_float(x[i / 16][i % 16 * 2]), __uint_as_float(x[i / 16][i % 16 * 2 + 1])), minus_delta));
-      if (diagonal) {
+        for (int i = 0; i < 32; ++i)
+          p[i] = mul2(p[i], add2(f2(__uint_as_float(x[i / 16][i % 16 * 2]), __uint_as_float(x[i / 16][i % 16 * 2 + 1])), minus_delta));
+        if (j + 1 == nb) {   // the diagonal
 #pragma unroll
-        for (int i = 0; i < 32; ++i) p[i] = hide(p[i], half * 64 + 2 * i > row, half * 64 + 2 * i + 1 > row);
+          for (int i = 0; i < 32; ++i) p[i] = hide(p[i], half * 64 + 2 * i > row, half * 64 + 2 * i + 1 > row);
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) ds[i] = f2_bf16(p[i]);
+        ptx::tmem_st_32x32(t_s(b) + lanes + half * 64, ds);
+        ptx::tmem_st_wait();
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(ds_ready);
       }
+      ok = ok && warp_wait(acc_full, r & 1, abort_flag);
+      if (!ok) break;
+      ptx::tc_fence_after();
+      uint32_t out[DP / 64][16];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) ds[i] = f2_bf16(p[i]);
-      ptx::tmem_st_32x32(t_s(j) + lanes + half * 64, ds);
-      ptx::tmem_st_wait();
+      for (int i = 0; i < DP / 64; ++i) {
+        uint32_t v[32];
+        ptx::tmem_ld_32x32(t_dq + lanes + half * (DP / 2) + i * 32, v);
+        ptx::tmem_ld_wait();
+        pack_row(out[i], v, a.scale);
+      }
       ptx::tc_fence_before();
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(ds_ready);
-    }
-    if (ok) ok = warp_wait(done, 0, abort_flag);
-    if (ok) {
-      ptx::tc_fence_after();
-      const long long out = ((long long)(w.start + q_row + row) * a.Hq + head) * a.D;
-#pragma unroll 1
-      for (int c = half * (DP / 2); c < (half + 1) * (DP / 2); c += 32) {
-        uint32_t x[32];
-        ptx::tmem_ld_32x32(t_dq + lanes + c, x);
-        ptx::tmem_ld_wait();
-        if (live) store_row32(a.dq + out + c, x, a.scale, a.D - c);
+      if (lane == 0) ptx::mbar_arrive(acc_empty);
+      const int row0 = w.level * kTile + (warp & 3) * 32;
+#pragma unroll
+      for (int i = 0; i < DP / 64; ++i) {
+        const int c = half * (DP / 2) + i * 32;
+        uint8_t* dst = reinterpret_cast<uint8_t*>(a.dq + ((long long)(w.start + row0) * a.Hq + w.sub) * a.D + c);
+        const long long stride = (long long)a.Hq * a.D * 2;
+        if constexpr (DqShape<DP>::kStaged) {
+          store_rows(attn_smem + (2 + ST) * TB + warp * 2048, out[i], dst, stride, w.len - row0, (a.D - c) * 2);
+        } else if (lane < w.len - row0) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (u * 8 < a.D - c) st_v4(dst + lane * stride + u * 16, make_uint4(out[i][4 * u], out[i][4 * u + 1], out[i][4 * u + 2], out[i][4 * u + 3]));
+        }
       }
     }
   }
@@ -954,6 +1183,7 @@ __global__ void __launch_bounds__(kDqThreads, 1) dq_kernel(const __grid_constant
     ptx::tc_fence_after();
     ptx::tmem_dealloc(tmem, 512);
   }
+  grid_wait();   // this kernel may have begun while the one for dK and dV was finishing; what follows it follows both
 }
 
 // ---------------------------------------------------------------- host side
@@ -965,14 +1195,29 @@ inline bool make_rows_map(CUtensorMap* m, const void* p, int T, int heads, int D
   return encode_tiled(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, p, dims, strides, box);
 }
 
-// How many CTAs share the heads of a group for a tile of dK and dV.  A tile of the first keys of a long sequence has all its queries, times G
-// heads, so few key heads leave a few long runs: as many parts as make 2 CTAs per SM, at least one head each.
-inline int dkv_parts(long long tiles, int Hkv, int G) {
-  const long long want = 2ll * num_sms(), have = tiles * Hkv;
-  return (int)(have >= want ? 1 : (want + have - 1) / have < G ? (want + have - 1) / have : G);
+// In how many parts, each a CTA's item, a group's heads are worked through for a tile of dK and dV.  The tile of a long sequence's first keys
+// has all its queries, times G heads, so few key heads leave a few long items, while parts cost their way through memory (float32, written and
+// read).  Taken is what comes out shortest of the longest item or an even share of everything, at 1.6 us per pair of tiles, and the parts'
+// bytes at 5 TB/s; where there are several sequences the longest is taken to be three times the mean.  One sequence of 1000, 16 heads over 2:
+// 128 us in one part, 30 in eight; of 16,384: 1975 and 1800 in two.
+inline int dkv_parts(int T, int n_seqs, int Hq, int Hkv, int D) {
+  const double tiles = (double)T / kTile + 0.5 * n_seqs, mean = tiles / n_seqs, longest = n_seqs == 1 ? mean : 3 * mean < tiles ? 3 * mean : tiles;
+  const double share = tiles * (mean + 1) / 2 * Hq / num_sms();
+  int best = 1;
+  double least = 0;
+  for (int p = 1; p <= Hq / Hkv; ++p) {
+    const double item = longest * ((Hq / Hkv + p - 1) / p), us = 1.6 * (item > share ? item : share) + (p > 1 ? 16.0 * T * Hkv * D * p / 5e6 : 0.0);
+    if (p == 1 || us < least) {
+      best = p;
+      least = us;
+    }
+  }
+  return best;
 }
 
-// Units that `n` sequences of together T rows can have at most, `per` per tile and one to round up per sequence.
+inline unsigned ctas(long long items) { return (unsigned)(items < num_sms() ? items : num_sms()); }
+
+// Tiles that `n` sequences of together T rows can have at most.
 inline long long most_tiles(int T, int n) { return (long long)T / kTile + n; }
 
 }  // namespace attn

@@ -71,9 +71,8 @@ template <int DP>
 int attention_fwd(cudaStream_t st, const attn::Args& a, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv) {
   static bool done[64] = {false};
   if (!allow_smem(attn::fwd_kernel<DP>, attn::FwdShape<DP>::kSmem, done)) return LEWI_ERR_CUDA;
-  // pairs of units of all sequences: half their tiles times heads, and one to round up for each
-  const long long pairs = (attn::most_tiles(a.seqs.T, a.seqs.n) * a.G + a.seqs.n + 1) / 2;
-  attn::fwd_kernel<DP><<<(unsigned)(pairs * a.Hkv), attn::kFwdThreads, attn::FwdShape<DP>::kSmem, st>>>(tq, tk, tv, a);
+  const long long items = a.G % 2 == 0 ? attn::most_tiles(a.seqs.T, a.seqs.n) * a.Hq / 2 : attn::most_tiles(a.seqs.T, a.seqs.n) * a.Hq;
+  attn::fwd_kernel<DP><<<attn::ctas(items), attn::kFwdThreads, attn::FwdShape<DP>::kSmem, st>>>(tq, tk, tv, a);
   LEWI_CHECK_LAUNCH();
   return LEWI_OK;
 }
@@ -88,19 +87,22 @@ int attention_bwd(cudaStream_t st, const attn::Args& a, const CUtensorMap& tq, c
   if (a.dk != nullptr) {
     static bool done[64] = {false};
     if (!allow_smem(attn::dkv_kernel<DP>, attn::DkvShape<DP>::kSmem, done)) return LEWI_ERR_CUDA;
-    attn::dkv_kernel<DP><<<(unsigned)(tiles * a.Hkv * a.parts), attn::kBwdThreads, attn::DkvShape<DP>::kSmem, st>>>(tq, tk, tv, td, a);
+    (void)launch_kernel(attn::dkv_kernel<DP>, (int)attn::ctas(tiles * a.Hkv * a.parts), attn::kBwdThreads, attn::DkvShape<DP>::kSmem, st, true, tq, tk,
+                        tv, td, a);
     LEWI_CHECK_LAUNCH();
+  }
+  if (a.dq != nullptr) {
+    static bool done[64] = {false};
+    if (!allow_smem(attn::dq_kernel<DP>, attn::DqShape<DP>::kSmem, done)) return LEWI_ERR_CUDA;
+    (void)launch_kernel(attn::dq_kernel<DP>, (int)attn::ctas(tiles * a.Hq), attn::kBwdThreads, attn::DqShape<DP>::kSmem, st, true, tq, tk, tv, td, a);
+    LEWI_CHECK_LAUNCH();
+  }
+  if (a.dk != nullptr) {
     if (a.parts > 1) {
       const long long vecs = (long long)a.seqs.T * a.Hkv * a.D / 4;
       attn::dkv_sum_kernel<<<(unsigned)((vecs + attn::kSumThreads - 1) / attn::kSumThreads), attn::kSumThreads, 0, st>>>(a);
       LEWI_CHECK_LAUNCH();
     }
-  }
-  if (a.dq != nullptr) {
-    static bool done[64] = {false};
-    if (!allow_smem(attn::dq_kernel<DP>, attn::DqShape<DP>::kSmem, done)) return LEWI_ERR_CUDA;
-    attn::dq_kernel<DP><<<(unsigned)(tiles * a.Hq), attn::kDqThreads, attn::DqShape<DP>::kSmem, st>>>(tq, tk, tv, td, a);
-    LEWI_CHECK_LAUNCH();
   }
   return LEWI_OK;
 }
@@ -215,7 +217,7 @@ int lewi_causal_attention_fwd(void* stream, const void* q, int64_t q_stride, con
 
 int64_t lewi_causal_attention_bwd_workspace_bytes(int T, int n_seqs, int Hq, int Hkv, int D) {
   if (T <= 0 || n_seqs <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || Hq % Hkv != 0) return LEWI_ERR_ARG;
-  const int parts = attn::dkv_parts(attn::most_tiles(T, n_seqs), Hkv, Hq / Hkv);
+  const int parts = attn::dkv_parts(T, n_seqs, Hq, Hkv, D);
   return delta_bytes(T, Hq) + (parts > 1 ? (int64_t)parts * 2 * T * Hkv * D * 4 : 0);
 }
 
@@ -234,7 +236,7 @@ int lewi_causal_attention_bwd(void* stream, const void* q, int64_t q_stride, con
   const attn::Args a{{cu_seqlens, n_seqs, T}, Hq, Hkv, Hq / Hkv, D, scale, scale * 1.4426950408889634f,
                      const_cast<bf16*>(reinterpret_cast<const bf16*>(o)), const_cast<float*>(lse), reinterpret_cast<float*>(workspace),
                      reinterpret_cast<bf16*>(dq), reinterpret_cast<bf16*>(dk), reinterpret_cast<bf16*>(dv),
-                     attn::dkv_parts(attn::most_tiles(T, n_seqs), Hkv, Hq / Hkv),
+                     attn::dkv_parts(T, n_seqs, Hq, Hkv, D),
                      reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(workspace) + delta_bytes(T, Hq))};
   const bf16* g = reinterpret_cast<const bf16*>(d_o);
   return D <= 64 ? attention_bwd<64>(as_stream(stream), a, tq, tk, tv, td, g) : attention_bwd<128>(as_stream(stream), a, tq, tk, tv, td, g);
