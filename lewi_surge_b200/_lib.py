@@ -187,19 +187,16 @@ def index_table(t, what):
 def rows_of(t, align):
   """`t` with its trailing dimensions packed (only rows may be apart) and rows and address multiples of `align` bytes, a copy where they
   are not; and the distance of its rows in elements."""
-  size = t.element_size()
-  n = 1
-  for m in t.shape[1:]:
-    n *= m
+  shape = t.shape
   if t.is_contiguous():
-    rows = n
+    rows = n = t.numel() // shape[0] if shape[0] else 0
   else:
-    packed, step = True, 1
-    for m, st in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
-      packed &= m == 1 or st == step
-      step *= m
-    rows = t.stride(0) if t.shape[0] > 1 else n
-    if not packed or rows < n or rows * size % align:
+    n, packed = 1, True
+    for m, step in zip(reversed(shape[1:]), reversed(t.stride()[1:])):
+      packed &= m == 1 or step == n
+      n *= m
+    rows = t.stride(0) if shape[0] > 1 else n
+    if not packed or rows < n or rows * t.element_size() % align:
       t, rows = t.contiguous(), n
   if t.data_ptr() % align:
     t, rows = t.new_empty(t.shape).copy_(t), n

@@ -11,19 +11,23 @@ from ._lib import LewiError, check, ptr, stream
 
 
 def _check_cache(what, key_cache, value_cache, block_tables, lengths):
-  if key_cache.dtype != torch.bfloat16 or value_cache.dtype != torch.bfloat16:
+  """Pages, tokens per page, heads and head dimension of the caches, and the distance of their pages."""
+  if not key_cache.dtype is value_cache.dtype is torch.bfloat16:
     raise LewiError(f"{what} takes bfloat16 caches")
-  if key_cache.dim() != 4 or value_cache.shape != key_cache.shape:
+  shape, tables = key_cache.shape, block_tables.shape
+  if len(shape) != 4 or value_cache.shape != shape:
     raise LewiError(f"{what}: caches [pages, page, Hkv, D] of one shape are required")
-  _, page, heads, d = key_cache.shape
+  pages, page, heads, d = shape
+  page_stride = page * heads * d
   if not (key_cache.is_contiguous() and value_cache.is_contiguous()):
     for t in (key_cache, value_cache):
-      if t.stride()[1:] != (heads * d, d, 1) or (t.shape[0] > 1 and t.stride(0) != key_cache.stride(0)):
+      if t.stride()[1:] != (heads * d, d, 1) or (pages > 1 and t.stride(0) != key_cache.stride(0)):
         raise LewiError(f"{what}: pages that are contiguous and as far apart in both caches are required")
-  if block_tables.dim() != 2 or lengths.shape != (block_tables.shape[0],):
+    if pages > 1:
+      page_stride = key_cache.stride(0)
+  if len(tables) != 2 or lengths.shape != tables[:1]:
     raise LewiError(f"{what}: block_tables [B, max_pages] and lengths [B] are required")
-  page_stride = key_cache.stride(0) if key_cache.shape[0] > 1 else page * heads * d
-  return page_stride, page, heads, d
+  return pages, page, heads, d, page_stride
 
 
 def paged_cache_write(key, value, key_cache, value_cache, block_tables, lengths, cu_seqlens=None):
@@ -34,10 +38,11 @@ def paged_cache_write(key, value, key_cache, value_cache, block_tables, lengths,
   outside its sequence's table or on a page that does not exist is left out with `LEWI_STATUS_BAD_INDEX` in `_lib.last_status()`.
   Two tokens written to one cell (a page named twice) leave either of them, piece by piece."""
   lib = _lib.load()
-  page_stride, page, heads, d = _check_cache("paged_cache_write", key_cache, value_cache, block_tables, lengths)
-  if key.dtype != torch.bfloat16 or value.dtype != torch.bfloat16 or key.dim() != 3 or key.shape[1:] != (heads, d) or value.shape != key.shape:
+  pages, page, heads, d, page_stride = _check_cache("paged_cache_write", key_cache, value_cache, block_tables, lengths)
+  new = key.shape
+  if not key.dtype is value.dtype is torch.bfloat16 or len(new) != 3 or new[1] != heads or new[2] != d or value.shape != new:
     raise LewiError("paged_cache_write: key, value [T, Hkv, D] bfloat16, as wide as the caches, are required")
-  t, b = key.shape[0], block_tables.shape[0]
+  t, (b, max_pages) = new[0], block_tables.shape
   if cu_seqlens is not None and cu_seqlens.shape != (b + 1,):
     raise LewiError("paged_cache_write: cu_seqlens [B + 1] is required")
   if cu_seqlens is None and t != b:
@@ -51,8 +56,7 @@ def paged_cache_write(key, value, key_cache, value_cache, block_tables, lengths,
   tables, lens = _lib.index_table(block_tables, "block_tables"), _lib.index_table(lengths, "lengths")
   cu = _lib.index_table(cu_seqlens, "cu_seqlens")
   check(lib.lewi_paged_cache_write(stream(), k.data_ptr(), ks, v.data_ptr(), vs, key_cache.data_ptr(), value_cache.data_ptr(), page_stride,
-                                   tables.data_ptr(), lens.data_ptr(), ptr(cu), t, b, heads, d, key_cache.shape[0], page, tables.shape[1]),
-        "lewi_paged_cache_write")
+                                   tables.data_ptr(), lens.data_ptr(), ptr(cu), t, b, heads, d, pages, page, max_pages), "lewi_paged_cache_write")
 
 
 def paged_attention(query, key_cache, value_cache, block_tables, lengths, scale=None):
@@ -62,61 +66,62 @@ def paged_attention(query, key_cache, value_cache, block_tables, lengths, scale=
   captured call follows them.  Cells past a sequence's length, whatever they hold, have no part in it; pages that do not exist
   and what a length has past its table are left out with `LEWI_STATUS_BAD_INDEX` in `_lib.last_status()`."""
   lib = _lib.load()
-  page_stride, page, heads, d = _check_cache("paged_attention", key_cache, value_cache, block_tables, lengths)
-  if query.dtype != torch.bfloat16 or query.dim() != 3 or query.shape[2] != d or query.shape[1] % heads or query.shape[0] != block_tables.shape[0]:
+  pages, page, heads, d, page_stride = _check_cache("paged_attention", key_cache, value_cache, block_tables, lengths)
+  shape, (b, max_pages) = query.shape, block_tables.shape
+  if query.dtype is not torch.bfloat16 or len(shape) != 3 or shape[2] != d or heads == 0 or shape[1] % heads or shape[0] != b:
     raise LewiError("paged_attention: query [B, Hq, D] bfloat16 with Hq a multiple of the caches' heads is required")
-  b, hq = query.shape[:2]
+  hq = shape[1]
   if _lib.elsewhere(query, key_cache, value_cache, block_tables, lengths):
     with torch.cuda.device(query.device):
       return paged_attention(query, key_cache, value_cache, block_tables, lengths, scale)
   q, qs = _lib.rows_of(query, 4)
-  o = torch.empty((b, hq, d), dtype=torch.bfloat16, device=q.device)
+  o = q.new_empty(shape)
   if b == 0 or hq == 0:
     return o
   tables, lens = _lib.index_table(block_tables, "block_tables"), _lib.index_table(lengths, "lengths")
   ws_bytes = lib.lewi_paged_attention_workspace_bytes(d)
-  ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+  ws = q.new_empty(ws_bytes // 2)
   check(lib.lewi_paged_attention(stream(), q.data_ptr(), qs, key_cache.data_ptr(), value_cache.data_ptr(), page_stride, tables.data_ptr(),
-                                 lens.data_ptr(), o.data_ptr(), ws.data_ptr(), ws_bytes, b, hq, heads, d, key_cache.shape[0], page, tables.shape[1],
+                                 lens.data_ptr(), o.data_ptr(), ws.data_ptr(), ws_bytes, b, hq, heads, d, pages, page, max_pages,
                                  d ** -0.5 if scale is None else float(scale)), "lewi_paged_attention")
   return o
 
 
 def _attention_fwd(q, k, v, cu, n_seqs, scale):
-  """Output, log-sum-exp and the operands as the kernels read them."""
-  (q, qs), (k, ks), (v, vs) = _lib.rows_of(q, 16), _lib.rows_of(k, 16), _lib.rows_of(v, 16)
+  """Output, log-sum-exp, the operands as the kernels read them and the distances of their rows."""
+  (q, q_rows), (k, k_rows), (v, v_rows) = _lib.rows_of(q, 16), _lib.rows_of(k, 16), _lib.rows_of(v, 16)
   cu = _lib.index_table(cu, "cu_seqlens")
   t, hq, d = q.shape
   o = torch.empty((t, hq, d), dtype=torch.bfloat16, device=q.device)
   lse = torch.empty((hq, t), dtype=torch.float32, device=q.device)
-  check(_lib.load().lewi_causal_attention_fwd(stream(), q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, ptr(cu), n_seqs, o.data_ptr(),
-                                              lse.data_ptr(), t, hq, k.shape[1], d, scale), "lewi_causal_attention_fwd")
-  return o, lse, q, k, v, cu
+  check(_lib.load().lewi_causal_attention_fwd(stream(), q.data_ptr(), q_rows, k.data_ptr(), k_rows, v.data_ptr(), v_rows, ptr(cu), n_seqs,
+                                              o.data_ptr(), lse.data_ptr(), t, hq, k.shape[1], d, scale), "lewi_causal_attention_fwd")
+  return o, lse, q, k, v, cu, (q_rows, k_rows, v_rows)
 
 
 class _CausalAttention(torch.autograd.Function):
 
   @staticmethod
   def forward(ctx, q, k, v, cu, n_seqs, scale):
-    o, lse, q, k, v, cu = _attention_fwd(q, k, v, cu, n_seqs, scale)
+    o, lse, q, k, v, cu, rows = _attention_fwd(q, k, v, cu, n_seqs, scale)
     ctx.save_for_backward(q, k, v, o, lse, cu)
-    ctx.call = n_seqs, scale
+    ctx.call = n_seqs, scale, rows
     return o
 
   @staticmethod
   def backward(ctx, g):
     lib = _lib.load()
     q, k, v, o, lse, cu = ctx.saved_tensors
-    n_seqs, scale = ctx.call
-    t, hq, d = q.shape
-    (q, qs), (k, ks), (v, vs) = _lib.rows_of(q, 16), _lib.rows_of(k, 16), _lib.rows_of(v, 16)
+    n_seqs, scale, (q_rows, k_rows, v_rows) = ctx.call
+    (t, hq, d), hkv = q.shape, k.shape[1]
     g, _ = _lib.rows_of(g.contiguous(), 16)
-    dq = torch.empty((t, hq, d), dtype=torch.bfloat16, device=q.device) if ctx.needs_input_grad[0] else None
-    dk, dv = (torch.empty(k.shape, dtype=torch.bfloat16, device=q.device) if any(ctx.needs_input_grad[1:3]) else None for _ in range(2))
-    ws_bytes = lib.lewi_causal_attention_bwd_workspace_bytes(t, n_seqs, hq, k.shape[1], d)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
-    check(lib.lewi_causal_attention_bwd(stream(), q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, o.data_ptr(), lse.data_ptr(), g.data_ptr(),
-                                        ptr(cu), n_seqs, ptr(dq), ptr(dk), ptr(dv), ws.data_ptr(), ws_bytes, t, hq, k.shape[1], d, scale),
+    need_q, need_k, need_v = ctx.needs_input_grad[:3]
+    dq = o.new_empty((t, hq, d)) if need_q else None
+    dk, dv = (o.new_empty((t, hkv, d)), o.new_empty((t, hkv, d))) if need_k or need_v else (None, None)
+    ws_bytes = lib.lewi_causal_attention_bwd_workspace_bytes(t, n_seqs, hq, hkv, d)
+    ws = lse.new_empty((ws_bytes + 3) // 4)
+    check(lib.lewi_causal_attention_bwd(stream(), q.data_ptr(), q_rows, k.data_ptr(), k_rows, v.data_ptr(), v_rows, o.data_ptr(), lse.data_ptr(),
+                                        g.data_ptr(), ptr(cu), n_seqs, ptr(dq), ptr(dk), ptr(dv), ws.data_ptr(), ws_bytes, t, hq, hkv, d, scale),
           "lewi_causal_attention_bwd")
     return dq, dk, dv, None, None, None
 

@@ -22,7 +22,7 @@ typedef __nv_bfloat16 bf16;
 int check_cache(const void* k, const void* v, const int32_t* tables, const int32_t* lengths, int B, int Hkv, int D, int64_t pages, int page,
                 int max_pages, int64_t page_stride) {
   if (!k || !v || !tables || !lengths || B <= 0 || Hkv <= 0 || D <= 0 || pages <= 0 || page <= 0 || max_pages <= 0) return LEWI_ERR_ARG;
-  if (D > 256 || pages > 0x7fffffff || (int64_t)max_pages * page > 0x7fffffff - 64) return LEWI_ERR_LIMIT;
+  if (D > 256 || pages > 0x7fffffff || (int64_t)max_pages * page > 0x7fffffff - 128) return LEWI_ERR_LIMIT;
   if (D % 8 != 0 || !aligned(k, 16) || !aligned(v, 16) || page_stride % 8 != 0 || page_stride < (int64_t)page * Hkv * D) return LEWI_ERR_SHAPE;
   return LEWI_OK;
 }
@@ -32,21 +32,22 @@ int launch_paged(cudaStream_t st, const paged::Args& a) {
   static bool done[64] = {false};
   using S = paged::Shape<D>;
   if (!allow_smem(paged::attend_kernel<D>, S::kSmem, done)) return LEWI_ERR_CUDA;
-  if (launch_kernel(paged::attend_kernel<D>, a.ctas, paged::kThreads, S::kSmem, st, false, a) != cudaSuccess) {
+  if (launch_kernel(paged::attend_kernel<D>, a.ctas, S::kThreads, S::kSmem, st, false, a) != cudaSuccess) {
     (void)cudaGetLastError();
     return LEWI_ERR_CUDA;
   }
   ++launch_counter();
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((a.Hq + paged::kWarps - 1) / paged::kWarps), (unsigned)a.c.B);
-  cfg.blockDim = dim3(paged::kThreads);
+  const bool few = (long long)a.c.B * a.Hq <= 2ll * num_sms();   // heads: a CTA each, or a warp each
+  cfg.gridDim = dim3((unsigned)(few ? a.Hq : (a.Hq + paged::kJoinWarps - 1) / paged::kJoinWarps), (unsigned)a.c.B);
+  cfg.blockDim = dim3(paged::kJoinWarps * 32);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, paged::join_kernel, a) != cudaSuccess) {
+  if ((few ? cudaLaunchKernelEx(&cfg, paged::join_kernel<S::kTile, paged::kJoinWarps>, a) : cudaLaunchKernelEx(&cfg, paged::join_kernel<S::kTile, 1>, a)) != cudaSuccess) {
     (void)cudaGetLastError();
     return LEWI_ERR_CUDA;
   }
@@ -109,7 +110,7 @@ int attention_bwd(cudaStream_t st, const attn::Args& a, const CUtensorMap& tq, c
 
 inline int64_t delta_bytes(int T, int Hq) { return ((int64_t)T * Hq * 4 + 255) / 256 * 256; }
 
-inline int paged_ctas(int D) { return num_sms() * (D > 128 ? 1 : 2); }
+inline int paged_ctas(int D) { return num_sms() * (D > 128 ? paged::Shape<256>::kCtas : paged::Shape<128>::kCtas); }
 
 }  // namespace
 

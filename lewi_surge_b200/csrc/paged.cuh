@@ -99,19 +99,22 @@ __global__ void __launch_bounds__(kWriteThreads) write_kernel(const WriteArgs a)
 // o[b,h] = sum_j p_j v_j, p = softmax(scale q.k_j) over the sequence's cells; one pass with a running maximum and sum (float32).
 //
 // Bound by the cache's way from HBM: 4 Hkv D bytes per cell.  The cells of all sequences and key heads are one long list of tiles of
-// 64 cells, of which every CTA takes an equal run, whatever the lengths (they are read on the device, so a captured launch follows
-// them).  The query heads that share a key head are the 16 rows of an `mma.sync` (m16n8k16), a warp's 16 cells its columns; a
+// 64 or 128 cells, of which every CTA takes an equal run, whatever the lengths (they are read on the device, so a captured launch follows
+// them).  The query heads that share a key head are the 16 rows of an `mma.sync` (m16n8k16), a warp's 16 cells (32 where D <= 64) its columns; a
 // warp has its own ring of tiles in shared memory (cp.async) and its own softmax, and nothing is synchronised before a head's
 // tiles end.  There the four warps' results are joined; a head that one CTA has whole is written out, of the others every CTA leaves
 // its part (at most two per CTA) and `join_kernel` adds them up in the order of the cells.
 // p is rounded to bf16 for its product with v (relative 2^-9, like the output's own rounding); its sum is taken before.
-constexpr int kWarps = 4, kThreads = kWarps * 32, kChunk = 16, kTile = kWarps * kChunk, kRows = 16, kJoinCols = 32;
+constexpr int kRows = 16, kJoinCols = 32;
 
+// What bounds a warp is the latency of its chain from scores to sums, so as many warps as there is room for share an SM: three CTAs of four with
+// two stages (64 sequences of up to 8192, 4 key heads: 101 us, two CTAs with three stages 105; 32 of up to 4000, 16 key heads, D = 64: 60 and
+// 64; D = 96, 16 of 16,384: 84 and 102), at D = 256 one of six.
 template <int D>
 struct Shape {
-  static constexpr int kStage = 2 * kChunk * D * 2;                    // a warp's K and V of 16 cells
-  static constexpr int kStages = D == 64 ? 6 : 3;
-  static constexpr int kCtas = D == 256 ? 1 : 2;                       // per SM
+  static constexpr int kWarps = D == 256 ? 6 : 4, kThreads = kWarps * 32, kCtas = D == 256 ? 1 : 3;   // CTAs per SM
+  static constexpr int kChunk = D == 64 ? 32 : 16, kTile = kWarps * kChunk;   // cells that a warp, and all of them, take at a time
+  static constexpr int kStage = 2 * kChunk * D * 2, kStages = 2;              // a warp's K and V of them
   static constexpr int kRing = kWarps * kStages * kStage;
   static constexpr int kSmem = kRing + kWarps * kRows * kJoinCols * 4 + 2 * kWarps * kRows * 4 + kWarps * kStages * 4 + 128;
 };
@@ -131,8 +134,12 @@ struct Cursor {
   int b, r, t, nt;
 };
 
-__device__ __forceinline__ int tiles_of(const Cache& c, int b) { return (length_of(c, b) + kTile - 1) / kTile; }
+template <int TILE>
+__device__ __forceinline__ int tiles_of(const Cache& c, int b) {
+  return (length_of(c, b) + TILE - 1) / TILE;
+}
 
+template <int TILE>
 __device__ __forceinline__ void next_tile(Cursor& u, const Cache& c, int R) {
   if (++u.t < u.nt) return;
   u.t = 0;
@@ -140,15 +147,16 @@ __device__ __forceinline__ void next_tile(Cursor& u, const Cache& c, int R) {
   u.r = 0;
   do {
     if (++u.b >= c.B) return;
-    u.nt = tiles_of(c, u.b);
+    u.nt = tiles_of<TILE>(c, u.b);
   } while (u.nt == 0);
 }
 
 // Tiles of all sequences and of those before `upto` (both times R: places in the list); all threads of the CTA call it.
-__device__ __forceinline__ longlong2 count_tiles(const Cache& c, int upto, long long (&s)[2][kWarps]) {
+template <int TILE, int WARPS>
+__device__ __forceinline__ longlong2 count_tiles(const Cache& c, int upto, long long (&s)[2][WARPS]) {
   long long all = 0, before = 0;
-  for (int b = threadIdx.x; b < c.B; b += kThreads) {
-    const int n = tiles_of(c, b);
+  for (int b = threadIdx.x; b < c.B; b += WARPS * 32) {
+    const int n = tiles_of<TILE>(c, b);
     all += n;
     if (b < upto) before += n;
   }
@@ -163,13 +171,21 @@ __device__ __forceinline__ longlong2 count_tiles(const Cache& c, int upto, long 
     s[1][threadIdx.x >> 5] = before;
   }
   __syncthreads();
-  return make_longlong2(s[0][0] + s[0][1] + s[0][2] + s[0][3], s[1][0] + s[1][1] + s[1][2] + s[1][3]);
+  all = before = 0;
+#pragma unroll
+  for (int x = 0; x < WARPS; ++x) {
+    all += s[0][x];
+    before += s[1][x];
+  }
+  return make_longlong2(all, before);
 }
 
 template <int D>
-__global__ void __launch_bounds__(kThreads, Shape<D>::kCtas) attend_kernel(const Args a) {
+__global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) attend_kernel(const Args a) {
   using S = Shape<D>;
-  constexpr int ST = S::kStages, KS = D / 16, VR = D / 8;   // 16-wide steps over D, 16-byte vectors of a row
+  constexpr int kWarps = S::kWarps;
+  constexpr int ST = S::kStages, KS = D / 16, VR = D / 8, CH = S::kChunk;   // 16-wide steps over D, 16-byte vectors of a row
+  constexpr int kRowBytes = CH * 128;                                       // a box of 64 columns
   extern __shared__ uint8_t smem_raw[];
   __shared__ long long s_count[2][kWarps];
   __shared__ Cursor s_start;
@@ -184,14 +200,14 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kCtas) attend_kernel(const
   const gdn::LaneOff L = gdn::lane_off(lane);
 
   // this CTA's run of the list, and where it starts
-  const long long total = count_tiles(a.c, 0, s_count).x * R;
+  const long long total = count_tiles<S::kTile, kWarps>(a.c, 0, s_count).x * R;
   const long long n_ctas = min(total, (long long)a.ctas);   // (so that no run is empty)
   if (blockIdx.x >= n_ctas) return;
   const long long w0 = blockIdx.x * total / n_ctas, w1 = (blockIdx.x + 1) * total / n_ctas;
   if (warp == 0) {   // 32 sequences at a time
     long long at = 0;
     for (int b0 = 0; b0 < a.c.B; b0 += 32) {
-      const int n = b0 + lane < a.c.B ? tiles_of(a.c, b0 + lane) : 0;
+      const int n = b0 + lane < a.c.B ? tiles_of<S::kTile>(a.c, b0 + lane) : 0;
       long long upto = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -212,39 +228,61 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kCtas) attend_kernel(const
   __syncthreads();
   Cursor use = s_start, get = use;
 
-  // The cells of the tile that is requested next: a lane (of the first 16) has one cell, whose page is looked up one request ahead.
+  // The cells of the tile that is requested next, looked up one request ahead: where pages hold whole chunks all of them follow the first,
+  // otherwise a lane has one.
+  const bool in_row = a.c.page % CH == 0;
+  const int step = a.c.Hkv * a.c.D, row0 = lane / VR, vec0 = (lane % VR) * 8;   // of this lane's first piece
   long long cell = -1;
+  int there = 0;   // cells of the chunk
   bool bad = false;
   auto look = [&] {
+    const int pos0 = get.t * S::kTile + warp * CH, pos = in_row ? pos0 : pos0 + lane;
+    there = min(max(length_of(a.c, get.b) - pos0, 0), CH);
     cell = -1;
-    const int pos = get.t * kTile + warp * kChunk + lane;
-    if (lane < kChunk && pos < length_of(a.c, get.b)) {
+    if (in_row ? there > 0 : lane < there) {
       cell = cell_of(a.c, get.b, pos);
       bad |= cell < 0;
     }
   };
-  const int vecs = a.c.D / 8;
   long long got = w0;
   look();
   auto request = [&](int stage) {
     if (got < w1) {
-      const uint32_t mask = __ballot_sync(0xffffffffu, cell >= 0);
-      if (lane == 0) s_mask[stage] = mask;
-      const uint32_t at = ring + stage * S::kStage;
-      const int head = get.r / a.MT * a.c.D;
+      const uint32_t at = ring + stage * S::kStage + (vec0 >> 6) * kRowBytes;
+      const int head = get.r / a.MT * a.c.D + vec0;
+      const bool col = vec0 < a.c.D;
+      uint32_t mask;
+      if (in_row) {
+        const int rows = cell < 0 ? 0 : there;
+        mask = rows >= 32 ? 0xffffffffu : (1u << rows) - 1u;
+        const __nv_bfloat16 *k = a.c.k + cell + head + (long long)row0 * step, *v = a.c.v + cell + head + (long long)row0 * step;
 #pragma unroll
-      for (int i = 0; i < VR / 2; ++i) {
-        const int row = (i * 32 + lane) / VR, vec = (i * 32 + lane) % VR;
-        const long long from = __shfl_sync(0xffffffffu, cell, row);
-        const bool in = from >= 0 && vec < vecs;
-        const long long e = in ? from + head + vec * 8 : 0;
-        const uint32_t dst = gdn::swz(at + (vec >> 3) * (kChunk * 128), row, vec & 7);
-        ptx::cp_async16(dst, a.c.k + e, in ? 16u : 0u);
-        ptx::cp_async16(dst + kChunk * D * 2, a.c.v + e, in ? 16u : 0u);
+        for (int i = 0; i < CH * VR / 32; ++i) {
+          const int row = row0 + i * (32 / VR);
+          const bool in = row < rows && col;
+          const uint32_t dst = gdn::swz(at, row, vec0 >> 3 & 7);
+          ptx::cp_async16(dst, in ? k : a.c.k, in ? 16u : 0u);
+          ptx::cp_async16(dst + CH * D * 2, in ? v : a.c.v, in ? 16u : 0u);
+          k += (32 / VR) * step;
+          v += (32 / VR) * step;
+        }
+      } else {
+        mask = __ballot_sync(0xffffffffu, cell >= 0);
+#pragma unroll 1
+        for (int i = 0; i < CH * VR / 32; ++i) {
+          const int row = row0 + i * (32 / VR);
+          const long long from = __shfl_sync(0xffffffffu, cell, row);
+          const bool in = from >= 0 && col;
+          const long long e = in ? from + head : 0;
+          const uint32_t dst = gdn::swz(at, row, vec0 >> 3 & 7);
+          ptx::cp_async16(dst, a.c.k + e, in ? 16u : 0u);
+          ptx::cp_async16(dst + CH * D * 2, a.c.v + e, in ? 16u : 0u);
+        }
       }
+      if (lane == 0) s_mask[stage] = mask;
       ++got;
       if (got < w1) {
-        next_tile(get, a.c, R);
+        next_tile<S::kTile>(get, a.c, R);
         look();
       }
     }
@@ -275,13 +313,28 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kCtas) attend_kernel(const
     request(stage == 0 ? ST - 1 : stage - 1);   // into the stage that was worked through last
     ptx::cp_async_wait<ST - 1>();
     __syncwarp();
-    const uint32_t kt = ring + stage * S::kStage, vt = kt + kChunk * D * 2, mask = s_mask[stage];
-    float s[2][4] = {};
+    const uint32_t kt = ring + stage * S::kStage, vt = kt + CH * D * 2, mask = s_mask[stage];
+    constexpr int NT = CH / 8;   // score tiles of 8 cells
+    float s[NT][4] = {};
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) gdn::mma2(s[0], s[1], qf[ks], gdn::ld_b(kt, 0, ks, L, kChunk * 128));
+    for (int c = 0; c < NT / 2; ++c) {
+      if constexpr (D <= 128) {   // two chains of products, half as long (at 256 there are no registers for it)
+        float odd[2][4] = {};
+#pragma unroll
+        for (int ks = 0; ks < KS; ks += 2) {
+          gdn::mma2(s[2 * c], s[2 * c + 1], qf[ks], gdn::ld_b(kt, c * 16, ks, L, kRowBytes));
+          gdn::mma2(odd[0], odd[1], qf[ks + 1], gdn::ld_b(kt, c * 16, ks + 1, L, kRowBytes));
+        }
+        gdn::add4(s[2 * c], odd[0]);
+        gdn::add4(s[2 * c + 1], odd[1]);
+      } else {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) gdn::mma2(s[2 * c], s[2 * c + 1], qf[ks], gdn::ld_b(kt, c * 16, ks, L, kRowBytes));
+      }
+    }
     float top[2] = {m[0], m[1]};
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const bool seen = mask >> (j * 8 + (lane & 3) * 2 + (e & 1)) & 1u;
@@ -306,20 +359,22 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kCtas) attend_kernel(const
         m[r] = top[r];
       }
     }
-    uint32_t p[4];
+    uint32_t p[NT / 2][4];
     {
       const float z0 = m[0] == -INFINITY ? 0.f : m[0], z1 = m[1] == -INFINITY ? 0.f : m[1];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < NT; ++j) {
         const float p0 = exp2f(s[j][0] - z0), p1 = exp2f(s[j][1] - z0), p2 = exp2f(s[j][2] - z1), p3 = exp2f(s[j][3] - z1);
         l[0] += p0 + p1;
         l[1] += p2 + p3;
-        p[2 * j] = pack_bf16(p0, p1);
-        p[2 * j + 1] = pack_bf16(p2, p3);
+        p[j / 2][j % 2 * 2] = pack_bf16(p0, p1);
+        p[j / 2][j % 2 * 2 + 1] = pack_bf16(p2, p3);
       }
     }
 #pragma unroll
-    for (int np = 0; np < D / 16; ++np) gdn::mma2(o[2 * np], o[2 * np + 1], p, gdn::ld_b_t(vt, 0, np, L, kChunk * 128));
+    for (int c = 0; c < NT / 2; ++c)
+#pragma unroll
+      for (int np = 0; np < D / 16; ++np) gdn::mma2(o[2 * np], o[2 * np + 1], p[c], gdn::ld_b_t(vt, c * 16, np, L, kRowBytes));
     __syncwarp();   // (the stage may be written again)
     stage = stage + 1 == ST ? 0 : stage + 1;
 
@@ -347,11 +402,11 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kCtas) attend_kernel(const
       const int row = threadIdx.x >> 3, c4 = (threadIdx.x & 7) * 4;   // what this thread joins: 4 columns of a row
       float mm = -INFINITY, ll = 0.f;
 #pragma unroll
-      for (int x = 0; x < kWarps; ++x) mm = fmaxf(mm, s_m[x * kRows + row]);
+      for (int x = 0; x < kWarps; ++x) mm = fmaxf(mm, s_m[x * kRows + row % kRows]);
 #pragma unroll
       for (int x = 0; x < kWarps; ++x) {
-        const float mx = s_m[x * kRows + row];
-        ll += mx == -INFINITY ? s_l[x * kRows + row] * 0.f : s_l[x * kRows + row] * (mx == mm ? 1.f : exp2f(mx - mm));
+        const float mx = s_m[x * kRows + row % kRows], lx = s_l[x * kRows + row % kRows];
+        ll += mx == -INFINITY ? lx * 0.f : lx * (mx == mm ? 1.f : exp2f(mx - mm));
       }
       const float inv = ll == 0.f ? 0.f : 1.f / ll;
 #pragma unroll
@@ -363,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kCtas) attend_kernel(const
             *reinterpret_cast<float2*>(s_o + (warp * kRows + r0 + r * 8) * kJoinCols + i * 8 + (lane & 3) * 2) =
                 make_float2(o[c0 / 8 + i][2 * r] * f[r], o[c0 / 8 + i][2 * r + 1] * f[r]);
         __syncthreads();
-        if (row < rows && c0 + c4 < a.c.D) {
+        if (row < rows && c0 + c4 < a.c.D) {   // (16 rows, the first 128 threads)
           float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
           for (int x = 0; x < kWarps; ++x) {
@@ -379,7 +434,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kCtas) attend_kernel(const
         }
         __syncthreads();
       }
-      if (!whole && (threadIdx.x & 7) == 0) {
+      if (!whole && row < kRows && (threadIdx.x & 7) == 0) {
         float* stats = a.part + (long long)2 * a.ctas * kRows * a.c.D + part * kRows + row;
         stats[0] = mm;
         stats[2 * a.ctas * kRows] = ll;
@@ -387,26 +442,31 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kCtas) attend_kernel(const
       __syncthreads();   // (s_m and s_l may be written again)
       part = 2 * blockIdx.x + 1;
     }
-    if (w + 1 < w1) next_tile(use, a.c, R);
+    if (w + 1 < w1) next_tile<S::kTile>(use, a.c, R);
   }
   ptx::cp_async_wait_all();
   if (bad) raise_status(LEWI_STATUS_BAD_INDEX);
 }
 
-// Adds up the parts of the heads that several CTAs worked on, in the order of the cells, and writes zeros for sequences without
-// cells.  A warp per query head.
-__global__ void __launch_bounds__(kThreads) join_kernel(const Args a) {
-  __shared__ long long s_count[2][kWarps];
-  const int b = blockIdx.y, lane = threadIdx.x & 31, R = a.c.Hkv * a.MT;
-  const int head = blockIdx.x * kWarps + (threadIdx.x >> 5);
-  const longlong2 count = count_tiles(a.c, b, s_count);
-  const int nt = tiles_of(a.c, b);
+// Adds up the parts of the heads that several CTAs worked on, in a fixed order, and writes zeros for sequences without cells.  `PER` warps
+// work on a query head and take every PER-th part each: 8 for few heads (one sequence of 100,001, 32 heads: 5 us, a warp each 19), one for many
+// (64 sequences x 32 heads: 5 us, eight each 16).
+constexpr int kJoinWarps = 8;
+template <int TILE, int PER>
+__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const Args a) {
+  __shared__ long long s_count[2][kJoinWarps];
+  __shared__ float s_m[kJoinWarps], s_l[kJoinWarps];
+  __shared__ float4 s_sum[PER > 1 ? kJoinWarps : 1][64];
+  const int b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, R = a.c.Hkv * a.MT;
+  const int head = blockIdx.x * (kJoinWarps / PER) + warp / PER, mine = warp % PER;
+  const longlong2 count = count_tiles<TILE, kJoinWarps>(a.c, b, s_count);
+  const int nt = tiles_of<TILE>(a.c, b);
   grid_wait();   // (every CTA, so that what follows this kernel follows the one before it, too)
   if (threadIdx.x == 0 && blockIdx.x == 0 && a.c.lengths[b] > (long long)a.c.max_pages * a.c.page) raise_status(LEWI_STATUS_BAD_INDEX);
-  if (head >= a.Hq) return;
+  if (head >= a.Hq) return;   // (whole warps, and only where each has a head of its own)
   __nv_bfloat16* o = a.o + ((long long)b * a.Hq + head) * a.c.D;
   if (nt == 0) {
-    for (int c = lane * 4; c < a.c.D; c += 128) *reinterpret_cast<uint2*>(o + c) = make_uint2(0u, 0u);
+    for (int c = (mine * 32 + lane) * 4; c < a.c.D; c += PER * 128) *reinterpret_cast<uint2*>(o + c) = make_uint2(0u, 0u);
     return;
   }
   const int g = head % a.G, row = g % kRows;
@@ -418,26 +478,53 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Args a) {
   const int slot0 = 2 * c0 + (w0 == c0 * total / n_ctas ? 0 : 1);   // (every other CTA's run starts inside the head)
   const float* stats = a.part + (long long)2 * a.ctas * kRows * a.c.D + row;
   auto slot_of = [&](int c) { return c == c0 ? slot0 : 2 * c; };
-  float mm = -INFINITY, ll = 0.f;
-  for (int c = c0 + lane; c <= c1; c += 32) mm = fmaxf(mm, stats[slot_of(c) * kRows]);
+  float mm = -INFINITY;
+  for (int c = c0 + mine * 32 + lane; c <= c1; c += PER * 32) mm = fmaxf(mm, stats[slot_of(c) * kRows]);
   mm = warp_max(mm);
-  for (int c = c0 + lane; c <= c1; c += 32) {
+  if constexpr (PER > 1) {
+    if (lane == 0) s_m[warp] = mm;
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < kJoinWarps; ++x) mm = fmaxf(mm, s_m[x]);
+  }
+  float ll = 0.f;
+  float4 sum[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};   // columns 4 lane, 128 + 4 lane
+#pragma unroll 8
+  for (int c = c0 + mine; c <= c1; c += PER) {
     const float mx = stats[slot_of(c) * kRows], lx = stats[(2 * a.ctas + slot_of(c)) * kRows];
-    ll += mx == -INFINITY ? lx * 0.f : lx * (mx == mm ? 1.f : exp2f(mx - mm));
+    const float f = mx == -INFINITY ? 0.f : mx == mm ? 1.f : exp2f(mx - mm);
+    const float* part = a.part + ((long long)slot_of(c) * kRows + row) * a.c.D;
+    ll = fmaf(f, lx, mx == -INFINITY ? lx * 0.f + ll : ll);   // (an lx that is not finite is not lost)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (h * 128 + lane * 4 < a.c.D) {
+        const float4 v = *reinterpret_cast<const float4*>(part + h * 128 + lane * 4);
+        sum[h].x = fmaf(f, v.x, sum[h].x); sum[h].y = fmaf(f, v.y, sum[h].y); sum[h].z = fmaf(f, v.z, sum[h].z); sum[h].w = fmaf(f, v.w, sum[h].w);
+      }
   }
-  ll = warp_sum(ll);
-  const float inv = ll == 0.f ? 0.f : 1.f / ll;
-  for (int col = lane * 4; col < a.c.D; col += 128) {
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int c = c0; c <= c1; ++c) {
-      const float mx = stats[slot_of(c) * kRows];
-      const float f = mx == -INFINITY ? 0.f : mx == mm ? 1.f : exp2f(mx - mm);
-      const float4 v = *reinterpret_cast<const float4*>(a.part + ((long long)slot_of(c) * kRows + row) * a.c.D + col);
-      sum.x = fmaf(f, v.x, sum.x); sum.y = fmaf(f, v.y, sum.y); sum.z = fmaf(f, v.z, sum.z); sum.w = fmaf(f, v.w, sum.w);
+  if constexpr (PER > 1) {
+    if (lane == 0) s_l[warp] = ll;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) s_sum[warp][h * 32 + lane] = sum[h];
+    __syncthreads();
+    if (warp > 0) return;
+    ll = 0.f;
+    sum[0] = sum[1] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int x = 0; x < kJoinWarps; ++x) {
+      ll += s_l[x];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float4 y = s_sum[x][h * 32 + lane];
+        sum[h].x += y.x; sum[h].y += y.y; sum[h].z += y.z; sum[h].w += y.w;
+      }
     }
-    *reinterpret_cast<uint2*>(o + col) = make_uint2(pack_bf16(sum.x * inv, sum.y * inv), pack_bf16(sum.z * inv, sum.w * inv));
   }
+  const float inv = ll == 0.f ? 0.f : 1.f / ll;
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    if (h * 128 + lane * 4 < a.c.D)
+      *reinterpret_cast<uint2*>(o + h * 128 + lane * 4) = make_uint2(pack_bf16(sum[h].x * inv, sum[h].y * inv), pack_bf16(sum[h].z * inv, sum[h].w * inv));
 }
 
 }  // namespace paged

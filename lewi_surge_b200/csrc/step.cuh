@@ -33,7 +33,7 @@ __device__ __forceinline__ int claim_slot(const int32_t* __restrict__ slots, int
 // that one pass over it is enough.  A CTA takes 32 columns of V and holds them in registers (8 lanes of 4 columns, 16 rows at a
 // time); sums over K are float32, joined over the lanes and the warps in a fixed order.
 // Bound by the state's way in and out: 8 bytes per element, 7 flops.
-constexpr int kCols = 32, kRowGroups = kThreads / 8, kMaxK = 128, kRowsPerThread = kMaxK / kRowGroups;
+constexpr int kCols = 64, kLanes = kCols / 4, kRowGroups = kThreads / kLanes, kMaxK = 128, kRowsPerThread = kMaxK / kRowGroups;
 
 struct GdnArgs {
   const __nv_bfloat16 *q, *k, *v;            // [B,Hk,K], [B,Hk,K], [B,H,V]; rows of the batch qs, ks, vs elements apart
@@ -53,9 +53,9 @@ __device__ __forceinline__ float ld_scalar(const void* p, long long i, int f32) 
 
 __global__ void __launch_bounds__(kThreads) gdn_step_kernel(const GdnArgs a) {
   __shared__ float s_q[kMaxK], s_k[kMaxK];
-  __shared__ float s_sum[kThreads / 32][8][9];
+  __shared__ float s_sum[kThreads / 32][kLanes][9];
   const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int l8 = tid & 7, rg = tid >> 3, col = blockIdx.x * kCols + l8 * 4;
+  const int l = tid % kLanes, rg = tid / kLanes, col = blockIdx.x * kCols + l * 4;
   const bool live = col < a.V;
   float4 s[kRowsPerThread];
   const int slot = claim_slot(a.slots, b, a.N, [&](int n) {
@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(kThreads) gdn_step_kernel(const GdnArgs a) {
 #pragma unroll
     for (int i = 0; i < kRowsPerThread; ++i) {
       const int r = rg + i * kRowGroups;
-      s[i] = live && r < a.K ? *reinterpret_cast<const float4*>(base + (long long)r * a.V) : make_float4(0.f, 0.f, 0.f, 0.f);
+      s[i] = live && r < a.K ? __ldcs(reinterpret_cast<const float4*>(base + (long long)r * a.V)) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
     const int hk = h / (a.H / a.Hk);
     s_q[tid] = tid < a.K ? __bfloat162float(a.q[b * a.qs + hk * a.K + tid]) : 0.f;
@@ -88,17 +88,14 @@ __global__ void __launch_bounds__(kThreads) gdn_step_kernel(const GdnArgs a) {
     sum[8] = fmaf(qq, kk, sum[8]);
   }
 #pragma unroll
-  for (int j = 0; j < 9; ++j) {
-    sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 8);
-    sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 16);
-  }
-  if (lane < 8) {
+  for (int j = 0; j < 9; ++j) sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 16);
+  if (lane < kLanes) {
 #pragma unroll
     for (int j = 0; j < 9; ++j) s_sum[warp][lane][j] = sum[j];
   }
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < 9; ++j) sum[j] = (s_sum[0][l8][j] + s_sum[1][l8][j]) + (s_sum[2][l8][j] + s_sum[3][l8][j]);
+  for (int j = 0; j < 9; ++j) sum[j] = (s_sum[0][l][j] + s_sum[1][l][j]) + (s_sum[2][l][j] + s_sum[3][l][j]);
   float d[4], out[4];
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
@@ -113,8 +110,8 @@ __global__ void __launch_bounds__(kThreads) gdn_step_kernel(const GdnArgs a) {
     const int r = rg + i * kRowGroups;
     if (r >= a.K) break;
     const float kk = s_k[r];
-    *reinterpret_cast<float4*>(base + (long long)r * a.V) =
-        make_float4(fmaf(kk, d[0], decay * s[i].x), fmaf(kk, d[1], decay * s[i].y), fmaf(kk, d[2], decay * s[i].z), fmaf(kk, d[3], decay * s[i].w));
+    __stcs(reinterpret_cast<float4*>(base + (long long)r * a.V),
+        make_float4(fmaf(kk, d[0], decay * s[i].x), fmaf(kk, d[1], decay * s[i].y), fmaf(kk, d[2], decay * s[i].z), fmaf(kk, d[3], decay * s[i].w)));
   }
 }
 

@@ -115,10 +115,11 @@ def chunk_gated_delta_rule(query, key, value, g, beta, chunk_size=64, initial_st
 _GATES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 
 
-def _check_slots(what, b, state, slots):
-  if slots is None and state.shape[0] < b:
-    raise LewiError(f"{what}: {b} rows and no slots, but {state.shape[0]} states")
-  if slots is not None and slots.shape != (b,):
+def _check_slots(what, b, n_states, slots):
+  if slots is None:
+    if n_states < b:
+      raise LewiError(f"{what}: {b} rows and no slots, but {n_states} states")
+  elif slots.shape != (b,):
     raise LewiError(f"{what}: slots [B] are required")
 
 
@@ -128,14 +129,15 @@ def causal_conv1d_step(x, w, state, slots=None):
   state b).  A negative slot is an idle row: zeros out, no state touched; a slot past the pool, or an earlier row's, as well, with
   `LEWI_STATUS_BAD_INDEX` in `_lib.last_status()`.  Not differentiable; the values are `causal_conv1d`'s bit for bit."""
   lib = _lib.load()
-  if x.dim() != 2 or w.dim() != 3 or w.shape[1] != 1 or w.shape[2] != x.shape[1]:
+  xs, ws, ss = x.shape, w.shape, state.shape
+  if len(xs) != 2 or len(ws) != 3 or ws[1] != 1 or ws[2] != xs[1]:
     raise LewiError("causal_conv1d_step: x [B,C] and a depthwise kernel w [K,1,C] are required")
-  if x.dtype != torch.bfloat16 or state.dtype != torch.bfloat16:
+  if x.dtype is not torch.bfloat16 or state.dtype is not torch.bfloat16:
     raise LewiError("causal_conv1d_step takes bfloat16 activations and state")
-  (b, c), k = x.shape, w.shape[0]
-  if state.dim() != 3 or state.shape[1:] != (k - 1, c):
+  (b, c), k = xs, ws[0]
+  if len(ss) != 3 or ss[1] != k - 1 or ss[2] != c:
     raise LewiError("causal_conv1d_step: state [N,K-1,C] is required")
-  _check_slots("causal_conv1d_step", b, state, slots)
+  _check_slots("causal_conv1d_step", b, ss[0], slots)
   if _lib.elsewhere(x, w, state, slots):
     with torch.cuda.device(x.device):
       return causal_conv1d_step(x, w, state, slots)
@@ -143,9 +145,9 @@ def causal_conv1d_step(x, w, state, slots=None):
   if w.dtype is not torch.bfloat16 or not w.is_contiguous():
     w = w.detach().to(torch.bfloat16).contiguous()
   slots = _lib.index_table(slots, "slots")
-  y = torch.empty((b, c), dtype=torch.bfloat16, device=x.device)
+  y = x.new_empty(xs)
   if b > 0:
-    check(lib.lewi_causal_conv1d_step(stream(), x.data_ptr(), x_rows, ptr(w), ptr(state), ptr(slots), y.data_ptr(), b, state.shape[0], c, k),
+    check(lib.lewi_causal_conv1d_step(stream(), x.data_ptr(), x_rows, ptr(w), ptr(state), ptr(slots), y.data_ptr(), b, ss[0], c, k),
           "lewi_causal_conv1d_step")
   return y
 
@@ -158,25 +160,27 @@ def gated_delta_step(query, key, value, g, beta, state, slots=None):
   Rows of the batch may lie apart (views of one projection need no copy).  Not differentiable.  Everything is float32 inside, where
   `chunk_gated_delta_rule` rounds some products to bf16 as the reference does, so the two agree to bf16's precision."""
   lib = _lib.load()
-  if not query.dtype == key.dtype == value.dtype == torch.bfloat16 or state.dtype != torch.float32:
+  if not query.dtype is key.dtype is value.dtype is torch.bfloat16 or state.dtype is not torch.float32:
     raise LewiError("gated_delta_step takes bfloat16 q, k, v and a float32 state")
-  if query.dim() != 3 or key.shape != query.shape or value.dim() != 3 or value.shape[0] != query.shape[0]:
+  qs, vs, ss = query.shape, value.shape, state.shape
+  if len(qs) != 3 or key.shape != qs or len(vs) != 3 or vs[0] != qs[0]:
     raise LewiError("gated_delta_step: query, key [B,Hk,K] and value [B,H,V] are required")
-  (b, hk, kd), (_, h, vd) = query.shape, value.shape
-  if state.dim() != 4 or state.shape[1:] != (h, kd, vd):
+  (b, hk, kd), (_, h, vd) = qs, vs
+  if len(ss) != 4 or ss[1] != h or ss[2] != kd or ss[3] != vd:
     raise LewiError("gated_delta_step: state [N,H,K,V] is required")
-  if g.shape != (b, h) or beta.shape != (b, h):
+  if g.shape != vs[:2] or beta.shape != vs[:2]:
     raise LewiError("gated_delta_step: g and beta [B,H] are required")
-  _check_slots("gated_delta_step", b, state, slots)
-  if g.dtype not in _GATES or beta.dtype not in _GATES:
+  _check_slots("gated_delta_step", b, ss[0], slots)
+  g_type, beta_type = _GATES.get(g.dtype), _GATES.get(beta.dtype)
+  if g_type is None or beta_type is None:
     raise LewiError("gated_delta_step takes float32 or bfloat16 g and beta")
   if _lib.elsewhere(query, key, value, g, beta, state, slots):
     with torch.cuda.device(query.device):
       return gated_delta_step(query, key, value, g, beta, state, slots)
-  (q, qs), (k, ks), (v, vs) = _lib.rows_of(query, 2), _lib.rows_of(key, 2), _lib.rows_of(value, 2)
+  (q, q_rows), (k, k_rows), (v, v_rows) = _lib.rows_of(query, 2), _lib.rows_of(key, 2), _lib.rows_of(value, 2)
   g, beta, slots = g.contiguous(), beta.contiguous(), _lib.index_table(slots, "slots")
-  o = torch.empty((b, h, vd), dtype=torch.bfloat16, device=q.device)
+  o = v.new_empty(vs)
   if b > 0:
-    check(lib.lewi_gdn_step(stream(), q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, g.data_ptr(), _GATES[g.dtype], beta.data_ptr(),
-                            _GATES[beta.dtype], ptr(state), ptr(slots), o.data_ptr(), b, state.shape[0], hk, h, kd, vd), "lewi_gdn_step")
+    check(lib.lewi_gdn_step(stream(), q.data_ptr(), q_rows, k.data_ptr(), k_rows, v.data_ptr(), v_rows, g.data_ptr(), g_type, beta.data_ptr(),
+                            beta_type, ptr(state), ptr(slots), o.data_ptr(), b, ss[0], hk, h, kd, vd), "lewi_gdn_step")
   return o
