@@ -48,7 +48,7 @@ struct Item {
 // Items are numbered by falling unit, all shares of a unit together, and CTA c has the items c, 2 n - 1 - c, 2 n + c, 4 n - 1 - c, .. of n
 // CTAs: long runs first, and about as much work for everybody, whatever the lengths.  No table is needed: F(i) = sum_s max(0, units(s) - i)
 // counts the units from number i on, so the x-th unit's number is the largest i with F(i) > x, and its sequence is the
-// (x - F(i + 1))-th of those that have it.
+// (x - F(i + 1))-th of those that have it.  A search is for a new number only; the sequences that have the same one are walked through.
 constexpr int kPlanned = 448;   // sequences whose units are kept in shared memory (further ones are looked up again)
 struct Plan {
   int4 item[2];
@@ -80,42 +80,40 @@ __device__ __forceinline__ void plan_items(const Seqs& q, int rows, int subs, Pl
     return __reduce_add_sync(0xffffffffu, v);
   };
   const int all = alike ? most * q.n : count(0);
-  int top = most;   // F(top) <= the next x
+  int lo = most, first = 0, end = 0;   // the unit number of the last item, F(lo + 1) and F(lo): units of this number are the x in between
+  int s0 = 0, passed = 0;              // the sequences before s0 have `passed` of them
   for (int r = 0;; ++r) {
     const long long id = (long long)r * n + ((r & 1) != 0 ? n - 1 - c : c);
     const int x = (int)min(id / subs, 0x7fffffffll);
     Item item{0, 0, -1, 0};
     if (x < all) {
-      item.sub = (int)(id % subs);
-      int s, lo = 0;
+      int s;
       if (alike) {
         lo = most - 1 - x / q.n;
         s = x % q.n;
       } else {
-        int hi = top;   // F(lo) > x, F(hi) <= x
-        while (hi - lo > 1) {
-          const int mid = (lo + hi) >> 1;
-          if (count(mid) > x) lo = mid;
-          else hi = mid;
-        }
-        int rank = x - count(lo + 1);
-        top = lo + 1;
-        s = 0;
-        for (int s0 = 0; s0 < q.n; s0 += 32) {
-          unsigned have = __ballot_sync(0xffffffffu, s0 + lane < q.n && units(min(s0 + lane, q.n - 1)) > lo);
-          if (rank >= __popc(have)) {
-            rank -= __popc(have);
-            continue;
+        if (x >= end) {
+          int hi = lo;   // F(hi) <= x
+          for (lo = 0; hi - lo > 1;) {
+            const int mid = (lo + hi) >> 1;
+            if (count(mid) > x) lo = mid;
+            else hi = mid;
           }
-          for (; rank > 0; --rank) have &= have - 1;
-          s = s0 + __ffs(have) - 1;
-          break;
+          first = count(lo + 1);
+          end = count(lo);
+          s0 = passed = 0;
         }
+        unsigned have;   // of 32 sequences those that have the unit
+        for (;; s0 += 32) {
+          have = __ballot_sync(0xffffffffu, s0 + lane < q.n && units(min(s0 + lane, q.n - 1)) > lo);
+          if (x - first < passed + __popc(have) || s0 + 32 >= q.n) break;
+          passed += __popc(have);
+        }
+        for (int rank = x - first - passed; rank > 0; --rank) have &= have - 1;
+        s = min(s0 + max(__ffs(have) - 1, 0), q.n - 1);
       }
       const Rows of = rows_of(q, s);
-      item.start = of.start;
-      item.len = of.len;
-      item.level = lo;
+      item = {of.start, of.len, lo, (int)(id % subs)};
     }
     if (!give(r, item) || item.level < 0) return;
   }
