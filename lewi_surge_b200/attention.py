@@ -92,7 +92,7 @@ def _attention_fwd(q, k, v, cu, n_seqs, scale):
   (q, q_rows), (k, k_rows), (v, v_rows) = _lib.rows_of(q, 16), _lib.rows_of(k, 16), _lib.rows_of(v, 16)
   cu = _lib.index_table(cu, "cu_seqlens")
   t, hq, d = q.shape
-  o = torch.empty((t, hq, d), dtype=torch.bfloat16, device=q.device)
+  o = q.new_empty((t, hq, d))
   lse = torch.empty((hq, t), dtype=torch.float32, device=q.device)
   check(_lib.load().lewi_causal_attention_fwd(stream(), q.data_ptr(), q_rows, k.data_ptr(), k_rows, v.data_ptr(), v_rows, ptr(cu), n_seqs,
                                               o.data_ptr(), lse.data_ptr(), t, hq, k.shape[1], d, scale), "lewi_causal_attention_fwd")
@@ -136,27 +136,30 @@ def causal_attention(query, key, value, cu_seqlens=None, scale=None):
 
   A value of v that is not finite reaches back to the start of its 128 rows of the sequence (as those of q, k and the upstream gradient do in the
   gradients), never into another sequence."""
-  if not query.dtype == key.dtype == value.dtype == torch.bfloat16:
+  if not query.dtype is key.dtype is value.dtype is torch.bfloat16:
     raise LewiError("causal_attention takes bfloat16 q, k, v")
-  if query.dim() not in (3, 4) or key.dim() != query.dim() or value.shape != key.shape or query.shape[:-2] != key.shape[:-2] or \
-      query.shape[-1] != key.shape[-1] or key.shape[-2] == 0 or query.shape[-2] % key.shape[-2]:
+  shape, other = query.shape, key.shape
+  n = len(shape)
+  if n not in (3, 4) or len(other) != n or value.shape != other or shape[:-2] != other[:-2] or shape[-1] != other[-1] or other[-2] == 0 or \
+      shape[-2] % other[-2]:
     raise LewiError("causal_attention: query [T, Hq, D] and key, value [T, Hkv, D], or all three [B, S, ..], Hq a multiple of Hkv, are required")
-  if cu_seqlens is not None and (query.dim() == 4 or cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 2):
-    raise LewiError("causal_attention: cu_seqlens [N + 1] belongs to packed rows [T, H, D]")
-  scale = query.shape[-1] ** -0.5 if scale is None else float(scale)
+  n_seqs = 1 if n == 3 else shape[0]
+  if cu_seqlens is not None:
+    if n == 4 or cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 2:
+      raise LewiError("causal_attention: cu_seqlens [N + 1] belongs to packed rows [T, H, D]")
+    n_seqs = cu_seqlens.shape[0] - 1
+  scale = shape[-1] ** -0.5 if scale is None else float(scale)
   if not scale > 0:
     raise LewiError("causal_attention: scale must be positive")
-  shape = query.shape
-  n_seqs = 1 if query.dim() == 3 else shape[0]
-  if query.dim() == 4:
-    query, key, value = (x.reshape(-1, *x.shape[2:]) for x in (query, key, value))
-  if cu_seqlens is not None:
-    n_seqs = cu_seqlens.shape[0] - 1
   if query.numel() == 0:
     return query.clone()
   if _lib.elsewhere(query, key, value, cu_seqlens):
     with torch.cuda.device(query.device):
-      return causal_attention(query.view(shape), key.view(*shape[:-2], *key.shape[-2:]), value.view(*shape[:-2], *key.shape[-2:]), cu_seqlens, scale)
+      return causal_attention(query, key, value, cu_seqlens, scale)
+  if n == 4:
+    query, key, value = (x.reshape(-1, *x.shape[2:]) for x in (query, key, value))
   if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad):
-    return _CausalAttention.apply(query, key, value, cu_seqlens, n_seqs, scale).view(shape)
-  return _attention_fwd(query, key, value, cu_seqlens, n_seqs, scale)[0].view(shape)
+    o = _CausalAttention.apply(query, key, value, cu_seqlens, n_seqs, scale)
+  else:
+    o = _attention_fwd(query, key, value, cu_seqlens, n_seqs, scale)[0]
+  return o if n == 3 else o.view(shape)

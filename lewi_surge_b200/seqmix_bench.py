@@ -1,6 +1,6 @@
-"""Times the two sequence-mixing operators on one GPU: `python -m lewi_surge_b200.seqmix_bench [--b 8 --s 4096 ...]`.
+"""Times the sequence-mixing operators on one GPU: `python -m lewi_surge_b200.seqmix_bench [--b 8 --s 4096 ...]`.
 
-Prints one line per operator (forward, forward+backward) from CUDA events around `--steps` calls after two warm-up
+Prints one line per operator (forward, forward+backward, or a decode step) from CUDA events around `--steps` calls after two warm-up
 calls.  With `--steps` small it is also the program to put under a profiler."""
 from __future__ import annotations
 
@@ -8,7 +8,7 @@ import argparse
 
 import torch
 
-from . import seqmix
+from . import attention, seqmix
 
 
 def main():
@@ -21,7 +21,12 @@ def main():
   ap.add_argument("--channels", type=int, default=4096, help="channels of the causal convolution")
   ap.add_argument("--taps", type=int, default=4)
   ap.add_argument("--steps", type=int, default=10)
-  ap.add_argument("--only", choices=["gdn", "conv"], default=None)
+  ap.add_argument("--heads", type=int, default=16, help="query heads of the attention")
+  ap.add_argument("--kv-heads", type=int, default=2)
+  ap.add_argument("--d", type=int, default=128, help="head dimension of the attention")
+  ap.add_argument("--rows", type=int, default=256, help="rows of a decode step")
+  ap.add_argument("--page", type=int, default=64)
+  ap.add_argument("--only", choices=["gdn", "conv", "attention", "step", "paged"], default=None)
   a = ap.parse_args()
   dev = torch.device("cuda:0")
   gen = torch.Generator(device=dev).manual_seed(0)
@@ -61,6 +66,34 @@ def main():
     nbytes = 2 * a.b * a.s * a.channels * 2
     print(f"causal conv B={a.b} T={a.s} C={a.channels} taps={a.taps}: forward {fwd:.4f} ms ({nbytes / fwd / 1e6:.0f} GB/s), "
           f"forward+backward {both:.4f} ms")
+  if a.only in (None, "attention"):
+    q, k, v = (rn(a.b, a.s, n, a.d).bfloat16().requires_grad_(True) for n in (a.heads, a.kv_heads, a.kv_heads))
+    d_o = rn(a.b, a.s, a.heads, a.d).bfloat16()
+    with torch.no_grad():
+      fwd = timed(lambda: attention.causal_attention(q, k, v))
+    both = timed(lambda: torch.autograd.grad(attention.causal_attention(q, k, v), (q, k, v), d_o))
+    flops = 2 * a.b * a.s * (a.s + 1) * a.heads * a.d
+    print(f"causal attention B={a.b} S={a.s} heads={a.heads}/{a.kv_heads} D={a.d}: forward {fwd:.3f} ms ({flops / fwd / 1e9:.0f} TFLOP/s), "
+          f"forward+backward {both:.3f} ms ({3.5 * flops / both / 1e9:.0f} TFLOP/s)")
+  if a.only in (None, "step"):
+    x, w, past = rn(a.rows, a.channels).bfloat16(), rn(a.taps, 1, a.channels).bfloat16(), rn(a.rows, a.taps - 1, a.channels).bfloat16()
+    conv = timed(lambda: seqmix.causal_conv1d_step(x, w, past))
+    q, k, v = (rn(a.rows, a.h, n).bfloat16() for n in (a.k, a.k, a.v))
+    k = (k / a.k ** 0.5).bfloat16()
+    g, beta, state = -torch.rand(a.rows, a.h, generator=gen, device=dev), torch.rand(a.rows, a.h, generator=gen, device=dev), rn(a.rows, a.h, a.k, a.v)
+    step = timed(lambda: seqmix.gated_delta_step(q, k, v, g, beta, state))
+    print(f"steps of {a.rows} rows: causal conv C={a.channels} taps={a.taps} {conv * 1e3:.1f} us, gated delta rule H={a.h} K={a.k} V={a.v} "
+          f"{step * 1e3:.1f} us ({8 * state.numel() / step / 1e6:.0f} GB/s)")
+  if a.only in (None, "paged"):
+    per = -(-a.s // a.page)
+    kc, vc = (rn(a.b * per, a.page, a.kv_heads, a.d).bfloat16() for _ in range(2))
+    tables = torch.randperm(a.b * per, generator=gen, device=dev).view(a.b, per).int()
+    lengths = torch.full((a.b,), a.s, dtype=torch.int32, device=dev)
+    q, k, v = (rn(a.b, n, a.d).bfloat16() for n in (a.heads, a.kv_heads, a.kv_heads))
+    write = timed(lambda: attention.paged_cache_write(k, v, kc, vc, tables, lengths))
+    att = timed(lambda: attention.paged_attention(q, kc, vc, tables, lengths))
+    print(f"paged cache B={a.b} tokens={a.s} heads={a.heads}/{a.kv_heads} D={a.d} page={a.page}: write {write * 1e3:.1f} us, attention of one token "
+          f"{att * 1e3:.1f} us ({4 * a.b * a.s * a.kv_heads * a.d / att / 1e6:.0f} GB/s)")
 
 
 if __name__ == "__main__":

@@ -254,3 +254,64 @@ def test_a_prompt_and_the_tokens_after_it_are_one_sequence(cuda):
   for b, n in enumerate(lens):
     want = formulas(*rows[b], [0, n + more], d ** -0.5)["o"]
     within(torch.cat([g[b] for g in got]), want, f"sequence {b}")
+
+
+@pytest.mark.gpu
+def test_more_sequences_than_are_kept_in_shared_memory(cuda):
+  gen = torch.Generator().manual_seed(7)
+  lens = torch.randint(0, 30, (1500,), generator=gen).tolist()
+  lens[700], lens[701] = 300, 131
+  hq, hkv, d, t = 2, 1, 32, sum(lens)
+  cu = torch.tensor([0] + lens).cumsum(0)
+  q, k, v, d_o = (rnd(gen, t, h, d) for h in (hq, hkv, hkv, hq))
+  want = formulas(q, k, v, cu.tolist(), d ** -0.5, d_o)
+  leaves = [x.to(cuda).requires_grad_(True) for x in (q, k, v)]
+  o = attention.causal_attention(*leaves, cu.to(cuda))
+  within(o, want["o"], "o")
+  for name, g in zip(("dq", "dk", "dv"), torch.autograd.grad(o, leaves, d_o.to(cuda))):
+    within(g, want[name], name)
+  assert _lib.last_status() == 0
+
+
+@pytest.mark.gpu
+def test_rows_past_32_bits_of_offset(cuda):
+  """Rows that begin behind 2^31 elements: the last sequences of many are what they are alone, bit for bit."""
+  n, s, h, d = 4200, 128, 32, 128
+  gen = torch.Generator(device=cuda).manual_seed(1)
+  assert n * s * h * d > 2 ** 31
+  q, k, v, d_o = (torch.randn(n * s, h, d, generator=gen, device=cuda, dtype=torch.bfloat16) for _ in range(4))
+  def call(rows):
+    leaves = [x[rows].detach().requires_grad_(True) for x in (q, k, v)]
+    m = leaves[0].shape[0] // s
+    o = attention.causal_attention(*leaves, torch.arange(0, m * s + 1, s, device=cuda))
+    return o.detach(), *torch.autograd.grad(o, leaves, d_o[rows])
+  whole = call(slice(0, n * s))
+  for got, want in zip(whole, call(slice((n - 3) * s, n * s))):
+    assert torch.equal(got[-3 * s:], want)
+  assert _lib.last_status() == 0
+
+
+@pytest.mark.gpu
+def test_shared_operands_and_modes(cuda):
+  """One tensor in three places, keys broadcast over heads, no gradient wanted: the values and gradients of separate operands."""
+  gen = torch.Generator().manual_seed(9)
+  x, w, d_o = rnd(gen, 260, 4, 64).to(cuda).requires_grad_(True), rnd(gen, 260, 1, 64).to(cuda).requires_grad_(True), rnd(gen, 260, 4, 64).to(cuda)
+  parts = [x.detach().clone().requires_grad_(True) for _ in range(3)]
+  o = attention.causal_attention(x, x, x)
+  g, = torch.autograd.grad(o, x, d_o)
+  o3 = attention.causal_attention(*parts)
+  gs = torch.autograd.grad(o3, parts, d_o)
+  assert torch.equal(o, o3) and torch.allclose(g.float(), sum(p.float() for p in gs), rtol=2 * U, atol=0.1)   # (autograd adds them in bf16)
+  with torch.no_grad():
+    assert torch.equal(attention.causal_attention(x, x, x), o)
+  with torch.inference_mode():
+    assert torch.equal(attention.causal_attention(x, x, x), o)
+  wide = w.expand(260, 4, 64)
+  a, = torch.autograd.grad(attention.causal_attention(x.detach(), wide, x.detach()), w, d_o)
+  full = w.detach().expand(260, 4, 64).clone().requires_grad_(True)
+  b, = torch.autograd.grad(attention.causal_attention(x.detach(), full, x.detach()), full, d_o)
+  assert torch.equal(a, b.sum(1, keepdim=True))
+  turned = x.detach().transpose(0, 1).contiguous().transpose(0, 1)   # heads outside
+  assert torch.equal(attention.causal_attention(turned, turned, turned), o)
+  shifted = torch.cat([x.detach().flatten()[:1], x.detach().flatten()])[1:].view(260, 4, 64)   # two bytes off
+  assert torch.equal(attention.causal_attention(shifted, shifted, shifted), o)

@@ -381,3 +381,47 @@ def test_two_streams_at_once(cuda):
   torch.cuda.synchronize()
   for i in range(2):
     assert all(torch.equal(g, want[i]) for g in got[i])
+
+
+@pytest.mark.gpu
+def test_states_past_32_bits_of_offset(cuda):
+  """A pool whose last states begin behind 2^31 elements."""
+  n, h, kd = 4200, 32, 128
+  assert n * h * kd * kd > 2 ** 31
+  gen = torch.Generator().manual_seed(8)
+  i = {m: t.to(cuda) for m, t in delta_inputs(gen, 2, 2, h, h, kd, kd).items()}
+  pool = torch.empty(n, h, kd, kd, device=cuda)
+  pool[-2:] = i["state"]
+  o = seqmix.gated_delta_step(*(i[m] for m in ("q", "k", "v", "g", "beta")), pool, torch.tensor([n - 2, n - 1], device=cuda))
+  o2 = seqmix.gated_delta_step(*(i[m] for m in ("q", "k", "v", "g", "beta", "state")))
+  assert torch.equal(o, o2) and torch.equal(pool[-2:], i["state"]) and _lib.last_status() == 0
+
+
+@pytest.mark.gpu
+def test_rows_at_any_distance_and_address(cuda):
+  """Rows apart, transposed, two bytes off: the results of packed rows."""
+  gen = torch.Generator().manual_seed(10)
+  b, h, kd = 5, 4, 32
+  i = {m: t.to(cuda) for m, t in delta_inputs(gen, b, b, h, h, kd, kd).items()}
+  want_state = i["state"].clone()
+  want = seqmix.gated_delta_step(i["q"], i["k"], i["v"], i["g"], i["beta"], want_state)
+  off = lambda t: torch.cat([t.flatten()[:1], t.flatten()])[1:].view(t.shape)
+  turned = lambda t: t.transpose(0, 1).contiguous().transpose(0, 1)
+  apart = lambda t: torch.cat([t, t, t], 1)[:, :t.shape[1]]
+  for f in (off, turned, apart):
+    state = i["state"].clone()
+    got = seqmix.gated_delta_step(f(i["q"]), f(i["k"]), f(i["v"]), f(i["g"]), f(i["beta"]), state)
+    assert torch.equal(got, want) and torch.equal(state, want_state)
+  kc, vc = rnd(gen, 6, 16, 2, 64).to(cuda), rnd(gen, 6, 16, 2, 64).to(cuda)
+  tables, lens, q = torch.tensor([[0, 1], [2, 3], [4, 5]], device=cuda), torch.tensor([20, 3, 32], device=cuda), rnd(gen, 3, 4, 64).to(cuda)
+  want = attention.paged_attention(q, kc, vc, tables, lens)
+  k = rnd(gen, 3, 2, 64).to(cuda)
+  for f in (off, turned, apart):
+    assert torch.equal(attention.paged_attention(f(q), kc, vc, f(tables), lens), want)
+    one, two = [c.clone() for c in (kc, vc)], [c.clone() for c in (kc, vc)]
+    attention.paged_cache_write(k, k, *one, tables, lens)
+    attention.paged_cache_write(f(k), f(k), *two, f(tables), f(lens[:, None])[:, 0])
+    assert all(torch.equal(x, y) for x, y in zip(one, two))
+  state = torch.zeros(h, kd, kd, device=cuda).expand(b, h, kd, kd)
+  with pytest.raises(LewiError):
+    seqmix.gated_delta_step(i["q"], i["k"], i["v"], i["g"], i["beta"], state)   # a pool that is not a pool
