@@ -229,7 +229,7 @@ struct Args {
 
 // A warp's 32 rows x 64 bytes go through shared memory (2 KB of its own), so that a store writes 8 rows x 64 bytes and not a piece of each of
 // 32 rows (which took 3700 cycles for a tile of 128 x 128 bf16).  `v`: this lane's row; rows dst + r * stride for r < valid, `bytes` of the 64.
-constexpr int kStaging = 8 * 2048, kBarriers = 384;
+constexpr int kStaging = 8 * 2048, kBarriers = 512;
 __device__ __forceinline__ void store_rows(uint8_t* stage, const uint32_t (&v)[16], uint8_t* dst, long long stride, int valid, int bytes) {
   const int lane = threadIdx.x & 31;
   uint4* mine = reinterpret_cast<uint4*>(stage) + lane * 4;
@@ -606,12 +606,13 @@ __global__ void __launch_bounds__(kDeltaThreads) delta_kernel(const __nv_bfloat1
 // An item is a tile of keys: its CTA works through the queries that see it, head by head of the group (or of a part of it: dkv_parts), so that
 // dK and dV stay in tensor memory and no sum needs an atomic.  Scores transposed (a row is a key): P^T and dS^T are the A operands of
 // dV = P^T dO and dK = dS^T Q.  Warps 0-7: elementwise, a thread has 64 of the 128 queries of a row; warp 8: TMA; warp 9: MMA; warp 10: items;
-// warp 11: lse and delta, and the rows of other sequences in a tile.  Order of products: S(0) dP(0) | dV(i) S(i+1) after P(i), dK(i) dP(i+1) after dS(i): exponentials are made while
-// dK and dP run, dS while dV and S do.
+// warp 11: lse and delta, and the rows of other sequences in a tile.  Scores have kScores places, P(i) takes that of S(i).  Order of products:
+// S(0) dP(0) .. S(kScores - 1) | dV(i) S(i + kScores) after P(i), dK(i) dP(i+1) after dS(i): exponentials are made while dK and dP
+// run, dS while dV and S do, and with two places, which dV and dK leave at D <= 64, the next scores are there when dS has been made.
 constexpr int kBwdThreads = 384;
 template <int DP>
 struct DkvShape {
-  static constexpr int kStages = 2;
+  static constexpr int kScores = DP == 64 ? 2 : 1, kStages = DP == 64 ? 4 : 2;
   static constexpr int kSmem = (2 + 2 * kStages) * kTileBytes<DP> + kStaging + kStages * 2 * kTile * 4 + kBarriers;
 };
 
@@ -619,7 +620,7 @@ template <int DP>
 __global__ void __launch_bounds__(kBwdThreads, 1) dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                                                              const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
                                                              const Args a) {
-  constexpr int ST = DkvShape<DP>::kStages, TB = kTileBytes<DP>;
+  constexpr int ST = DkvShape<DP>::kStages, NS = DkvShape<DP>::kScores, TB = kTileBytes<DP>;
   extern __shared__ __align__(1024) uint8_t attn_smem[];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
@@ -633,7 +634,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dkv_kernel(const __grid_consta
   const uint32_t k_at = base, v_at = base + TB, ring = base + 2 * TB;   // [stage][Q, dO]
   float* stats = reinterpret_cast<float*>(attn_smem + (2 + 2 * ST) * TB + kStaging);   // [stage][-lse, -delta][128]
   const uint32_t bars = base + (2 + 2 * ST) * TB + kStaging + ST * 2 * kTile * 4;
-  const uint32_t k_full = bars, v_full = bars + 8, s_full = bars + 16, dp_full = bars + 24, p_ready = bars + 32, ds_ready = bars + 40, acc_full = bars + 48,
+  const uint32_t k_full = bars, v_full = bars + 8, dp_full = bars + 24, p_ready = bars + 32, ds_ready = bars + 40, acc_full = bars + 48,
                  k_empty = bars + 64, v_empty = bars + 72, acc_empty = bars + 80;
   auto q_full = [&](int n) { return bars + 88u + 8u * (n % ST); };
   auto q_empty = [&](int n) { return bars + 88u + 8u * (ST + n % ST); };
@@ -643,10 +644,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dkv_kernel(const __grid_consta
   auto st_empty = [&](int n) { return bars + 88u + 8u * (5 * ST + n % ST); };
   auto q_raw = [&](int n) { return bars + 88u + 8u * (6 * ST + n % ST); };
   auto do_raw = [&](int n) { return bars + 88u + 8u * (7 * ST + n % ST); };
+  auto s_full = [&](int n) { return bars + 88u + 8u * (8 * ST + n % NS); };
   volatile int* abort_flag = &s_abort;
-  const ItemQueue items{&s_plan, bars + 88u + 8u * (8 * ST), abort_flag};
+  const ItemQueue items{&s_plan, bars + 88u + 8u * (8 * ST + NS), abort_flag};
   if (threadIdx.x == 0) {
-    for (uint32_t b : {k_full, v_full, k_empty, v_empty, s_full, dp_full, acc_full}) ptx::mbar_init(b, 1);
+    for (uint32_t b : {k_full, v_full, k_empty, v_empty, dp_full, acc_full}) ptx::mbar_init(b, 1);
+    for (int n = 0; n < NS; ++n) ptx::mbar_init(s_full(n), 1);
     for (uint32_t b : {p_ready, ds_ready, acc_empty}) ptx::mbar_init(b, 8);
     for (int s = 0; s < ST; ++s) {
       for (uint32_t b : {q_full(s), q_empty(s), do_full(s), do_empty(s), st_full(s), q_raw(s), do_raw(s)}) ptx::mbar_init(b, 1);
@@ -668,7 +671,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dkv_kernel(const __grid_consta
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
-  const uint32_t tmem = s_tmem, t_s = tmem, t_dp = tmem + 128, t_dv = tmem + 256, t_dk = tmem + 384;
+  const uint32_t tmem = s_tmem, t_dp = tmem + NS * 128, t_dv = t_dp + 128, t_dk = t_dv + DP;
+  auto t_s = [&](int n) { return tmem + n % NS * 128; };
 
   // An item's products: tile `key` of the keys with the tiles key .. key + per_head - 1 of the queries, head by head.
   struct Span {
@@ -734,8 +738,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dkv_kernel(const __grid_consta
           const int x = n + it;
           if (!ptx::mbar_wait(q_full(x), x / ST & 1, abort_flag)) return false;
           ptx::tc_fence_after();
-          mma_kk<DP>(t_s, k_at, ring + x % ST * 2 * TB, id_s);
-          ptx::mma_commit(s_full);
+          mma_kk<DP>(t_s(x), k_at, ring + x % ST * 2 * TB, id_s);
+          ptx::mma_commit(s_full(x));
           if (it + 1 == n_it) ptx::mma_commit(k_empty);
           return true;
         };
@@ -748,15 +752,16 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dkv_kernel(const __grid_consta
           if (it + 1 == n_it) ptx::mma_commit(v_empty);
           return true;
         };
-        ok = ptx::mbar_wait(k_full, r & 1, abort_flag) && scores(0) && ptx::mbar_wait(v_full, r & 1, abort_flag) && dps(0);
+        ok = ptx::mbar_wait(k_full, r & 1, abort_flag) && scores(0) && ptx::mbar_wait(v_full, r & 1, abort_flag) && dps(0) &&
+             (NS == 1 || n_it == 1 || scores(1));
         for (int it = 0; ok && it < n_it; ++it) {
           const int x = n + it, at = ring + x % ST * 2 * TB;
           ok = ptx::mbar_wait(p_ready, x & 1, abort_flag) && (it > 0 || ptx::mbar_wait(acc_empty, (r & 1) ^ 1u, abort_flag));
           if (!ok) break;
           ptx::tc_fence_after();
-          mma_tm<0, 8>(t_dv, t_s, at + TB, id_d, it > 0, 64);
+          mma_tm<0, 8>(t_dv, t_s(x), at + TB, id_d, it > 0, 64);
           ptx::mma_commit(do_empty(x));
-          if (it + 1 < n_it) ok = scores(it + 1);
+          if (it + NS < n_it) ok = scores(it + NS);
           ok = ok && ptx::mbar_wait(ds_ready, x & 1, abort_flag);
           if (!ok) break;
           ptx::tc_fence_after();
@@ -825,13 +830,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dkv_kernel(const __grid_consta
         const bool diagonal = it % sp.per_head == 0;
         const ulonglong2* lse = reinterpret_cast<const ulonglong2*>(stats + n % ST * 2 * kTile + half * 64);   // (both negative, in pairs)
         const ulonglong2* delta = reinterpret_cast<const ulonglong2*>(stats + (n % ST * 2 + 1) * kTile + half * 64);
-        ok = warp_wait(st_full(n), n / ST & 1, abort_flag) && warp_wait(s_full, n & 1, abort_flag);
+        ok = warp_wait(st_full(n), n / ST & 1, abort_flag) && warp_wait(s_full(n), n / NS & 1, abort_flag);
         if (!ok) break;
         ptx::tc_fence_after();
         F2 p[32];
         uint32_t x[2][32], out[32];
-        ptx::tmem_ld_32x32(t_s + lanes + half * 64, x[0]);
-        ptx::tmem_ld_32x32(t_s + lanes + half * 64 + 32, x[1]);
+        ptx::tmem_ld_32x32(t_s(n) + lanes + half * 64, x[0]);
+        ptx::tmem_ld_32x32(t_s(n) + lanes + half * 64 + 32, x[1]);
         ptx::tmem_ld_wait();
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
@@ -845,7 +850,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dkv_kernel(const __grid_consta
         }
 #pragma unroll
         for (int i = 0; i < 32; ++i) out[i] = f2_bf16(p[i]);
-        ptx::tmem_st_32x32(t_s + lanes + half * 64, out);
+        ptx::tmem_st_32x32(t_s(n) + lanes + half * 64, out);
         ptx::tmem_st_wait();
         ptx::tc_fence_before();
         __syncwarp();
