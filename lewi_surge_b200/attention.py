@@ -75,7 +75,7 @@ def paged_attention(query, key_cache, value_cache, block_tables, lengths, scale=
     with torch.cuda.device(query.device):
       return paged_attention(query, key_cache, value_cache, block_tables, lengths, scale)
   q, qs = _lib.rows_of(query, 4)
-  o = q.new_empty(shape)
+  o = torch.empty_like(q, memory_format=torch.contiguous_format)
   if b == 0 or hq == 0:
     return o
   tables, lens = _lib.index_table(block_tables, "block_tables"), _lib.index_table(lengths, "lengths")
@@ -92,7 +92,7 @@ def _attention_fwd(q, k, v, cu, n_seqs, scale):
   (q, q_rows), (k, k_rows), (v, v_rows) = _lib.rows_of(q, 16), _lib.rows_of(k, 16), _lib.rows_of(v, 16)
   cu = _lib.index_table(cu, "cu_seqlens")
   t, hq, d = q.shape
-  o = q.new_empty((t, hq, d))
+  o = torch.empty_like(q, memory_format=torch.contiguous_format)
   lse = torch.empty((hq, t), dtype=torch.float32, device=q.device)
   check(_lib.load().lewi_causal_attention_fwd(stream(), q.data_ptr(), q_rows, k.data_ptr(), k_rows, v.data_ptr(), v_rows, ptr(cu), n_seqs,
                                               o.data_ptr(), lse.data_ptr(), t, hq, k.shape[1], d, scale), "lewi_causal_attention_fwd")

@@ -62,6 +62,7 @@ int check_attention(const void* q, int64_t q_stride, const void* k, int64_t k_st
   if (!cu && T % n_seqs != 0) return LEWI_ERR_ARG;
   if (D > attn::kMaxD || T > 0x7fffffff - attn::kTile) return LEWI_ERR_LIMIT;
   if ((attn::most_tiles(T, n_seqs) + n_seqs) * Hq > 0x7fffffff) return LEWI_ERR_LIMIT;
+  if ((int64_t)T * (Hq / Hkv) > attn::kMaxGroupRows) return LEWI_ERR_LIMIT;
   if (D % 8 != 0 || Hq % Hkv != 0 || !aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(o, 16)) return LEWI_ERR_SHAPE;
   if (q_stride % 8 != 0 || k_stride % 8 != 0 || v_stride % 8 != 0) return LEWI_ERR_SHAPE;
   if (q_stride < (int64_t)Hq * D || k_stride < (int64_t)Hkv * D || v_stride < (int64_t)Hkv * D) return LEWI_ERR_SHAPE;

@@ -34,7 +34,7 @@ __device__ __forceinline__ long long cell_of(const Cache& c, int b, int pos) {
 // ---------------------------------------------------------------- write
 // Token i of sequence b (tokens cu[b] .. cu[b+1]; without cu one token per sequence) goes to cell lengths[b] - n_b + i.  A warp per
 // token: 16-byte pieces, every one requested before the first is stored.  Tokens of no sequence are left out; a token before
-// the cache's start or past its table raises LEWI_STATUS_BAD_INDEX and is left out.
+// the cache's start or past its table raises LEWI_STATUS_BAD_INDEX and is left out.  8191 tokens x 4 heads x 128 (34 MB): 5.7 us, 5.9 TB/s.
 constexpr int kWriteThreads = 128;
 struct WriteArgs {
   Cache c;
@@ -98,7 +98,8 @@ __global__ void __launch_bounds__(kWriteThreads) write_kernel(const WriteArgs a)
 // ---------------------------------------------------------------- attention of one token
 // o[b,h] = sum_j p_j v_j, p = softmax(scale q.k_j) over the sequence's cells; one pass with a running maximum and sum (float32).
 //
-// Bound by the cache's way from HBM: 4 Hkv D bytes per cell.  The cells of all sequences and key heads are one long list of tiles of
+// Bound by the cache's way from HBM: 4 Hkv D bytes per cell (64 sequences of up to 8192, 4 key heads, D = 128: 101 us, 5.3 TB/s, of which 15 us are
+// the first loads, which depend on one another, and the join).  The cells of all sequences and key heads are one long list of tiles of
 // 64 or 128 cells, of which every CTA takes an equal run, whatever the lengths (they are read on the device, so a captured launch follows
 // them).  The query heads that share a key head are the 16 rows of an `mma.sync` (m16n8k16), a warp's 16 cells (32 where D <= 64) its columns; a
 // warp has its own ring of tiles in shared memory (cp.async) and its own softmax, and nothing is synchronised before a head's
@@ -449,8 +450,8 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) attend_ke
 }
 
 // Adds up the parts of the heads that several CTAs worked on, in a fixed order, and writes zeros for sequences without cells.  `PER` warps
-// work on a query head and take every PER-th part each: 8 for few heads (one sequence of 100,001, 32 heads: 5 us, a warp each 19), one for many
-// (64 sequences x 32 heads: 5 us, eight each 16).
+// work on a query head and take every PER-th part each: 8 for few heads (one sequence of 100,001, 32 heads, the whole call: 73 us, with one
+// 83), one for many (64 sequences x 32 heads: 111, with eight 113).
 constexpr int kJoinWarps = 8;
 template <int TILE, int PER>
 __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const Args a) {

@@ -145,7 +145,7 @@ def causal_conv1d_step(x, w, state, slots=None):
   if w.dtype is not torch.bfloat16 or not w.is_contiguous():
     w = w.detach().to(torch.bfloat16).contiguous()
   slots = _lib.index_table(slots, "slots")
-  y = x.new_empty(xs)
+  y = torch.empty_like(x, memory_format=torch.contiguous_format)
   if b > 0:
     check(lib.lewi_causal_conv1d_step(stream(), x.data_ptr(), x_rows, ptr(w), ptr(state), ptr(slots), y.data_ptr(), b, ss[0], c, k),
           "lewi_causal_conv1d_step")
@@ -179,7 +179,7 @@ def gated_delta_step(query, key, value, g, beta, state, slots=None):
       return gated_delta_step(query, key, value, g, beta, state, slots)
   (q, q_rows), (k, k_rows), (v, v_rows) = _lib.rows_of(query, 2), _lib.rows_of(key, 2), _lib.rows_of(value, 2)
   g, beta, slots = g.contiguous(), beta.contiguous(), _lib.index_table(slots, "slots")
-  o = v.new_empty(vs)
+  o = torch.empty_like(v, memory_format=torch.contiguous_format)
   if b > 0:
     check(lib.lewi_gdn_step(stream(), q.data_ptr(), q_rows, k.data_ptr(), k_rows, v.data_ptr(), v_rows, g.data_ptr(), g_type, beta.data_ptr(),
                             beta_type, ptr(state), ptr(slots), o.data_ptr(), b, ss[0], hk, h, kd, vd), "lewi_gdn_step")

@@ -71,6 +71,7 @@ def test_refusals():
   lib, at = _lib.load(), 1 << 20   # (addresses that are never used)
   call = lambda q=at, qs=256, n=1, t=64, hq=4, hkv=2, d=64, scale=1.0: lib.lewi_causal_attention_fwd(None, q, qs, at, 128, at, 128, None, n, at, at, t, hq, hkv, d, scale)
   assert call(q=None) == -1 and call(t=0) == -1 and call(n=3) == -1 and call(scale=float("nan")) == -1
+  assert call(t=2 ** 25) == -5 and call(hq=64, qs=4096, t=2 ** 21) == -5
   assert call(q=at + 2) == -2 and call(qs=255) == -2 and call(qs=264 - 16) == -2 and call(hq=3) == -2 and call(d=60) == -2 and call(d=136) == -5
   bwd = lambda dq=at, dk=at, dv=at, ws=1 << 20: lib.lewi_causal_attention_bwd(None, at, 256, at, 128, at, 128, at, at, at, None, 1, dq, dk, dv, at, ws, 64, 4, 2, 64, 1.0)
   assert bwd(dq=None, dk=None, dv=None) == -1 and bwd(dv=None) == -1 and bwd(dq=at + 8) == -2 and bwd(ws=16) == -3
