@@ -62,7 +62,7 @@ def paged_cache_write(key, value, key_cache, value_cache, block_tables, lengths,
 def paged_attention(query, key_cache, value_cache, block_tables, lengths, scale=None):
   """Attention of one new token per sequence over the sequence's cells, its own among them (write it first): query [B, Hq, D] bf16 ->
   [B, Hq, D] bf16, head h with the keys of head h // (Hq // Hkv); zeros where lengths[b] is 0.  Caches and tables as in
-  `paged_cache_write`; D up to 256, a multiple of 8.  `scale` defaults to D ** -0.5.  Lengths and tables are read on the device, so a
+  `paged_cache_write`; D up to 256, a multiple of 8.  `scale` defaults to D ** -0.5.  Not differentiable.  Lengths and tables are read on the device, so a
   captured call follows them.  Cells past a sequence's length, whatever they hold, have no part in it; pages that do not exist
   and what a length has past its table are left out with `LEWI_STATUS_BAD_INDEX` in `_lib.last_status()`."""
   lib = _lib.load()
@@ -87,23 +87,23 @@ def paged_attention(query, key_cache, value_cache, block_tables, lengths, scale=
   return o
 
 
-def _attention_fwd(q, k, v, cu, n_seqs, scale):
-  """Output, log-sum-exp, the operands as the kernels read them and the distances of their rows."""
+def _attention_fwd(q, k, v, cu, n_seqs, scale, lse=None):
+  """Output, the operands as the kernels read them and the distances of their rows; `lse` [Hq, T] receives the log-sum-exp."""
   (q, q_rows), (k, k_rows), (v, v_rows) = _lib.rows_of(q, 16), _lib.rows_of(k, 16), _lib.rows_of(v, 16)
   cu = _lib.index_table(cu, "cu_seqlens")
   t, hq, d = q.shape
   o = torch.empty_like(q, memory_format=torch.contiguous_format)
-  lse = torch.empty((hq, t), dtype=torch.float32, device=q.device)
   check(_lib.load().lewi_causal_attention_fwd(stream(), q.data_ptr(), q_rows, k.data_ptr(), k_rows, v.data_ptr(), v_rows, ptr(cu), n_seqs,
-                                              o.data_ptr(), lse.data_ptr(), t, hq, k.shape[1], d, scale), "lewi_causal_attention_fwd")
-  return o, lse, q, k, v, cu, (q_rows, k_rows, v_rows)
+                                              o.data_ptr(), ptr(lse), t, hq, k.shape[1], d, scale), "lewi_causal_attention_fwd")
+  return o, q, k, v, cu, (q_rows, k_rows, v_rows)
 
 
 class _CausalAttention(torch.autograd.Function):
 
   @staticmethod
   def forward(ctx, q, k, v, cu, n_seqs, scale):
-    o, lse, q, k, v, cu, rows = _attention_fwd(q, k, v, cu, n_seqs, scale)
+    lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device)
+    o, q, k, v, cu, rows = _attention_fwd(q, k, v, cu, n_seqs, scale, lse)
     ctx.save_for_backward(q, k, v, o, lse, cu)
     ctx.call = n_seqs, scale, rows
     return o

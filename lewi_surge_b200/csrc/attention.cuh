@@ -222,7 +222,7 @@ struct Args {
   int Hq, Hkv, G, D;
   float scale, scale_log2;
   __nv_bfloat16* o;        // [T][Hq][D]
-  float *lse, *delta;      // [Hq][T], lse in units of log 2
+  float *lse, *delta;      // [Hq][T], lse in units of log 2 (null in a forward pass that none back follows)
   __nv_bfloat16 *dq, *dk, *dv;
   int parts;               // of a group's heads, one CTA each for dK and dV
   float* sums;             // [part][dV, dK][T][Hkv][D] where there are several
@@ -573,7 +573,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
 #pragma unroll
       for (int c = 0; c < DP / 32; ++c)
         store_rows(attn_smem + (2 + ST) * TB + warp * 2048, out[c], dst + c * 64, (long long)a.Hq * a.D * 2, valid, (a.D - c * 32) * 2);
-      if (lane < valid) a.lse[(long long)head * a.seqs.T + w.start + row0 + lane] = m * a.scale_log2 + log2f(l);
+      if (a.lse != nullptr && lane < valid) a.lse[(long long)head * a.seqs.T + w.start + row0 + lane] = m * a.scale_log2 + log2f(l);
     }
   }
   ptx::tc_fence_before();

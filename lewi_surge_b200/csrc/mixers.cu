@@ -57,8 +57,8 @@ int launch_paged(cudaStream_t st, const paged::Args& a) {
 
 // Checks of what forward and backward of causal attention share.
 int check_attention(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride, const int32_t* cu, int n_seqs,
-                    const void* o, const float* lse, int T, int Hq, int Hkv, int D, float scale) {
-  if (!q || !k || !v || !o || !lse || T <= 0 || n_seqs <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || !(scale > 0.f)) return LEWI_ERR_ARG;
+                    const void* o, int T, int Hq, int Hkv, int D, float scale) {
+  if (!q || !k || !v || !o || T <= 0 || n_seqs <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || !(scale > 0.f)) return LEWI_ERR_ARG;
   if (!cu && T % n_seqs != 0) return LEWI_ERR_ARG;
   if (D > attn::kMaxD || T > 0x7fffffff - attn::kTile) return LEWI_ERR_LIMIT;
   if ((attn::most_tiles(T, n_seqs) + n_seqs) * Hq > 0x7fffffff) return LEWI_ERR_LIMIT;
@@ -207,7 +207,7 @@ int lewi_paged_attention(void* stream, const void* q, int64_t q_stride, const vo
 
 int lewi_causal_attention_fwd(void* stream, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
                               const int32_t* cu_seqlens, int n_seqs, void* o, float* lse, int T, int Hq, int Hkv, int D, float scale) {
-  if (const int rc = check_attention(q, q_stride, k, k_stride, v, v_stride, cu_seqlens, n_seqs, o, lse, T, Hq, Hkv, D, scale)) return rc;
+  if (const int rc = check_attention(q, q_stride, k, k_stride, v, v_stride, cu_seqlens, n_seqs, o, T, Hq, Hkv, D, scale)) return rc;
   CUtensorMap tq, tk, tv;
   if (!attn::make_rows_map(&tq, q, T, Hq, D, q_stride) || !attn::make_rows_map(&tk, k, T, Hkv, D, k_stride) ||
       !attn::make_rows_map(&tv, v, T, Hkv, D, v_stride))
@@ -226,8 +226,8 @@ int64_t lewi_causal_attention_bwd_workspace_bytes(int T, int n_seqs, int Hq, int
 int lewi_causal_attention_bwd(void* stream, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
                               const void* o, const float* lse, const void* d_o, const int32_t* cu_seqlens, int n_seqs, void* dq, void* dk,
                               void* dv, void* workspace, int64_t workspace_bytes, int T, int Hq, int Hkv, int D, float scale) {
-  if (const int rc = check_attention(q, q_stride, k, k_stride, v, v_stride, cu_seqlens, n_seqs, o, lse, T, Hq, Hkv, D, scale)) return rc;
-  if (!d_o || (!dq && !dk) || !dk != !dv) return LEWI_ERR_ARG;
+  if (const int rc = check_attention(q, q_stride, k, k_stride, v, v_stride, cu_seqlens, n_seqs, o, T, Hq, Hkv, D, scale)) return rc;
+  if (!d_o || !lse || (!dq && !dk) || !dk != !dv) return LEWI_ERR_ARG;
   if (!aligned(d_o, 16) || !aligned(dq, 16) || !aligned(dk, 16) || !aligned(dv, 16)) return LEWI_ERR_SHAPE;
   if (!workspace || !aligned(workspace, 16) || workspace_bytes < lewi_causal_attention_bwd_workspace_bytes(T, n_seqs, Hq, Hkv, D))
     return LEWI_ERR_WORKSPACE;
