@@ -389,20 +389,20 @@ int lewi_paged_attention(void* stream, const void* q, int64_t q_stride, const vo
  * sequence, with the key head h / (Hq / Hkv).  q, o bf16 [T][Hq][D], k, v bf16 [T][Hkv][D]; sequence s has the rows
  * cu_seqlens[s] .. cu_seqlens[s+1] (i32 [n_seqs + 1], ascending; null: n_seqs sequences of T / n_seqs rows).  Rows of no sequence get zeros, in o
  * and in the gradients, whatever they hold.  Bounds that fall or leave the rows raise LEWI_STATUS_BAD_INDEX; what they cut is
- * undefined.  lse f32 [Hq][T] is for the backward pass (log2 of the softmax's denominator; rows of no sequence are left as they are; may be null where
- * none follows).
+ * undefined.  lse f32 [Hq][T] (log2 of the softmax's denominator) and o_rest bf16 [T][Hq][D] (what rounding o left
+ * of it) are for the backward pass and both null where none follows; their rows of no sequence are left as they are.
  * D <= 128, a multiple of 8; T * Hq / Hkv <= 2^25; scale > 0; all tensors 16-byte aligned, `*_stride` (elements from row to row; heads are contiguous) multiples
  * of 8.  Scores, softmax and sums float32; p and the gradient of the scores are rounded to bf16 for their products.
  * The backward call makes dq and/or dk and dv (bf16, contiguous; dk and dv together) out of d_o (bf16 [T][Hq][D], contiguous).  No
  * atomics: equal calls have equal bits.
  * ---------------------------------------------------------------------------------------------- */
 int lewi_causal_attention_fwd(void* stream, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
-                              int64_t v_stride, const int32_t* cu_seqlens, int n_seqs, void* o, float* lse, int T, int Hq, int Hkv, int D,
-                              float scale);
+                              int64_t v_stride, const int32_t* cu_seqlens, int n_seqs, void* o, void* o_rest, float* lse, int T, int Hq,
+                              int Hkv, int D, float scale);
 int64_t lewi_causal_attention_bwd_workspace_bytes(int T, int n_seqs, int Hq, int Hkv, int D);
 int lewi_causal_attention_bwd(void* stream, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
-                              int64_t v_stride, const void* o, const float* lse, const void* d_o, const int32_t* cu_seqlens, int n_seqs,
-                              void* dq, void* dk, void* dv, void* workspace, int64_t workspace_bytes, int T, int Hq, int Hkv, int D,
+                              int64_t v_stride, const void* o, const void* o_rest, const float* lse, const void* d_o, const int32_t* cu_seqlens,
+                              int n_seqs, void* dq, void* dk, void* dv, void* workspace, int64_t workspace_bytes, int T, int Hq, int Hkv, int D,
                               float scale);
 
 /* ------------------------------------------------------------------------------------------------

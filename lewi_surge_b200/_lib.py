@@ -80,9 +80,9 @@ SIGNATURES = {
     "lewi_paged_attention_workspace_bytes": (c_int64, [c_int]),
     "lewi_paged_attention": (c_int, [P, P, c_int64, P, P, c_int64, P, P, P, P, c_int64, c_int, c_int, c_int, c_int, c_int64, c_int, c_int,
                                      c_float]),
-    "lewi_causal_attention_fwd": (c_int, [P, P, c_int64, P, c_int64, P, c_int64, P, c_int, P, P] + [c_int] * 4 + [c_float]),
+    "lewi_causal_attention_fwd": (c_int, [P, P, c_int64, P, c_int64, P, c_int64, P, c_int, P, P, P] + [c_int] * 4 + [c_float]),
     "lewi_causal_attention_bwd_workspace_bytes": (c_int64, [c_int] * 5),
-    "lewi_causal_attention_bwd": (c_int, [P, P, c_int64, P, c_int64, P, c_int64, P, P, P, P, c_int, P, P, P, P, c_int64] + [c_int] * 4 +
+    "lewi_causal_attention_bwd": (c_int, [P, P, c_int64, P, c_int64, P, c_int64, P, P, P, P, P, c_int, P, P, P, P, c_int64] + [c_int] * 4 +
                                   [c_float]),
     "lewi_moe_residual_layout": (c_int64, [c_int64, c_int, c_int, c_int, c_int, c_int, c_int, P]),
     "lewi_moe_workspace_bytes": (c_int64, [c_int64, c_int, c_int, c_int, c_int, c_int, c_int]),

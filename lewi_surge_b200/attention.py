@@ -87,14 +87,15 @@ def paged_attention(query, key_cache, value_cache, block_tables, lengths, scale=
   return o
 
 
-def _attention_fwd(q, k, v, cu, n_seqs, scale, lse=None):
-  """Output, the operands as the kernels read them and the distances of their rows; `lse` [Hq, T] receives the log-sum-exp."""
+def _attention_fwd(q, k, v, cu, n_seqs, scale, o_rest=None, lse=None):
+  """Output, the operands as the kernels read them and the distances of their rows; `o_rest` like the output and `lse` [Hq, T] receive
+  what the backward pass needs."""
   (q, q_rows), (k, k_rows), (v, v_rows) = _lib.rows_of(q, 16), _lib.rows_of(k, 16), _lib.rows_of(v, 16)
   cu = _lib.index_table(cu, "cu_seqlens")
   t, hq, d = q.shape
   o = torch.empty_like(q, memory_format=torch.contiguous_format)
   check(_lib.load().lewi_causal_attention_fwd(stream(), q.data_ptr(), q_rows, k.data_ptr(), k_rows, v.data_ptr(), v_rows, ptr(cu), n_seqs,
-                                              o.data_ptr(), ptr(lse), t, hq, k.shape[1], d, scale), "lewi_causal_attention_fwd")
+                                              o.data_ptr(), ptr(o_rest), ptr(lse), t, hq, k.shape[1], d, scale), "lewi_causal_attention_fwd")
   return o, q, k, v, cu, (q_rows, k_rows, v_rows)
 
 
@@ -103,15 +104,16 @@ class _CausalAttention(torch.autograd.Function):
   @staticmethod
   def forward(ctx, q, k, v, cu, n_seqs, scale):
     lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device)
-    o, q, k, v, cu, rows = _attention_fwd(q, k, v, cu, n_seqs, scale, lse)
-    ctx.save_for_backward(q, k, v, o, lse, cu)
+    o_rest = torch.empty_like(q, memory_format=torch.contiguous_format)
+    o, q, k, v, cu, rows = _attention_fwd(q, k, v, cu, n_seqs, scale, o_rest, lse)
+    ctx.save_for_backward(q, k, v, o, o_rest, lse, cu)
     ctx.call = n_seqs, scale, rows
     return o
 
   @staticmethod
   def backward(ctx, g):
     lib = _lib.load()
-    q, k, v, o, lse, cu = ctx.saved_tensors
+    q, k, v, o, o_rest, lse, cu = ctx.saved_tensors
     n_seqs, scale, (q_rows, k_rows, v_rows) = ctx.call
     (t, hq, d), hkv = q.shape, k.shape[1]
     g, _ = _lib.rows_of(g.contiguous(), 16)
@@ -120,8 +122,9 @@ class _CausalAttention(torch.autograd.Function):
     dk, dv = (o.new_empty((t, hkv, d)), o.new_empty((t, hkv, d))) if need_k or need_v else (None, None)
     ws_bytes = lib.lewi_causal_attention_bwd_workspace_bytes(t, n_seqs, hq, hkv, d)
     ws = lse.new_empty((ws_bytes + 3) // 4)
-    check(lib.lewi_causal_attention_bwd(stream(), q.data_ptr(), q_rows, k.data_ptr(), k_rows, v.data_ptr(), v_rows, o.data_ptr(), lse.data_ptr(),
-                                        g.data_ptr(), ptr(cu), n_seqs, ptr(dq), ptr(dk), ptr(dv), ws.data_ptr(), ws_bytes, t, hq, hkv, d, scale),
+    check(lib.lewi_causal_attention_bwd(stream(), q.data_ptr(), q_rows, k.data_ptr(), k_rows, v.data_ptr(), v_rows, o.data_ptr(),
+                                        o_rest.data_ptr(), lse.data_ptr(), g.data_ptr(), ptr(cu), n_seqs, ptr(dq), ptr(dk), ptr(dv),
+                                        ws.data_ptr(), ws_bytes, t, hq, hkv, d, scale),
           "lewi_causal_attention_bwd")
     return dq, dk, dv, None, None, None
 

@@ -83,7 +83,7 @@ template <int DP>
 int attention_bwd(cudaStream_t st, const attn::Args& a, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& td,
                   const bf16* d_o) {
   const long long rows = (long long)a.seqs.T * a.Hq, per = attn::kDeltaThreads / (DP / 8);
-  attn::delta_kernel<DP><<<(unsigned)((rows + per - 1) / per), attn::kDeltaThreads, 0, st>>>(a.o, d_o, a.delta, a.seqs.T, a.Hq, a.D);
+  attn::delta_kernel<DP><<<(unsigned)((rows + per - 1) / per), attn::kDeltaThreads, 0, st>>>(a.o, a.o_rest, d_o, a.delta, a.seqs.T, a.Hq, a.D);
   LEWI_CHECK_LAUNCH();
   const long long tiles = attn::most_tiles(a.seqs.T, a.seqs.n);
   if (a.dk != nullptr) {
@@ -206,14 +206,17 @@ int lewi_paged_attention(void* stream, const void* q, int64_t q_stride, const vo
 // ------------------------------------------------------------------------------------------------ causal attention
 
 int lewi_causal_attention_fwd(void* stream, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
-                              const int32_t* cu_seqlens, int n_seqs, void* o, float* lse, int T, int Hq, int Hkv, int D, float scale) {
+                              const int32_t* cu_seqlens, int n_seqs, void* o, void* o_rest, float* lse, int T, int Hq, int Hkv, int D,
+                              float scale) {
   if (const int rc = check_attention(q, q_stride, k, k_stride, v, v_stride, cu_seqlens, n_seqs, o, T, Hq, Hkv, D, scale)) return rc;
+  if (!lse != !o_rest) return LEWI_ERR_ARG;
+  if (!aligned(o_rest, 16)) return LEWI_ERR_SHAPE;
   CUtensorMap tq, tk, tv;
   if (!attn::make_rows_map(&tq, q, T, Hq, D, q_stride) || !attn::make_rows_map(&tk, k, T, Hkv, D, k_stride) ||
       !attn::make_rows_map(&tv, v, T, Hkv, D, v_stride))
     return LEWI_ERR_CUDA;
-  const attn::Args a{{cu_seqlens, n_seqs, T}, Hq, Hkv, Hq / Hkv, D, scale, scale * 1.4426950408889634f, reinterpret_cast<bf16*>(o), lse,
-                     nullptr, nullptr, nullptr, nullptr, 1, nullptr};
+  const attn::Args a{{cu_seqlens, n_seqs, T}, Hq, Hkv, Hq / Hkv, D, scale, scale * 1.4426950408889634f, reinterpret_cast<bf16*>(o),
+                     reinterpret_cast<bf16*>(o_rest), lse, nullptr, nullptr, nullptr, nullptr, 1, nullptr};
   return D <= 64 ? attention_fwd<64>(as_stream(stream), a, tq, tk, tv) : attention_fwd<128>(as_stream(stream), a, tq, tk, tv);
 }
 
@@ -224,11 +227,11 @@ int64_t lewi_causal_attention_bwd_workspace_bytes(int T, int n_seqs, int Hq, int
 }
 
 int lewi_causal_attention_bwd(void* stream, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
-                              const void* o, const float* lse, const void* d_o, const int32_t* cu_seqlens, int n_seqs, void* dq, void* dk,
-                              void* dv, void* workspace, int64_t workspace_bytes, int T, int Hq, int Hkv, int D, float scale) {
+                              const void* o, const void* o_rest, const float* lse, const void* d_o, const int32_t* cu_seqlens, int n_seqs,
+                              void* dq, void* dk, void* dv, void* workspace, int64_t workspace_bytes, int T, int Hq, int Hkv, int D, float scale) {
   if (const int rc = check_attention(q, q_stride, k, k_stride, v, v_stride, cu_seqlens, n_seqs, o, T, Hq, Hkv, D, scale)) return rc;
-  if (!d_o || !lse || (!dq && !dk) || !dk != !dv) return LEWI_ERR_ARG;
-  if (!aligned(d_o, 16) || !aligned(dq, 16) || !aligned(dk, 16) || !aligned(dv, 16)) return LEWI_ERR_SHAPE;
+  if (!d_o || !o_rest || !lse || (!dq && !dk) || !dk != !dv) return LEWI_ERR_ARG;
+  if (!aligned(d_o, 16) || !aligned(o_rest, 16) || !aligned(dq, 16) || !aligned(dk, 16) || !aligned(dv, 16)) return LEWI_ERR_SHAPE;
   if (!workspace || !aligned(workspace, 16) || workspace_bytes < lewi_causal_attention_bwd_workspace_bytes(T, n_seqs, Hq, Hkv, D))
     return LEWI_ERR_WORKSPACE;
   CUtensorMap tq, tk, tv, td;
@@ -236,7 +239,8 @@ int lewi_causal_attention_bwd(void* stream, const void* q, int64_t q_stride, con
       !attn::make_rows_map(&tv, v, T, Hkv, D, v_stride) || !attn::make_rows_map(&td, d_o, T, Hq, D, (int64_t)Hq * D))
     return LEWI_ERR_CUDA;
   const attn::Args a{{cu_seqlens, n_seqs, T}, Hq, Hkv, Hq / Hkv, D, scale, scale * 1.4426950408889634f,
-                     const_cast<bf16*>(reinterpret_cast<const bf16*>(o)), const_cast<float*>(lse), reinterpret_cast<float*>(workspace),
+                     const_cast<bf16*>(reinterpret_cast<const bf16*>(o)), const_cast<bf16*>(reinterpret_cast<const bf16*>(o_rest)),
+                     const_cast<float*>(lse), reinterpret_cast<float*>(workspace),
                      reinterpret_cast<bf16*>(dq), reinterpret_cast<bf16*>(dk), reinterpret_cast<bf16*>(dv),
                      attn::dkv_parts(T, n_seqs, Hq, Hkv, D),
                      reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(workspace) + delta_bytes(T, Hq))};

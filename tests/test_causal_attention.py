@@ -69,11 +69,11 @@ def test_refusals():
     with pytest.raises(LewiError):
       bad()
   lib, at = _lib.load(), 1 << 20   # (addresses that are never used)
-  call = lambda q=at, qs=256, n=1, t=64, hq=4, hkv=2, d=64, scale=1.0: lib.lewi_causal_attention_fwd(None, q, qs, at, 128, at, 128, None, n, at, at, t, hq, hkv, d, scale)
+  call = lambda q=at, qs=256, n=1, t=64, hq=4, hkv=2, d=64, scale=1.0: lib.lewi_causal_attention_fwd(None, q, qs, at, 128, at, 128, None, n, at, at, at, t, hq, hkv, d, scale)
   assert call(q=None) == -1 and call(t=0) == -1 and call(n=3) == -1 and call(scale=float("nan")) == -1
   assert call(t=2 ** 25) == -5 and call(hq=64, qs=4096, t=2 ** 21) == -5
   assert call(q=at + 2) == -2 and call(qs=255) == -2 and call(qs=264 - 16) == -2 and call(hq=3) == -2 and call(d=60) == -2 and call(d=136) == -5
-  bwd = lambda dq=at, dk=at, dv=at, ws=1 << 20: lib.lewi_causal_attention_bwd(None, at, 256, at, 128, at, 128, at, at, at, None, 1, dq, dk, dv, at, ws, 64, 4, 2, 64, 1.0)
+  bwd = lambda dq=at, dk=at, dv=at, ws=1 << 20: lib.lewi_causal_attention_bwd(None, at, 256, at, 128, at, 128, at, at, at, at, None, 1, dq, dk, dv, at, ws, 64, 4, 2, 64, 1.0)
   assert bwd(dq=None, dk=None, dv=None) == -1 and bwd(dv=None) == -1 and bwd(dq=at + 8) == -2 and bwd(ws=16) == -3
 
 
@@ -316,3 +316,21 @@ def test_shared_operands_and_modes(cuda):
   assert torch.equal(attention.causal_attention(turned, turned, turned), o)
   shifted = torch.cat([x.detach().flatten()[:1], x.detach().flatten()])[1:].view(260, 4, 64)   # two bytes off
   assert torch.equal(attention.causal_attention(shifted, shifted, shifted), o)
+
+
+@pytest.mark.gpu
+def test_gradients_where_a_softmax_is_nearly_all_on_one_key(cuda):
+  """dP - delta is a small difference there.  Every term of dS is rounded once (2^-8 of it at most, 2^-9 / sqrt(3) in the mean), p to as much and
+  the gradients themselves, so the norm of their error is below 2^-8 of theirs, as long as delta is not off by 2^-8 of itself."""
+  gen = torch.Generator().manual_seed(11)
+  for lens in ([2] * 5 + [1] * 9, [700]):
+    t, d = sum(lens), 64
+    q, k, v, d_o = (rnd(gen, t, 1, d) for _ in range(4))
+    q = 8 * q
+    cu = torch.tensor([0] + lens).cumsum(0)
+    want = formulas(q, k, v, cu.tolist(), d ** -0.5, d_o)
+    leaves = [x.to(cuda).requires_grad_(True) for x in (q, k, v)]
+    o = attention.causal_attention(*leaves, cu.to(cuda))
+    for name, g in zip(("dq", "dk", "dv"), torch.autograd.grad(o, leaves, d_o.to(cuda))):
+      within(g, want[name], name)
+      assert (g.cpu().to(F64) - want[name][0]).norm() <= U * want[name][0].norm(), name
