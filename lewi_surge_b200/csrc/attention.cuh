@@ -155,11 +155,12 @@ __device__ __forceinline__ F2 hide(F2 v, bool lo_hidden, bool hi_hidden) {
 constexpr int kBox = kTile * 128;
 template <int DP> constexpr int kTileBytes = kTile * DP * 2;
 // K-major (rows are M or N, columns K) and MN-major (rows are K, columns N)
+// (a step is a constant added to a tile's descriptor, whose address field holds all of shared memory: nothing is masked or shifted again)
 __device__ __forceinline__ uint64_t desc_k(uint32_t tile, int step) {
-  return ptx::smem_desc(ptx::smem_desc_hi_sw128(16, 1024), tile + (step >> 2) * kBox + (step & 3) * 32);
+  return ptx::smem_desc_hi_sw128(16, 1024) + ((tile >> 4) + (((step >> 2) * kBox + (step & 3) * 32) >> 4));
 }
 __device__ __forceinline__ uint64_t desc_mn(uint32_t tile, int step) {
-  return ptx::smem_desc(ptx::smem_desc_hi_sw128(kBox, 1024), tile + step * 2048);
+  return ptx::smem_desc_hi_sw128(kBox, 1024) + ((tile >> 4) + (step * 2048 >> 4));
 }
 // D (+)= A B over the DP columns of two tiles
 template <int DP>
@@ -216,6 +217,19 @@ __device__ __forceinline__ void settle() {
   const unsigned long long t0 = ptx::globaltimer_ns();
   while (ptx::globaltimer_ns() - t0 < 4000000ull) {}
 }
+
+// A place in a ring of ST and the parity of its phase, moved on instead of divided out of a count.
+template <int ST>
+struct At {
+  uint32_t s, phase;
+  __device__ __forceinline__ void on(uint32_t by) {
+    s += by;
+    if (s >= ST) {
+      s -= ST;
+      phase ^= 1u;
+    }
+  }
+};
 
 struct Args {
   Seqs seqs;
@@ -669,7 +683,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dkv_kernel(const __grid_consta
   const uint32_t k_at = base, v_at = base + TB, ring = base + 2 * TB;   // [stage][Q, dO]
   float* stats = reinterpret_cast<float*>(attn_smem + (2 + 2 * ST) * TB + kStaging);   // [stage][-lse, -delta][128]
   const uint32_t bars = base + (2 + 2 * ST) * TB + kStaging + ST * 2 * kTile * 4;
-  const uint32_t k_full = bars, v_full = bars + 8, dp_full = bars + 24, p_ready = bars + 32, ds_ready = bars + 40, acc_full = bars + 48,
+  const uint32_t k_full = bars, v_full = bars + 8, dp_full = bars + 24, ds_ready = bars + 40, acc_full = bars + 48,
                  k_empty = bars + 64, v_empty = bars + 72, acc_empty = bars + 80;
   auto q_full = [&](int n) { return bars + 88u + 8u * (n % ST); };
   auto q_empty = [&](int n) { return bars + 88u + 8u * (ST + n % ST); };
@@ -680,12 +694,16 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dkv_kernel(const __grid_consta
   auto q_raw = [&](int n) { return bars + 88u + 8u * (6 * ST + n % ST); };
   auto do_raw = [&](int n) { return bars + 88u + 8u * (7 * ST + n % ST); };
   auto s_full = [&](int n) { return bars + 88u + 8u * (8 * ST + n % NS); };
+  auto p_ready = [&](int n) { return bars + 32u + 24u * (n % NS); };   // (with two places the next P can be there before this one is waited for)
   volatile int* abort_flag = &s_abort;
   const ItemQueue items{&s_plan, bars + 88u + 8u * (8 * ST + NS), abort_flag};
   if (threadIdx.x == 0) {
     for (uint32_t b : {k_full, v_full, k_empty, v_empty, dp_full, acc_full}) ptx::mbar_init(b, 1);
-    for (int n = 0; n < NS; ++n) ptx::mbar_init(s_full(n), 1);
-    for (uint32_t b : {p_ready, ds_ready, acc_empty}) ptx::mbar_init(b, 8);
+    for (int n = 0; n < NS; ++n) {
+      ptx::mbar_init(s_full(n), 1);
+      ptx::mbar_init(p_ready(n), 8);
+    }
+    for (uint32_t b : {ds_ready, acc_empty}) ptx::mbar_init(b, 8);
     for (int s = 0; s < ST; ++s) {
       for (uint32_t b : {q_full(s), q_empty(s), do_full(s), do_empty(s), st_full(s), q_raw(s), do_raw(s)}) ptx::mbar_init(b, 1);
       ptx::mbar_init(st_empty(s), 8);
@@ -791,7 +809,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dkv_kernel(const __grid_consta
              (NS == 1 || n_it == 1 || scores(1));
         for (int it = 0; ok && it < n_it; ++it) {
           const int x = n + it, at = ring + x % ST * 2 * TB;
-          ok = ptx::mbar_wait(p_ready, x & 1, abort_flag) && (it > 0 || ptx::mbar_wait(acc_empty, (r & 1) ^ 1u, abort_flag));
+          ok = ptx::mbar_wait(p_ready(x), x / NS & 1, abort_flag) && (it > 0 || ptx::mbar_wait(acc_empty, (r & 1) ^ 1u, abort_flag));
           if (!ok) break;
           ptx::tc_fence_after();
           mma_tm<0, 8>(t_dv, t_s(x), at + TB, id_d, it > 0, 64);
@@ -889,7 +907,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dkv_kernel(const __grid_consta
         ptx::tmem_st_wait();
         ptx::tc_fence_before();
         __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(p_ready);
+        if (lane == 0) ptx::mbar_arrive(p_ready(n));
         ok = warp_wait(dp_full, n & 1, abort_flag);
         if (!ok) break;
         ptx::tc_fence_after();
@@ -1000,18 +1018,22 @@ __global__ void __launch_bounds__(kSumThreads) dkv_sum_kernel(const Args a) {
 // of keys, in an order that changes, or wait for its turn.  One sequence of 16,384, 16 heads over 2, D = 128: 1.2 ms.
 // S(j+2) waits for K(j+2), whose place is that of K(j) where there are four: five places take what the staging would (8192 x 32 heads, D = 128:
 // 650 us with five, 780 with four), so at D = 128 dQ is stored row by row.
+// At D = 64 three products take 770 cycles of 1640 for a pair of tiles, and what the warp that issues them does between them counts: it loops as a whole over
+// values that all its lanes share, with one elected for the instructions (8192 x 32 heads: 442 us as a loop of one thread, 405 so), and K and V come
+// as pairs on one barrier (398).  The forward pass and the kernel for dK and dV, which wait for their exponentials, lose 2 % by the former.
 template <int DP>
 struct DqShape {
-  static constexpr int kStages = DP == 64 ? 6 : 5;
-  static constexpr bool kStaged = DP == 64;
-  static constexpr int kSmem = (2 + kStages) * kTileBytes<DP> + (kStaged ? kStaging : 0) + kBarriers;
+  static constexpr bool kPairs = DP == 64, kStaged = DP == 64;   // (a place is K's and V's)
+  static constexpr int kStages = kPairs ? 4 : 5;
+  static constexpr int kSmem = (2 + (kPairs ? 2 : 1) * kStages) * kTileBytes<DP> + (kStaged ? kStaging : 0) + kBarriers;
 };
 
 template <int DP>
 __global__ void __launch_bounds__(kBwdThreads, 1) dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                                                             const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
                                                             const Args a) {
-  constexpr int ST = DqShape<DP>::kStages, TB = kTileBytes<DP>;
+  constexpr bool PAIRS = DqShape<DP>::kPairs;
+  constexpr int ST = DqShape<DP>::kStages, TB = kTileBytes<DP>, PLACE = PAIRS ? 2 * TB : TB;
   extern __shared__ __align__(1024) uint8_t attn_smem[];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
@@ -1022,7 +1044,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dq_kernel(const __grid_constan
     return;
   }
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const uint32_t q_at = base, do_at = base + TB, kv = base + 2 * TB, bars = kv + ST * TB + (DqShape<DP>::kStaged ? kStaging : 0);
+  const uint32_t q_at = base, do_at = base + TB, kv = base + 2 * TB, bars = kv + ST * PLACE + (DqShape<DP>::kStaged ? kStaging : 0);
   const uint32_t q_full = bars, do_full = bars + 8, q_empty = bars + 16, do_empty = bars + 24, dp_full = bars + 32, ds_ready = bars + 40, acc_full = bars + 48,
                  acc_empty = bars + 56;
   auto s_full = [&](int b) { return bars + 72u + 8u * (b & 1); };
@@ -1035,7 +1057,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dq_kernel(const __grid_constan
     for (uint32_t b : {q_full, do_full, q_empty, do_empty, dp_full, acc_full, s_full(0), s_full(1)}) ptx::mbar_init(b, 1);
     for (uint32_t b : {ds_ready, acc_empty}) ptx::mbar_init(b, 8);
     for (int s = 0; s < ST; ++s) {
-      for (uint32_t b : {full(s), empty(s), raw(s)}) ptx::mbar_init(b, 1);
+      ptx::mbar_init(full(s), PAIRS ? 2 : 1);
+      for (uint32_t b : {empty(s), raw(s)}) ptx::mbar_init(b, 1);
     }
     items.init(11);
     s_abort = 0;
@@ -1072,59 +1095,72 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dq_kernel(const __grid_constan
         load_tile<DP>(do_at, &tm_do, do_full, w.sub, q_row);
       }
       __syncwarp();
-      for (int i = 0; ok && i < 2 * nb; ++i, ++n) {
-        const int j = i >> 1, valid = (i & 1) == 0 ? w.len - j * kTile : kTile;   // (of V a foreign row only reaches pairs that are masked)
+      for (int j = 0; ok && j < nb; ++j, ++n) {
         ok = warp_wait(empty(n), (n / ST & 1) ^ 1u, abort_flag);
         if (!ok) break;
-        bring_tile<DP>(kv + n % ST * TB, (i & 1) != 0 ? &tm_v : &tm_k, full(n), raw(n), hk, w.start + j * kTile, valid);
+        bring_tile<DP>(kv + n % ST * PLACE, &tm_k, full(n), raw(n), hk, w.start + j * kTile, w.len - j * kTile);
+        if (!PAIRS) {
+          ++n;
+          ok = warp_wait(empty(n), (n / ST & 1) ^ 1u, abort_flag);
+          if (!ok) break;
+        }   // (of V a foreign row only reaches pairs that are masked)
+        bring_tile<DP>(kv + n % ST * PLACE + (PAIRS ? TB : 0), &tm_v, full(n), raw(n), hk, w.start + j * kTile, kTile);
       }
     }
     if (s_abort) settle();
   } else if (warp == 9) {
     const uint32_t id_s = ptx::instr_desc_bf16(128, 128, 0, 0), id_d = ptx::instr_desc_bf16(128, DP, 0, 1);
-    if (ptx::elect_one()) {
-      bool ok = true;
-      int n = 0, b = 0;   // ring position, blocks so far
-      for (int r = 0; ok; ++r) {
-        const Item w = items.take_alone(r);
-        if (w.level < 0) break;
-        const int nb = w.level + 1;
-        auto scores = [&](int j) {
-          const int x = n + 2 * j;
-          if (!ptx::mbar_wait(full(x), x / ST & 1, abort_flag)) return false;
+    bool ok = true;
+    constexpr int STEP = PAIRS ? 1 : 2;
+    At<ST> ks{0, 0}, vs{PAIRS ? 0 : 1, 0}, ds{0, 0};   // K of the next S, V of the next dP, K of the next dQ
+    uint32_t bs = 0, b = 0;                // blocks of S and of dQ so far
+    for (uint32_t r = 0; ok; ++r) {
+      const Item w = items.take(r);
+      const int nb = __shfl_sync(0xffffffffu, w.level, 0) + 1;
+      if (nb <= 0) break;
+      auto scores = [&](int j) {
+        if (!warp_wait(full(ks.s), ks.phase, abort_flag)) return false;
+        if (ptx::elect_one()) {
           ptx::tc_fence_after();
-          mma_kk<DP>(t_s(b + j), q_at, kv + x % ST * TB, id_s);
-          ptx::mma_commit(s_full(b + j));
+          mma_kk<DP>(t_s(bs), q_at, kv + ks.s * PLACE, id_s);
+          ptx::mma_commit(s_full(bs));
           if (j + 1 == nb) ptx::mma_commit(q_empty);
-          return true;
-        };
-        auto dps = [&](int j) {
-          const int x = n + 2 * j + 1;
-          if (!ptx::mbar_wait(full(x), x / ST & 1, abort_flag)) return false;
-          ptx::tc_fence_after();
-          mma_kk<DP>(t_dp, do_at, kv + x % ST * TB, id_s);
-          ptx::mma_commit(dp_full);
-          ptx::mma_commit(empty(x));
-          if (j + 1 == nb) ptx::mma_commit(do_empty);
-          return true;
-        };
-        ok = ptx::mbar_wait(q_full, r & 1, abort_flag) && scores(0) && ptx::mbar_wait(do_full, r & 1, abort_flag) && dps(0) && (nb < 2 || scores(1));
-        for (int j = 0; ok && j < nb; ++j) {
-          const int x = n + 2 * j;
-          ok = ptx::mbar_wait(ds_ready, (b + j) & 1, abort_flag) && (j + 1 >= nb || dps(j + 1)) &&
-               (j > 0 || ptx::mbar_wait(acc_empty, (r & 1) ^ 1u, abort_flag));
-          if (!ok) break;
-          ptx::tc_fence_after();
-          mma_tm<0, 8>(t_dq, t_s(b + j), kv + x % ST * TB, id_d, j > 0, 64);
-          ptx::mma_commit(empty(x));
-          if (j + 1 == nb) ptx::mma_commit(acc_full);
-          if (j + 2 < nb) ok = scores(j + 2);
         }
-        n += 2 * nb;
-        b += nb;
+        __syncwarp();
+        ++bs;
+        ks.on(STEP);
+        return true;
+      };
+      auto dps = [&](int j) {
+        if (!PAIRS && !warp_wait(full(vs.s), vs.phase, abort_flag)) return false;
+        if (ptx::elect_one()) {
+          ptx::tc_fence_after();
+          mma_kk<DP>(t_dp, do_at, kv + vs.s * PLACE + (PAIRS ? TB : 0), id_s);
+          ptx::mma_commit(dp_full);
+          if (!PAIRS) ptx::mma_commit(empty(vs.s));
+          if (j + 1 == nb) ptx::mma_commit(do_empty);
+        }
+        __syncwarp();
+        vs.on(STEP);
+        return true;
+      };
+      ok = warp_wait(q_full, r & 1, abort_flag) && scores(0) && warp_wait(do_full, r & 1, abort_flag) && dps(0) && (nb < 2 || scores(1));
+      for (int j = 0; ok && j < nb; ++j) {
+        ok = warp_wait(ds_ready, b & 1, abort_flag) && (j + 1 >= nb || dps(j + 1)) && (j > 0 || warp_wait(acc_empty, (r & 1) ^ 1u, abort_flag));
+        if (!ok) break;
+        if (ptx::elect_one()) {
+          ptx::tc_fence_after();
+          mma_tm<0, 8>(t_dq, t_s(b), kv + ds.s * PLACE, id_d, j > 0, 64);
+          ptx::mma_commit(empty(ds.s));
+          if (j + 1 == nb) ptx::mma_commit(acc_full);
+        }
+        __syncwarp();
+        ++b;
+        ds.on(STEP);
+        if (j + 2 < nb) ok = scores(j + 2);
       }
-      if (s_abort) settle();
     }
+    if (s_abort) settle();
     __syncwarp();
   } else if (warp == 10) {
     items.run(a.seqs, kTile, a.Hq);
@@ -1136,10 +1172,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dq_kernel(const __grid_constan
     for (int r = 0; ok; ++r) {
       const Item w = items.take(r);
       if (w.level < 0) break;
-      const int valid = w.len - w.level * kTile, s = (n + 2 * w.level) % ST;   // of the last keys
-      n += 2 * (w.level + 1);
+      const int valid = w.len - w.level * kTile, s = (n + (PAIRS ? 1 : 2) * w.level) % ST;   // of the last keys
+      n += (PAIRS ? 1 : 2) * (w.level + 1);
       if (valid >= kTile) continue;
-      ok = mend_tile<DP>(kv + s * TB, full(s), raw(s), phases >> s, valid, abort_flag);
+      ok = mend_tile<DP>(kv + s * PLACE, full(s), raw(s), phases >> s, valid, abort_flag);
       phases ^= 1u << s;
     }
   } else {
@@ -1209,7 +1245,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dq_kernel(const __grid_constan
         uint8_t* dst = reinterpret_cast<uint8_t*>(a.dq + ((long long)(w.start + row0) * a.Hq + w.sub) * a.D + c);
         const long long stride = (long long)a.Hq * a.D * 2;
         if constexpr (DqShape<DP>::kStaged) {
-          store_rows(attn_smem + (2 + ST) * TB + warp * 2048, out[i], dst, stride, w.len - row0, (a.D - c) * 2);
+          store_rows(attn_smem + 2 * TB + ST * PLACE + warp * 2048, out[i], dst, stride, w.len - row0, (a.D - c) * 2);
         } else if (lane < w.len - row0) {
 #pragma unroll
           for (int u = 0; u < 4; ++u)
