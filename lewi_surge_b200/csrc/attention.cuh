@@ -231,6 +231,8 @@ struct At {
   }
 };
 
+enum FwdItem { kTwoHeads, kTwoTiles, kOneTile };
+
 struct Args {
   Seqs seqs;
   int Hq, Hkv, G, D;
@@ -240,6 +242,7 @@ struct Args {
   __nv_bfloat16 *dq, *dk, *dv;
   int parts;               // of a group's heads, one CTA each for dK and dV
   float* sums;             // [part][dV, dK][T][Hkv][D] where there are several
+  FwdItem shape;           // of the forward pass
 };
 
 // A warp's 32 rows x 64 bytes go through shared memory (2 KB of its own), so that a store writes 8 rows x 64 bytes and not a piece of each of
@@ -321,6 +324,9 @@ struct ItemQueue {
 // grown by more than 8 (in powers of 2; p stays below 2^8, which bf16 and float32 hold as well as 1).  The next item's queries, first keys
 // and scores are on their way while O of this one is written out.  p is rounded to bf16 for its product, its sum l is taken before.
 //
+// Where such items are too few for the SMs an item is one tile (fwd_item).  Its scores have both places, so that those of the next block are there
+// when a softmax ends, which then scales O after the product before (pv_done).  Each row's steps are the same, and so are its bits.
+//
 // What bounds it: a tile's chain S -> softmax -> P -> S, 2900 cycles for both tiles of a block where their products take 2048 (D = 128) or
 // 1024 (D = 64) and their exponentials 2048 of the special function unit.  One sequence of 16,384, 16 heads over 2, D = 128: 0.80 ms,
 // 1370 TFLOP/s; 8192, 32 over 8, D = 64: 0.40 ms, 680 TFLOP/s.
@@ -357,6 +363,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
   auto raw = [&](int n) { return bars + 8u * (2 * ST + 14 + n % ST); };
   volatile int* abort_flag = &s_abort;
   const ItemQueue items{&s_plan, bars + 8u * (3 * ST + 14), abort_flag};
+  const uint32_t pv_done = bars + 8u * (3 * ST + 18);
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) {
       for (uint32_t b : {full(s), empty(s), raw(s)}) ptx::mbar_init(b, 1);
@@ -365,6 +372,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
       for (uint32_t b : {q_full(t), q_empty(t), s_full(t), o_full(t)}) ptx::mbar_init(b, 1);
       for (uint32_t b : {p_full(t, 0), p_full(t, 1), o_empty(t)}) ptx::mbar_init(b, 4);
     }
+    ptx::mbar_init(pv_done, 1);
     items.init(11);
     s_abort = 0;
     ptx::mbar_fence_init();
@@ -383,10 +391,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
   const uint32_t tmem = s_tmem;
   auto s_at = [&](int t) { return tmem + t * 128; };
   auto o_at = [&](int t) { return tmem + 256 + t * 128; };
-  const bool two_heads = a.G % 2 == 0;
-  auto tile_of = [&](const Item& w, int t) { return two_heads ? w.level : 2 * w.level + t; };
-  auto head_of = [&](const Item& w, int t) { return two_heads ? 2 * w.sub + t : w.sub; };
-  auto blocks_of = [&](const Item& w, int t) { return tile_of(w, t) * kTile < w.len ? tile_of(w, t) + 1 : 0; };
+  auto tile_of = [&](const Item& w, int t) { return a.shape == kTwoTiles ? 2 * w.level + t : w.level; };
+  auto head_of = [&](const Item& w, int t) { return a.shape == kTwoHeads ? 2 * w.sub + t : w.sub; };
+  auto blocks_of = [&](const Item& w, int t) { return tile_of(w, t) * kTile < w.len && (t == 0 || a.shape != kOneTile) ? tile_of(w, t) + 1 : 0; };
 
   // registers: 8 x 216 + 4 x 72 = 12 x 168 a thread, what the launch has
   if (warp >= 8) {
@@ -427,6 +434,39 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
           const Item w = items.take_alone(r);
           if (w.level < 0) break;
           const int blocks[2] = {blocks_of(w, 0), blocks_of(w, 1)}, nb = max(blocks[0], blocks[1]);
+          if (a.shape == kOneTile) {   // S(0) S(1) | P(j) V(j), S(j + 2) after P(j)
+            auto scores = [&](int j) {
+              const int x = n + 2 * j;
+              if (!ptx::mbar_wait(full(x), x / ST & 1, abort_flag)) return false;
+              ptx::tc_fence_after();
+              mma_kk<DP>(s_at(done[0] + j & 1), base, kv + x % ST * TB, id_s);
+              ptx::mma_commit(s_full(done[0] + j & 1));
+              ptx::mma_commit(empty(x));
+              if (j + 1 == nb) ptx::mma_commit(q_empty(0));
+              return true;
+            };
+            ok = ptx::mbar_wait(q_full(0), used[0] & 1, abort_flag) && scores(0) && (nb == 1 || scores(1)) &&
+                 ptx::mbar_wait(o_empty(0), (used[0] & 1) ^ 1u, abort_flag);
+            for (int j = 0; ok && j < nb; ++j) {
+              const int x = n + 2 * j + 1, b = done[0] + j;
+              ok = ptx::mbar_wait(full(x), x / ST & 1, abort_flag) && ptx::mbar_wait(p_full(b & 1, 0), b >> 1 & 1, abort_flag);
+              if (!ok) break;
+              ptx::tc_fence_after();
+              mma_tm<0, 4>(o_at(0), s_at(b & 1), kv + x % ST * TB, id_o, j > 0, 32);
+              ok = ptx::mbar_wait(p_full(b & 1, 1), b >> 1 & 1, abort_flag);
+              if (!ok) break;
+              ptx::tc_fence_after();
+              mma_tm<4, 8>(o_at(0), s_at(b & 1), kv + x % ST * TB, id_o, true, 32);
+              ptx::mma_commit(pv_done);
+              ptx::mma_commit(empty(x));
+              if (j + 1 == nb) ptx::mma_commit(o_full(0));
+              if (j + 2 < nb) ok = scores(j + 2);
+            }
+            n += 2 * nb;
+            done[0] += nb;
+            ++used[0];
+            continue;
+          }
           auto scores = [&](int t, int j) {
             ptx::tc_fence_after();
             mma_kk<DP>(s_at(t), base + t * TB, kv + (n + 2 * j) % ST * TB, id_s);
@@ -473,7 +513,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
       }
       __syncwarp();
     } else if (warp == 10) {
-      items.run(a.seqs, two_heads ? kTile : 2 * kTile, two_heads ? a.Hq / 2 : a.Hq);
+      items.run(a.seqs, a.shape == kTwoTiles ? 2 * kTile : kTile, a.shape == kTwoHeads ? a.Hq / 2 : a.Hq);
     } else {
       zero_gaps(a.seqs, a.o, a.Hq * a.D / 8);
       bool ok = true;
@@ -495,7 +535,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const int t = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;   // this warp's lanes of tensor memory
-    const uint32_t sp = s_at(t) + lanes, op = o_at(t) + lanes;
+    const uint32_t op = o_at(t) + lanes;
+    const bool one = a.shape == kOneTile;
     const F2 scale = f2(a.scale_log2, a.scale_log2);
     int used = 0, done = 0;
     bool ok = true;
@@ -504,9 +545,12 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
       if (w.level < 0) break;
       const int tile = tile_of(w, t), head = head_of(w, t), n_blocks = blocks_of(w, t);
       if (n_blocks == 0) continue;
+      const bool mine = tile * kTile + row < w.len;   // (what other sequences' rows hold decides nothing)
       float m = 0.f, l = 0.f;
       for (int j = 0; j < n_blocks; ++j, ++done) {
-        ok = warp_wait(s_full(t), done & 1, abort_flag);
+        const int place = one ? done & 1 : t;
+        const uint32_t sp = s_at(place) + lanes;
+        ok = warp_wait(s_full(place), (one ? done >> 1 : done) & 1, abort_flag);
         if (!ok) break;
         ptx::tc_fence_after();
         uint32_t s[4][32];
@@ -530,7 +574,12 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
         if (j == 0) {
           m = top;
-        } else if (__any_sync(0xffffffffu, (top - m) * a.scale_log2 > 8.f)) {
+        } else if (__any_sync(0xffffffffu, mine && (top - m) * a.scale_log2 > 8.f)) {
+          if (one && !warp_wait(pv_done, (done & 1) ^ 1u, abort_flag)) {   // of the block before
+            ok = false;
+            break;
+          }
+          ptx::tc_fence_after();
           const float grown = fmaxf(m, top), f = grown == m ? 1.f : ex2((m - grown) * a.scale_log2);
           m = grown;
           l *= f;
@@ -560,7 +609,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
           ptx::tmem_st_wait();
           ptx::tc_fence_before();
           __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(p_full(t, half));
+          if (lane == 0) ptx::mbar_arrive(p_full(place, half));
         }
         float lo, hi;
         f2_split(add2(sum[0], sum[1]), lo, hi);
@@ -1272,14 +1321,32 @@ inline bool make_rows_map(CUtensorMap* m, const void* p, int T, int heads, int D
   return encode_tiled(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, p, dims, strides, box);
 }
 
+// Pairs of tiles of the longest row of tiles, and an SM's share of all of them.  What lengths several sequences have only the device knows: the longest
+// is taken to be three times the mean.
+struct Blocks {
+  double longest, share;
+};
+inline Blocks blocks_of(int T, int n_seqs, int Hq) {
+  const double tiles = (double)T / kTile + 0.5 * n_seqs, mean = tiles / n_seqs, longest = n_seqs == 1 ? mean : 3 * mean < tiles ? 3 * mean : tiles;
+  return {longest, tiles * (mean + 1) / 2 * Hq / num_sms()};
+}
+
+// An item of the forward pass is two heads or two tiles, or one tile where that is over sooner: a block of the former takes 1.6 us for its two
+// tiles, of the latter 1.15 us for one, and an SM is done with its share or with the longest item.  One sequence, 16 heads over 2, D = 128, two
+// heads and one tile: of 256 rows 9.9 and 8.1 us, 1000 19 and 14, 2048 32 and 23, 4096 57 and 65.
+inline FwdItem fwd_item(int T, int n_seqs, int Hq, int G) {
+  const Blocks b = blocks_of(T, n_seqs, Hq);
+  const double two = b.longest > b.share / 2 ? 1.6 * b.longest : 0.8 * b.share, one = 1.15 * (b.longest > b.share ? b.longest : b.share);
+  return one < two ? kOneTile : G % 2 == 0 ? kTwoHeads : kTwoTiles;
+}
+
 // In how many parts, each a CTA's item, a group's heads are worked through for a tile of dK and dV.  The tile of a long sequence's first keys
 // has all its queries, times G heads, so few key heads leave a few long items, while parts cost their way through memory (float32, written and
 // read).  Taken is what comes out shortest of the longest item or an even share of everything, at 1.6 us per pair of tiles, and the parts'
-// bytes at 5 TB/s; where there are several sequences the longest is taken to be three times the mean.  One sequence of 1000, 16 heads over 2:
+// bytes at 5 TB/s.  One sequence of 1000, 16 heads over 2:
 // 128 us in one part, 30 in eight; of 16,384: 1975 and 1800 in two.
 inline int dkv_parts(int T, int n_seqs, int Hq, int Hkv, int D) {
-  const double tiles = (double)T / kTile + 0.5 * n_seqs, mean = tiles / n_seqs, longest = n_seqs == 1 ? mean : 3 * mean < tiles ? 3 * mean : tiles;
-  const double share = tiles * (mean + 1) / 2 * Hq / num_sms();
+  const auto [longest, share] = blocks_of(T, n_seqs, Hq);
   int best = 1;
   double least = 0;
   for (int p = 1; p <= Hq / Hkv; ++p) {

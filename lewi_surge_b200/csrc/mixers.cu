@@ -70,10 +70,11 @@ int check_attention(const void* q, int64_t q_stride, const void* k, int64_t k_st
 }
 
 template <int DP>
-int attention_fwd(cudaStream_t st, const attn::Args& a, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv) {
+int attention_fwd(cudaStream_t st, attn::Args a, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv) {
   static bool done[64] = {false};
   if (!allow_smem(attn::fwd_kernel<DP>, attn::FwdShape<DP>::kSmem, done)) return LEWI_ERR_CUDA;
-  const long long items = a.G % 2 == 0 ? attn::most_tiles(a.seqs.T, a.seqs.n) * a.Hq / 2 : attn::most_tiles(a.seqs.T, a.seqs.n) * a.Hq;
+  a.shape = attn::fwd_item(a.seqs.T, a.seqs.n, a.Hq, a.G);
+  const long long items = attn::most_tiles(a.seqs.T, a.seqs.n) * (a.shape == attn::kTwoHeads ? a.Hq / 2 : a.Hq);
   attn::fwd_kernel<DP><<<attn::ctas(items), attn::kFwdThreads, attn::FwdShape<DP>::kSmem, st>>>(tq, tk, tv, a);
   LEWI_CHECK_LAUNCH();
   return LEWI_OK;

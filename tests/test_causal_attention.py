@@ -334,3 +334,17 @@ def test_gradients_where_a_softmax_is_nearly_all_on_one_key(cuda):
     for name, g in zip(("dq", "dk", "dv"), torch.autograd.grad(o, leaves, d_o.to(cuda))):
       within(g, want[name], name)
       assert (g.cpu().to(F64) - want[name][0]).norm() <= U * want[name][0].norm(), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,s,hq,hkv,d", [(120, 300, 4, 2, 64), (120, 300, 3, 1, 128), (90, 300, 6, 6, 96), (40, 520, 12, 2, 128), (1, 4500, 16, 2, 64)])
+def test_a_sequence_among_many_has_the_bits_that_it_has_alone(cuda, n, s, hq, hkv, d):
+  """How queries are shared out depends on how many there are (here on heads of one sequence too); what a row gets does not."""
+  gen = torch.Generator(device=cuda).manual_seed(n + d)
+  q, k, v = (torch.randn(n, s, h, d, generator=gen, device=cuda, dtype=torch.bfloat16) for h in (hq, hkv, hkv))
+  k *= torch.linspace(0.1, 6, s, device=cuda, dtype=torch.bfloat16)[:, None, None]   # maxima that grow
+  whole = attention.causal_attention(q, k, v)
+  for i in {0, n // 2, n - 1}:
+    for h in range(hkv):
+      heads = slice(h * (hq // hkv), (h + 1) * (hq // hkv))
+      assert torch.equal(whole[i][:, heads], attention.causal_attention(q[i][:, heads], k[i][:, h:h + 1], v[i][:, h:h + 1]))
