@@ -392,7 +392,8 @@ int lewi_paged_attention(void* stream, const void* q, int64_t q_stride, const vo
  * undefined.  lse f32 [Hq][T] (log2 of the softmax's denominator) and o_rest bf16 [T][Hq][D] (what rounding o left
  * of it) are for the backward pass and both null where none follows; their rows of no sequence are left as they are.
  * D <= 128, a multiple of 8; T * Hq / Hkv <= 2^25; scale > 0; all tensors 16-byte aligned, `*_stride` (elements from row to row; heads are contiguous) multiples
- * of 8.  Scores, softmax and sums float32; p and the gradient of the scores are rounded to bf16 for their products.
+ * of 8.  Scores, softmax and sums float32; p and the gradient of the scores are rounded to bf16 for their products (where lse is given and in the
+ * backward call, pairs of a sequence's first 128 rows in two parts, to 2^-16).
  * The backward call makes dq and/or dk and dv (bf16, contiguous; dk and dv together) out of d_o (bf16 [T][Hq][D], contiguous).  No
  * atomics: equal calls have equal bits.
  * ---------------------------------------------------------------------------------------------- */

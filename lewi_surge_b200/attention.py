@@ -137,6 +137,8 @@ def causal_attention(query, key, value, cu_seqlens=None, scale=None):
   Rows of no sequence give zeros and get zero gradients, whatever they hold.  Bounds that fall or leave the rows:
   `LEWI_STATUS_BAD_INDEX` in `_lib.last_status()`.  Rows may lie apart (views of one projection need no copy).
 
+  Outputs with and without gradients wanted may differ by a rounding in the first 128 rows of a sequence, whose p are kept to 2^-16 for the former.
+
   A value of v that is not finite reaches back to the start of its 128 rows of the sequence (as those of q, k and the upstream gradient do in the
   gradients), never into another sequence."""
   if not query.dtype is key.dtype is value.dtype is torch.bfloat16:

@@ -12,6 +12,8 @@
 // gradients.
 #pragma once
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "f32x2.cuh"
 #include "tcgen05.cuh"
@@ -150,6 +152,12 @@ __device__ __forceinline__ F2 hide(F2 v, bool lo_hidden, bool hi_hidden) {
   float lo, hi;
   f2_split(v, lo, hi);
   return f2(lo_hidden ? 0.f : lo, hi_hidden ? 0.f : hi);
+}
+// What rounding `p` to `rounded` left, rounded as well
+__device__ __forceinline__ uint32_t rest_bf16(F2 p, uint32_t rounded) {
+  float lo, hi;
+  f2_split(p, lo, hi);
+  return pack_bf16(lo - bf16_lo(rounded), hi - bf16_hi(rounded));
 }
 // Operand tiles in shared memory: boxes of [128 rows][64 columns], 128-byte swizzled, 16 KB apart.
 constexpr int kBox = kTile * 128;
@@ -322,7 +330,8 @@ struct ItemQueue {
 // sequence, and those of other sequences in a tile.  Products are issued in the order S0(j+1) after P0 V(j), S1(j+1) after P1 V(j): a
 // softmax that finds its scores knows that the product before them is done, so it may scale O then.  It does so only where the maximum has
 // grown by more than 8 (in powers of 2; p stays below 2^8, which bf16 and float32 hold as well as 1).  The next item's queries, first keys
-// and scores are on their way while O of this one is written out.  p is rounded to bf16 for its product, its sum l is taken before.
+// and scores are on their way while O of this one is written out.  p is rounded to bf16 for its product, its sum l is taken before; in training
+// (TRAIN) the first tile of a sequence, whose rows have few keys and errors that no sum averages, is multiplied by what that left as well.
 //
 // Where such items are too few for the SMs an item is one tile (fwd_item).  Its scores have both places, so that those of the next block are there
 // when a softmax ends, which then scales O after the product before (pv_done).  Each row's steps are the same, and so are its bits.
@@ -337,7 +346,7 @@ struct FwdShape {
   static constexpr int kSmem = (2 + kStages) * kTileBytes<DP> + kStaging + kBarriers;
 };
 
-template <int DP>
+template <int DP, bool TRAIN>
 __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                                                              const __grid_constant__ CUtensorMap tm_v, const Args a) {
   constexpr int ST = FwdShape<DP>::kStages, TB = kTileBytes<DP>;
@@ -457,6 +466,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
               if (!ok) break;
               ptx::tc_fence_after();
               mma_tm<4, 8>(o_at(0), s_at(b & 1), kv + x % ST * TB, id_o, true, 32);
+              if (TRAIN && nb == 1) mma_tm<0, 8>(o_at(0), s_at(b & 1) + 64, kv + x % ST * TB, id_o, true, 32);
               ptx::mma_commit(pv_done);
               ptx::mma_commit(empty(x));
               if (j + 1 == nb) ptx::mma_commit(o_full(0));
@@ -494,6 +504,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
               if (!ok) break;
               ptx::tc_fence_after();
               mma_tm<4, 8>(o_at(t), s_at(t), kv + nv % ST * TB, id_o, true, 32);
+              if (TRAIN && blocks[t] == 1) mma_tm<0, 8>(o_at(t), s_at(t) + 64, kv + nv % ST * TB, id_o, true, 32);
               ++done[t];
               if (j + 1 < blocks[t]) {
                 ok = ptx::mbar_wait(full(nk), nk / ST & 1, abort_flag);
@@ -547,11 +558,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
       if (n_blocks == 0) continue;
       const bool mine = tile * kTile + row < w.len;   // (what other sequences' rows hold decides nothing)
       float m = 0.f, l = 0.f;
-      for (int j = 0; j < n_blocks; ++j, ++done) {
+      auto block = [&](int j, auto first) {   // (first: in training and of a sequence's first tile; apart, so that the others do not pay for it)
         const int place = one ? done & 1 : t;
         const uint32_t sp = s_at(place) + lanes;
-        ok = warp_wait(s_full(place), (one ? done >> 1 : done) & 1, abort_flag);
-        if (!ok) break;
+        if (!warp_wait(s_full(place), (one ? done >> 1 : done) & 1, abort_flag)) return false;
         ptx::tc_fence_after();
         uint32_t s[4][32];
 #pragma unroll
@@ -575,10 +585,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
         if (j == 0) {
           m = top;
         } else if (__any_sync(0xffffffffu, mine && (top - m) * a.scale_log2 > 8.f)) {
-          if (one && !warp_wait(pv_done, (done & 1) ^ 1u, abort_flag)) {   // of the block before
-            ok = false;
-            break;
-          }
+          if (one && !warp_wait(pv_done, (done & 1) ^ 1u, abort_flag)) return false;   // of the block before
           ptx::tc_fence_after();
           const float grown = fmaxf(m, top), f = grown == m ? 1.f : ex2((m - grown) * a.scale_log2);
           m = grown;
@@ -601,11 +608,24 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
           uint32_t p[32];
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
-            const F2 x = ex2_pair<4>(s[2 * half + i / 16][i % 16 * 2], s[2 * half + i / 16][i % 16 * 2 + 1], scale, shift, i);
+            uint32_t &s0 = s[2 * half + i / 16][i % 16 * 2], &s1 = s[2 * half + i / 16][i % 16 * 2 + 1];
+            const F2 x = ex2_pair<4>(s0, s1, scale, shift, i);
             sum[i & 1] = add2(sum[i & 1], x);
             p[i] = f2_bf16(x);
+            if constexpr (first.value) {
+              float lo, hi;
+              f2_split(x, lo, hi);
+              s0 = __float_as_uint(lo);
+              s1 = __float_as_uint(hi);
+            }
           }
           ptx::tmem_st_32x32(sp + half * 32, p);
+          if constexpr (first.value) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              p[i] = rest_bf16(f2(__uint_as_float(s[2 * half + i / 16][i % 16 * 2]), __uint_as_float(s[2 * half + i / 16][i % 16 * 2 + 1])), p[i]);
+            ptx::tmem_st_32x32(sp + 64 + half * 32, p);
+          }
           ptx::tmem_st_wait();
           ptx::tc_fence_before();
           __syncwarp();
@@ -614,6 +634,13 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
         float lo, hi;
         f2_split(add2(sum[0], sum[1]), lo, hi);
         l += lo + hi;
+        ++done;
+        return true;
+      };
+      if (__builtin_expect(!TRAIN || n_blocks > 1, 1)) {
+        for (int j = 0; ok && j < n_blocks; ++j) ok = block(j, std::false_type());
+      } else {
+        ok = block(0, std::bool_constant<TRAIN>());
       }
       ok = ok && warp_wait(o_full(t), used & 1, abort_flag);
       if (!ok) break;
@@ -635,7 +662,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
       auto store = [&](__nv_bfloat16* to, const uint32_t (&x)[16], int c) {
         store_rows(stage, x, reinterpret_cast<uint8_t*>(to + at + c * 32), stride, valid, (a.D - c * 32) * 2);
       };
-      if (a.o_rest != nullptr) {
+      if constexpr (TRAIN) {
 #pragma unroll 1
         for (int c = 0; c < DP / 32; ++c) {
           uint32_t v[32], out[16], rest[16];
@@ -673,8 +700,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
 
 // ---------------------------------------------------------------- backward: delta
 // delta[h][t] = sum_d dO O, DP / 8 lanes per row.  Where a softmax is nearly all on one key, dP - delta is a small difference of large numbers:
-// O is therefore taken with what its rounding left.  dQ is off by 2.4e-3 of its norm for scores of N(0,1), 3.1e-3 for N(0,100) (with the rounded O
-// 2.4e-3 and 5.5e-3, for single rows 5e-2).  Dividing O by the sum of the rounded p would bring that to 2.5e-3 and the forward pass 6 % more time.
+// O is therefore taken with what its rounding left.  dQ of 3000 rows is off by 2.1e-3 of its norm for scores of N(0,1), 3.0e-3 for N(0,100) (with
+// the rounded O alone 2.4e-3 and 5.5e-3, for single rows 5e-2); its own rounding is 1.7e-3.
 constexpr int kDeltaThreads = 256;
 template <int DP>
 __global__ void __launch_bounds__(kDeltaThreads) delta_kernel(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict__ o_rest,
@@ -705,7 +732,8 @@ __global__ void __launch_bounds__(kDeltaThreads) delta_kernel(const __nv_bfloat1
 // S(0) dP(0) .. S(kScores - 1) | dV(i) S(i + kScores) after P(i), dK(i) dP(i+1) after dS(i): exponentials are made while dK and dP
 // run, dS while dV and S do, and with two places, which dV and dK leave at D <= 64, the next scores are there when dS has been made (8192
 // rows, 32 heads over 8: 575 us, with one place 715).  dS is rounded to bf16 for its products, as p is: of the error of dQ and dK (2.5e-3 of their
-// norm) that is as much as their own rounding.
+// norm) that is as much as their own rounding; where both tiles are a sequence's first (the norm is largest there) what that left of dS and p is
+// multiplied too (8191 rows in 13 sequences, 16 heads over 4, D = 64: 97 us and an error of 2.0e-3, without 90 and 2.4e-3).
 // One sequence of 16,384, 16 heads over 2, D = 128: 1.75 ms, 2650 cycles for a pair of tiles whose four products take 2048.
 constexpr int kBwdThreads = 384;
 template <int DP>
@@ -835,7 +863,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dkv_kernel(const __grid_consta
       for (int r = 0; ok; ++r) {
         const Item w = items.take_alone(r);
         if (w.level < 0) break;
-        const int n_it = span_of(w).n_it;
+        const Span sp = span_of(w);
+        const int n_it = sp.n_it, to_first = sp.per_head;   // pairs of tiles from a first one of both to the next
+        int at_first = sp.key == 0 ? 0 : to_first + 1;       // (there is none)
         auto scores = [&](int it) {   // S^T = K Q^T
           const int x = n + it;
           if (!ptx::mbar_wait(q_full(x), x / ST & 1, abort_flag)) return false;
@@ -862,12 +892,16 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dkv_kernel(const __grid_consta
           if (!ok) break;
           ptx::tc_fence_after();
           mma_tm<0, 8>(t_dv, t_s(x), at + TB, id_d, it > 0, 64);
+          const bool first = at_first == 0;
+          if (++at_first == to_first) at_first = 0;
+          if (first) mma_tm<0, 8>(t_dv, t_s(x) + 32, at + TB, id_d, true, 64);
           ptx::mma_commit(do_empty(x));
           if (it + NS < n_it) ok = scores(it + NS);
           ok = ok && ptx::mbar_wait(ds_ready, x & 1, abort_flag);
           if (!ok) break;
           ptx::tc_fence_after();
           mma_tm<0, 8>(t_dk, t_dp, at, id_d, it > 0, 64);
+          if (first) mma_tm<0, 8>(t_dk, t_dp + 32, at, id_d, true, 64);
           ptx::mma_commit(q_empty(x));
           if (it + 1 < n_it) ok = dps(it + 1);
           else ptx::mma_commit(acc_full);
@@ -928,12 +962,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dkv_kernel(const __grid_consta
       const Item w = items.take(r);
       if (w.level < 0) break;
       const Span sp = span_of(w);
-      for (int it = 0; it < sp.n_it; ++it, ++n) {
-        const bool diagonal = it % sp.per_head == 0;
+      auto block = [&](bool diagonal, auto first) {   // (first: both tiles are a sequence's first; apart, so that the others do not pay for it)
         const ulonglong2* lse = reinterpret_cast<const ulonglong2*>(stats + n % ST * 2 * kTile + half * 64);   // (both negative, in pairs)
         const ulonglong2* delta = reinterpret_cast<const ulonglong2*>(stats + (n % ST * 2 + 1) * kTile + half * 64);
-        ok = warp_wait(st_full(n), n / ST & 1, abort_flag) && warp_wait(s_full(n), n / NS & 1, abort_flag);
-        if (!ok) break;
+        if (!warp_wait(st_full(n), n / ST & 1, abort_flag) || !warp_wait(s_full(n), n / NS & 1, abort_flag)) return false;
         ptx::tc_fence_after();
         F2 p[32];
         uint32_t x[2][32], out[32];
@@ -953,12 +985,16 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dkv_kernel(const __grid_consta
 #pragma unroll
         for (int i = 0; i < 32; ++i) out[i] = f2_bf16(p[i]);
         ptx::tmem_st_32x32(t_s(n) + lanes + half * 64, out);
+        if constexpr (first.value) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) out[i] = rest_bf16(p[i], out[i]);
+          ptx::tmem_st_32x32(t_s(n) + lanes + half * 64 + 32, out);
+        }
         ptx::tmem_st_wait();
         ptx::tc_fence_before();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(p_ready(n));
-        ok = warp_wait(dp_full, n & 1, abort_flag);
-        if (!ok) break;
+        if (!warp_wait(dp_full, n & 1, abort_flag)) return false;
         ptx::tc_fence_after();
         ptx::tmem_ld_32x32(t_dp + lanes + half * 64, x[0]);
         ptx::tmem_ld_32x32(t_dp + lanes + half * 64 + 32, x[1]);
@@ -976,6 +1012,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dkv_kernel(const __grid_consta
 #pragma unroll
         for (int i = 0; i < 32; ++i) out[i] = f2_bf16(p[i]);
         ptx::tmem_st_32x32(t_dp + lanes + half * 64, out);
+        if constexpr (first.value) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) out[i] = rest_bf16(p[i], out[i]);
+          ptx::tmem_st_32x32(t_dp + lanes + half * 64 + 32, out);
+        }
         ptx::tmem_st_wait();
         ptx::tc_fence_before();
         __syncwarp();
@@ -983,6 +1024,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dkv_kernel(const __grid_consta
           ptx::mbar_arrive(ds_ready);
           ptx::mbar_arrive(st_empty(n));
         }
+        ++n;
+        return true;
+      };
+      for (int it = 0, i = 0; ok && it < sp.n_it; ++it) {
+        if (__builtin_expect(i > 0 || sp.key > 0, 1)) ok = block(i == 0, std::false_type());
+        else ok = block(true, std::true_type());
+        if (++i == sp.per_head) i = 0;
       }
       ok = ok && warp_wait(acc_full, r & 1, abort_flag);
       if (!ok) break;
@@ -1200,6 +1248,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dq_kernel(const __grid_constan
         if (ptx::elect_one()) {
           ptx::tc_fence_after();
           mma_tm<0, 8>(t_dq, t_s(b), kv + ds.s * PLACE, id_d, j > 0, 64);
+          if (nb == 1) mma_tm<0, 8>(t_dq, t_s(b) + 32, kv + ds.s * PLACE, id_d, true, 64);
           ptx::mma_commit(empty(ds.s));
           if (j + 1 == nb) ptx::mma_commit(acc_full);
         }
@@ -1241,9 +1290,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dq_kernel(const __grid_constan
       const long long at = (long long)w.sub * a.seqs.T + w.start + in_seq;
       const float lse = in_seq < w.len ? a.lse[at] : INFINITY, delta = in_seq < w.len ? a.delta[at] : 0.f;
       const F2 shift = f2(-lse, -lse), minus_delta = f2(-delta, -delta);
-      for (int j = 0; j < nb; ++j, ++b) {
-        ok = warp_wait(s_full(b), b >> 1 & 1, abort_flag);
-        if (!ok) break;
+      auto block = [&](int j, auto first) {   // (first: the rows and the keys are a sequence's first; apart, so that the others do not pay for it)
+        if (!warp_wait(s_full(b), b >> 1 & 1, abort_flag)) return false;
         ptx::tc_fence_after();
         F2 p[32];
         uint32_t x[2][32], ds[32];
@@ -1252,8 +1300,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dq_kernel(const __grid_constan
         ptx::tmem_ld_wait();
 #pragma unroll
         for (int i = 0; i < 32; ++i) p[i] = ex2_pair<kBwdPoly<DP>>(x[i / 16][i % 16 * 2], x[i / 16][i % 16 * 2 + 1], scale, shift, i);
-        ok = warp_wait(dp_full, b & 1, abort_flag);
-        if (!ok) break;
+        if (!warp_wait(dp_full, b & 1, abort_flag)) return false;
         ptx::tc_fence_after();
         ptx::tmem_ld_32x32(t_dp + lanes + half * 64, x[0]);
         ptx::tmem_ld_32x32(t_dp + lanes + half * 64 + 32, x[1]);
@@ -1268,10 +1315,22 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dq_kernel(const __grid_constan
 #pragma unroll
         for (int i = 0; i < 32; ++i) ds[i] = f2_bf16(p[i]);
         ptx::tmem_st_32x32(t_s(b) + lanes + half * 64, ds);
+        if constexpr (first.value) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) ds[i] = rest_bf16(p[i], ds[i]);
+          ptx::tmem_st_32x32(t_s(b) + lanes + half * 64 + 32, ds);
+        }
         ptx::tmem_st_wait();
         ptx::tc_fence_before();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(ds_ready);
+        ++b;
+        return true;
+      };
+      if (__builtin_expect(nb > 1, 1)) {
+        for (int j = 0; ok && j < nb; ++j) ok = block(j, std::false_type());
+      } else {
+        ok = block(0, std::true_type());
       }
       ok = ok && warp_wait(acc_full, r & 1, abort_flag);
       if (!ok) break;

@@ -69,13 +69,13 @@ int check_attention(const void* q, int64_t q_stride, const void* k, int64_t k_st
   return LEWI_OK;
 }
 
-template <int DP>
+template <int DP, bool TRAIN>
 int attention_fwd(cudaStream_t st, attn::Args a, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv) {
   static bool done[64] = {false};
-  if (!allow_smem(attn::fwd_kernel<DP>, attn::FwdShape<DP>::kSmem, done)) return LEWI_ERR_CUDA;
+  if (!allow_smem(attn::fwd_kernel<DP, TRAIN>, attn::FwdShape<DP>::kSmem, done)) return LEWI_ERR_CUDA;
   a.shape = attn::fwd_item(a.seqs.T, a.seqs.n, a.Hq, a.G);
   const long long items = attn::most_tiles(a.seqs.T, a.seqs.n) * (a.shape == attn::kTwoHeads ? a.Hq / 2 : a.Hq);
-  attn::fwd_kernel<DP><<<attn::ctas(items), attn::kFwdThreads, attn::FwdShape<DP>::kSmem, st>>>(tq, tk, tv, a);
+  attn::fwd_kernel<DP, TRAIN><<<attn::ctas(items), attn::kFwdThreads, attn::FwdShape<DP>::kSmem, st>>>(tq, tk, tv, a);
   LEWI_CHECK_LAUNCH();
   return LEWI_OK;
 }
@@ -218,7 +218,9 @@ int lewi_causal_attention_fwd(void* stream, const void* q, int64_t q_stride, con
     return LEWI_ERR_CUDA;
   const attn::Args a{{cu_seqlens, n_seqs, T}, Hq, Hkv, Hq / Hkv, D, scale, scale * 1.4426950408889634f, reinterpret_cast<bf16*>(o),
                      reinterpret_cast<bf16*>(o_rest), lse, nullptr, nullptr, nullptr, nullptr, 1, nullptr};
-  return D <= 64 ? attention_fwd<64>(as_stream(stream), a, tq, tk, tv) : attention_fwd<128>(as_stream(stream), a, tq, tk, tv);
+  cudaStream_t st = as_stream(stream);
+  if (o_rest != nullptr) return D <= 64 ? attention_fwd<64, true>(st, a, tq, tk, tv) : attention_fwd<128, true>(st, a, tq, tk, tv);
+  return D <= 64 ? attention_fwd<64, false>(st, a, tq, tk, tv) : attention_fwd<128, false>(st, a, tq, tk, tv);
 }
 
 int64_t lewi_causal_attention_bwd_workspace_bytes(int T, int n_seqs, int Hq, int Hkv, int D) {

@@ -1,8 +1,9 @@
 """Causal attention over packed sequences, forward and backward, against its formulas in 64 bits.
 
 Tolerances: a rounding to bf16 is off by u = 2^-8 of the value at most.  p is rounded for its product with v, so o is off by u sum p |v| and its
-own rounding.  delta is a sum over the rounded o.  dS is rounded for its products, so dQ is off by scale (u |dS| + p |delta's error|) |K|
-and its own rounding, and so on.  1e-4 of the magnitudes is room for float32: scores of magnitude up to 40 with sums of 128 products."""
+own rounding.  delta is a sum over o and what that rounding left (to u^2).  dS is rounded for its products, so dQ is off by
+scale (u |dS| + p |delta's error|) |K| and its own rounding, and so on.  In training, pairs of the first 128 rows of a sequence have p and dS
+in two roundings, that is to u^2.  1e-4 of the magnitudes is room for float32: scores of magnitude up to 40 with sums of 128 products."""
 import pytest
 import torch
 
@@ -12,8 +13,8 @@ U, F32 = 2.0 ** -8, 1e-4
 F64 = torch.float64
 
 
-def formulas(q, k, v, cu, scale, d_o=None, f32=F32):
-  """Outputs and gradients in 64 bits with their bounds, {name: (value, bound)}; rows of no sequence are zero."""
+def formulas(q, k, v, cu, scale, d_o=None, f32=F32, u=U):
+  """Outputs and gradients in 64 bits with their bounds, {name: (value, bound)}; rows of no sequence are zero.  p and dS are off by `u`."""
   t, hq, d = q.shape
   g = hq // k.shape[1]
   q, k, v = (x.to(F64) for x in (q, k, v))
@@ -27,15 +28,15 @@ def formulas(q, k, v, cu, scale, d_o=None, f32=F32):
       qh, kh, vh = q[a:b, h], k[a:b, h // g], v[a:b, h // g]
       p = torch.softmax((qh @ kh.t() * scale).masked_fill(~seen, float("-inf")), -1)
       oh = p @ vh
-      o[a:b, h], ob[a:b, h] = oh, U * oh.abs() + (U + f32) * (p @ vh.abs())
+      o[a:b, h], ob[a:b, h] = oh, U * oh.abs() + (u + f32) * (p @ vh.abs())
       if d_o is None:
         continue
       do = d_o[a:b, h].to(F64)
       dv[a:b, h // g] += p.t() @ do
-      dvb[a:b, h // g] += (U + f32) * (p.t() @ do.abs())
-      delta, delta_b = (do * oh).sum(-1, keepdim=True), (do.abs() * ob[a:b, h]).sum(-1, keepdim=True)
+      dvb[a:b, h // g] += (u + f32) * (p.t() @ do.abs())
+      delta, delta_b = (do * oh).sum(-1, keepdim=True), (do.abs() * (U * U * oh.abs() + (u + f32) * (p @ vh.abs()))).sum(-1, keepdim=True)
       ds = p * (do @ vh.t() - delta)
-      ds_b = U * ds.abs() + p * (delta_b + f32 * (do.abs() @ vh.abs().t() + (do * oh).abs().sum(-1, keepdim=True)))
+      ds_b = u * ds.abs() + p * (delta_b + f32 * (do.abs() @ vh.abs().t() + (do * oh).abs().sum(-1, keepdim=True)))
       dq[a:b, h], dqb[a:b, h] = scale * (ds @ kh), scale * (ds_b @ kh.abs())
       dk[a:b, h // g] += scale * (ds.t() @ qh)
       dkb[a:b, h // g] += scale * (ds_b.t() @ qh.abs())
@@ -303,8 +304,12 @@ def test_shared_operands_and_modes(cuda):
   o3 = attention.causal_attention(*parts)
   gs = torch.autograd.grad(o3, parts, d_o)
   assert torch.equal(o, o3) and torch.allclose(g.float(), sum(p.float() for p in gs), rtol=2 * U, atol=0.1)   # (autograd adds them in bf16)
-  with torch.no_grad():
-    assert torch.equal(attention.causal_attention(x, x, x), o)
+  want = formulas(*[x.detach().cpu()] * 3, [0, 260], 64 ** -0.5)["o"]
+  within(o, want, "o")
+  with torch.no_grad():   # (p is rounded in the first rows too)
+    o = attention.causal_attention(x, x, x)
+  within(o, want, "o without gradients")
+  assert torch.equal(o[128:], o3[128:])
   with torch.inference_mode():
     assert torch.equal(attention.causal_attention(x, x, x), o)
   wide = w.expand(260, 4, 64)
@@ -316,6 +321,23 @@ def test_shared_operands_and_modes(cuda):
   assert torch.equal(attention.causal_attention(turned, turned, turned), o)
   shifted = torch.cat([x.detach().flatten()[:1], x.detach().flatten()])[1:].view(260, 4, 64)   # two bytes off
   assert torch.equal(attention.causal_attention(shifted, shifted, shifted), o)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,hq,hkv,d,sharp", [([2, 1, 128, 77, 3, 0, 127], 4, 2, 64, 1), ([2] * 9, 3, 1, 128, 3), ([128, 5, 64, 65], 2, 2, 96, 5), ([100], 8, 1, 8, 2)])
+def test_first_rows_in_training_are_rounded_once(cuda, lens, hq, hkv, d, sharp):
+  """Rows of few keys, whose roundings no sum averages: results are off by their own rounding, and by u^2 and float32 of the magnitudes."""
+  gen = torch.Generator().manual_seed(sum(lens) + d)
+  t = sum(lens)
+  q, k, v, d_o = (rnd(gen, t, h, d) for h in (hq, hkv, hkv, hq))
+  q = sharp * q
+  cu = torch.tensor([0] + lens).cumsum(0)
+  want = formulas(q, k, v, cu.tolist(), d ** -0.5, d_o, u=U * U)
+  leaves = [x.to(cuda).requires_grad_(True) for x in (q, k, v)]
+  o = attention.causal_attention(*leaves, cu.to(cuda))
+  within(o, want["o"], "o")
+  for name, g in zip(("dq", "dk", "dv"), torch.autograd.grad(o, leaves, d_o.to(cuda))):
+    within(g, want[name], name)
 
 
 @pytest.mark.gpu
