@@ -112,6 +112,8 @@ class _CausalAttention(torch.autograd.Function):
 
   @staticmethod
   def backward(ctx, g):
+    if torch.is_grad_enabled():   # (create_graph: what these kernels do would be missing from it)
+      raise LewiError("causal_attention is differentiable once")
     lib = _lib.load()
     q, k, v, o, o_rest, lse, cu = ctx.saved_tensors
     n_seqs, scale, (q_rows, k_rows, v_rows) = ctx.call
@@ -133,7 +135,7 @@ def causal_attention(query, key, value, cu_seqlens=None, scale=None):
   """softmax(scale q k^T) v over the rows of a sequence up to the query's own.  Packed: query [T, Hq, D], key, value [T, Hkv, D] bf16, sequence s
   the rows cu_seqlens[s] .. cu_seqlens[s+1] (int32 or int64 [N + 1], ascending, empty ones among them; none: one sequence), or sequences of one
   length: query [B, S, Hq, D], key, value [B, S, Hkv, D].  Head h has the keys of head h // (Hq // Hkv); D up to 128, a multiple of 8;
-  `scale` > 0 defaults to D ** -0.5.  Returns bf16 of the query's shape; differentiable through `torch.autograd` in query, key and value.
+  `scale` > 0 defaults to D ** -0.5.  Returns bf16 of the query's shape; differentiable through `torch.autograd`, once, in query, key and value.
   Rows of no sequence give zeros and get zero gradients, whatever they hold.  Bounds that fall or leave the rows:
   `LEWI_STATUS_BAD_INDEX` in `_lib.last_status()`.  Rows may lie apart (views of one projection need no copy).
 

@@ -321,6 +321,8 @@ def test_shared_operands_and_modes(cuda):
   assert torch.equal(attention.causal_attention(turned, turned, turned), o)
   shifted = torch.cat([x.detach().flatten()[:1], x.detach().flatten()])[1:].view(260, 4, 64)   # two bytes off
   assert torch.equal(attention.causal_attention(shifted, shifted, shifted), o)
+  with pytest.raises(LewiError, match="differentiable once"):
+    torch.autograd.grad(attention.causal_attention(x, x, x), x, d_o, create_graph=True)
 
 
 @pytest.mark.gpu
