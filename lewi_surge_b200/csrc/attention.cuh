@@ -333,7 +333,7 @@ struct ItemQueue {
 // and scores are on their way while O of this one is written out.  p is rounded to bf16 for its product, its sum l is taken before; in training
 // (TRAIN) the first tile of a sequence, whose rows have few keys and errors that no sum averages, is multiplied by what that left as well.
 //
-// Where such items are too few for the SMs an item is one tile (fwd_item).  Its scores have both places, so that those of the next block are there
+// Where such items are too few for the SMs an item is one tile (ONE, by fwd_item).  Its scores have both places, so that those of the next block are there
 // when a softmax ends, which then scales O after the product before (pv_done).  Each row's steps are the same, and so are its bits.
 //
 // What bounds it: a tile's chain S -> softmax -> P -> S, 2900 cycles for both tiles of a block where their products take 2048 (D = 128) or
@@ -346,7 +346,7 @@ struct FwdShape {
   static constexpr int kSmem = (2 + kStages) * kTileBytes<DP> + kStaging + kBarriers;
 };
 
-template <int DP, bool TRAIN>
+template <int DP, bool TRAIN, bool ONE>
 __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                                                              const __grid_constant__ CUtensorMap tm_v, const Args a) {
   constexpr int ST = FwdShape<DP>::kStages, TB = kTileBytes<DP>;
@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
   auto o_at = [&](int t) { return tmem + 256 + t * 128; };
   auto tile_of = [&](const Item& w, int t) { return a.shape == kTwoTiles ? 2 * w.level + t : w.level; };
   auto head_of = [&](const Item& w, int t) { return a.shape == kTwoHeads ? 2 * w.sub + t : w.sub; };
-  auto blocks_of = [&](const Item& w, int t) { return tile_of(w, t) * kTile < w.len && (t == 0 || a.shape != kOneTile) ? tile_of(w, t) + 1 : 0; };
+  auto blocks_of = [&](const Item& w, int t) { return tile_of(w, t) * kTile < w.len && (t == 0 || !ONE) ? tile_of(w, t) + 1 : 0; };
 
   // registers: 8 x 216 + 4 x 72 = 12 x 168 a thread, what the launch has
   if (warp >= 8) {
@@ -443,7 +443,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
           const Item w = items.take_alone(r);
           if (w.level < 0) break;
           const int blocks[2] = {blocks_of(w, 0), blocks_of(w, 1)}, nb = max(blocks[0], blocks[1]);
-          if (a.shape == kOneTile) {   // S(0) S(1) | P(j) V(j), S(j + 2) after P(j)
+          if constexpr (ONE) {   // S(0) S(1) | P(j) V(j), S(j + 2) after P(j)
             auto scores = [&](int j) {
               const int x = n + 2 * j;
               if (!ptx::mbar_wait(full(x), x / ST & 1, abort_flag)) return false;
@@ -475,50 +475,50 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
             n += 2 * nb;
             done[0] += nb;
             ++used[0];
-            continue;
-          }
-          auto scores = [&](int t, int j) {
-            ptx::tc_fence_after();
-            mma_kk<DP>(s_at(t), base + t * TB, kv + (n + 2 * j) % ST * TB, id_s);
-            ptx::mma_commit(s_full(t));
-            if (j + 1 == blocks[t]) ptx::mma_commit(q_empty(t));
-          };
-          ok = ptx::mbar_wait(full(n), n / ST & 1, abort_flag);
-          for (int t = 0; ok && t < 2; ++t)
-            if (blocks[t] > 0) {
-              ok = ptx::mbar_wait(q_full(t), used[t] & 1, abort_flag);
-              if (ok) scores(t, 0);
-            }
-          if (!ok) break;
-          ptx::mma_commit(empty(n));
-          for (int j = 0; ok && j < nb; ++j) {
-            const int nv = n + 2 * j + 1, nk = nv + 1;
-            ok = ptx::mbar_wait(full(nv), nv / ST & 1, abort_flag);
-            for (int t = 0; ok && t < 2; ++t) {
-              if (j >= blocks[t]) continue;
-              ok = (j > 0 || ptx::mbar_wait(o_empty(t), (used[t] & 1) ^ 1u, abort_flag)) && ptx::mbar_wait(p_full(t, 0), done[t] & 1, abort_flag);
-              if (!ok) break;
+          } else {
+            auto scores = [&](int t, int j) {
               ptx::tc_fence_after();
-              mma_tm<0, 4>(o_at(t), s_at(t), kv + nv % ST * TB, id_o, j > 0, 32);
-              ok = ptx::mbar_wait(p_full(t, 1), done[t] & 1, abort_flag);
-              if (!ok) break;
-              ptx::tc_fence_after();
-              mma_tm<4, 8>(o_at(t), s_at(t), kv + nv % ST * TB, id_o, true, 32);
-              if (TRAIN && blocks[t] == 1) mma_tm<0, 8>(o_at(t), s_at(t) + 64, kv + nv % ST * TB, id_o, true, 32);
-              ++done[t];
-              if (j + 1 < blocks[t]) {
-                ok = ptx::mbar_wait(full(nk), nk / ST & 1, abort_flag);
-                if (ok) scores(t, j + 1);
-              } else {
-                ptx::mma_commit(o_full(t));
+              mma_kk<DP>(s_at(t), base + t * TB, kv + (n + 2 * j) % ST * TB, id_s);
+              ptx::mma_commit(s_full(t));
+              if (j + 1 == blocks[t]) ptx::mma_commit(q_empty(t));
+            };
+            ok = ptx::mbar_wait(full(n), n / ST & 1, abort_flag);
+            for (int t = 0; ok && t < 2; ++t)
+              if (blocks[t] > 0) {
+                ok = ptx::mbar_wait(q_full(t), used[t] & 1, abort_flag);
+                if (ok) scores(t, 0);
               }
-            }
             if (!ok) break;
-            ptx::mma_commit(empty(nv));
-            if (j + 1 < nb) ptx::mma_commit(empty(nk));
+            ptx::mma_commit(empty(n));
+            for (int j = 0; ok && j < nb; ++j) {
+              const int nv = n + 2 * j + 1, nk = nv + 1;
+              ok = ptx::mbar_wait(full(nv), nv / ST & 1, abort_flag);
+              for (int t = 0; ok && t < 2; ++t) {
+                if (j >= blocks[t]) continue;
+                ok = (j > 0 || ptx::mbar_wait(o_empty(t), (used[t] & 1) ^ 1u, abort_flag)) && ptx::mbar_wait(p_full(t, 0), done[t] & 1, abort_flag);
+                if (!ok) break;
+                ptx::tc_fence_after();
+                mma_tm<0, 4>(o_at(t), s_at(t), kv + nv % ST * TB, id_o, j > 0, 32);
+                ok = ptx::mbar_wait(p_full(t, 1), done[t] & 1, abort_flag);
+                if (!ok) break;
+                ptx::tc_fence_after();
+                mma_tm<4, 8>(o_at(t), s_at(t), kv + nv % ST * TB, id_o, true, 32);
+                if (TRAIN && blocks[t] == 1) mma_tm<0, 8>(o_at(t), s_at(t) + 64, kv + nv % ST * TB, id_o, true, 32);
+                ++done[t];
+                if (j + 1 < blocks[t]) {
+                  ok = ptx::mbar_wait(full(nk), nk / ST & 1, abort_flag);
+                  if (ok) scores(t, j + 1);
+                } else {
+                  ptx::mma_commit(o_full(t));
+                }
+              }
+              if (!ok) break;
+              ptx::mma_commit(empty(nv));
+              if (j + 1 < nb) ptx::mma_commit(empty(nk));
+            }
+            n += 2 * nb;
+            for (int t = 0; t < 2; ++t) used[t] += blocks[t] > 0;
           }
-          n += 2 * nb;
-          for (int t = 0; t < 2; ++t) used[t] += blocks[t] > 0;
         }
         if (s_abort) settle();
       }
@@ -547,7 +547,6 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
     const int t = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;   // this warp's lanes of tensor memory
     const uint32_t op = o_at(t) + lanes;
-    const bool one = a.shape == kOneTile;
     const F2 scale = f2(a.scale_log2, a.scale_log2);
     int used = 0, done = 0;
     bool ok = true;
@@ -559,9 +558,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
       const bool mine = tile * kTile + row < w.len;   // (what other sequences' rows hold decides nothing)
       float m = 0.f, l = 0.f;
       auto block = [&](int j, auto first) {   // (first: in training and of a sequence's first tile; apart, so that the others do not pay for it)
-        const int place = one ? done & 1 : t;
+        const int place = ONE ? done & 1 : t;
         const uint32_t sp = s_at(place) + lanes;
-        if (!warp_wait(s_full(place), (one ? done >> 1 : done) & 1, abort_flag)) return false;
+        if (!warp_wait(s_full(place), (ONE ? done >> 1 : done) & 1, abort_flag)) return false;
         ptx::tc_fence_after();
         uint32_t s[4][32];
 #pragma unroll
@@ -585,7 +584,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
         if (j == 0) {
           m = top;
         } else if (__any_sync(0xffffffffu, mine && (top - m) * a.scale_log2 > 8.f)) {
-          if (one && !warp_wait(pv_done, (done & 1) ^ 1u, abort_flag)) return false;   // of the block before
+          if (ONE && !warp_wait(pv_done, (done & 1) ^ 1u, abort_flag)) return false;   // of the block before
           ptx::tc_fence_after();
           const float grown = fmaxf(m, top), f = grown == m ? 1.f : ex2((m - grown) * a.scale_log2);
           m = grown;

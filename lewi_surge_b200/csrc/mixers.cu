@@ -69,15 +69,21 @@ int check_attention(const void* q, int64_t q_stride, const void* k, int64_t k_st
   return LEWI_OK;
 }
 
-template <int DP, bool TRAIN>
-int attention_fwd(cudaStream_t st, attn::Args a, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv) {
+template <int DP, bool TRAIN, bool ONE>
+int attention_fwd(cudaStream_t st, const attn::Args& a, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv) {
   static bool done[64] = {false};
-  if (!allow_smem(attn::fwd_kernel<DP, TRAIN>, attn::FwdShape<DP>::kSmem, done)) return LEWI_ERR_CUDA;
-  a.shape = attn::fwd_item(a.seqs.T, a.seqs.n, a.Hq, a.G);
+  if (!allow_smem(attn::fwd_kernel<DP, TRAIN, ONE>, attn::FwdShape<DP>::kSmem, done)) return LEWI_ERR_CUDA;
   const long long items = attn::most_tiles(a.seqs.T, a.seqs.n) * (a.shape == attn::kTwoHeads ? a.Hq / 2 : a.Hq);
-  attn::fwd_kernel<DP, TRAIN><<<attn::ctas(items), attn::kFwdThreads, attn::FwdShape<DP>::kSmem, st>>>(tq, tk, tv, a);
+  attn::fwd_kernel<DP, TRAIN, ONE><<<attn::ctas(items), attn::kFwdThreads, attn::FwdShape<DP>::kSmem, st>>>(tq, tk, tv, a);
   LEWI_CHECK_LAUNCH();
   return LEWI_OK;
+}
+
+template <int DP>
+int attention_fwd(cudaStream_t st, const attn::Args& a, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv) {
+  const bool one = a.shape == attn::kOneTile;
+  if (a.o_rest != nullptr) return one ? attention_fwd<DP, true, true>(st, a, tq, tk, tv) : attention_fwd<DP, true, false>(st, a, tq, tk, tv);
+  return one ? attention_fwd<DP, false, true>(st, a, tq, tk, tv) : attention_fwd<DP, false, false>(st, a, tq, tk, tv);
 }
 
 template <int DP>
@@ -217,10 +223,9 @@ int lewi_causal_attention_fwd(void* stream, const void* q, int64_t q_stride, con
       !attn::make_rows_map(&tv, v, T, Hkv, D, v_stride))
     return LEWI_ERR_CUDA;
   const attn::Args a{{cu_seqlens, n_seqs, T}, Hq, Hkv, Hq / Hkv, D, scale, scale * 1.4426950408889634f, reinterpret_cast<bf16*>(o),
-                     reinterpret_cast<bf16*>(o_rest), lse, nullptr, nullptr, nullptr, nullptr, 1, nullptr};
+                     reinterpret_cast<bf16*>(o_rest), lse, nullptr, nullptr, nullptr, nullptr, 1, nullptr, attn::fwd_item(T, n_seqs, Hq, Hq / Hkv)};
   cudaStream_t st = as_stream(stream);
-  if (o_rest != nullptr) return D <= 64 ? attention_fwd<64, true>(st, a, tq, tk, tv) : attention_fwd<128, true>(st, a, tq, tk, tv);
-  return D <= 64 ? attention_fwd<64, false>(st, a, tq, tk, tv) : attention_fwd<128, false>(st, a, tq, tk, tv);
+  return D <= 64 ? attention_fwd<64>(st, a, tq, tk, tv) : attention_fwd<128>(st, a, tq, tk, tv);
 }
 
 int64_t lewi_causal_attention_bwd_workspace_bytes(int T, int n_seqs, int Hq, int Hkv, int D) {
