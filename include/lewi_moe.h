@@ -388,8 +388,8 @@ int lewi_paged_attention(void* stream, const void* q, int64_t q_stride, const vo
  * Causal attention over packed sequences, forward and backward: o[t,h] = softmax_j(scale q[t,h].k[j]) v[j] over the rows j <= t of t's own
  * sequence, with the key head h / (Hq / Hkv).  q, o bf16 [T][Hq][D], k, v bf16 [T][Hkv][D]; sequence s has the rows
  * cu_seqlens[s] .. cu_seqlens[s+1] (i32 [n_seqs + 1], ascending; null: n_seqs sequences of T / n_seqs rows).  Rows of no sequence get zeros, in o
- * and in the gradients, whatever they hold.  Bounds that fall or leave the rows raise LEWI_STATUS_BAD_INDEX; what they cut is
- * undefined.  lse f32 [Hq][T] (log2 of the softmax's denominator) and o_rest bf16 [T][Hq][D] (what rounding o left
+ * and in the gradients, whatever they hold.  Bounds that leave the rows are cut to them; where bounds fall, no
+ * sequence of the call is worked on and what its outputs hold is undefined; LEWI_STATUS_BAD_INDEX either way.  lse f32 [Hq][T] (log2 of the softmax's denominator) and o_rest bf16 [T][Hq][D] (what rounding o left
  * of it) are for the backward pass and both null where none follows; their rows of no sequence are left as they are.
  * D <= 128, a multiple of 8; T * Hq / Hkv <= 2^25; scale > 0; all tensors 16-byte aligned, `*_stride` (elements from row to row; heads are contiguous) multiples
  * of 8.  Scores, softmax and sums float32; p and the gradient of the scores are rounded to bf16 for their products (where lse is given and in the

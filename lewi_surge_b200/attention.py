@@ -136,8 +136,8 @@ def causal_attention(query, key, value, cu_seqlens=None, scale=None):
   the rows cu_seqlens[s] .. cu_seqlens[s+1] (int32 or int64 [N + 1], ascending, empty ones among them; none: one sequence), or sequences of one
   length: query [B, S, Hq, D], key, value [B, S, Hkv, D].  Head h has the keys of head h // (Hq // Hkv); D up to 128, a multiple of 8;
   `scale` > 0 defaults to D ** -0.5.  Returns bf16 of the query's shape; differentiable through `torch.autograd`, once, in query, key and value.
-  Rows of no sequence give zeros and get zero gradients, whatever they hold.  Bounds that fall or leave the rows:
-  `LEWI_STATUS_BAD_INDEX` in `_lib.last_status()`.  Rows may lie apart (views of one projection need no copy).
+  Rows of no sequence give zeros and get zero gradients, whatever they hold.  Bounds that leave the rows are cut to them; where bounds fall, no
+  sequence is worked on and the results are undefined; either way `LEWI_STATUS_BAD_INDEX` in `_lib.last_status()`.  Rows may lie apart (views of one projection need no copy).
 
   Outputs with and without gradients wanted may differ by a rounding in the first 128 rows of a sequence, whose p are kept to 2^-16 for the former.
 

@@ -68,12 +68,17 @@ __device__ __forceinline__ void plan_items(const Seqs& q, int rows, int subs, Pl
   if (alike) {
     most = unit_count(0);
   } else {
+    bool falls = false;
     for (int s = lane; s < q.n; s += 32) {
       const int u = unit_count(s);
       if (kept) plan.units[s] = u;
       most = max(most, u);
+      falls |= q.cu[s + 1] < q.cu[s];
     }
     most = __reduce_max_sync(0xffffffffu, most);
+    // Sequences whose bounds ascend share no row, so that there are at most T / rows + n units.  Where bounds fall they could name all rows again
+    // and again (more work than any grid should have, more units than 32 bits count): such a call has no sequence at all.
+    if (__any_sync(0xffffffffu, falls)) most = 0;
     __syncwarp();
   }
   auto units = [&](int s) { return kept ? plan.units[s] : unit_count(s); };
@@ -82,7 +87,7 @@ __device__ __forceinline__ void plan_items(const Seqs& q, int rows, int subs, Pl
     for (int s = lane; s < q.n; s += 32) v += max(0, units(s) - i);
     return __reduce_add_sync(0xffffffffu, v);
   };
-  const int all = alike ? most * q.n : count(0);
+  const int all = most == 0 ? 0 : alike ? most * q.n : count(0);
   int lo = most, first = 0, end = 0;   // the unit number of the last item, F(lo + 1) and F(lo): units of this number are the x in between
   int s0 = 0, passed = 0;              // the sequences before s0 have `passed` of them
   for (int r = 0;; ++r) {

@@ -372,3 +372,23 @@ def test_a_sequence_among_many_has_the_bits_that_it_has_alone(cuda, n, s, hq, hk
     for h in range(hkv):
       heads = slice(h * (hq // hkv), (h + 1) * (hq // hkv))
       assert torch.equal(whole[i][:, heads], attention.causal_attention(q[i][:, heads], k[i][:, h:h + 1], v[i][:, h:h + 1]))
+
+
+@pytest.mark.gpu
+def test_bounds_that_fall_again_and_again_name_no_rows(cuda):
+  """Every other sequence would be all rows: T / 128 units each, past any grid and, with enough of them, past 32 bits.  Nothing is worked on."""
+  t, n, h, d = 4096, 2001, 1, 64
+  q = torch.randn(t, h, d, device=cuda).bfloat16()
+  cu = torch.tensor([0, t] * ((n + 1) // 2), dtype=torch.int32, device=cuda)
+  lib, at = _lib.load(), lambda x: x.data_ptr()
+  mark = lambda: torch.full_like(q, 7.0)
+  o, rest, dq, dk, dv, lse = mark(), mark(), mark(), mark(), mark(), torch.full((h, t), 7.0, device=cuda)
+  rows = [at(q), h * d] * 3
+  assert lib.lewi_causal_attention_fwd(_lib.stream(), *rows, at(cu), n, at(o), at(rest), at(lse), t, h, h, d, 0.1) == 0
+  assert _lib.last_status() == _lib.STATUS_BAD_INDEX
+  ws = torch.empty(lib.lewi_causal_attention_bwd_workspace_bytes(t, n, h, h, d), dtype=torch.uint8, device=cuda)
+  assert lib.lewi_causal_attention_bwd(_lib.stream(), *rows, at(o), at(rest), at(lse), at(q), at(cu), n, at(dq), at(dk), at(dv), at(ws), ws.numel(),
+                                       t, h, h, d, 0.1) == 0
+  assert _lib.last_status() == _lib.STATUS_BAD_INDEX
+  for x in (o, rest, dq, dk, dv, lse):
+    assert (x == 7).all()
