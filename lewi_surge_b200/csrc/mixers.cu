@@ -96,8 +96,8 @@ int attention_bwd(cudaStream_t st, const attn::Args& a, const CUtensorMap& tq, c
   if (a.dk != nullptr) {
     static bool done[64] = {false};
     if (!allow_smem(attn::dkv_kernel<DP>, attn::DkvShape<DP>::kSmem, done)) return LEWI_ERR_CUDA;
-    (void)launch_kernel(attn::dkv_kernel<DP>, (int)attn::ctas(tiles * a.Hkv * a.parts), attn::kBwdThreads, attn::DkvShape<DP>::kSmem, st, true, tq, tk,
-                        tv, td, a);
+    (void)launch_kernel(attn::dkv_kernel<DP>, (int)attn::ctas(tiles * a.Hkv * a.parts), attn::kBwdThreads, attn::DkvShape<DP>::kSmem, st, false, tq, tk,
+                        tv, td, a);   // (not early: dQ's kernel, which is, reads delta too)
     LEWI_CHECK_LAUNCH();
   }
   if (a.dq != nullptr) {

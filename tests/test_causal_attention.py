@@ -392,3 +392,18 @@ def test_bounds_that_fall_again_and_again_name_no_rows(cuda):
   assert _lib.last_status() == _lib.STATUS_BAD_INDEX
   for x in (o, rest, dq, dk, dv, lse):
     assert (x == 7).all()
+
+
+@pytest.mark.gpu
+def test_dq_beside_dk_and_dv_is_dq_alone(cuda):
+  """dQ's kernel begins while the one for dK and dV runs and reads a sum that a third one made: small calls of new values one behind another."""
+  gen = torch.Generator(device=cuda).manual_seed(12)
+  data = [[torch.randn(40 + i, h, 64, generator=gen, device=cuda).bfloat16() for h in (2, 1, 1, 2)] for i in range(150)]
+  def grads(wanted):
+    out = []
+    for *operands, d_o in data:
+      leaves = [x.detach().requires_grad_(w) for x, w in zip(operands, wanted)]
+      out.append(torch.autograd.grad(attention.causal_attention(*leaves), leaves[0], d_o)[0])
+    return out
+  for both, alone in zip(grads((True, True, True)), grads((True, False, False))):
+    assert torch.equal(both, alone)
