@@ -390,7 +390,9 @@ int lewi_paged_attention(void* stream, const void* q, int64_t q_stride, const vo
  * cu_seqlens[s] .. cu_seqlens[s+1] (i32 [n_seqs + 1], ascending; null: n_seqs sequences of T / n_seqs rows).  Rows of no sequence get zeros, in o
  * and in the gradients, whatever they hold.  Bounds that leave the rows are cut to them; where bounds fall, no
  * sequence of the call is worked on and what its outputs hold is undefined; LEWI_STATUS_BAD_INDEX either way.  lse f32 [Hq][T] (log2 of the softmax's denominator) and o_rest bf16 [T][Hq][D] (what rounding o left
- * of it) are for the backward pass and both null where none follows; their rows of no sequence are left as they are.
+ * of it) are for the backward pass; where none follows lse is null, and o_rest may be too up to T = 32768 (beyond it is a place for sums,
+ * LEWI_ERR_WORKSPACE without it).  Their rows of no sequence are left as they are.  No accumulator of the tensor cores, which truncate, sums
+ * more than 32768 rows: sums of one sign come out short by 2^-12 of themselves at most, whatever the length.
  * D <= 128, a multiple of 8; T * Hq / Hkv <= 2^25; scale > 0; all tensors 16-byte aligned, `*_stride` (elements from row to row; heads are contiguous) multiples
  * of 8.  Scores, softmax and sums float32; p and the gradient of the scores are rounded to bf16 for their products (where lse is given and in the
  * backward call, pairs of a sequence's first 128 rows in two parts, to 2^-16).

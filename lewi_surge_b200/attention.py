@@ -87,6 +87,9 @@ def paged_attention(query, key_cache, value_cache, block_tables, lengths, scale=
   return o
 
 
+_CHAIN_ROWS = 32768   # rows of a sequence from which on the forward pass keeps sums in `o_rest` (more go into no accumulator)
+
+
 def _attention_fwd(q, k, v, cu, n_seqs, scale, o_rest=None, lse=None):
   """Output, the operands as the kernels read them and the distances of their rows; `o_rest` like the output and `lse` [Hq, T] receive
   what the backward pass needs."""
@@ -94,6 +97,8 @@ def _attention_fwd(q, k, v, cu, n_seqs, scale, o_rest=None, lse=None):
   cu = _lib.index_table(cu, "cu_seqlens")
   t, hq, d = q.shape
   o = torch.empty_like(q, memory_format=torch.contiguous_format)
+  if o_rest is None and t > _CHAIN_ROWS:
+    o_rest = torch.empty_like(o)
   check(_lib.load().lewi_causal_attention_fwd(stream(), q.data_ptr(), q_rows, k.data_ptr(), k_rows, v.data_ptr(), v_rows, ptr(cu), n_seqs,
                                               o.data_ptr(), ptr(o_rest), ptr(lse), t, hq, k.shape[1], d, scale), "lewi_causal_attention_fwd")
   return o, q, k, v, cu, (q_rows, k_rows, v_rows)

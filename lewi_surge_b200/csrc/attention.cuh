@@ -24,6 +24,10 @@ namespace attn {
 
 constexpr int kTile = 128;
 constexpr int kMaxD = 128;
+// Tiles whose products go into one accumulator.  The tensor core truncates every sum that it makes: a sum of one sign over n rows comes out short by about
+// n 2^-27 of itself (o of 2^20 rows, v and the weights alike, by 2^-7).  After so many tiles an accumulator is therefore added to float32 sums kept in
+// memory, which rounds to nearest, and starts from zero: 2^-12 at most.
+constexpr int kChain = 256;
 constexpr int64_t kMaxGroupRows = 1 << 25;   // rows times heads per key head: an item of dK and dV (0.4 s) stays below what a wait may last
 
 // ---------------------------------------------------------------- which tiles there are
@@ -250,11 +254,12 @@ struct Args {
   Seqs seqs;
   int Hq, Hkv, G, D;
   float scale, scale_log2;
-  __nv_bfloat16 *o, *o_rest;   // [T][Hq][D]; what rounding o left of it, for the backward pass
-  float *lse, *delta;      // [Hq][T], lse in units of log 2 (null, as o_rest, in a forward pass that none back follows)
+  __nv_bfloat16 *o, *o_rest;   // [T][Hq][D]; what rounding o left of it, for the backward pass and for sums of chains
+  float *lse, *delta;      // [Hq][T], lse in units of log 2 (null in a forward pass that none back follows)
   __nv_bfloat16 *dq, *dk, *dv;
   int parts;               // of a group's heads, one CTA each for dK and dV
   float* sums;             // [part][dV, dK][T][Hkv][D] where there are several
+  float4 *chain_kv, *chain_q;   // per CTA [dV, dK or dQ][DP / 4][128]: sums of an item's chains so far (null where none is longer than kChain)
   FwdItem shape;           // of the forward pass
 };
 
@@ -283,6 +288,23 @@ __device__ __forceinline__ void pack_row(uint32_t (&out)[16], const uint32_t (&v
 __device__ __forceinline__ void half_row(uint32_t (&out)[16], const uint32_t (&v)[32], int half, float f) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) out[i] = __float_as_uint(__uint_as_float(v[16 * half + i]) * f);
+}
+
+// 32 columns of a row to or from the sums of chains: `at` is the place of the row and the first column, four columns are 128 rows apart.
+__device__ __forceinline__ void add_chain(uint32_t (&v)[32], const float4* at) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float4 x = __ldcg(at + i * kTile);
+    v[4 * i] = __float_as_uint(__uint_as_float(v[4 * i]) + x.x);
+    v[4 * i + 1] = __float_as_uint(__uint_as_float(v[4 * i + 1]) + x.y);
+    v[4 * i + 2] = __float_as_uint(__uint_as_float(v[4 * i + 2]) + x.z);
+    v[4 * i + 3] = __float_as_uint(__uint_as_float(v[4 * i + 3]) + x.w);
+  }
+}
+__device__ __forceinline__ void put_chain(const uint32_t (&v)[32], float4* at) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    __stcg(at + i * kTile, make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]), __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3])));
 }
 
 // What the roles of a kernel share: barriers of the items, the planning warp's loop, and how a warp or a thread takes an item.
@@ -359,6 +381,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   __shared__ Plan s_plan;
+  __shared__ float s_kept[2 * kTile];   // the maximum that a row's kept sums are relative to
   const uint32_t base = ptx::smem_u32(attn_smem);
   if ((base & 1023u) != 0) {
     if (threadIdx.x == 0) raise_status(LEWI_STATUS_SMEM_LAYOUT);
@@ -466,7 +489,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
               ok = ptx::mbar_wait(full(x), x / ST & 1, abort_flag) && ptx::mbar_wait(p_full(b & 1, 0), b >> 1 & 1, abort_flag);
               if (!ok) break;
               ptx::tc_fence_after();
-              mma_tm<0, 4>(o_at(0), s_at(b & 1), kv + x % ST * TB, id_o, j > 0, 32);
+              mma_tm<0, 4>(o_at(0), s_at(b & 1), kv + x % ST * TB, id_o, j % kChain != 0, 32);
               ok = ptx::mbar_wait(p_full(b & 1, 1), b >> 1 & 1, abort_flag);
               if (!ok) break;
               ptx::tc_fence_after();
@@ -503,7 +526,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
                 ok = (j > 0 || ptx::mbar_wait(o_empty(t), (used[t] & 1) ^ 1u, abort_flag)) && ptx::mbar_wait(p_full(t, 0), done[t] & 1, abort_flag);
                 if (!ok) break;
                 ptx::tc_fence_after();
-                mma_tm<0, 4>(o_at(t), s_at(t), kv + nv % ST * TB, id_o, j > 0, 32);
+                mma_tm<0, 4>(o_at(t), s_at(t), kv + nv % ST * TB, id_o, j % kChain != 0, 32);
                 ok = ptx::mbar_wait(p_full(t, 1), done[t] & 1, abort_flag);
                 if (!ok) break;
                 ptx::tc_fence_after();
@@ -562,6 +585,43 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
       if (n_blocks == 0) continue;
       const bool mine = tile * kTile + row < w.len;   // (what other sequences' rows hold decides nothing)
       float m = 0.f, l = 0.f;
+      const int row0 = tile * kTile + (warp & 3) * 32, valid = w.len - row0;   // of this warp's rows
+      const long long at = ((long long)(w.start + row0) * a.Hq + head) * a.D, stride = (long long)a.Hq * a.D * 2;
+      uint8_t* stage = attn_smem + (2 + ST) * TB + warp * 2048;
+      auto store = [&](__nv_bfloat16* to, const uint32_t (&x)[16], int c) {
+        store_rows(stage, x, reinterpret_cast<uint8_t*>(to + at + c * 32), stride, valid, (a.D - c * 32) * 2);
+      };
+      auto column = [&](int c, uint32_t (&v)[32]) {
+        ptx::tmem_ld_32x32(op + c * 32, v);
+        ptx::tmem_ld_wait();
+      };
+      // adds what earlier chains left in o and o_rest, which is relative to an earlier maximum
+      auto add_kept = [&](int c, uint32_t (&v)[32]) {
+        const float before = s_kept[threadIdx.x], f = before == m ? 1.f : ex2((before - m) * a.scale_log2);
+        const long long from = at + (long long)lane * a.Hq * a.D + c * 32;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (lane >= valid || c * 32 + i * 8 >= a.D) continue;
+          const uint4 x = __ldcg(reinterpret_cast<const uint4*>(a.o + from + i * 8)), y = __ldcg(reinterpret_cast<const uint4*>(a.o_rest + from + i * 8));
+          const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t &lo = v[i * 8 + 2 * e], &hi = v[i * 8 + 2 * e + 1];
+            lo = __float_as_uint(fmaf(bf16_lo(xs[e]) + bf16_lo(ys[e]), f, __uint_as_float(lo)));
+            hi = __float_as_uint(fmaf(bf16_hi(xs[e]) + bf16_hi(ys[e]), f, __uint_as_float(hi)));
+          }
+        }
+      };
+      // columns times `inv` to o and, what their rounding leaves, to o_rest
+      auto store_twice = [&](int c, const uint32_t (&v)[32], float inv) {
+        uint32_t out[16], rest[16];
+        pack_row(out, v, inv);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          rest[i] = pack_bf16(__uint_as_float(v[2 * i]) * inv - bf16_lo(out[i]), __uint_as_float(v[2 * i + 1]) * inv - bf16_hi(out[i]));
+        store(a.o, out, c);
+        store(a.o_rest, rest, c);
+      };
       auto block = [&](int j, auto first) {   // (first: in training and of a sequence's first tile; apart, so that the others do not pay for it)
         const int place = ONE ? done & 1 : t;
         const uint32_t sp = s_at(place) + lanes;
@@ -642,7 +702,24 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
         return true;
       };
       if (__builtin_expect(!TRAIN || n_blocks > 1, 1)) {
-        for (int j = 0; ok && j < n_blocks; ++j) ok = block(j, std::false_type());
+        int j = 0;
+        for (;;) {
+          for (const int end = min(j + kChain, n_blocks); ok && j < end; ++j) ok = block(j, std::false_type());
+          if (!ok || j == n_blocks) break;
+          // a chain ends: O so far is kept in o and o_rest, and starts from zero.  (Its last product is done when the next scores are, as in `block`.)
+          ok = ONE ? warp_wait(pv_done, (done & 1) ^ 1u, abort_flag) : warp_wait(s_full(t), done & 1, abort_flag);
+          if (!ok) break;
+          ptx::tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < DP / 32; ++c) {
+            uint32_t v[32];
+            column(c, v);
+            if (j > kChain) add_kept(c, v);
+            store_twice(c, v, 1.f);
+          }
+          __syncwarp();   // (rows are read again by other lanes than have stored them)
+          s_kept[threadIdx.x] = m;
+        }
       } else {
         ok = block(0, std::bool_constant<TRAIN>());
       }
@@ -650,33 +727,28 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
       if (!ok) break;
       ++used;
       ptx::tc_fence_after();
+      if (__builtin_expect(n_blocks > kChain, 0)) {   // (the last chain and the others, for what follows)
+#pragma unroll 1
+        for (int c = 0; c < DP / 32; ++c) {
+          uint32_t v[32];
+          column(c, v);
+          add_kept(c, v);
+          ptx::tmem_st_32x32(op + c * 32, v);
+        }
+        ptx::tmem_st_wait();
+      }
       const float inv = 1.f / l;
-      const int row0 = tile * kTile + (warp & 3) * 32, valid = w.len - row0;   // of this warp's rows
-      const long long at = ((long long)(w.start + row0) * a.Hq + head) * a.D, stride = (long long)a.Hq * a.D * 2;
-      uint8_t* stage = attn_smem + (2 + ST) * TB + warp * 2048;
       auto free_o = [&] {
         ptx::tc_fence_before();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(o_empty(t));
       };
-      auto column = [&](int c, uint32_t (&v)[32]) {
-        ptx::tmem_ld_32x32(op + c * 32, v);
-        ptx::tmem_ld_wait();
-      };
-      auto store = [&](__nv_bfloat16* to, const uint32_t (&x)[16], int c) {
-        store_rows(stage, x, reinterpret_cast<uint8_t*>(to + at + c * 32), stride, valid, (a.D - c * 32) * 2);
-      };
       if constexpr (TRAIN) {
 #pragma unroll 1
         for (int c = 0; c < DP / 32; ++c) {
-          uint32_t v[32], out[16], rest[16];
+          uint32_t v[32];
           column(c, v);
-          pack_row(out, v, inv);
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            rest[i] = pack_bf16(__uint_as_float(v[2 * i]) * inv - bf16_lo(out[i]), __uint_as_float(v[2 * i + 1]) * inv - bf16_hi(out[i]));
-          store(a.o, out, c);
-          store(a.o_rest, rest, c);
+          store_twice(c, v, inv);
         }
         free_o();
       } else {
@@ -863,7 +935,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dkv_kernel(const __grid_consta
     const uint32_t id_s = ptx::instr_desc_bf16(128, 128, 0, 0), id_d = ptx::instr_desc_bf16(128, DP, 0, 1);
     if (ptx::elect_one()) {
       bool ok = true;
-      int n = 0;
+      int n = 0, chain = 0;   // chains so far
       for (int r = 0; ok; ++r) {
         const Item w = items.take_alone(r);
         if (w.level < 0) break;
@@ -890,25 +962,28 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dkv_kernel(const __grid_consta
         };
         ok = ptx::mbar_wait(k_full, r & 1, abort_flag) && scores(0) && ptx::mbar_wait(v_full, r & 1, abort_flag) && dps(0) &&
              (NS == 1 || n_it == 1 || scores(1));
-        for (int it = 0; ok && it < n_it; ++it) {
-          const int x = n + it, at = ring + x % ST * 2 * TB;
-          ok = ptx::mbar_wait(p_ready(x), x / NS & 1, abort_flag) && (it > 0 || ptx::mbar_wait(acc_empty, (r & 1) ^ 1u, abort_flag));
-          if (!ok) break;
-          ptx::tc_fence_after();
-          mma_tm<0, 8>(t_dv, t_s(x), at + TB, id_d, it > 0, 64);
-          const bool first = at_first == 0;
-          if (++at_first == to_first) at_first = 0;
-          if (first) mma_tm<0, 8>(t_dv, t_s(x) + 32, at + TB, id_d, true, 64);
-          ptx::mma_commit(do_empty(x));
-          if (it + NS < n_it) ok = scores(it + NS);
-          ok = ok && ptx::mbar_wait(ds_ready, x & 1, abort_flag);
-          if (!ok) break;
-          ptx::tc_fence_after();
-          mma_tm<0, 8>(t_dk, t_dp, at, id_d, it > 0, 64);
-          if (first) mma_tm<0, 8>(t_dk, t_dp + 32, at, id_d, true, 64);
-          ptx::mma_commit(q_empty(x));
-          if (it + 1 < n_it) ok = dps(it + 1);
-          else ptx::mma_commit(acc_full);
+        for (int it = 0; ok && it < n_it; ++chain) {
+          const int len = min(kChain, n_it - it);
+          for (int k = 0; ok && k < len; ++k, ++it) {
+            const int x = n + it, at = ring + x % ST * 2 * TB;
+            ok = ptx::mbar_wait(p_ready(x), x / NS & 1, abort_flag) && (k > 0 || ptx::mbar_wait(acc_empty, (chain & 1) ^ 1u, abort_flag));
+            if (!ok) break;
+            ptx::tc_fence_after();
+            mma_tm<0, 8>(t_dv, t_s(x), at + TB, id_d, k > 0, 64);
+            const bool first = at_first == 0;
+            if (++at_first == to_first) at_first = 0;
+            if (first) mma_tm<0, 8>(t_dv, t_s(x) + 32, at + TB, id_d, true, 64);
+            ptx::mma_commit(do_empty(x));
+            if (it + NS < n_it) ok = scores(it + NS);
+            ok = ok && ptx::mbar_wait(ds_ready, x & 1, abort_flag);
+            if (!ok) break;
+            ptx::tc_fence_after();
+            mma_tm<0, 8>(t_dk, t_dp, at, id_d, k > 0, 64);
+            if (first) mma_tm<0, 8>(t_dk, t_dp + 32, at, id_d, true, 64);
+            ptx::mma_commit(q_empty(x));
+            if (k + 1 == len) ptx::mma_commit(acc_full);
+            if (it + 1 < n_it) ok = dps(it + 1);
+          }
         }
         n += n_it;
       }
@@ -960,7 +1035,20 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dkv_kernel(const __grid_consta
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
     const F2 scale = f2(a.scale_log2, a.scale_log2);
     bool ok = true;
-    int n = 0;
+    int n = 0, chain = 0;
+    // this warp's pieces of 32 columns: of dV, then of dK
+    auto column = [&](int i) { return half * (DP / 2) + i % (DP / 64) * 32; };
+    auto kept_at = [&](int i) { return a.chain_kv + ((long long)blockIdx.x * (DP / 2) + (i < DP / 64 ? 0 : DP / 4) + column(i) / 4) * kTile + row; };
+    auto piece = [&](int i, uint32_t (&v)[32]) {
+      ptx::tmem_ld_32x32((i < DP / 64 ? t_dv : t_dk) + lanes + column(i), v);
+      ptx::tmem_ld_wait();
+    };
+    auto free_sums = [&] {
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(acc_empty);
+      ++chain;
+    };
     for (int r = 0; ok; ++r) {
       const Item w = items.take(r);
       if (w.level < 0) break;
@@ -1030,28 +1118,41 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dkv_kernel(const __grid_consta
         ++n;
         return true;
       };
-      for (int it = 0, i = 0; ok && it < sp.n_it; ++it) {
-        if (__builtin_expect(i > 0 || sp.key > 0, 1)) ok = block(i == 0, std::false_type());
-        else ok = block(true, std::true_type());
-        if (++i == sp.per_head) i = 0;
+      for (int it = 0, i = 0;;) {
+        for (const int end = min(it + kChain, sp.n_it); ok && it < end; ++it) {
+          if (__builtin_expect(i > 0 || sp.key > 0, 1)) ok = block(i == 0, std::false_type());
+          else ok = block(true, std::true_type());
+          if (++i == sp.per_head) i = 0;
+        }
+        if (!ok || it == sp.n_it) break;
+        ok = warp_wait(acc_full, chain & 1, abort_flag);   // a chain ends: the sums so far are kept, and start from zero
+        if (!ok) break;
+        ptx::tc_fence_after();
+#pragma unroll 1
+        for (int c = 0; c < DP / 32; ++c) {
+          uint32_t v[32];
+          piece(c, v);
+          if (it > kChain) add_chain(v, kept_at(c));
+          put_chain(v, kept_at(c));
+        }
+        free_sums();
       }
-      ok = ok && warp_wait(acc_full, r & 1, abort_flag);
+      ok = ok && warp_wait(acc_full, chain & 1, abort_flag);
       if (!ok) break;
       ptx::tc_fence_after();
+      if (__builtin_expect(sp.n_it > kChain, 0)) {   // (the last chain and the others, for what follows)
+#pragma unroll 1
+        for (int c = 0; c < DP / 32; ++c) {
+          uint32_t v[32];
+          piece(c, v);
+          add_chain(v, kept_at(c));
+          ptx::tmem_st_32x32((c < DP / 64 ? t_dv : t_dk) + lanes + column(c), v);
+        }
+        ptx::tmem_st_wait();
+      }
       const int row0 = sp.key * kTile + (warp & 3) * 32, valid = w.len - row0;
       const long long at = ((long long)(w.start + row0) * a.Hkv + sp.hk) * a.D, plane = (long long)a.seqs.T * a.Hkv * a.D;
       uint8_t* stage = attn_smem + (2 + 2 * ST) * TB + warp * 2048;
-      // this warp's pieces of 32 columns: of dV, then of dK
-      auto column = [&](int i) { return half * (DP / 2) + i % (DP / 64) * 32; };
-      auto piece = [&](int i, uint32_t (&v)[32]) {
-        ptx::tmem_ld_32x32((i < DP / 64 ? t_dv : t_dk) + lanes + column(i), v);
-        ptx::tmem_ld_wait();
-      };
-      auto free_sums = [&] {
-        ptx::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(acc_empty);
-      };
       if (a.parts == 1) {
         uint32_t out[DP / 32][16];
 #pragma unroll
@@ -1215,7 +1316,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dq_kernel(const __grid_constan
     bool ok = true;
     constexpr int STEP = PAIRS ? 1 : 2;
     At<ST> ks{0, 0}, vs{PAIRS ? 0 : 1, 0}, ds{0, 0};   // K of the next S, V of the next dP, K of the next dQ
-    uint32_t bs = 0, b = 0;                // blocks of S and of dQ so far
+    uint32_t bs = 0, b = 0, chain = 0;     // blocks of S and of dQ and chains so far
     for (uint32_t r = 0; ok; ++r) {
       const Item w = items.take(r);
       const int nb = __shfl_sync(0xffffffffu, w.level, 0) + 1;
@@ -1247,20 +1348,23 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dq_kernel(const __grid_constan
         return true;
       };
       ok = warp_wait(q_full, r & 1, abort_flag) && scores(0) && warp_wait(do_full, r & 1, abort_flag) && dps(0) && (nb < 2 || scores(1));
-      for (int j = 0; ok && j < nb; ++j) {
-        ok = warp_wait(ds_ready, b & 1, abort_flag) && (j + 1 >= nb || dps(j + 1)) && (j > 0 || warp_wait(acc_empty, (r & 1) ^ 1u, abort_flag));
-        if (!ok) break;
-        if (ptx::elect_one()) {
-          ptx::tc_fence_after();
-          mma_tm<0, 8>(t_dq, t_s(b), kv + ds.s * PLACE, id_d, j > 0, 64);
-          if (nb == 1) mma_tm<0, 8>(t_dq, t_s(b) + 32, kv + ds.s * PLACE, id_d, true, 64);
-          ptx::mma_commit(empty(ds.s));
-          if (j + 1 == nb) ptx::mma_commit(acc_full);
+      for (int j = 0; ok && j < nb; ++chain) {
+        const int len = min(kChain, nb - j);
+        for (int k = 0; ok && k < len; ++k, ++j) {
+          ok = warp_wait(ds_ready, b & 1, abort_flag) && (j + 1 >= nb || dps(j + 1)) && (k > 0 || warp_wait(acc_empty, (chain & 1) ^ 1u, abort_flag));
+          if (!ok) break;
+          if (ptx::elect_one()) {
+            ptx::tc_fence_after();
+            mma_tm<0, 8>(t_dq, t_s(b), kv + ds.s * PLACE, id_d, k > 0, 64);
+            if (nb == 1) mma_tm<0, 8>(t_dq, t_s(b) + 32, kv + ds.s * PLACE, id_d, true, 64);
+            ptx::mma_commit(empty(ds.s));
+            if (k + 1 == len) ptx::mma_commit(acc_full);
+          }
+          __syncwarp();
+          ++b;
+          ds.on(STEP);
+          if (j + 2 < nb) ok = scores(j + 2);
         }
-        __syncwarp();
-        ++b;
-        ds.on(STEP);
-        if (j + 2 < nb) ok = scores(j + 2);
       }
     }
     if (s_abort) settle();
@@ -1286,7 +1390,18 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dq_kernel(const __grid_constan
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
     const F2 scale = f2(a.scale_log2, a.scale_log2);
     bool ok = true;
-    int b = 0;
+    int b = 0, chain = 0;
+    auto kept_at = [&](int i) { return a.chain_q + ((long long)blockIdx.x * (DP / 4) + (half * (DP / 2) + i * 32) / 4) * kTile + row; };
+    auto piece = [&](int i, uint32_t (&v)[32]) {
+      ptx::tmem_ld_32x32(t_dq + lanes + half * (DP / 2) + i * 32, v);
+      ptx::tmem_ld_wait();
+    };
+    auto free_sums = [&] {
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(acc_empty);
+      ++chain;
+    };
     // delta: from the kernel before this one, or from one that was complete, with its writes visible, before that one (dK and dV) began
     if (a.dk == nullptr) grid_wait();
     for (int r = 0; ok; ++r) {
@@ -1334,24 +1449,45 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dq_kernel(const __grid_constan
         return true;
       };
       if (__builtin_expect(nb > 1, 1)) {
-        for (int j = 0; ok && j < nb; ++j) ok = block(j, std::false_type());
+        for (int j = 0;;) {
+          for (const int end = min(j + kChain, nb); ok && j < end; ++j) ok = block(j, std::false_type());
+          if (!ok || j == nb) break;
+          ok = warp_wait(acc_full, chain & 1, abort_flag);   // a chain ends: dQ so far is kept, and starts from zero
+          if (!ok) break;
+          ptx::tc_fence_after();
+#pragma unroll 1
+          for (int i = 0; i < DP / 64; ++i) {
+            uint32_t v[32];
+            piece(i, v);
+            if (j > kChain) add_chain(v, kept_at(i));
+            put_chain(v, kept_at(i));
+          }
+          free_sums();
+        }
       } else {
         ok = block(0, std::true_type());
       }
-      ok = ok && warp_wait(acc_full, r & 1, abort_flag);
+      ok = ok && warp_wait(acc_full, chain & 1, abort_flag);
       if (!ok) break;
       ptx::tc_fence_after();
+      if (__builtin_expect(nb > kChain, 0)) {   // (the last chain and the others, for what follows)
+#pragma unroll 1
+        for (int i = 0; i < DP / 64; ++i) {
+          uint32_t v[32];
+          piece(i, v);
+          add_chain(v, kept_at(i));
+          ptx::tmem_st_32x32(t_dq + lanes + half * (DP / 2) + i * 32, v);
+        }
+        ptx::tmem_st_wait();
+      }
       uint32_t out[DP / 64][16];
 #pragma unroll
       for (int i = 0; i < DP / 64; ++i) {
         uint32_t v[32];
-        ptx::tmem_ld_32x32(t_dq + lanes + half * (DP / 2) + i * 32, v);
-        ptx::tmem_ld_wait();
+        piece(i, v);
         pack_row(out[i], v, a.scale);
       }
-      ptx::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(acc_empty);
+      free_sums();
       const int row0 = w.level * kTile + (warp & 3) * 32;
 #pragma unroll
       for (int i = 0; i < DP / 64; ++i) {
@@ -1425,6 +1561,12 @@ inline int dkv_parts(int T, int n_seqs, int Hq, int Hkv, int D) {
 }
 
 inline unsigned ctas(long long items) { return (unsigned)(items < num_sms() ? items : num_sms()); }
+
+// Bytes of the sums of chains, for dV and dK and for dQ: none where no item can have more than kChain pairs of tiles.
+inline long long chain_kv_bytes(int T, int G, int parts, int D) {
+  return ((long long)T + kTile - 1) / kTile * ((G + parts - 1) / parts) > kChain ? (long long)num_sms() * (D <= 64 ? 64 : 128) * kTile * 8 : 0;
+}
+inline long long chain_q_bytes(int T, int D) { return T > kChain * kTile ? (long long)num_sms() * (D <= 64 ? 64 : 128) * kTile * 4 : 0; }
 
 // Tiles that `n` sequences of together T rows can have at most.
 inline long long most_tiles(int T, int n) { return (long long)T / kTile + n; }

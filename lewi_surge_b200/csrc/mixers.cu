@@ -82,7 +82,7 @@ int attention_fwd(cudaStream_t st, const attn::Args& a, const CUtensorMap& tq, c
 template <int DP>
 int attention_fwd(cudaStream_t st, const attn::Args& a, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv) {
   const bool one = a.shape == attn::kOneTile;
-  if (a.o_rest != nullptr) return one ? attention_fwd<DP, true, true>(st, a, tq, tk, tv) : attention_fwd<DP, true, false>(st, a, tq, tk, tv);
+  if (a.lse != nullptr) return one ? attention_fwd<DP, true, true>(st, a, tq, tk, tv) : attention_fwd<DP, true, false>(st, a, tq, tk, tv);
   return one ? attention_fwd<DP, false, true>(st, a, tq, tk, tv) : attention_fwd<DP, false, false>(st, a, tq, tk, tv);
 }
 
@@ -117,6 +117,7 @@ int attention_bwd(cudaStream_t st, const attn::Args& a, const CUtensorMap& tq, c
 }
 
 inline int64_t delta_bytes(int T, int Hq) { return ((int64_t)T * Hq * 4 + 255) / 256 * 256; }
+inline int64_t sums_bytes(int T, int Hkv, int D, int parts) { return parts > 1 ? (int64_t)parts * 2 * T * Hkv * D * 4 : 0; }
 
 inline int paged_ctas(int D) { return num_sms() * (D > 128 ? paged::Shape<256>::kCtas : paged::Shape<128>::kCtas); }
 
@@ -216,14 +217,15 @@ int lewi_causal_attention_fwd(void* stream, const void* q, int64_t q_stride, con
                               const int32_t* cu_seqlens, int n_seqs, void* o, void* o_rest, float* lse, int T, int Hq, int Hkv, int D,
                               float scale) {
   if (const int rc = check_attention(q, q_stride, k, k_stride, v, v_stride, cu_seqlens, n_seqs, o, T, Hq, Hkv, D, scale)) return rc;
-  if (!lse != !o_rest) return LEWI_ERR_ARG;
+  if (lse && !o_rest) return LEWI_ERR_ARG;
+  if (!o_rest && T > attn::kChain * attn::kTile) return LEWI_ERR_WORKSPACE;
   if (!aligned(o_rest, 16)) return LEWI_ERR_SHAPE;
   CUtensorMap tq, tk, tv;
   if (!attn::make_rows_map(&tq, q, T, Hq, D, q_stride) || !attn::make_rows_map(&tk, k, T, Hkv, D, k_stride) ||
       !attn::make_rows_map(&tv, v, T, Hkv, D, v_stride))
     return LEWI_ERR_CUDA;
   const attn::Args a{{cu_seqlens, n_seqs, T}, Hq, Hkv, Hq / Hkv, D, scale, scale * 1.4426950408889634f, reinterpret_cast<bf16*>(o),
-                     reinterpret_cast<bf16*>(o_rest), lse, nullptr, nullptr, nullptr, nullptr, 1, nullptr, attn::fwd_item(T, n_seqs, Hq, Hq / Hkv)};
+                     reinterpret_cast<bf16*>(o_rest), lse, nullptr, nullptr, nullptr, nullptr, 1, nullptr, nullptr, nullptr, attn::fwd_item(T, n_seqs, Hq, Hq / Hkv)};
   cudaStream_t st = as_stream(stream);
   return D <= 64 ? attention_fwd<64>(st, a, tq, tk, tv) : attention_fwd<128>(st, a, tq, tk, tv);
 }
@@ -231,7 +233,7 @@ int lewi_causal_attention_fwd(void* stream, const void* q, int64_t q_stride, con
 int64_t lewi_causal_attention_bwd_workspace_bytes(int T, int n_seqs, int Hq, int Hkv, int D) {
   if (T <= 0 || n_seqs <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || Hq % Hkv != 0) return LEWI_ERR_ARG;
   const int parts = attn::dkv_parts(T, n_seqs, Hq, Hkv, D);
-  return delta_bytes(T, Hq) + (parts > 1 ? (int64_t)parts * 2 * T * Hkv * D * 4 : 0);
+  return delta_bytes(T, Hq) + sums_bytes(T, Hkv, D, parts) + attn::chain_kv_bytes(T, Hq / Hkv, parts, D) + attn::chain_q_bytes(T, D);
 }
 
 int lewi_causal_attention_bwd(void* stream, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
@@ -246,12 +248,14 @@ int lewi_causal_attention_bwd(void* stream, const void* q, int64_t q_stride, con
   if (!attn::make_rows_map(&tq, q, T, Hq, D, q_stride) || !attn::make_rows_map(&tk, k, T, Hkv, D, k_stride) ||
       !attn::make_rows_map(&tv, v, T, Hkv, D, v_stride) || !attn::make_rows_map(&td, d_o, T, Hq, D, (int64_t)Hq * D))
     return LEWI_ERR_CUDA;
+  const int parts = attn::dkv_parts(T, n_seqs, Hq, Hkv, D);
+  uint8_t* at = reinterpret_cast<uint8_t*>(workspace) + delta_bytes(T, Hq);
+  const int64_t sums = sums_bytes(T, Hkv, D, parts), kept = attn::chain_kv_bytes(T, Hq / Hkv, parts, D);
   const attn::Args a{{cu_seqlens, n_seqs, T}, Hq, Hkv, Hq / Hkv, D, scale, scale * 1.4426950408889634f,
                      const_cast<bf16*>(reinterpret_cast<const bf16*>(o)), const_cast<bf16*>(reinterpret_cast<const bf16*>(o_rest)),
                      const_cast<float*>(lse), reinterpret_cast<float*>(workspace),
                      reinterpret_cast<bf16*>(dq), reinterpret_cast<bf16*>(dk), reinterpret_cast<bf16*>(dv),
-                     attn::dkv_parts(T, n_seqs, Hq, Hkv, D),
-                     reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(workspace) + delta_bytes(T, Hq))};
+                     parts, reinterpret_cast<float*>(at), reinterpret_cast<float4*>(at + sums), reinterpret_cast<float4*>(at + sums + kept)};
   const bf16* g = reinterpret_cast<const bf16*>(d_o);
   return D <= 64 ? attention_bwd<64>(as_stream(stream), a, tq, tk, tv, td, g) : attention_bwd<128>(as_stream(stream), a, tq, tk, tv, td, g);
 }

@@ -407,3 +407,58 @@ def test_dq_beside_dk_and_dv_is_dq_alone(cuda):
     return out
   for both, alone in zip(grads((True, True, True)), grads((True, False, False))):
     assert torch.equal(both, alone)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("log_t,hq,d,empty", [(17, 1, 64, 0), (17, 1, 128, 0), (17, 2, 128, 0), (16, 2, 64, 0), (16, 1, 128, 400), (16, 1, 40, 400), (15, 8, 64, 0)])
+def test_long_sums_of_one_sign_do_not_come_out_short(cuda, log_t, hq, d, empty):
+  """A tensor core truncates every sum that it makes, so a long chain of products of one sign comes out short.  Scores of zero make every p of row t
+  1 / (t + 1) and the exact results running sums (but for the first key's, in o).  What is looked at is the mean of the relative errors of 10^6
+  values and more, whose own roundings (2^-9 / sqrt(3) each, as many up as down) leave less than 2^-18 of it, and those of p and dS, alike for all
+  of a row but different from row to row, 2^-16; 2^-14 is room for them and for float32.  An accumulator may lose 2^-12.  Empty sequences
+  beside the long one make one tile an item in the forward pass."""
+  gen = torch.Generator(device=cuda).manual_seed(13)
+  t, scale = 1 << log_t, 0.5
+  cu = torch.tensor([0] * (empty // 2 + 1) + [t] * (empty // 2 + 1), device=cuda)
+  call = lambda *operands: attention.causal_attention(*operands, cu, scale=scale)
+  rn = lambda *s: torch.rand(*s, generator=gen, device=cuda)
+  grow = (1 + torch.arange(t, device=cuda) / t)[:, None, None]
+  wide = lambda h=1: ((1 + rn(1, h, d)) * grow * (0.9 + 0.2 * rn(t, h, d))).bfloat16()   # of one sign, their mantissas anywhere
+  sign = torch.where(torch.arange(t, device=cuda) % 2 == 0, 1.0, -1.0).bfloat16()[:, None, None]
+  zero = lambda h=1: torch.zeros(t, h, d, device=cuda).bfloat16()
+  w = 1 / torch.arange(1, t + 1, device=cuda, dtype=F64)[:, None, None]
+  behind = lambda x: x.flip(0).cumsum(0).flip(0)
+  late, early = slice(t // 2, None), slice(0, t // 2)
+  short = lambda got, want, rows: ((got.detach().to(F64) - want) / want)[rows].mean().abs().item()
+  off = {}
+  # o: the first key of every row has its own score, so that the p of all others, one value per row, has all its bits
+  q, k, v = wide(hq), zero(), wide()
+  k[0] = 1 / d
+  first = torch.exp(scale * (q.to(F64) @ k[0, 0].to(F64)))[..., None]
+  want = (v.to(F64).cumsum(0) + (first - 1) * v[:1].to(F64)) / (first + 1 / w - 1)
+  off["o"] = short(call(q, k, v), want, late)
+  off["o in training"] = short(call(q, k, v.requires_grad_(True)), want, late)
+  # v = +-1 / d and an upstream gradient of ones: dP = +-1, and dS times keys, or queries, that go with that sign, is of one sign
+  ones, v = torch.ones_like(q), (sign / d).expand(t, 1, d).contiguous()
+  a = v.to(F64).sum(2, keepdim=True)
+  delta = a.cumsum(0) * w
+  k, q = (sign * wide()).bfloat16(), zero(hq).requires_grad_(True)
+  dq, = torch.autograd.grad(call(q, k, v), q, ones)
+  off["dq"] = short(dq, scale * w * ((a * k.to(F64)).cumsum(0) - delta * k.to(F64).cumsum(0)), late)
+  q, d_o, k = wide(hq), wide(hq), zero().requires_grad_(True)
+  dk, = torch.autograd.grad(call(q, k, v), k, ones)
+  q_sum = q.to(F64).sum(1, keepdim=True)
+  off["dk"] = short(dk, scale * (a * behind(w * q_sum) - behind(w * delta * q_sum)), early)
+  dv, = torch.autograd.grad(call(q, k.detach(), v.requires_grad_(True)), v, d_o)
+  off["dv"] = short(dv, behind(w * d_o.to(F64).sum(1, keepdim=True)), early)
+  assert _lib.last_status() == 0
+  assert max(off.values()) <= 2.0 ** -12 + 2.0 ** -14, off
+
+
+def test_a_long_forward_pass_wants_a_place_for_sums():
+  """More rows than go into one accumulator: o_rest is needed without a backward pass too (addresses that are never used)."""
+  lib, at = _lib.load(), 1 << 20
+  call = lambda t, rest, lse: lib.lewi_causal_attention_fwd(None, at, 64, at, 64, at, 64, None, 1, at, rest, lse, t, 1, 1, 64, 1.0)
+  assert call(32769, None, None) == -3 and call(64, None, at) == -1
+  few, many = (lib.lewi_causal_attention_bwd_workspace_bytes(t, 1, 1, 1, 64) - 4 * t for t in (32768, 32768 + 64))
+  assert few == 0 and many > 0
