@@ -12,6 +12,7 @@
 // gradients.
 #pragma once
 
+#include <cfloat>
 #include <type_traits>
 
 #include "common.cuh"
@@ -576,6 +577,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;   // this warp's lanes of tensor memory
     const uint32_t op = o_at(t) + lanes;
     const F2 scale = f2(a.scale_log2, a.scale_log2);
+    const float lowest = -0.5f * FLT_MAX / fmaxf(1.f, a.scale_log2);   // (times the scale it is finite)
     int used = 0, done = 0;
     bool ok = true;
     for (int r = 0; ok; ++r) {
@@ -647,7 +649,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) fwd_kernel(const __grid_consta
         }
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
         if (j == 0) {
-          m = top;
+          m = fmaxf(top, lowest);   // (scores of -inf only: their p are zero, and what follows is larger)
         } else if (__any_sync(0xffffffffu, mine && (top - m) * a.scale_log2 > 8.f)) {
           if (ONE && !warp_wait(pv_done, (done & 1) ^ 1u, abort_flag)) return false;   // of the block before
           ptx::tc_fence_after();

@@ -462,3 +462,30 @@ def test_a_long_forward_pass_wants_a_place_for_sums():
   assert call(32769, None, None) == -3 and call(64, None, at) == -1
   few, many = (lib.lewi_causal_attention_bwd_workspace_bytes(t, 1, 1, 1, 64) - 4 * t for t in (32768, 32768 + 64))
   assert few == 0 and many > 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,scale", [(1, 0.125), (200, 0.125), (1, 1.5)])
+def test_scores_of_minus_infinity_at_the_start_of_a_row(cuda, n, scale):
+  """Later rows have scores of -inf with the whole first tile of keys and more (products that float32 cannot hold): their softmax is that of the rest."""
+  gen = torch.Generator().manual_seed(14)
+  s, d = 300, 64
+  q, k, v, d_o = (rnd(gen, n * s, h, d) for h in (4, 2, 2, 4))
+  pos = torch.arange(n * s) % s
+  q[..., 0] = torch.where(pos < 200, 0.0, 40.0)[:, None].bfloat16()
+  k[..., 0] = torch.where(pos < 140, -1e38, 0.0)[:, None].bfloat16()
+  cu = list(range(0, n * s + 1, s))
+  want = formulas(q, k, v, cu, scale, d_o)
+  leaves = [x.to(cuda).requires_grad_(True) for x in (q, k, v)]
+  seqs = torch.tensor(cu, device=cuda)
+  within(attention.causal_attention(*(x.detach() for x in leaves), seqs, scale), want["o"], "o")
+  o = attention.causal_attention(*leaves, seqs, scale)
+  within(o, want["o"], "o in training")
+  grads = [g.cpu() for g in torch.autograd.grad(o, leaves, d_o.to(cuda))]
+  # dq is scale times a sum over dS k in float32, whose terms reach 20 * 1e38: it is looked at where sum |dS k|, which is the bound / (u scale) at most, is
+  # one that float32 holds.  (That leaves out the first element of rows that see keys of -1e38, not of those whose p for them is zero.)
+  held = want["dq"][1] / (U * scale) < 2.0 ** 127
+  assert held[pos >= 200].all() and held[..., 1:].all()
+  within(grads[0][held], [x[held] for x in want["dq"]], "dq")
+  within(grads[1], want["dk"], "dk")
+  within(grads[2], want["dv"], "dv")
