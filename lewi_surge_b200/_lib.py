@@ -172,6 +172,13 @@ def elsewhere(*tensors):
   return index != torch._C._cuda_getDevice()
 
 
+def written(*tensors):
+  """Tells autograd that a kernel has written these: a backward pass that had saved one of them raises, as after any in-place operation."""
+  from torch.autograd.graph import increment_version
+  for t in tensors:
+    increment_version(t)
+
+
 def index_table(t, what):
   """A table of int32 as the kernels read it; int64 values that int32 cannot hold stay out of range."""
   import torch

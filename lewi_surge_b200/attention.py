@@ -57,6 +57,7 @@ def paged_cache_write(key, value, key_cache, value_cache, block_tables, lengths,
   cu = _lib.index_table(cu_seqlens, "cu_seqlens")
   check(lib.lewi_paged_cache_write(stream(), k.data_ptr(), ks, v.data_ptr(), vs, key_cache.data_ptr(), value_cache.data_ptr(), page_stride,
                                    tables.data_ptr(), lens.data_ptr(), ptr(cu), t, b, heads, d, pages, page, max_pages), "lewi_paged_cache_write")
+  _lib.written(key_cache, value_cache)
 
 
 def paged_attention(query, key_cache, value_cache, block_tables, lengths, scale=None):

@@ -149,6 +149,7 @@ def causal_conv1d_step(x, w, state, slots=None):
   if b > 0:
     check(lib.lewi_causal_conv1d_step(stream(), x.data_ptr(), x_rows, ptr(w), ptr(state), ptr(slots), y.data_ptr(), b, ss[0], c, k),
           "lewi_causal_conv1d_step")
+    _lib.written(state)
   return y
 
 
@@ -183,4 +184,5 @@ def gated_delta_step(query, key, value, g, beta, state, slots=None):
   if b > 0:
     check(lib.lewi_gdn_step(stream(), q.data_ptr(), q_rows, k.data_ptr(), k_rows, v.data_ptr(), v_rows, g.data_ptr(), g_type, beta.data_ptr(),
                             beta_type, ptr(state), ptr(slots), o.data_ptr(), b, ss[0], hk, h, kd, vd), "lewi_gdn_step")
+    _lib.written(state)
   return o

@@ -425,3 +425,34 @@ def test_rows_at_any_distance_and_address(cuda):
   state = torch.zeros(h, kd, kd, device=cuda).expand(b, h, kd, kd)
   with pytest.raises(LewiError):
     seqmix.gated_delta_step(i["q"], i["k"], i["v"], i["g"], i["beta"], state)   # a pool that is not a pool
+
+
+# ------------------------------------------------------------------------------------------------ autograd
+@pytest.mark.gpu
+def test_what_a_step_writes_is_no_longer_what_a_backward_pass_saved(cuda):
+  gen = torch.Generator().manual_seed(20)
+  w = torch.ones((), device=cuda, requires_grad=True)
+  x, taps, past = rnd(gen, 2, 16).to(cuda), rnd(gen, 4, 1, 16).to(cuda), rnd(gen, 3, 3, 16).to(cuda)
+  i = {m: t.to(cuda) for m, t in delta_inputs(gen, 2, 3, 2, 2, 16, 16).items()}
+  kc, vc = (rnd(gen, 4, 2, 16, 1, 8).to(cuda)[:, j] for j in range(2))   # views of tensors that hold more
+  k, tables, lens = rnd(gen, 2, 1, 8).to(cuda), torch.tensor([[0], [1]], device=cuda), torch.tensor([1, 1], device=cuda)
+  for call, targets in ((lambda: seqmix.causal_conv1d_step(x, taps, past), (past,)),
+                        (lambda: seqmix.gated_delta_step(*(i[m] for m in ("q", "k", "v", "g", "beta", "state"))), (i["state"],)),
+                        (lambda: attention.paged_cache_write(k, k, kc, vc, tables, lens), (kc, vc))):
+    for t in targets:
+      losses = [(t * w).sum(), (t._base * w).sum() if t._is_view() else (t[:1] * w).sum()]
+      call()
+      for loss in losses:
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+          loss.backward()
+    with torch.inference_mode():
+      call()
+  # the state that a prompt started from
+  s = 64
+  q, k, v = (rnd(gen, 1, s, 2, 16).to(cuda).requires_grad_(True) for _ in range(3))
+  g, beta, state = -torch.rand(1, s, 2, generator=gen).to(cuda), torch.rand(1, s, 2, generator=gen).to(cuda), torch.zeros(1, 2, 16, 16, device=cuda)
+  o, _ = seqmix.chunk_gated_delta_rule(q, k, v, g, beta, initial_state=state)
+  with torch.no_grad():
+    seqmix.gated_delta_step(q[:, 0], k[:, 0], v[:, 0], g[:, 0], beta[:, 0], state)
+  with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+    o.sum().backward()
