@@ -172,6 +172,12 @@ def elsewhere(*tensors):
   return index != torch._C._cuda_getDevice()
 
 
+def has_tangent(*tensors):
+  """Whether one of these is a dual tensor of forward-mode differentiation, which no kernel here carries on."""
+  from torch.autograd import forward_ad
+  return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def written(*tensors):
   """Tells autograd that a kernel has written these: a backward pass that had saved one of them raises, as after any in-place operation."""
   from torch.autograd.graph import increment_version

@@ -141,7 +141,8 @@ def causal_attention(query, key, value, cu_seqlens=None, scale=None):
   """softmax(scale q k^T) v over the rows of a sequence up to the query's own.  Packed: query [T, Hq, D], key, value [T, Hkv, D] bf16, sequence s
   the rows cu_seqlens[s] .. cu_seqlens[s+1] (int32 or int64 [N + 1], ascending, empty ones among them; none: one sequence), or sequences of one
   length: query [B, S, Hq, D], key, value [B, S, Hkv, D].  Head h has the keys of head h // (Hq // Hkv); D up to 128, a multiple of 8;
-  `scale` > 0 defaults to D ** -0.5.  Returns bf16 of the query's shape; differentiable through `torch.autograd`, once, in query, key and value.
+  `scale` > 0 defaults to D ** -0.5.  Returns bf16 of the query's shape; differentiable through `torch.autograd`, once and
+  in reverse mode, in query, key and value.
   Rows of no sequence give zeros and get zero gradients, whatever they hold.  Bounds that leave the rows are cut to them; where bounds fall, no
   sequence is worked on and the results are undefined; either way `LEWI_STATUS_BAD_INDEX` in `_lib.last_status()`.  Rows may lie apart (views of one projection need no copy).
 
@@ -164,6 +165,8 @@ def causal_attention(query, key, value, cu_seqlens=None, scale=None):
   scale = shape[-1] ** -0.5 if scale is None else float(scale)
   if not scale > 0:
     raise LewiError("causal_attention: scale must be positive")
+  if _lib.has_tangent(query, key, value):
+    raise LewiError("causal_attention has no forward-mode derivative")
   if query.numel() == 0:
     return query.clone()
   if _lib.elsewhere(query, key, value, cu_seqlens):

@@ -489,3 +489,15 @@ def test_scores_of_minus_infinity_at_the_start_of_a_row(cuda, n, scale):
   within(grads[0][held], [x[held] for x in want["dq"]], "dq")
   within(grads[1], want["dk"], "dk")
   within(grads[2], want["dv"], "dv")
+
+
+def test_forward_mode_is_refused():
+  """A dual operand, of which no gradient is wanted, is not one without a derivative."""
+  from torch.autograd import forward_ad
+  q, k = torch.zeros(6, 4, 16).bfloat16(), torch.zeros(6, 2, 16).bfloat16()
+  with forward_ad.dual_level():
+    dual = lambda x: forward_ad.make_dual(x, torch.ones_like(x))
+    for operands in ((dual(q), k, k), (q, dual(k), k), (q, k, dual(k)), (dual(q).requires_grad_(True), k, k)):
+      for mode in (torch.enable_grad, torch.no_grad):
+        with mode(), pytest.raises(LewiError, match="forward-mode"):
+          attention.causal_attention(*operands)
