@@ -148,10 +148,11 @@ def ptr(t):
   return t.data_ptr()
 
 
-def stream():
-  """Handle of the current stream (read directly: wrapping it in a Stream object takes several microseconds per call)."""
+def stream(on=None):
+  """Handle of the current stream (read directly: wrapping it in a Stream object takes several microseconds per call) of the current device,
+  or of the device of the CUDA tensor `on`."""
   import torch
-  return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+  return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if on is None else on.get_device())
 
 
 def last_status():
@@ -175,14 +176,24 @@ def elsewhere(*tensors):
 def has_tangent(*tensors):
   """Whether one of these is a dual tensor of forward-mode differentiation, which no kernel here carries on."""
   from torch.autograd import forward_ad
-  return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+  return any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+def no_derivative(what, *tensors):
+  """Refuses operands that a derivative is wanted of, which `what` has none for: the term would be missing without an error."""
+  import torch
+  if torch.is_grad_enabled():
+    for t in tensors:
+      if t.requires_grad:
+        raise LewiError(f"{what} is not differentiable: operands that require a gradient are taken under torch.no_grad() only")
+  if torch.autograd.forward_ad._current_level >= 0 and has_tangent(*tensors):   # (-1: no forward mode, and nothing to look at)
+    raise LewiError(f"{what} has no forward-mode derivative")
 
 
 def written(*tensors):
   """Tells autograd that a kernel has written these: a backward pass that had saved one of them raises, as after any in-place operation."""
-  from torch.autograd.graph import increment_version
-  for t in tensors:
-    increment_version(t)
+  import torch
+  torch.autograd.graph.increment_version(tensors)
 
 
 def index_table(t, what):

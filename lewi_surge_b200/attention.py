@@ -36,7 +36,7 @@ def paged_cache_write(key, value, key_cache, value_cache, block_tables, lengths,
   of length 0 is idle.  Caches [pages, page, Hkv, D] bf16 (pages may lie apart: views of one tensor that interleaves both);
   sequence b's tokens lie in the pages block_tables[b] (int32 or int64) names.  Tokens of no sequence are left out.  A token that lies
   outside its sequence's table or on a page that does not exist is left out with `LEWI_STATUS_BAD_INDEX` in `_lib.last_status()`.
-  Two tokens written to one cell (a page named twice) leave either of them, piece by piece."""
+  Two tokens written to one cell (a page named twice) leave either of them, piece by piece.  Not differentiable, as `paged_attention`."""
   lib = _lib.load()
   pages, page, heads, d, page_stride = _check_cache("paged_cache_write", key_cache, value_cache, block_tables, lengths)
   new = key.shape
@@ -47,6 +47,7 @@ def paged_cache_write(key, value, key_cache, value_cache, block_tables, lengths,
     raise LewiError("paged_cache_write: cu_seqlens [B + 1] is required")
   if cu_seqlens is None and t != b:
     raise LewiError("paged_cache_write: without cu_seqlens there is one token per sequence")
+  _lib.no_derivative("paged_cache_write", key, value, key_cache, value_cache)
   if t == 0 or b == 0:
     return
   if _lib.elsewhere(key_cache, key, value, value_cache, block_tables, lengths, cu_seqlens):
@@ -55,7 +56,7 @@ def paged_cache_write(key, value, key_cache, value_cache, block_tables, lengths,
   (k, ks), (v, vs) = _lib.rows_of(key, 16), _lib.rows_of(value, 16)
   tables, lens = _lib.index_table(block_tables, "block_tables"), _lib.index_table(lengths, "lengths")
   cu = _lib.index_table(cu_seqlens, "cu_seqlens")
-  check(lib.lewi_paged_cache_write(stream(), k.data_ptr(), ks, v.data_ptr(), vs, key_cache.data_ptr(), value_cache.data_ptr(), page_stride,
+  check(lib.lewi_paged_cache_write(stream(k), k.data_ptr(), ks, v.data_ptr(), vs, key_cache.data_ptr(), value_cache.data_ptr(), page_stride,
                                    tables.data_ptr(), lens.data_ptr(), ptr(cu), t, b, heads, d, pages, page, max_pages), "lewi_paged_cache_write")
   _lib.written(key_cache, value_cache)
 
@@ -63,7 +64,8 @@ def paged_cache_write(key, value, key_cache, value_cache, block_tables, lengths,
 def paged_attention(query, key_cache, value_cache, block_tables, lengths, scale=None):
   """Attention of one new token per sequence over the sequence's cells, its own among them (write it first): query [B, Hq, D] bf16 ->
   [B, Hq, D] bf16, head h with the keys of head h // (Hq // Hkv); zeros where lengths[b] is 0.  Caches and tables as in
-  `paged_cache_write`; D up to 256, a multiple of 8.  `scale` defaults to D ** -0.5.  Not differentiable.  Lengths and tables are read on the device, so a
+  `paged_cache_write`; D up to 256, a multiple of 8.  `scale` defaults to D ** -0.5.  Not differentiable: operands that
+  require a gradient are refused while gradients are recorded.  Lengths and tables are read on the device, so a
   captured call follows them.  Cells past a sequence's length, whatever they hold, have no part in it; pages that do not exist
   and what a length has past its table are left out with `LEWI_STATUS_BAD_INDEX` in `_lib.last_status()`."""
   lib = _lib.load()
@@ -71,6 +73,7 @@ def paged_attention(query, key_cache, value_cache, block_tables, lengths, scale=
   shape, (b, max_pages) = query.shape, block_tables.shape
   if query.dtype is not torch.bfloat16 or len(shape) != 3 or shape[2] != d or heads == 0 or shape[1] % heads or shape[0] != b:
     raise LewiError("paged_attention: query [B, Hq, D] bfloat16 with Hq a multiple of the caches' heads is required")
+  _lib.no_derivative("paged_attention", query, key_cache, value_cache)
   hq = shape[1]
   if _lib.elsewhere(query, key_cache, value_cache, block_tables, lengths):
     with torch.cuda.device(query.device):
@@ -82,7 +85,7 @@ def paged_attention(query, key_cache, value_cache, block_tables, lengths, scale=
   tables, lens = _lib.index_table(block_tables, "block_tables"), _lib.index_table(lengths, "lengths")
   ws_bytes = lib.lewi_paged_attention_workspace_bytes(d)
   ws = q.new_empty(ws_bytes // 2)
-  check(lib.lewi_paged_attention(stream(), q.data_ptr(), qs, key_cache.data_ptr(), value_cache.data_ptr(), page_stride, tables.data_ptr(),
+  check(lib.lewi_paged_attention(stream(q), q.data_ptr(), qs, key_cache.data_ptr(), value_cache.data_ptr(), page_stride, tables.data_ptr(),
                                  lens.data_ptr(), o.data_ptr(), ws.data_ptr(), ws_bytes, b, hq, heads, d, pages, page, max_pages,
                                  d ** -0.5 if scale is None else float(scale)), "lewi_paged_attention")
   return o
@@ -100,7 +103,7 @@ def _attention_fwd(q, k, v, cu, n_seqs, scale, o_rest=None, lse=None):
   o = torch.empty_like(q, memory_format=torch.contiguous_format)
   if o_rest is None and t > _CHAIN_ROWS:
     o_rest = torch.empty_like(o)
-  check(_lib.load().lewi_causal_attention_fwd(stream(), q.data_ptr(), q_rows, k.data_ptr(), k_rows, v.data_ptr(), v_rows, ptr(cu), n_seqs,
+  check(_lib.load().lewi_causal_attention_fwd(stream(q), q.data_ptr(), q_rows, k.data_ptr(), k_rows, v.data_ptr(), v_rows, ptr(cu), n_seqs,
                                               o.data_ptr(), ptr(o_rest), ptr(lse), t, hq, k.shape[1], d, scale), "lewi_causal_attention_fwd")
   return o, q, k, v, cu, (q_rows, k_rows, v_rows)
 
@@ -165,7 +168,7 @@ def causal_attention(query, key, value, cu_seqlens=None, scale=None):
   scale = shape[-1] ** -0.5 if scale is None else float(scale)
   if not scale > 0:
     raise LewiError("causal_attention: scale must be positive")
-  if _lib.has_tangent(query, key, value):
+  if torch.autograd.forward_ad._current_level >= 0 and _lib.has_tangent(query, key, value):
     raise LewiError("causal_attention has no forward-mode derivative")
   if query.numel() == 0:
     return query.clone()

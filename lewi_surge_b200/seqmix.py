@@ -127,7 +127,8 @@ def causal_conv1d_step(x, w, state, slots=None):
   """One more input of the sequences of `causal_conv1d`: x [B,C] bf16, w [K,1,C], state [N,K-1,C] bf16 holds the K-1 inputs before this
   one, oldest first (zeros at the start of a sequence) and is moved on in place.  Row b has the state slots[b] (int32 or int64; none:
   state b).  A negative slot is an idle row: zeros out, no state touched; a slot past the pool, or an earlier row's, as well, with
-  `LEWI_STATUS_BAD_INDEX` in `_lib.last_status()`.  Not differentiable; the values are `causal_conv1d`'s bit for bit."""
+  `LEWI_STATUS_BAD_INDEX` in `_lib.last_status()`.  Not differentiable (operands that require a gradient are
+  refused while gradients are recorded); the values are `causal_conv1d`'s bit for bit."""
   lib = _lib.load()
   xs, ws, ss = x.shape, w.shape, state.shape
   if len(xs) != 2 or len(ws) != 3 or ws[1] != 1 or ws[2] != xs[1]:
@@ -138,6 +139,7 @@ def causal_conv1d_step(x, w, state, slots=None):
   if len(ss) != 3 or ss[1] != k - 1 or ss[2] != c:
     raise LewiError("causal_conv1d_step: state [N,K-1,C] is required")
   _check_slots("causal_conv1d_step", b, ss[0], slots)
+  _lib.no_derivative("causal_conv1d_step", x, w, state)
   if _lib.elsewhere(x, w, state, slots):
     with torch.cuda.device(x.device):
       return causal_conv1d_step(x, w, state, slots)
@@ -147,7 +149,7 @@ def causal_conv1d_step(x, w, state, slots=None):
   slots = _lib.index_table(slots, "slots")
   y = torch.empty_like(x, memory_format=torch.contiguous_format)
   if b > 0:
-    check(lib.lewi_causal_conv1d_step(stream(), x.data_ptr(), x_rows, ptr(w), ptr(state), ptr(slots), y.data_ptr(), b, ss[0], c, k),
+    check(lib.lewi_causal_conv1d_step(stream(x), x.data_ptr(), x_rows, ptr(w), ptr(state), ptr(slots), y.data_ptr(), b, ss[0], c, k),
           "lewi_causal_conv1d_step")
     _lib.written(state)
   return y
@@ -158,7 +160,7 @@ def gated_delta_step(query, key, value, g, beta, state, slots=None):
   value [B,H,V] bf16, g (log decay), beta [B,H] (float32 or bf16) and the state [N,H,K,V] float32, which is moved on in place; returns
   o [B,H,V] bf16.  H is a multiple of Hk: value head h has the query and key of head h // (H // Hk).  Row b has the state slots[b]
   (int32 or int64; none: state b); idle and refused rows are those of `causal_conv1d_step`.  K up to 128, K and V multiples of 8.
-  Rows of the batch may lie apart (views of one projection need no copy).  Not differentiable.  Everything is float32 inside, where
+  Rows of the batch may lie apart (views of one projection need no copy).  Not differentiable, as `causal_conv1d_step`.  Everything is float32 inside, where
   `chunk_gated_delta_rule` rounds some products to bf16 as the reference does, so the two agree to bf16's precision."""
   lib = _lib.load()
   if not query.dtype is key.dtype is value.dtype is torch.bfloat16 or state.dtype is not torch.float32:
@@ -175,6 +177,7 @@ def gated_delta_step(query, key, value, g, beta, state, slots=None):
   g_type, beta_type = _GATES.get(g.dtype), _GATES.get(beta.dtype)
   if g_type is None or beta_type is None:
     raise LewiError("gated_delta_step takes float32 or bfloat16 g and beta")
+  _lib.no_derivative("gated_delta_step", query, key, value, g, beta, state)
   if _lib.elsewhere(query, key, value, g, beta, state, slots):
     with torch.cuda.device(query.device):
       return gated_delta_step(query, key, value, g, beta, state, slots)
@@ -182,7 +185,7 @@ def gated_delta_step(query, key, value, g, beta, state, slots=None):
   g, beta, slots = g.contiguous(), beta.contiguous(), _lib.index_table(slots, "slots")
   o = torch.empty_like(v, memory_format=torch.contiguous_format)
   if b > 0:
-    check(lib.lewi_gdn_step(stream(), q.data_ptr(), q_rows, k.data_ptr(), k_rows, v.data_ptr(), v_rows, g.data_ptr(), g_type, beta.data_ptr(),
+    check(lib.lewi_gdn_step(stream(q), q.data_ptr(), q_rows, k.data_ptr(), k_rows, v.data_ptr(), v_rows, g.data_ptr(), g_type, beta.data_ptr(),
                             beta_type, ptr(state), ptr(slots), o.data_ptr(), b, ss[0], hk, h, kd, vd), "lewi_gdn_step")
     _lib.written(state)
   return o

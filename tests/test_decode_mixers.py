@@ -456,3 +456,30 @@ def test_what_a_step_writes_is_no_longer_what_a_backward_pass_saved(cuda):
     seqmix.gated_delta_step(q[:, 0], k[:, 0], v[:, 0], g[:, 0], beta[:, 0], state)
   with pytest.raises(RuntimeError, match="modified by an inplace operation"):
     o.sum().backward()
+
+
+def step_calls():
+  """Every operator without a derivative, as a call of one list of float operands."""
+  bf = torch.bfloat16
+  x, w, past = torch.zeros(2, 16, dtype=bf), torch.zeros(4, 1, 16), torch.zeros(2, 3, 16, dtype=bf)
+  q, v, g, s = torch.zeros(2, 2, 16, dtype=bf), torch.zeros(2, 4, 24, dtype=bf), torch.zeros(2, 4), torch.zeros(3, 4, 16, 24)
+  kc, tab, ln, k = torch.zeros(5, 16, 2, 64, dtype=bf), torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), torch.zeros(3, 2, 64, dtype=bf)
+  return ((seqmix.causal_conv1d_step, [x, w, past]), (seqmix.gated_delta_step, [q, q.clone(), v, g, g.clone(), s]),
+          (lambda a, b, c, d: attention.paged_cache_write(a, b, c, d, tab, ln), [k, k.clone(), kc, kc.clone()]),
+          (lambda a, b, c: attention.paged_attention(a, b, c, tab, ln), [torch.zeros(3, 4, 64, dtype=bf), kc, kc.clone()]))
+
+
+def test_operands_that_a_derivative_is_wanted_of_are_refused():
+  """On CPU tensors, which are refused afterwards: gradients and tangents first, and only where they are recorded."""
+  from torch.autograd import forward_ad
+  for call, operands in step_calls():
+    for i in range(len(operands)):
+      with_grad = [t.clone().requires_grad_(True) if j == i else t for j, t in enumerate(operands)]
+      with pytest.raises(LewiError, match="not differentiable"):
+        call(*with_grad)
+      with torch.no_grad(), pytest.raises(LewiError, match="expected CUDA tensors"):
+        call(*with_grad)
+      with forward_ad.dual_level(), pytest.raises(LewiError, match="forward-mode"):
+        call(*(forward_ad.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate(operands)))
+    with pytest.raises(LewiError, match="expected CUDA tensors"):
+      call(*operands)
