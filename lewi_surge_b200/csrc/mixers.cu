@@ -182,7 +182,7 @@ int lewi_paged_cache_write(void* stream, const void* k, int64_t k_stride, const 
                             (int)pages, page, max_pages},
                            reinterpret_cast<const bf16*>(k), reinterpret_cast<const bf16*>(v), k_stride, v_stride, cu_seqlens, T};
   constexpr int per = paged::kWriteThreads / 32;
-  paged::write_kernel<<<(unsigned)((T + per - 1) / per), paged::kWriteThreads, 0, as_stream(stream)>>>(a);
+  paged::write_kernel<<<(unsigned)(((int64_t)T + per - 1) / per), paged::kWriteThreads, 0, as_stream(stream)>>>(a);
   LEWI_CHECK_LAUNCH();
   return LEWI_OK;
 }

@@ -65,8 +65,9 @@ __device__ __forceinline__ void write_row(const __nv_bfloat16* __restrict__ src,
 }
 
 __global__ void __launch_bounds__(kWriteThreads) write_kernel(const WriteArgs a) {
-  const int t = (blockIdx.x * kWriteThreads + threadIdx.x) >> 5, lane = threadIdx.x & 31;
-  if (t >= a.T) return;
+  const long long at = (long long)blockIdx.x * (kWriteThreads / 32) + (threadIdx.x >> 5);   // (threads of 2^27 tokens pass 32 bits)
+  if (at >= a.T) return;
+  const int t = (int)at, lane = threadIdx.x & 31;
   int b = t, back = 1;   // the token's sequence, and how far from its end it is
   if (a.cu != nullptr) {
     // the last b with cu[b] <= t, 32 bounds at a time; [lo, hi) holds it

@@ -483,3 +483,16 @@ def test_operands_that_a_derivative_is_wanted_of_are_refused():
         call(*(forward_ad.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate(operands)))
     with pytest.raises(LewiError, match="expected CUDA tensors"):
       call(*operands)
+
+
+@pytest.mark.gpu
+def test_cache_write_of_more_tokens_than_32_bits_count_threads(cuda):
+  """2^27 tokens of a warp each and a few more: the last ones arrive, the first ones stay."""
+  page, t = 8, 2 ** 27 + 1000
+  k = torch.arange(t * 4, dtype=torch.int32, device=cuda).view(torch.bfloat16).view(t, 1, 8)
+  kc, vc = (torch.zeros(t // page, page, 1, 8, dtype=torch.bfloat16, device=cuda) for _ in range(2))
+  tables = torch.arange(t // page - 1, -1, -1, dtype=torch.int32, device=cuda)[None]
+  attention.paged_cache_write(k, k, kc, vc, tables, torch.tensor([t], device=cuda), torch.tensor([0, t], device=cuda))
+  assert _lib.last_status() == 0
+  for c in (kc, vc):
+    assert torch.equal(c.flip(0).view(torch.int16), k.view(t // page, page, 1, 8).view(torch.int16))
