@@ -351,7 +351,7 @@ int lewi_gdn_chunk_bwd(void* stream, const void* q, const void* k, const void* v
  * Single-token steps of both, for decoding.  A row of the batch has its state at slots[b] of a pool of N (slots null: at b, N >= B);
  * the state is read, moved one token on and written back.  slots[b] < 0: an idle row, zeros out, no state touched.  A slot past the
  * pool, or one that an earlier row of the batch has: the same, and LEWI_STATUS_BAD_INDEX.  `*_stride` is the distance of two rows of
- * the batch in elements; within a row inputs are contiguous.
+ * the batch in elements; within a row inputs are contiguous.  B and H up to 65,535, C and V up to 2^31 - 2049.
  *   convolution: y[b,c] = sum_{j<K} w[j,c] z[j,c], z = (state, x); state <- z[1..].  x, y bf16 [B,C], w bf16 [K,C], state bf16 [N,K-1,C]
  *     (the K-1 inputs before this one, oldest first; zeros where there were none).  K <= 8, C a multiple of 8, all 16-byte aligned.
  *   gated delta rule: S <- S exp(g), S <- S + k (x) beta (v - k^T S), o = (q / sqrt(K))^T S.  q, k bf16 [B,Hk,K], v, o bf16 [B,H,V],
@@ -367,7 +367,7 @@ int lewi_gdn_step(void* stream, const void* q, int64_t q_stride, const void* k, 
 /* ------------------------------------------------------------------------------------------------
  * A paged key-value cache: k_cache, v_cache bf16 [pages][page][Hkv][D], pages page_stride elements apart; sequence b has the pages
  * tables[b][0..max_pages) (i32) and lengths[b] (i32) tokens in them, the new ones among them.  D <= 256, a multiple of 8; caches
- * 16-byte aligned, page_stride a multiple of 8.  Table entries past a sequence's length are not read.  A length past the table counts
+ * 16-byte aligned, page_stride a multiple of 8; Hkv D and Hq D up to 2^31 - 2049, in the attention B up to 65,535.  Table entries past a sequence's length are not read.  A length past the table counts
  * as the table's, a page that does not exist is left out, both with LEWI_STATUS_BAD_INDEX; a length of zero or less is an idle row.
  *   write: tokens cu_seqlens[b] .. cu_seqlens[b+1] of k, v bf16 [T][Hkv][D] (i32, ascending; null: one token per sequence, T = B) become
  *     the last ones of sequence b.  Tokens of no sequence are left out.  Two tokens on one cell leave either.
@@ -393,7 +393,7 @@ int lewi_paged_attention(void* stream, const void* q, int64_t q_stride, const vo
  * of it) are for the backward pass; where none follows lse is null, and o_rest may be too up to T = 32768 (beyond it is a place for sums,
  * LEWI_ERR_WORKSPACE without it).  Their rows of no sequence are left as they are.  No accumulator of the tensor cores, which truncate, sums
  * more than 32768 rows: sums of one sign come out short by 2^-12 of themselves at most, whatever the length.
- * D <= 128, a multiple of 8; T * Hq / Hkv <= 2^25; scale > 0; all tensors 16-byte aligned, `*_stride` (elements from row to row; heads are contiguous) multiples
+ * D <= 128, a multiple of 8; T * Hq / Hkv <= 2^25, Hq D <= 2^31 - 2049; scale > 0; all tensors 16-byte aligned, `*_stride` (elements from row to row; heads are contiguous) multiples
  * of 8.  Scores, softmax and sums float32; p and the gradient of the scores are rounded to bf16 for their products (where lse is given and in the
  * backward call, pairs of a sequence's first 128 rows in two parts, to 2^-16).
  * The backward call makes dq and/or dk and dv (bf16, contiguous; dk and dv together) out of d_o (bf16 [T][Hq][D], contiguous).  No

@@ -173,6 +173,12 @@ def elsewhere(*tensors):
   return index != torch._C._cuda_getDevice()
 
 
+def fits(what, *sizes):
+  """Refuses sizes that the C entries' 32 bits would cut."""
+  if max(sizes) > 0x7fffffff:
+    raise LewiError(f"{what}: a size of {max(sizes)} does not fit into 32 bits")
+
+
 def has_tangent(*tensors):
   """Whether one of these is a dual tensor of forward-mode differentiation, which no kernel here carries on."""
   from torch.autograd import forward_ad

@@ -27,6 +27,7 @@ def _check_cache(what, key_cache, value_cache, block_tables, lengths):
       page_stride = key_cache.stride(0)
   if len(tables) != 2 or lengths.shape != tables[:1]:
     raise LewiError(f"{what}: block_tables [B, max_pages] and lengths [B] are required")
+  _lib.fits(what, page, heads, tables[0], tables[1])
   return pages, page, heads, d, page_stride
 
 
@@ -43,6 +44,7 @@ def paged_cache_write(key, value, key_cache, value_cache, block_tables, lengths,
   if not key.dtype is value.dtype is torch.bfloat16 or len(new) != 3 or new[1] != heads or new[2] != d or value.shape != new:
     raise LewiError("paged_cache_write: key, value [T, Hkv, D] bfloat16, as wide as the caches, are required")
   t, (b, max_pages) = new[0], block_tables.shape
+  _lib.fits("paged_cache_write", t, b)
   if cu_seqlens is not None and cu_seqlens.shape != (b + 1,):
     raise LewiError("paged_cache_write: cu_seqlens [B + 1] is required")
   if cu_seqlens is None and t != b:
@@ -75,6 +77,7 @@ def paged_attention(query, key_cache, value_cache, block_tables, lengths, scale=
     raise LewiError("paged_attention: query [B, Hq, D] bfloat16 with Hq a multiple of the caches' heads is required")
   _lib.no_derivative("paged_attention", query, key_cache, value_cache)
   hq = shape[1]
+  _lib.fits("paged_attention", hq, b)
   if _lib.elsewhere(query, key_cache, value_cache, block_tables, lengths):
     with torch.cuda.device(query.device):
       return paged_attention(query, key_cache, value_cache, block_tables, lengths, scale)
@@ -161,10 +164,12 @@ def causal_attention(query, key, value, cu_seqlens=None, scale=None):
       shape[-2] % other[-2]:
     raise LewiError("causal_attention: query [T, Hq, D] and key, value [T, Hkv, D], or all three [B, S, ..], Hq a multiple of Hkv, are required")
   n_seqs = 1 if n == 3 else shape[0]
+  _lib.fits("causal_attention", shape[0] * (shape[1] if n == 4 else 1), shape[-2])
   if cu_seqlens is not None:
     if n == 4 or cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 2:
       raise LewiError("causal_attention: cu_seqlens [N + 1] belongs to packed rows [T, H, D]")
     n_seqs = cu_seqlens.shape[0] - 1
+    _lib.fits("causal_attention", n_seqs)
   scale = shape[-1] ** -0.5 if scale is None else float(scale)
   if not scale > 0:
     raise LewiError("causal_attention: scale must be positive")

@@ -18,11 +18,14 @@ inline bool aligned(const void* p, int to) { return (reinterpret_cast<uintptr_t>
 inline bool is_dtype(int d) { return d == LEWI_BF16 || d == LEWI_F32; }
 typedef __nv_bfloat16 bf16;
 
+// Elements of a row, and channels that a grid covers, are counted in 32 bits; past its end a grid may reach by as much as this.
+constexpr int64_t kMaxRow = 0x7fffffff - 2048;
+
 // Checks of a paged cache; 0 or an error code.
 int check_cache(const void* k, const void* v, const int32_t* tables, const int32_t* lengths, int B, int Hkv, int D, int64_t pages, int page,
                 int max_pages, int64_t page_stride) {
   if (!k || !v || !tables || !lengths || B <= 0 || Hkv <= 0 || D <= 0 || pages <= 0 || page <= 0 || max_pages <= 0) return LEWI_ERR_ARG;
-  if (D > 256 || pages > 0x7fffffff || (int64_t)max_pages * page > 0x7fffffff - 128) return LEWI_ERR_LIMIT;
+  if (D > 256 || pages > 0x7fffffff || (int64_t)max_pages * page > 0x7fffffff - 128 || (int64_t)Hkv * D > kMaxRow) return LEWI_ERR_LIMIT;
   if (D % 8 != 0 || !aligned(k, 16) || !aligned(v, 16) || page_stride % 8 != 0 || page_stride < (int64_t)page * Hkv * D) return LEWI_ERR_SHAPE;
   return LEWI_OK;
 }
@@ -60,7 +63,7 @@ int check_attention(const void* q, int64_t q_stride, const void* k, int64_t k_st
                     const void* o, int T, int Hq, int Hkv, int D, float scale) {
   if (!q || !k || !v || !o || T <= 0 || n_seqs <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || !(scale > 0.f)) return LEWI_ERR_ARG;
   if (!cu && T % n_seqs != 0) return LEWI_ERR_ARG;
-  if (D > attn::kMaxD || T > 0x7fffffff - attn::kTile) return LEWI_ERR_LIMIT;
+  if (D > attn::kMaxD || T > 0x7fffffff - attn::kTile || (int64_t)Hq * D > kMaxRow || (int64_t)Hkv * D > kMaxRow) return LEWI_ERR_LIMIT;
   if ((attn::most_tiles(T, n_seqs) + n_seqs) * Hq > 0x7fffffff) return LEWI_ERR_LIMIT;
   if ((int64_t)T * (Hq / Hkv) > attn::kMaxGroupRows) return LEWI_ERR_LIMIT;
   if (D % 8 != 0 || Hq % Hkv != 0 || !aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(o, 16)) return LEWI_ERR_SHAPE;
@@ -130,7 +133,7 @@ extern "C" {
 int lewi_causal_conv1d_step(void* stream, const void* x, int64_t x_stride, const void* w, void* state, const int32_t* slots, void* y, int B,
                             int N, int C, int K) {
   if (!x || !w || !y || B <= 0 || N <= 0 || C <= 0 || K <= 0 || (K > 1 && !state) || (!slots && N < B)) return LEWI_ERR_ARG;
-  if (K > 8 || B > 65535) return LEWI_ERR_LIMIT;
+  if (K > 8 || B > 65535 || C > kMaxRow) return LEWI_ERR_LIMIT;
   if (C % 8 != 0 || x_stride % 8 != 0 || x_stride < C || !aligned(x, 16) || !aligned(w, 16) || !aligned(state, 16) || !aligned(y, 16))
     return LEWI_ERR_SHAPE;
   const step::ConvArgs a{reinterpret_cast<const bf16*>(x), x_stride, reinterpret_cast<const bf16*>(w), reinterpret_cast<bf16*>(state), slots,
@@ -156,7 +159,7 @@ int lewi_gdn_step(void* stream, const void* q, int64_t q_stride, const void* k, 
                   int Hk, int H, int K, int V) {
   if (!q || !k || !v || !g || !beta || !state || !o || B <= 0 || N <= 0 || Hk <= 0 || H <= 0 || K <= 0 || V <= 0) return LEWI_ERR_ARG;
   if (!is_dtype(g_dtype) || !is_dtype(beta_dtype) || (!slots && N < B)) return LEWI_ERR_ARG;
-  if (K > step::kMaxK || H > 65535 || B > 65535) return LEWI_ERR_LIMIT;
+  if (K > step::kMaxK || H > 65535 || B > 65535 || V > kMaxRow) return LEWI_ERR_LIMIT;
   if (K % 8 != 0 || V % 8 != 0 || H % Hk != 0 || !aligned(state, 16) || !aligned(o, 8)) return LEWI_ERR_SHAPE;
   if (q_stride < (int64_t)Hk * K || k_stride < (int64_t)Hk * K || v_stride < (int64_t)H * V) return LEWI_ERR_SHAPE;
   const step::GdnArgs a{reinterpret_cast<const bf16*>(q), reinterpret_cast<const bf16*>(k), reinterpret_cast<const bf16*>(v), q_stride, k_stride,
@@ -197,7 +200,7 @@ int lewi_paged_attention(void* stream, const void* q, int64_t q_stride, const vo
                          int Hkv, int D, int64_t pages, int page, int max_pages, float scale) {
   if (!q || !o || Hq <= 0) return LEWI_ERR_ARG;
   if (const int rc = check_cache(k_cache, v_cache, tables, lengths, B, Hkv, D, pages, page, max_pages, page_stride)) return rc;
-  if (B > 65535) return LEWI_ERR_LIMIT;
+  if (B > 65535 || (int64_t)Hq * D > kMaxRow) return LEWI_ERR_LIMIT;
   if (Hq % Hkv != 0 || !aligned(q, 4) || q_stride % 2 != 0 || q_stride < (int64_t)Hq * D || !aligned(o, 8)) return LEWI_ERR_SHAPE;
   if (!workspace || !aligned(workspace, 16) || workspace_bytes < lewi_paged_attention_workspace_bytes(D)) return LEWI_ERR_WORKSPACE;
   const int G = Hq / Hkv, MT = (G + paged::kRows - 1) / paged::kRows;

@@ -496,3 +496,63 @@ def test_cache_write_of_more_tokens_than_32_bits_count_threads(cuda):
   assert _lib.last_status() == 0
   for c in (kc, vc):
     assert torch.equal(c.flip(0).view(torch.int16), k.view(t // page, page, 1, 8).view(torch.int16))
+
+
+def test_sizes_past_32_bits_are_refused():
+  """Tensors of one element that seem large: a size that the C entries' arguments would cut must not become a small one."""
+  huge, bf = 2 ** 32 + 2, torch.bfloat16
+  e = lambda *shape, dtype=bf: torch.zeros((), dtype=dtype).expand(*shape)
+  i32 = torch.int32
+  for call in (lambda: seqmix.causal_conv1d_step(e(huge, 8), e(4, 1, 8), e(huge, 3, 8)), lambda: seqmix.causal_conv1d_step(e(2, 8), e(1, 1, 8), e(huge, 0, 8)),
+               lambda: seqmix.gated_delta_step(e(huge, 1, 8), e(huge, 1, 8), e(huge, 1, 8), e(huge, 1), e(huge, 1), e(huge, 1, 8, 8, dtype=torch.float32)),
+               lambda: attention.paged_attention(e(huge, 2, 8), e(4, 16, 1, 8).contiguous(), e(4, 16, 1, 8).contiguous(), e(huge, 2, dtype=i32), e(huge, dtype=i32)),
+               lambda: attention.paged_attention(e(2, 2, 8), e(4, 16, 1, 8).contiguous(), e(4, 16, 1, 8).contiguous(), e(2, huge, dtype=i32), e(2, dtype=i32)),
+               lambda: attention.paged_cache_write(e(huge, 1, 8), e(huge, 1, 8), e(4, 16, 1, 8).contiguous(), e(4, 16, 1, 8).contiguous(), e(2, 2, dtype=i32),
+                                                   e(2, dtype=i32), e(3, dtype=i32)),
+               lambda: attention.causal_attention(e(huge, 2, 8), e(huge, 1, 8), e(huge, 1, 8)),
+               lambda: attention.causal_attention(e(2 ** 16, 2 ** 16 + 1, 2, 8), e(2 ** 16, 2 ** 16 + 1, 1, 8), e(2 ** 16, 2 ** 16 + 1, 1, 8)),
+               lambda: attention.causal_attention(e(4, 2, 8), e(4, 1, 8), e(4, 1, 8), e(huge, dtype=i32))):
+    with pytest.raises(LewiError, match="32 bits"):
+      call()
+
+
+def test_the_c_entries_refuse_rows_that_32_bits_do_not_count():
+  """Channels and columns whose grid would pass 2^31 - 1, and as many elements of a row of heads (addresses that are never used)."""
+  lib, at, last = _lib.load(), 1 << 20, 2 ** 31 - 8
+  assert lib.lewi_causal_conv1d_step(None, at, last, at, at, None, at, 1, 1, last, 4) == -5
+  assert lib.lewi_gdn_step(None, at, 8, at, 8, at, last, at, 1, at, 1, at, None, at, 1, 1, 1, 1, 8, last) == -5
+  heads = 2 ** 28
+  write = lambda hkv, stride: lib.lewi_paged_cache_write(None, at, stride, at, stride, at, at, stride, at, at, None, 1, 1, hkv, 8, 1, 1, 1)
+  assert write(heads, 8 * heads) == -5
+  attend = lambda hq, hkv: lib.lewi_paged_attention(None, at, 8 * hq, at, at, 8 * hkv, at, at, at, at, 1 << 40, 1, hq, hkv, 8, 1, 1, 1, 1.0)
+  assert attend(heads, heads) == -5 and attend(heads, 1) == -5
+  assert lib.lewi_causal_attention_fwd(None, at, 8 * heads, at, 8 * heads, at, 8 * heads, None, 1, at, at, at, 1, heads, heads, 8, 1.0) == -5
+
+
+@pytest.mark.parametrize("change,code", [(dict(K=9), -5), (dict(B=65536, N=65536), -5), (dict(C=12), -2), (dict(xs=8), -2), (dict(xs=20), -2), (dict(x=2), -2), (dict(N=1), -1),
+                                         (dict(C=0), -1), (dict(state=None), -1), (dict(y=None), -1)])
+def test_the_c_entry_of_the_convolution_step_checks_its_arguments(change, code):
+  at = 1 << 20
+  a = dict(x=at, xs=16, state=at, y=at, B=2, N=2, C=16, K=4)
+  a.update({n: v + at if n == "x" else v for n, v in change.items()})
+  assert _lib.load().lewi_causal_conv1d_step(None, a["x"], a["xs"], at, a["state"], None, a["y"], a["B"], a["N"], a["C"], a["K"]) == code
+
+
+@pytest.mark.parametrize("change,code", [(dict(K=136), -5), (dict(H=65536, vs=65536 * 16), -5), (dict(B=65536, N=65536), -5), (dict(K=12), -2), (dict(V=12), -2), (dict(H=3), -2), (dict(qs=16), -2),
+                                         (dict(vs=32), -2), (dict(state=8), -2), (dict(o=4), -2), (dict(N=1), -1), (dict(g_type=7), -1), (dict(B=0), -1)])
+def test_the_c_entry_of_the_delta_step_checks_its_arguments(change, code):
+  at = 1 << 20
+  a = dict(qs=32, vs=64, state=0, o=0, B=2, N=2, Hk=2, H=4, K=16, V=16, g_type=_lib.F32)
+  a.update(change)
+  assert _lib.load().lewi_gdn_step(None, at, a["qs"], at, 32, at, a["vs"], at, a["g_type"], at, _lib.BF16, at + a["state"], None, at + a["o"], a["B"], a["N"], a["Hk"], a["H"],
+                                   a["K"], a["V"]) == code
+
+
+@pytest.mark.parametrize("change,code", [(dict(D=264), -5), (dict(max_pages=2 ** 30), -5), (dict(D=60), -2), (dict(ks=120), -2), (dict(ks=132), -2), (dict(k=8), -2), (dict(page_stride=8), -2),
+                                         (dict(T=3), -1), (dict(T=0), -1), (dict(pages=0), -1)])
+def test_the_c_entry_of_the_cache_write_checks_its_arguments(change, code):
+  at = 1 << 20
+  a = dict(k=0, ks=128, page_stride=16 * 128, T=2, B=2, D=64, pages=4, page=16, max_pages=2)
+  a.update(change)
+  assert _lib.load().lewi_paged_cache_write(None, at + a["k"], a["ks"], at, 128, at, at, a["page_stride"], at, at, None, a["T"], a["B"], 2, a["D"], a["pages"], a["page"],
+                                            a["max_pages"]) == code
