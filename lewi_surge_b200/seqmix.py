@@ -99,17 +99,21 @@ class _ChunkGatedDeltaRule(torch.autograd.Function):
     return dq, dk, dv, dg.to(g_dt), db.to(b_dt), (dh0.to(h_dt) if dh0 is not None else None)
 
 
-def chunk_gated_delta_rule(query, key, value, g, beta, chunk_size=64, initial_state=None):
+def chunk_gated_delta_rule(query, key, value, g, beta, chunk_size=64, initial_state=None, final_state_dtype=torch.bfloat16):
   """The chunked gated delta rule with the signature of the reference's `fast_chunk_gated_delta_rule`
   (modal/gdn_fast.py:37): query, key [B,S,H,K], value [B,S,H,V] bf16, g [B,S,H] (log decay), beta [B,S,H]; returns
   (o [B,S,H,V] bf16, final state [B,H,K,V] bf16 or None when no initial state was given, as the reference does).
+  `final_state_dtype=torch.float32` returns the final state as the kernel holds it, which is what `gated_delta_step` or a further piece of the
+  sequence goes on from without a rounding.
   Differentiable through `torch.autograd` in q, k, v, g, beta and the initial state (head dimensions up to 128)."""
   if chunk_size != 64:
     raise LewiError("chunk_gated_delta_rule: the kernels work in chunks of 64 tokens")
   if query.dtype != torch.bfloat16 or key.dtype != torch.bfloat16 or value.dtype != torch.bfloat16:
     raise LewiError("chunk_gated_delta_rule takes bfloat16 q, k, v")
+  if final_state_dtype not in _GATES:
+    raise LewiError("chunk_gated_delta_rule returns its final state as bfloat16 or float32")
   o, hf = _ChunkGatedDeltaRule.apply(query, key, value, g, beta, initial_state)
-  return o, (hf.to(torch.bfloat16) if initial_state is not None else None)
+  return o, (hf.to(final_state_dtype) if initial_state is not None else None)
 
 
 _GATES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}

@@ -556,3 +556,43 @@ def test_the_c_entry_of_the_cache_write_checks_its_arguments(change, code):
   a.update(change)
   assert _lib.load().lewi_paged_cache_write(None, at + a["k"], a["ks"], at, 128, at, at, a["page_stride"], at, at, None, a["T"], a["B"], 2, a["D"], a["pages"], a["page"],
                                             a["max_pages"]) == code
+
+
+def test_the_type_of_the_final_state_is_checked():
+  x, g = torch.zeros(1, 64, 1, 16).bfloat16(), torch.zeros(1, 64, 1)
+  with pytest.raises(LewiError, match="final state"):
+    seqmix.chunk_gated_delta_rule(x, x, x, g, g, initial_state=torch.zeros(1, 1, 16, 16), final_state_dtype=torch.float16)
+
+
+@pytest.mark.gpu
+def test_a_float32_final_state_goes_on_without_a_rounding(cuda):
+  """A sequence in two pieces has the operands of the whole one in every product, and a state in float32 between them, so what it ends with differs by
+  float32 at most (2^-14 is room for it); bf16 between them is 2^-9 / sqrt(3) of the state, of which the decay leaves most."""
+  gen = torch.Generator().manual_seed(21)
+  b, s, h, kd, cut = 2, 256, 2, 64, 192
+  unit = lambda x: (x / x.norm(dim=-1, keepdim=True)).bfloat16()
+  q, k = (unit(torch.randn(b, s, h, kd, generator=gen)).to(cuda) for _ in range(2))
+  v = rnd(gen, b, s, h, kd).to(cuda)
+  g, beta = -0.002 * torch.rand(b, s, h, generator=gen).to(cuda), torch.rand(b, s, h, generator=gen).bfloat16().to(cuda)
+  start = torch.randn(b, h, kd, kd, generator=gen).to(cuda)
+  piece = lambda rows, state, **how: seqmix.chunk_gated_delta_rule(q[:, rows], k[:, rows], v[:, rows], g[:, rows], beta[:, rows], initial_state=state, **how)
+  f32 = dict(final_state_dtype=torch.float32)
+  _, whole = piece(slice(0, s), start, **f32)
+  assert whole.dtype is torch.float32 and torch.equal(piece(slice(0, s), start)[1], whole.bfloat16())
+  _, middle = piece(slice(0, cut), start, **f32)
+  _, end = piece(slice(cut, s), middle, **f32)
+  assert (end - whole).norm() <= 2.0 ** -14 * whole.norm()
+  # tokens one by one from the middle: float32 all the way, as far from the recurrence in 64 bits as its own sums (2 K + 8 roundings each, 64 steps)
+  pool, exact = middle.clone(), middle.to(F64).cpu()
+  for i in range(cut, s):
+    seqmix.gated_delta_step(q[:, i], k[:, i], v[:, i], g[:, i], beta[:, i], pool)
+    ki, vi, bi = (t[:, i].to(F64).cpu() for t in (k, v, beta))
+    exact = exact * g[:, i].to(F64).cpu().exp()[..., None, None]
+    exact = exact + ki[..., None] * (bi[..., None] * (vi - torch.einsum("bhk,bhkv->bhv", ki, exact)))[:, :, None]
+  assert (pool.cpu().to(F64) - exact).norm() <= (s - cut) * (2 * kd + 8) * 2.0 ** -24 * exact.norm()
+  # gradients through either form of it
+  leaves = [x.detach().requires_grad_(True) for x in (q, k, v, g, beta, start)]
+  up = rnd(gen, b, h, kd, kd).to(cuda)
+  run = lambda **how: seqmix.chunk_gated_delta_rule(*leaves[:5], initial_state=leaves[5], **how)[1]
+  for x, y in zip(torch.autograd.grad(run(), leaves[1:], up), torch.autograd.grad(run(**f32), leaves[1:], up.float())):
+    assert torch.equal(x, y)
