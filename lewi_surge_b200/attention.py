@@ -21,7 +21,8 @@ def _check_cache(what, key_cache, value_cache, block_tables, lengths):
   page_stride = page * heads * d
   if not (key_cache.is_contiguous() and value_cache.is_contiguous()):
     for t in (key_cache, value_cache):
-      if t.stride()[1:] != (heads * d, d, 1) or (pages > 1 and t.stride(0) != key_cache.stride(0)):
+      inside = all(n == 1 or step == packed for n, step, packed in zip(shape[1:], t.stride()[1:], (heads * d, d, 1)))
+      if not inside or (pages > 1 and t.stride(0) != key_cache.stride(0)):
         raise LewiError(f"{what}: pages that are contiguous and as far apart in both caches are required")
     if pages > 1:
       page_stride = key_cache.stride(0)

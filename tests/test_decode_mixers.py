@@ -596,3 +596,32 @@ def test_a_float32_final_state_goes_on_without_a_rounding(cuda):
   run = lambda **how: seqmix.chunk_gated_delta_rule(*leaves[:5], initial_state=leaves[5], **how)[1]
   for x, y in zip(torch.autograd.grad(run(), leaves[1:], up), torch.autograd.grad(run(**f32), leaves[1:], up.float())):
     assert torch.equal(x, y)
+
+
+def test_distances_along_dimensions_of_one_mean_nothing():
+  """Pages of one token or heads of which there is one, cut out of larger tensors, are taken (CPU tensors: up to where those are refused)."""
+  tab, ln = torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+  one_token, one_head, split = torch.zeros(5, 3, 2, 64).bfloat16()[:, ::3], torch.zeros(5, 16, 64, 3).bfloat16()[..., ::3].permute(0, 1, 3, 2), torch.zeros(5, 16, 4, 64).bfloat16()[:, :, :2]
+  assert one_token.shape == (5, 1, 2, 64) and one_token.stride(1) != 128
+  for caches, heads, match in (((one_token, one_token), 2, "expected CUDA"), ((one_token, one_token.clone()), 2, "contiguous"), ((split, split), 2, "contiguous"),
+                               ((one_head, one_head), 1, "contiguous")):
+    q, k = torch.zeros(3, 4, 64).bfloat16(), torch.zeros(3, heads, 64).bfloat16()
+    with pytest.raises(LewiError, match=match):
+      attention.paged_attention(q, *caches, tab, ln)
+    with pytest.raises(LewiError, match=match):
+      attention.paged_cache_write(k, k, *caches, tab, ln)
+
+
+@pytest.mark.gpu
+def test_pages_of_one_token_at_a_distance(cuda):
+  gen = torch.Generator().manual_seed(22)
+  base = rnd(gen, 9, 6, 2, 64).to(cuda)
+  kc, vc = base[:, 0:1].as_strided((9, 1, 2, 64), (6 * 128, 999, 64, 1)), base[:, 3:4]
+  tables, lens = torch.tensor([[4, 0, 7], [2, 8, 1]], device=cuda), torch.tensor([3, 2], device=cuda)
+  q, k = rnd(gen, 2, 4, 64).to(cuda), rnd(gen, 2, 2, 64).to(cuda)
+  packed = [c.contiguous().clone() for c in (kc, vc)]
+  other = base[:, [1, 2, 4, 5]].clone()
+  for caches in ((kc, vc), packed):
+    attention.paged_cache_write(k, -k, *caches, tables, lens)
+  assert torch.equal(kc, packed[0]) and torch.equal(vc, packed[1]) and torch.equal(base[:, [1, 2, 4, 5]], other)
+  assert torch.equal(attention.paged_attention(q, kc, vc, tables, lens), attention.paged_attention(q, *packed, tables, lens)) and _lib.last_status() == 0
