@@ -15,7 +15,7 @@ def _check_cache(what, key_cache, value_cache, block_tables, lengths):
   if not key_cache.dtype is value_cache.dtype is torch.bfloat16:
     raise LewiError(f"{what} takes bfloat16 caches")
   shape, tables = key_cache.shape, block_tables.shape
-  if len(shape) != 4 or value_cache.shape != shape:
+  if len(shape) != 4 or value_cache.shape != shape or shape[3] == 0:
     raise LewiError(f"{what}: caches [pages, page, Hkv, D] of one shape are required")
   pages, page, heads, d = shape
   page_stride = page * heads * d
@@ -171,13 +171,13 @@ def causal_attention(query, key, value, cu_seqlens=None, scale=None):
       raise LewiError("causal_attention: cu_seqlens [N + 1] belongs to packed rows [T, H, D]")
     n_seqs = cu_seqlens.shape[0] - 1
     _lib.fits("causal_attention", n_seqs)
-  scale = shape[-1] ** -0.5 if scale is None else float(scale)
+  scale = max(shape[-1], 1) ** -0.5 if scale is None else float(scale)
   if not scale > 0:
     raise LewiError("causal_attention: scale must be positive")
   if torch.autograd.forward_ad._current_level >= 0 and _lib.has_tangent(query, key, value):
     raise LewiError("causal_attention has no forward-mode derivative")
   if query.numel() == 0:
-    return query.clone()
+    return query + 0 * (key.sum() + value.sum())   # (nothing, with gradients of zero)
   if _lib.elsewhere(query, key, value, cu_seqlens):
     with torch.cuda.device(query.device):
       return causal_attention(query, key, value, cu_seqlens, scale)

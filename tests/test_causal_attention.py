@@ -501,3 +501,12 @@ def test_forward_mode_is_refused():
       for mode in (torch.enable_grad, torch.no_grad):
         with mode(), pytest.raises(LewiError, match="forward-mode"):
           attention.causal_attention(*operands)
+
+
+def test_nothing_has_gradients_of_zero():
+  for t, hq, hkv, d in ((0, 4, 2, 16), (5, 0, 2, 16), (3, 2, 2, 0)):
+    q, k, v = (torch.ones(t, h, d).bfloat16().requires_grad_(True) for h in (hq, hkv, hkv))
+    o = attention.causal_attention(q, k, v)
+    assert o.shape == q.shape and o.dtype is torch.bfloat16
+    for g, x in zip(torch.autograd.grad(o.sum(), (q, k, v)), (q, k, v)):
+      assert g.shape == x.shape and not g.any()
