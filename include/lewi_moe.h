@@ -393,7 +393,7 @@ int lewi_paged_attention(void* stream, const void* q, int64_t q_stride, const vo
  * of it) are for the backward pass; where none follows lse is null, and o_rest may be too up to T = 32768 (beyond it is a place for sums,
  * LEWI_ERR_WORKSPACE without it).  Their rows of no sequence are left as they are.  No accumulator of the tensor cores, which truncate, sums
  * more than 32768 rows: sums of one sign come out short by 2^-12 of themselves at most, whatever the length.
- * D <= 128, a multiple of 8; T * Hq / Hkv <= 2^25, Hq D <= 2^31 - 2049; scale > 0; all tensors 16-byte aligned, `*_stride` (elements from row to row; heads are contiguous) multiples
+ * D <= 128, a multiple of 8; T * Hq / Hkv <= 2^25, Hq D <= 2^31 - 2049; 0 < scale < 2e38; all tensors 16-byte aligned, `*_stride` (elements from row to row; heads are contiguous) multiples
  * of 8.  Scores, softmax and sums float32; p and the gradient of the scores are rounded to bf16 for their products (where lse is given and in the
  * backward call, pairs of a sequence's first 128 rows in two parts, to 2^-16).
  * The backward call makes dq and/or dk and dv (bf16, contiguous; dk and dv together) out of d_o (bf16 [T][Hq][D], contiguous).  No

@@ -172,8 +172,8 @@ def causal_attention(query, key, value, cu_seqlens=None, scale=None):
     n_seqs = cu_seqlens.shape[0] - 1
     _lib.fits("causal_attention", n_seqs)
   scale = max(shape[-1], 1) ** -0.5 if scale is None else float(scale)
-  if not scale > 0:
-    raise LewiError("causal_attention: scale must be positive")
+  if not 0 < scale < 2e38:
+    raise LewiError("causal_attention: scale must be positive, and float32 must hold it")
   if torch.autograd.forward_ad._current_level >= 0 and _lib.has_tangent(query, key, value):
     raise LewiError("causal_attention has no forward-mode derivative")
   if query.numel() == 0:

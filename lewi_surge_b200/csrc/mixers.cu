@@ -61,7 +61,7 @@ int launch_paged(cudaStream_t st, const paged::Args& a) {
 // Checks of what forward and backward of causal attention share.
 int check_attention(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride, const int32_t* cu, int n_seqs,
                     const void* o, int T, int Hq, int Hkv, int D, float scale) {
-  if (!q || !k || !v || !o || T <= 0 || n_seqs <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || !(scale > 0.f)) return LEWI_ERR_ARG;
+  if (!q || !k || !v || !o || T <= 0 || n_seqs <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || !(scale > 0.f && scale < 2e38f)) return LEWI_ERR_ARG;
   if (!cu && T % n_seqs != 0) return LEWI_ERR_ARG;
   if (D > attn::kMaxD || T > 0x7fffffff - attn::kTile || (int64_t)Hq * D > kMaxRow || (int64_t)Hkv * D > kMaxRow) return LEWI_ERR_LIMIT;
   if ((attn::most_tiles(T, n_seqs) + n_seqs) * Hq > 0x7fffffff) return LEWI_ERR_LIMIT;
@@ -198,7 +198,7 @@ int64_t lewi_paged_attention_workspace_bytes(int D) {
 int lewi_paged_attention(void* stream, const void* q, int64_t q_stride, const void* k_cache, const void* v_cache, int64_t page_stride,
                          const int32_t* tables, const int32_t* lengths, void* o, void* workspace, int64_t workspace_bytes, int B, int Hq,
                          int Hkv, int D, int64_t pages, int page, int max_pages, float scale) {
-  if (!q || !o || Hq <= 0) return LEWI_ERR_ARG;
+  if (!q || !o || Hq <= 0 || !(scale > -2e38f && scale < 2e38f)) return LEWI_ERR_ARG;
   if (const int rc = check_cache(k_cache, v_cache, tables, lengths, B, Hkv, D, pages, page, max_pages, page_stride)) return rc;
   if (B > 65535 || (int64_t)Hq * D > kMaxRow) return LEWI_ERR_LIMIT;
   if (Hq % Hkv != 0 || !aligned(q, 4) || q_stride % 2 != 0 || q_stride < (int64_t)Hq * D || !aligned(o, 8)) return LEWI_ERR_SHAPE;

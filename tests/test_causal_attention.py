@@ -510,3 +510,14 @@ def test_nothing_has_gradients_of_zero():
     assert o.shape == q.shape and o.dtype is torch.bfloat16
     for g, x in zip(torch.autograd.grad(o.sum(), (q, k, v)), (q, k, v)):
       assert g.shape == x.shape and not g.any()
+
+
+def test_scales_that_float32_does_not_hold_are_refused():
+  q = torch.zeros(6, 4, 16).bfloat16()
+  for scale in (float("inf"), float("nan"), 1e39):
+    with pytest.raises(LewiError, match="scale"):
+      attention.causal_attention(q, q, q, scale=scale)
+  lib, at, inf = _lib.load(), 1 << 20, float("inf")
+  assert lib.lewi_causal_attention_fwd(None, at, 64, at, 64, at, 64, None, 1, at, at, at, 64, 1, 1, 64, inf) == -1
+  for scale in (inf, -inf, float("nan")):
+    assert lib.lewi_paged_attention(None, at, 64, at, at, 64, at, at, at, at, 1 << 30, 1, 1, 1, 64, 1, 1, 1, scale) == -1
