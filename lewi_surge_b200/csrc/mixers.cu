@@ -30,12 +30,12 @@ int check_cache(const void* k, const void* v, const int32_t* tables, const int32
   return LEWI_OK;
 }
 
-template <int D>
+template <int D, bool LONG>
 int launch_paged(cudaStream_t st, const paged::Args& a) {
   static bool done[64] = {false};
   using S = paged::Shape<D>;
-  if (!allow_smem(paged::attend_kernel<D>, S::kSmem, done)) return LEWI_ERR_CUDA;
-  if (launch_kernel(paged::attend_kernel<D>, a.ctas, S::kThreads, S::kSmem, st, false, a) != cudaSuccess) {
+  if (!allow_smem(paged::attend_kernel<D, LONG>, S::kSmem, done)) return LEWI_ERR_CUDA;
+  if (launch_kernel(paged::attend_kernel<D, LONG>, a.ctas, S::kThreads, S::kSmem, st, false, a) != cudaSuccess) {
     (void)cudaGetLastError();
     return LEWI_ERR_CUDA;
   }
@@ -56,6 +56,12 @@ int launch_paged(cudaStream_t st, const paged::Args& a) {
   }
   ++launch_counter();
   return LEWI_OK;
+}
+
+template <int D>
+int launch_paged(cudaStream_t st, const paged::Args& a) {
+  using S = paged::Shape<D>;
+  return (int64_t)a.c.max_pages * a.c.page > (int64_t)S::kTile * S::kChain ? launch_paged<D, true>(st, a) : launch_paged<D, false>(st, a);
 }
 
 // Checks of what forward and backward of causal attention share.
@@ -123,6 +129,11 @@ inline int64_t delta_bytes(int T, int Hq) { return ((int64_t)T * Hq * 4 + 255) /
 inline int64_t sums_bytes(int T, int Hkv, int D, int parts) { return parts > 1 ? (int64_t)parts * 2 * T * Hkv * D * 4 : 0; }
 
 inline int paged_ctas(int D) { return num_sms() * (D > 128 ? paged::Shape<256>::kCtas : paged::Shape<128>::kCtas); }
+inline int64_t paged_parts_bytes(int D) { return ((int64_t)2 * paged_ctas(D) * paged::kRows * (D + 2) * 4 + 15) / 16 * 16; }
+inline int64_t paged_kept_bytes(int D) {
+  const int columns = D > 128 ? 256 : D > 64 ? 128 : 64, warps = D > 128 ? paged::Shape<256>::kWarps : paged::Shape<128>::kWarps;
+  return (int64_t)paged_ctas(D) * warps * 32 * (columns / 8 * 16 + 8);
+}
 
 }  // namespace
 
@@ -192,7 +203,7 @@ int lewi_paged_cache_write(void* stream, const void* k, int64_t k_stride, const 
 
 int64_t lewi_paged_attention_workspace_bytes(int D) {
   if (D <= 0) return LEWI_ERR_ARG;
-  return (int64_t)2 * paged_ctas(D) * paged::kRows * (D + 2) * 4;
+  return paged_parts_bytes(D) + paged_kept_bytes(D);
 }
 
 int lewi_paged_attention(void* stream, const void* q, int64_t q_stride, const void* k_cache, const void* v_cache, int64_t page_stride,
@@ -206,7 +217,8 @@ int lewi_paged_attention(void* stream, const void* q, int64_t q_stride, const vo
   const int G = Hq / Hkv, MT = (G + paged::kRows - 1) / paged::kRows;
   const paged::Args a{{tables, lengths, const_cast<bf16*>(reinterpret_cast<const bf16*>(k_cache)),
                        const_cast<bf16*>(reinterpret_cast<const bf16*>(v_cache)), page_stride, B, Hkv, D, (int)pages, page, max_pages},
-                      reinterpret_cast<const bf16*>(q), q_stride, reinterpret_cast<bf16*>(o), reinterpret_cast<float*>(workspace), Hq, G, MT,
+                      reinterpret_cast<const bf16*>(q), q_stride, reinterpret_cast<bf16*>(o), reinterpret_cast<float*>(workspace),
+                      reinterpret_cast<float4*>(reinterpret_cast<uint8_t*>(workspace) + paged_parts_bytes(D)), Hq, G, MT,
                       paged_ctas(D), scale * 1.4426950408889634f};
   cudaStream_t st = as_stream(stream);
   if (D <= 64) return launch_paged<64>(st, a);

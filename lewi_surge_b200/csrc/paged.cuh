@@ -117,6 +117,9 @@ struct Shape {
   static constexpr int kWarps = D == 256 ? 6 : 4, kThreads = kWarps * 32, kCtas = D == 256 ? 1 : 3;   // CTAs per SM
   static constexpr int kChunk = D == 64 ? 32 : 16, kTile = kWarps * kChunk;   // cells that a warp, and all of them, take at a time
   static constexpr int kStage = 2 * kChunk * D * 2, kStages = 2;              // a warp's K and V of them
+  // Tiles that a warp sums up in one chain of products, which the tensor core truncates one by one: a sum of one sign over n cells comes out short by about
+  // n 2^-28 of itself (10^6 cells, four warps: 7e-4).  Then its sums are added, rounded to nearest, to those it keeps in memory.
+  static constexpr int kChain = 32768 / kChunk;
   static constexpr int kRing = kWarps * kStages * kStage;
   static constexpr int kSmem = kRing + kWarps * kRows * kJoinCols * 4 + 2 * kWarps * kRows * 4 + kWarps * kStages * 4 + 128;
 };
@@ -127,6 +130,7 @@ struct Args {
   long long qs;
   __nv_bfloat16* o;         // [B][Hq][D]
   float* part;              // [2 per CTA][16][D] sums, then [2 per CTA][16] maxima, then as many sums of p
+  float4* kept;             // per warp [D / 8][32 lanes] sums of a head's chains so far, then per warp [32] maxima of two rows
   int Hq, G, MT, ctas;      // query heads per key head, groups of 16 of them, CTAs of the list
   float scale_log2;
 };
@@ -182,7 +186,8 @@ __device__ __forceinline__ longlong2 count_tiles(const Cache& c, int upto, long 
   return make_longlong2(all, before);
 }
 
-template <int D>
+// LONG: a head may have more than kChain tiles (apart: the registers that this takes cost 64 sequences of up to 8192, 4 key heads, 104.7 us instead of 101).
+template <int D, bool LONG>
 __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) attend_kernel(const Args a) {
   using S = Shape<D>;
   constexpr int kWarps = S::kWarps;
@@ -295,6 +300,29 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) attend_ke
 
   uint32_t qf[KS][4];
   float o[D / 8][4], m[2], l[2];
+  // o and what earlier chains of the head left, relative to the present maximum; `keep`: goes there, and o starts from zero
+  auto join_chains = [&](bool earlier, bool keep) {
+    float4* at = a.kept + ((long long)blockIdx.x * kWarps + warp) * (D / 8) * 32 + lane;
+    float2* max_at = reinterpret_cast<float2*>(a.kept + (long long)a.ctas * kWarps * (D / 8) * 32) + (blockIdx.x * kWarps + warp) * 32 + lane;
+    float f[2] = {0.f, 0.f};
+    if (earlier) {
+      const float2 before = *max_at;
+      f[0] = before.x == m[0] ? 1.f : exp2f(before.x - m[0]);
+      f[1] = before.y == m[1] ? 1.f : exp2f(before.y - m[1]);
+    }
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) {
+      if (earlier) {
+        const float4 x = at[i * 32];
+        o[i][0] = fmaf(x.x, f[0], o[i][0]); o[i][1] = fmaf(x.y, f[0], o[i][1]); o[i][2] = fmaf(x.z, f[1], o[i][2]); o[i][3] = fmaf(x.w, f[1], o[i][3]);
+      }
+      if (keep) {
+        at[i * 32] = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
+        gdn::zero4(o[i]);
+      }
+    }
+    if (keep) *max_at = make_float2(m[0], m[1]);
+  };
   int stage = 0, part = 2 * blockIdx.x;   // where a part is left: the first head's, then the last one's
   for (long long w = w0; w < w1; ++w) {
     if (w == w0 || use.t == 0) {   // a head starts: its queries, nothing seen yet
@@ -380,7 +408,13 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) attend_ke
     __syncwarp();   // (the stage may be written again)
     stage = stage + 1 == ST ? 0 : stage + 1;
 
-    if (use.t + 1 == use.nt || w + 1 == w1) {   // the head ends here, or this CTA's share of it
+    const bool ends = use.t + 1 == use.nt || w + 1 == w1;   // the head, or this CTA's share of it
+    if (LONG && __builtin_expect((use.t + 1) % S::kChain == 0 || (ends && use.t >= S::kChain), 0)) {
+      const int first = max(0, use.t - (int)min(w - w0, (long long)use.t));   // the share's first tile
+      const bool earlier = first / S::kChain != use.t / S::kChain;
+      if (earlier || !ends) join_chains(earlier, !ends);
+    }
+    if (ends) {
       const int rows = min(kRows, a.G - use.r % a.MT * kRows), r0 = lane >> 2;
       const bool from_start = w - w0 >= use.t, whole = from_start && use.t + 1 == use.nt;
 #pragma unroll

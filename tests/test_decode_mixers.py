@@ -625,3 +625,29 @@ def test_pages_of_one_token_at_a_distance(cuda):
     attention.paged_cache_write(k, -k, *caches, tables, lens)
   assert torch.equal(kc, packed[0]) and torch.equal(vc, packed[1]) and torch.equal(base[:, [1, 2, 4, 5]], other)
   assert torch.equal(attention.paged_attention(q, kc, vc, tables, lens), attention.paged_attention(q, *packed, tables, lens)) and _lib.last_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,b,g", [(64, 480, 3), (128, 480, 16), (256, 160, 2)])
+def test_paged_attention_over_long_sequences_of_one_sign_does_not_come_out_short(cuda, d, b, g):
+  """More sequences than CTAs share one long run of pages, so that a warp sums over a fourth or sixth of a sequence.  The tensor core truncates every sum that it
+  makes: v of one sign would come out short by that.  What is looked at is the mean of the relative errors of outputs whose mantissas lie anywhere
+  (their own roundings, 2^-9 / sqrt(3) of each, and those of p leave less than 2^-13 of it in 64 x D different values); a chain may lose 2^-12."""
+  gen = torch.Generator(device=cuda).manual_seed(23)
+  page, t = 64, 1 << 20
+  rn = lambda *s: torch.rand(*s, generator=gen, device=cuda)
+  grow = 1 + torch.arange(t, device=cuda)[:, None] / t
+  k = torch.randn(t // page, page, 1, d, generator=gen, device=cuda).bfloat16()
+  v = ((1 + rn(1, d)) * grow * (0.9 + 0.2 * rn(t, d))).bfloat16().view(t // page, page, 1, d)
+  lens = torch.randint(t // 2, t + 1, (b,), generator=gen, device=cuda)
+  tables = torch.arange(t // page, dtype=torch.int32, device=cuda).expand(b, -1)
+  q = 0.5 * torch.randn(b, g, d, generator=gen, device=cuda).bfloat16()
+  o = attention.paged_attention(q, k, v, tables, lens)
+  assert _lib.last_status() == 0
+  off = []
+  for i in range(0, b, b // 64 + 1):
+    n = int(lens[i])
+    x = (q[i].to(F64) @ k.view(t, d)[:n].to(F64).t()) * d ** -0.5
+    want = torch.softmax(x, -1) @ v.view(t, d)[:n].to(F64)
+    off.append(((o[i].to(F64) - want) / want).mean())
+  assert abs(torch.stack(off).mean().item()) <= 2.0 ** -12 + 2.0 ** -13, off
