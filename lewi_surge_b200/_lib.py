@@ -8,6 +8,8 @@ import ctypes
 import os
 from ctypes import c_char_p, c_float, c_int, c_int32, c_int64, c_void_p
 
+import torch
+
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "liblewi_moe.so")
 
@@ -151,7 +153,6 @@ def ptr(t):
 def stream(on=None):
   """Handle of the current stream (read directly: wrapping it in a Stream object takes several microseconds per call) of the current device,
   or of the device of the CUDA tensor `on`."""
-  import torch
   return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if on is None else on.get_device())
 
 
@@ -165,7 +166,6 @@ def last_status():
 
 def elsewhere(*tensors):
   """Whether these CUDA tensors (None is left out) lie on a device that is not the current one; they have to lie on one."""
-  import torch
   index = tensors[0].get_device()
   for t in tensors:
     if t is not None and (t.get_device() != index or index < 0):
@@ -187,7 +187,6 @@ def has_tangent(*tensors):
 
 def no_derivative(what, *tensors):
   """Refuses operands that a derivative is wanted of, which `what` has none for: the term would be missing without an error."""
-  import torch
   if torch.is_grad_enabled():
     for t in tensors:
       if t.requires_grad:
@@ -198,13 +197,11 @@ def no_derivative(what, *tensors):
 
 def written(*tensors):
   """Tells autograd that a kernel has written these: a backward pass that had saved one of them raises, as after any in-place operation."""
-  import torch
   torch.autograd.graph.increment_version(tensors)
 
 
 def index_table(t, what):
   """A table of int32 as the kernels read it; int64 values that int32 cannot hold stay out of range."""
-  import torch
   if t is None or (t.dtype is torch.int32 and t.is_contiguous()):
     return t
   if t.dtype is torch.int64:
