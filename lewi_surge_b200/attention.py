@@ -88,6 +88,8 @@ def paged_attention(query, key_cache, value_cache, block_tables, lengths, scale=
     return o
   tables, lens = _lib.index_table(block_tables, "block_tables"), _lib.index_table(lengths, "lengths")
   ws_bytes = lib.lewi_paged_attention_workspace_bytes(d)
+  if ws_bytes < 0:
+    check(ws_bytes, "lewi_paged_attention_workspace_bytes")
   ws = q.new_empty(ws_bytes // 2)
   check(lib.lewi_paged_attention(stream(q), q.data_ptr(), qs, key_cache.data_ptr(), value_cache.data_ptr(), page_stride, tables.data_ptr(),
                                  lens.data_ptr(), o.data_ptr(), ws.data_ptr(), ws_bytes, b, hq, heads, d, pages, page, max_pages,

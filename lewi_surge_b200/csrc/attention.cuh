@@ -1558,6 +1558,7 @@ inline int dkv_parts(int T, int n_seqs, int Hq, int Hkv, int D) {
       best = p;
       least = us;
     }
+    if (item <= share) break;   // (more parts only cost their bytes; after some hundreds at most, however many heads share keys)
   }
   return best;
 }

@@ -203,6 +203,7 @@ int lewi_paged_cache_write(void* stream, const void* k, int64_t k_stride, const 
 
 int64_t lewi_paged_attention_workspace_bytes(int D) {
   if (D <= 0) return LEWI_ERR_ARG;
+  if (D > 256) return LEWI_ERR_LIMIT;
   return paged_parts_bytes(D) + paged_kept_bytes(D);
 }
 
@@ -247,6 +248,7 @@ int lewi_causal_attention_fwd(void* stream, const void* q, int64_t q_stride, con
 
 int64_t lewi_causal_attention_bwd_workspace_bytes(int T, int n_seqs, int Hq, int Hkv, int D) {
   if (T <= 0 || n_seqs <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || Hq % Hkv != 0) return LEWI_ERR_ARG;
+  if (D > attn::kMaxD || (int64_t)T * (Hq / Hkv) > attn::kMaxGroupRows) return LEWI_ERR_LIMIT;
   const int parts = attn::dkv_parts(T, n_seqs, Hq, Hkv, D);
   return delta_bytes(T, Hq) + sums_bytes(T, Hkv, D, parts) + attn::chain_kv_bytes(T, Hq / Hkv, parts, D) + attn::chain_q_bytes(T, D);
 }

@@ -521,3 +521,12 @@ def test_scales_that_float32_does_not_hold_are_refused():
   assert lib.lewi_causal_attention_fwd(None, at, 64, at, 64, at, 64, None, 1, at, at, at, 64, 1, 1, 64, inf) == -1
   for scale in (inf, -inf, float("nan")):
     assert lib.lewi_paged_attention(None, at, 64, at, at, 64, at, at, at, at, 1 << 30, 1, 1, 1, 64, 1, 1, 1, scale) == -1
+
+
+def test_workspace_sizes_of_what_is_refused():
+  """Sizes past the limits get the limit's code, at once: the search for shares of a group of 2^31 - 1 heads would not end."""
+  lib = _lib.load()
+  size = lib.lewi_causal_attention_bwd_workspace_bytes
+  assert size(1, 1, 2 ** 31 - 1, 1, 8) == -5 and size(2 ** 20, 1, 64, 1, 64) == -5 and size(64, 1, 4, 2, 136) == -5 and size(64, 1, 3, 2, 64) == -1
+  assert size(1, 1, 2 ** 25, 1, 8) > 0
+  assert lib.lewi_paged_attention_workspace_bytes(264) == -5 and lib.lewi_paged_attention_workspace_bytes(0) == -1
