@@ -530,3 +530,40 @@ def test_workspace_sizes_of_what_is_refused():
   assert size(1, 1, 2 ** 31 - 1, 1, 8) == -5 and size(2 ** 20, 1, 64, 1, 64) == -5 and size(64, 1, 4, 2, 136) == -5 and size(64, 1, 3, 2, 64) == -1
   assert size(1, 1, 2 ** 25, 1, 8) > 0
   assert lib.lewi_paged_attention_workspace_bytes(264) == -5 and lib.lewi_paged_attention_workspace_bytes(0) == -1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,d", [(2, 2, 96), (2, 1, 64)])
+def test_a_long_ragged_sequence_between_others(cuda, hq, hkv, d):
+  """Sums kept in memory, of a sequence whose last tile is not full, between short ones and rows of none: the bits that each has alone, o against 64 bits."""
+  gen = torch.Generator(device=cuda).manual_seed(24)
+  lens = [5, 40001, 0, 300]
+  cu = (torch.tensor([0] + lens).cumsum(0) + 7).tolist()
+  t = cu[-1] + 50
+  q, k, v, d_o = (torch.randn(t, h, d, generator=gen, device=cuda).bfloat16() for h in (hq, hkv, hkv, hq))
+  def call(rows, bounds):
+    leaves = [x[rows].detach().requires_grad_(True) for x in (q, k, v)]
+    o = attention.causal_attention(*leaves, torch.tensor(bounds, device=cuda))
+    return o.detach(), *torch.autograd.grad(o, leaves, d_o[rows])
+  whole = call(slice(0, t), cu)
+  exact_heads = hq == hkv   # (a group's heads are summed in shares that depend on the whole call)
+  for a, b in zip(cu, cu[1:]):
+    if a < b:
+      alone = call(slice(a, b), [0, b - a])
+      for got, want in zip(whole[:4 if exact_heads else 2], alone):
+        assert torch.equal(got[a:b], want)
+      for got, want in zip(whole[2:], alone[2:]):
+        assert (got[a:b].float() - want.float()).norm() <= 2.0 ** -8 * want.float().norm()
+  for x in whole:
+    assert not x[:7].any() and not x[cu[-1]:].any()
+  with torch.no_grad():
+    o = attention.causal_attention(q, k, v, torch.tensor(cu, device=cuda))
+  rows = torch.tensor([0, 127, 128, 32767, 32768, 32769, 36000, 39999, 40000], device=cuda)
+  for h in range(hq):
+    kh, vh = (x[cu[1]:cu[2], h // (hq // hkv)].to(F64) for x in (k, v))
+    x = (q[cu[1]:cu[2], h][rows].to(F64) @ kh.t()) * d ** -0.5
+    p = torch.softmax(x.masked_fill(torch.arange(lens[1], device=cuda) > rows[:, None], float("-inf")), -1)
+    want = (p @ vh).cpu(), (U * (p @ vh).abs() + (U + F32) * (p @ vh.abs())).cpu()
+    within(o[cu[1]:cu[2], h][rows], want, "o")
+    within(whole[0][cu[1]:cu[2], h][rows], want, "o in training")
+  assert _lib.last_status() == 0
