@@ -809,7 +809,7 @@ __global__ void __launch_bounds__(kDeltaThreads) delta_kernel(const __nv_bfloat1
 // warp 11: lse and delta, and the rows of other sequences in a tile.  Scores have kScores places, P(i) takes that of S(i).  Order of products:
 // S(0) dP(0) .. S(kScores - 1) | dV(i) S(i + kScores) after P(i), dK(i) dP(i+1) after dS(i): exponentials are made while dK and dP
 // run, dS while dV and S do, and with two places, which dV and dK leave at D <= 64, the next scores are there when dS has been made (8192
-// rows, 32 heads over 8: 575 us, with one place 715).  dS is rounded to bf16 for its products, as p is: of the error of dQ and dK (2.5e-3 of their
+// rows, 32 heads over 8: 567 us, with one place 715).  dS is rounded to bf16 for its products, as p is: of the error of dQ and dK (2.5e-3 of their
 // norm) that is as much as their own rounding; where both tiles are a sequence's first (the norm is largest there) what that left of dS and p is
 // multiplied too (8191 rows in 13 sequences, 16 heads over 4, D = 64: 97 us and an error of 2.0e-3, without 90 and 2.4e-3).
 // One sequence of 16,384, 16 heads over 2, D = 128: 1.75 ms, 2650 cycles for a pair of tiles whose four products take 2048.
@@ -1225,7 +1225,7 @@ __global__ void __launch_bounds__(kSumThreads) dkv_sum_kernel(const Args a) {
 // 650 us with five, 780 with four), so at D = 128 dQ is stored row by row.
 // At D = 64 three products take 770 cycles of 1640 for a pair of tiles, and what the warp that issues them does between them counts: it loops as a whole over
 // values that all its lanes share, with one elected for the instructions (8192 x 32 heads: 442 us as a loop of one thread, 405 so), and K and V come
-// as pairs on one barrier (398).  The forward pass and the kernel for dK and dV, which wait for their exponentials, lose 2 % by the former.
+// as pairs on one barrier (398; 408 since there are chains).  The forward pass and the kernel for dK and dV, which wait for their exponentials, lose 2 % by the former.
 template <int DP>
 struct DqShape {
   static constexpr bool kPairs = DP == 64, kStaged = DP == 64;   // (a place is K's and V's)
@@ -1525,7 +1525,8 @@ inline bool make_rows_map(CUtensorMap* m, const void* p, int T, int heads, int D
 }
 
 // Pairs of tiles of the longest row of tiles, and an SM's share of all of them.  What lengths several sequences have only the device knows: the longest
-// is taken to be three times the mean.
+// is taken to be three times the mean, which is far off where one is long and many are short (4096 + 400 x 10 rows, 32 heads over 1: two parts for dK
+// and dV, where by the costs below six would be best).
 struct Blocks {
   double longest, share;
 };
@@ -1535,7 +1536,7 @@ inline Blocks blocks_of(int T, int n_seqs, int Hq) {
 }
 
 // An item of the forward pass is two heads or two tiles, or one tile where that is over sooner: a block of the former takes 1.6 us for its two
-// tiles, of the latter 1.15 us for one, and an SM is done with its share or with the longest item.  One sequence, 16 heads over 2, D = 128, two
+// tiles, of the latter 1.15 us for one (at D = 128; D = 64 goes by the same), and an SM is done with its share or with the longest item.  One sequence, 16 heads over 2, D = 128, two
 // heads and one tile: of 256 rows 9.9 and 8.1 us, 1000 19 and 14, 2048 32 and 23, 4096 57 and 65.
 inline FwdItem fwd_item(int T, int n_seqs, int Hq, int G) {
   const Blocks b = blocks_of(T, n_seqs, Hq);

@@ -101,12 +101,13 @@ __global__ void __launch_bounds__(kWriteThreads) write_kernel(const WriteArgs a)
 //
 // Bound by the cache's way from HBM: 4 Hkv D bytes per cell (64 sequences of up to 8192, 4 key heads, D = 128: 101 us, 5.3 TB/s, of which 15 us are
 // the first loads, which depend on one another, and the join).  The cells of all sequences and key heads are one long list of tiles of
-// 64 or 128 cells, of which every CTA takes an equal run, whatever the lengths (they are read on the device, so a captured launch follows
-// them).  The query heads that share a key head are the 16 rows of an `mma.sync` (m16n8k16), a warp's 16 cells (32 where D <= 64) its columns; a
+// 64 cells (128 where D <= 64, 96 where D > 128), of which every CTA takes an equal run, whatever the lengths (they are read on the device, so a
+// captured launch follows them).  The query heads that share a key head are the 16 rows of an `mma.sync` (m16n8k16), a warp's 16 cells (32 where D <= 64) its columns; a
 // warp has its own ring of tiles in shared memory (cp.async) and its own softmax, and nothing is synchronised before a head's
-// tiles end.  There the four warps' results are joined; a head that one CTA has whole is written out, of the others every CTA leaves
+// tiles end.  There the four (six) warps' results are joined; a head that one CTA has whole is written out, of the others every CTA leaves
 // its part (at most two per CTA) and `join_kernel` adds them up in the order of the cells.
-// p is rounded to bf16 for its product with v (relative 2^-9, like the output's own rounding); its sum is taken before.
+// p is rounded to bf16 for its product with v (relative 2^-8 at most, as the output's own rounding); its sum is taken before.  A second product with what
+// that left would bring errors of 2.1e-3 of the output's norm down to its own rounding's 1.7e-3, and takes 104.5 instead of 101 us (D = 96: 89, 82).
 constexpr int kRows = 16, kJoinCols = 32;
 
 // What bounds a warp is the latency of its chain from scores to sums, so as many warps as there is room for share an SM: three CTAs of four with
@@ -117,8 +118,8 @@ struct Shape {
   static constexpr int kWarps = D == 256 ? 6 : 4, kThreads = kWarps * 32, kCtas = D == 256 ? 1 : 3;   // CTAs per SM
   static constexpr int kChunk = D == 64 ? 32 : 16, kTile = kWarps * kChunk;   // cells that a warp, and all of them, take at a time
   static constexpr int kStage = 2 * kChunk * D * 2, kStages = 2;              // a warp's K and V of them
-  // Tiles that a warp sums up in one chain of products, which the tensor core truncates one by one: a sum of one sign over n cells comes out short by about
-  // n 2^-28 of itself (10^6 cells, four warps: 7e-4).  Then its sums are added, rounded to nearest, to those it keeps in memory.
+  // Tiles that a warp sums up in one chain of products, which the tensor core truncates one by one: a sum of one sign over n of its cells comes out short by
+  // about n 2^-28 of itself (of 10^6 cells, shared by four warps: 7e-4).  Then its sums are added, rounded to nearest, to those it keeps in memory.
   static constexpr int kChain = 32768 / kChunk;
   static constexpr int kRing = kWarps * kStages * kStage;
   static constexpr int kSmem = kRing + kWarps * kRows * kJoinCols * 4 + 2 * kWarps * kRows * 4 + kWarps * kStages * 4 + 128;

@@ -414,7 +414,7 @@ def test_dq_beside_dk_and_dv_is_dq_alone(cuda):
 def test_long_sums_of_one_sign_do_not_come_out_short(cuda, log_t, hq, d, empty):
   """A tensor core truncates every sum that it makes, so a long chain of products of one sign comes out short.  Scores of zero make every p of row t
   1 / (t + 1) and the exact results running sums (but for the first key's, in o).  What is looked at is the mean of the relative errors of 10^6
-  values and more, whose own roundings (2^-9 / sqrt(3) each, as many up as down) leave less than 2^-18 of it, and those of p and dS, alike for all
+  values and more, whose own roundings (2^-8 / sqrt(3) each at most, as many up as down) leave less than 2^-18 of it, and those of p and dS, alike for all
   of a row but different from row to row, 2^-16; 2^-14 is room for them and for float32.  An accumulator may lose 2^-12.  Empty sequences
   beside the long one make one tile an item in the forward pass."""
   gen = torch.Generator(device=cuda).manual_seed(13)
