@@ -28,7 +28,7 @@ def _check_cache(what, key_cache, value_cache, block_tables, lengths):
       page_stride = key_cache.stride(0)
   if len(tables) != 2 or lengths.shape != tables[:1]:
     raise LewiError(f"{what}: block_tables [B, max_pages] and lengths [B] are required")
-  _lib.fits(what, page, heads, tables[0], tables[1])
+  _lib.fits(what, page, heads, d, tables[0], tables[1])
   return pages, page, heads, d, page_stride
 
 
@@ -167,7 +167,7 @@ def causal_attention(query, key, value, cu_seqlens=None, scale=None):
       shape[-2] % other[-2]:
     raise LewiError("causal_attention: query [T, Hq, D] and key, value [T, Hkv, D], or all three [B, S, ..], Hq a multiple of Hkv, are required")
   n_seqs = 1 if n == 3 else shape[0]
-  _lib.fits("causal_attention", shape[0] * (shape[1] if n == 4 else 1), shape[-2])
+  _lib.fits("causal_attention", shape[0] * (shape[1] if n == 4 else 1), shape[-2], shape[-1])
   if cu_seqlens is not None:
     if n == 4 or cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 2:
       raise LewiError("causal_attention: cu_seqlens [N + 1] belongs to packed rows [T, H, D]")

@@ -143,7 +143,7 @@ def causal_conv1d_step(x, w, state, slots=None):
   if len(ss) != 3 or ss[1] != k - 1 or ss[2] != c:
     raise LewiError("causal_conv1d_step: state [N,K-1,C] is required")
   _check_slots("causal_conv1d_step", b, ss[0], slots)
-  _lib.fits("causal_conv1d_step", b, ss[0], c)
+  _lib.fits("causal_conv1d_step", b, ss[0], c, k)
   _lib.no_derivative("causal_conv1d_step", x, w, state)
   if _lib.elsewhere(x, w, state, slots):
     with torch.cuda.device(x.device):
@@ -182,7 +182,7 @@ def gated_delta_step(query, key, value, g, beta, state, slots=None):
   g_type, beta_type = _GATES.get(g.dtype), _GATES.get(beta.dtype)
   if g_type is None or beta_type is None:
     raise LewiError("gated_delta_step takes float32 or bfloat16 g and beta")
-  _lib.fits("gated_delta_step", b, ss[0], hk, h, vd)
+  _lib.fits("gated_delta_step", b, ss[0], hk, h, kd, vd)
   _lib.no_derivative("gated_delta_step", query, key, value, g, beta, state)
   if _lib.elsewhere(query, key, value, g, beta, state, slots):
     with torch.cuda.device(query.device):

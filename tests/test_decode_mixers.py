@@ -510,6 +510,8 @@ def test_sizes_past_32_bits_are_refused():
                lambda: attention.paged_cache_write(e(huge, 1, 8), e(huge, 1, 8), e(4, 16, 1, 8).contiguous(), e(4, 16, 1, 8).contiguous(), e(2, 2, dtype=i32),
                                                    e(2, dtype=i32), e(3, dtype=i32)),
                lambda: attention.causal_attention(e(huge, 2, 8), e(huge, 1, 8), e(huge, 1, 8)),
+               lambda: attention.causal_attention(e(2, 2, huge), e(2, 1, huge), e(2, 1, huge)), lambda: seqmix.causal_conv1d_step(e(2, 8), e(huge, 1, 8), e(2, huge - 1, 8)),
+               lambda: seqmix.gated_delta_step(e(2, 1, huge), e(2, 1, huge), e(2, 1, 8), e(2, 1), e(2, 1), e(2, 1, huge, 8, dtype=torch.float32)),
                lambda: attention.causal_attention(e(2 ** 16, 2 ** 16 + 1, 2, 8), e(2 ** 16, 2 ** 16 + 1, 1, 8), e(2 ** 16, 2 ** 16 + 1, 1, 8)),
                lambda: attention.causal_attention(e(4, 2, 8), e(4, 1, 8), e(4, 1, 8), e(huge, dtype=i32))):
     with pytest.raises(LewiError, match="32 bits"):
